@@ -18,9 +18,16 @@ from __future__ import annotations
 
 import functools
 import math
+import sys
+from pathlib import Path
 
 import numpy as np
 import torch
+
+#: where this repository keeps its package
+_PACKAGE = str(Path(__file__).resolve().parent.parent / "tq-local_amd")
+if _PACKAGE not in sys.path:
+    sys.path.insert(0, _PACKAGE)
 
 own = False
 
