@@ -322,6 +322,59 @@ int tq_dense_attention(const void* q, int q_is_f32, int batch, int q_heads, int 
                        float scale, float* partials, int slots, int first_slot, int n_split, int accumulate,
                        const float* prev, const float* prev_lse, float* out_f32, uint16_t* out_bf16, void* stream);
 
+/*
+ * Causal attention over whole prompts: row i of a sequence attends to its rows up to i.  No counterpart
+ * in the reference, whose prompts run on the framework's own attention (runtime/attention.py:75-99).
+ *
+ *   q, k, v  bf16, or fp16 with is_f16, [batch][heads][tokens][dim] with element strides (multiples of 8;
+ *            dim contiguous, rows 16-byte aligned); q_heads a multiple of kv_heads
+ *   out      the same type, likewise strided
+ *   lse      fp32 [batch][q_heads][tokens] log-sum-exp of the scaled logits (nullable; -inf for a row
+ *            without tokens), for merging with attention over other tokens
+ *   cu_seqlens  int32 [n_seqs + 1] (device, nullable), ascending: packed sequences, sequence i the rows
+ *            [cu_seqlens[i], cu_seqlens[i + 1]); batch is 1 then.  Rows of no sequence get 0 (lse -inf)
+ *            with zero_outside, else they stay as they were
+ *   seq_starts, seq_ends  int32 [batch] (device, nullable; not with cu_seqlens): row b's sequence is
+ *            [start, end), for padded batches; the other rows get 0 (lse -inf)
+ *   scale    logit scale, > 0 and finite
+ * Offsets are clamped to [0, tokens].  TQ_ERR_UNSUPPORTED beyond 2^30 tokens, or 2^24 blocks of 128 rows
+ * over all query heads.
+ */
+int tq_prompt_attention(const void* q, const void* k, const void* v, void* out, float* lse, int is_f16, int batch,
+                        int q_heads, int kv_heads, int64_t tokens, int dim, int64_t q_sb, int64_t q_sh, int64_t q_st,
+                        int64_t k_sb, int64_t k_sh, int64_t k_st, int64_t v_sb, int64_t v_sh, int64_t v_st,
+                        int64_t o_sb, int64_t o_sh, int64_t o_st, const int32_t* cu_seqlens, int n_seqs,
+                        const int32_t* seq_starts, const int32_t* seq_ends, int zero_outside, float scale,
+                        void* stream);
+
+/*
+ * A new cache of chosen batch rows and tokens: for every buffer, batch row b, head and j < n
+ *   dst[b][head][j] = src[rows[b]][head][index[b][head][j]],   dst[b][head][n..dst_cap) = 0
+ * with n = n_index, or tokens (the source's valid slots) without an index.  Replaces the torch
+ * operations per buffer of the reference's containers (runtime/packed_qmse_cache.py:81-92, 135-140).
+ *   src, dst   HOST arrays of n_buffers (1..16) device pointers, [batch][heads][cap] rows of row_bytes[i]
+ *              bytes (host array, 1..TQ_MAX_ROW_BYTES); src and dst must not overlap
+ *   rows       int32 [dst_batch] (device, nullable: row b is row b)
+ *   index      int32 (device, nullable), element (b, head, j) at b index_sb + head index_sh + j
+ * A row outside [0, src_batch), or an index outside [0, tokens), gives zeros.
+ */
+#define TQ_MAX_ROW_BYTES 256
+int tq_gather_tokens(int n_buffers, const void* const* src, void* const* dst, const int* row_bytes, int src_batch,
+                     int heads, int64_t src_cap, int64_t tokens, int dst_batch, int64_t dst_cap, const int32_t* rows,
+                     const int32_t* index, int64_t index_sb, int64_t index_sh, int64_t n_index, void* stream);
+
+/*
+ * In place: of the slots [first, first + tokens) of every buffer, batch row and head, slot first + j becomes
+ * slot first + index[b][head][j] for j < n_index <= TQ_MAX_KEEP (an accepted path of drafted tokens closed
+ * up).  All are read before any is written: the index may have any order and name a slot more than once; an
+ * index outside [0, tokens) gives zeros.  The slots from first + n_index on stay as they were.  Arguments as
+ * for tq_gather_tokens.
+ */
+#define TQ_MAX_KEEP 256
+int tq_keep_tokens(int n_buffers, void* const* buffers, const int* row_bytes, int batch, int heads, int64_t cap,
+                   int64_t first, int64_t tokens, const int32_t* index, int64_t index_sb, int64_t index_sh,
+                   int n_index, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -350,6 +350,18 @@ def chunked_turboquant_attention(query_states: torch.Tensor, packed_layer: "Pack
     return (o / s.clamp(min=1e-8)).to(query_states.dtype)
 
 
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *,
+                     cu_seqlens: torch.Tensor | None = None, seq_starts: torch.Tensor | None = None,
+                     seq_ends: torch.Tensor | None = None, scale: float | None = None,
+                     out: torch.Tensor | None = None, return_lse: bool = False):
+    """Causal attention over whole prompts, [B, Hq, S, D] against [B, Hkv, S, D] (bf16 or fp16) -> [B, Hq, S, D].
+
+    A padded batch gives each row's [``seq_starts``, ``seq_ends``); prompts packed behind one another (B = 1)
+    give ``cu_seqlens``.  See ``kernels.prompt_attention``."""
+    return K.prompt_attention(query, key, value, cu_seqlens=cu_seqlens, seq_starts=seq_starts, seq_ends=seq_ends,
+                              scale=scale, out=out, want_lse=return_lse)
+
+
 def _sdpa_fallback(module, query, key, value, attention_mask, scaling):
     """Standard SDPA for prefill and norm-guarded dense layers (reference :75-99)."""
     causal = attention_mask is None and query.shape[-2] > 1

@@ -528,6 +528,183 @@ class DenseAttention:
         return None if o is None else o.to(out)
 
 
+def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no backward pass: call it under torch.no_grad()")
+
+
+def _on_device(fn: str, device: torch.device, *args) -> None:
+    """The C call, made with ``device`` as the current one (a stream belongs to its device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        _lib.call(fn, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(fn, *args)
+
+
+def _int32_on(t: torch.Tensor | None, device: torch.device, name: str, shape: tuple) -> torch.Tensor | None:
+    """``t`` as a contiguous int32 tensor of ``shape`` on ``device`` (itself when it is one)."""
+    if t is None:
+        return None
+    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be int32 or int64 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: torch.Tensor | None = None,
+                     seq_starts: torch.Tensor | None = None, seq_ends: torch.Tensor | None = None,
+                     scale: float | None = None, out: torch.Tensor | None = None, want_lse: bool = False):
+    """Causal attention over whole prompts (tq_prompt_attention).
+
+    q [B, Hq, S, D], k and v [B, Hkv, S, D], bf16 or fp16, any strides with D contiguous; Hq a multiple of
+    Hkv.  ``seq_starts`` / ``seq_ends`` int [B] bound each row's sequence in a padded batch (the other
+    rows get 0).  ``cu_seqlens`` int [n + 1], ascending from 0: sequences packed behind one another (B = 1);
+    rows behind the last one stay as they were in a given ``out``, and are 0 otherwise.  Returns
+    [B, Hq, S, D] laid out token by token ([B, S, Hq, D] in memory), and with ``want_lse`` the fp32
+    log-sum-exp [B, Hq, S] of the scaled logits (-inf for a row without tokens).
+    """
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"expected q [B, Hq, S, D] and k, v [B, Hkv, S, D], got {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(v.shape)}")
+    B, Hq, S, D = q.shape
+    Hkv = k.shape[1]
+    if D != HEAD_DIM:
+        raise ValueError(f"head_dim {D} unsupported (kernels are built for {HEAD_DIM})")
+    if k.shape[0] != B or k.shape[2] != S or k.shape[3] != D or Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"k, v {tuple(k.shape)} do not match q {tuple(q.shape)}: a whole prompt has as many keys as rows")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v must all be bf16 or all fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    _no_gradient("prompt_attention", q, k, v)
+    _require_gpu(q, k, v)
+    dev = q.device
+    if k.device != dev or v.device != dev:
+        raise ValueError("q, k and v must be on one device")
+    n_seqs = 0
+    if cu_seqlens is not None:
+        if B != 1 or seq_starts is not None or seq_ends is not None:
+            raise ValueError("cu_seqlens takes packed sequences [1, H, tokens, D], without seq_starts / seq_ends")
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+            raise ValueError(f"cu_seqlens must be [sequences + 1], got {tuple(cu_seqlens.shape)}")
+        n_seqs = cu_seqlens.numel() - 1
+        cu_seqlens = _int32_on(cu_seqlens, dev, "cu_seqlens", (n_seqs + 1,))
+    seq_starts = _int32_on(seq_starts, dev, "seq_starts", (B,))
+    seq_ends = _int32_on(seq_ends, dev, "seq_ends", (B,))
+    zero_outside = out is None
+    if out is None:
+        out = torch.empty(B, S, Hq, D, dtype=q.dtype, device=dev).transpose(1, 2)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or rows16(out) is not out:
+        raise ValueError("out must have q's shape, dtype and device, with 16-byte aligned rows")
+    lse = torch.empty(B, Hq, S, dtype=torch.float32, device=dev) if want_lse else None
+    if q.numel() == 0:
+        return (out, lse) if want_lse else out
+    if want_lse and not zero_outside:
+        lse.fill_(float("-inf"))
+    q, k, v = rows16(q), rows16(k), rows16(v)
+    s = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    _on_device("tq_prompt_attention", dev, _vp(q), _vp(k), _vp(v), _vp(out), _vp(lse), int(q.dtype == torch.float16), B,
+               Hq, Hkv, S, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], _vp(cu_seqlens),
+               n_seqs, _vp(seq_starts), _vp(seq_ends), int(zero_outside), s, _stream(dev))
+    return (out, lse) if want_lse else out
+
+
+#: most buffers of one launch, and the limits of TQ_MAX_KEEP and TQ_MAX_ROW_BYTES
+_MOVE_BUFFERS = 16
+MAX_KEEP = 256
+_MAX_ROW_BYTES = 256
+
+
+def _move_buffers(name: str, buffers: list[torch.Tensor]) -> tuple[int, int, int, list[int]]:
+    """(batch, heads, cap, row bytes) of a layer's [B, H, cap, ...] buffers."""
+    if not buffers:
+        raise ValueError(f"{name}: no buffers")
+    first = buffers[0]
+    rows = []
+    for b in buffers:
+        if b.dim() < 3 or b.shape[:3] != first.shape[:3] or not b.is_contiguous() or b.device != first.device:
+            raise ValueError(f"{name}: expected contiguous [B, H, cap, ...] buffers of one shape and device, got "
+                             f"{tuple(b.shape)}")
+        rows.append(math.prod(b.shape[3:]) * b.element_size())
+        if not 1 <= rows[-1] <= _MAX_ROW_BYTES:
+            raise ValueError(f"{name}: {rows[-1]} bytes to a token ({_MAX_ROW_BYTES} at most)")
+    _require_gpu(*buffers)
+    return int(first.shape[0]), int(first.shape[1]), int(first.shape[2]), rows
+
+
+def _token_index(name: str, index: torch.Tensor, batch: int, heads: int, device: torch.device):
+    """``index`` [n], [B, n] or [B, H, n] as int32, with its strides over batch and heads."""
+    if index.dtype not in (torch.int32, torch.int64) or not 1 <= index.dim() <= 3:
+        raise ValueError(f"{name}: index must be int32 or int64 [n], [B, n] or [B, H, n]")
+    lead = (batch, heads)[:index.dim() - 1]
+    if tuple(index.shape[:-1]) != lead:
+        raise ValueError(f"{name}: index {tuple(index.shape)} does not match batch {batch}, heads {heads}")
+    index = index.to(device=device, dtype=torch.int32).contiguous()
+    n = int(index.shape[-1])
+    return index, (n * heads if index.dim() == 3 else n if index.dim() == 2 else 0), (n if index.dim() == 3 else 0), n
+
+
+def _pointers(tensors) -> ctypes.Array:
+    return (ctypes.c_void_p * len(tensors))(*(t.data_ptr() for t in tensors))
+
+
+def gather_tokens(buffers: list[torch.Tensor], *, tokens: int, rows: torch.Tensor | None = None,
+                  index: torch.Tensor | None = None, capacity: int | None = None) -> list[torch.Tensor]:
+    """New buffers with chosen batch rows and tokens of a layer's buffers [B, H, cap, ...] (tq_gather_tokens).
+
+    ``tokens`` slots of the source are valid.  ``rows`` int [R]: batch row r of the result is row rows[r]
+    (the same rows without).  ``index`` int [n], [R, n] or [R, H, n]: its tokens (all of them without).
+    The result has ``capacity`` slots (as many as it has tokens without), zero behind its tokens.  A row or
+    an index outside the source gives zeros.
+    """
+    B, H, cap, row_bytes = _move_buffers("gather_tokens", buffers)
+    dev = buffers[0].device
+    if not 0 <= tokens <= cap:
+        raise ValueError(f"gather_tokens: {tokens} tokens of a capacity of {cap}")
+    R = B
+    if rows is not None:
+        if rows.dim() != 1:
+            raise ValueError("gather_tokens: rows must be [R]")
+        R = int(rows.numel())
+        rows = _int32_on(rows, dev, "rows", (R,))
+    n, sb, sh = tokens, 0, 0
+    if index is not None:
+        index, sb, sh, n = _token_index("gather_tokens", index, R, H, dev)
+    slots = n if capacity is None else int(capacity)
+    if slots < n:
+        raise ValueError(f"gather_tokens: {n} tokens do not fit a capacity of {slots}")
+    out = [torch.empty(R, H, slots, *b.shape[3:], dtype=b.dtype, device=dev) for b in buffers]
+    if R == 0 or H == 0 or slots == 0:
+        return out
+    if B == 0 or n == 0:
+        return [o.zero_() for o in out]
+    for a in range(0, len(buffers), _MOVE_BUFFERS):
+        part = slice(a, a + _MOVE_BUFFERS)
+        count = len(buffers[part])
+        _on_device("tq_gather_tokens", dev, count, _pointers(buffers[part]), _pointers(out[part]),
+                   (ctypes.c_int * count)(*row_bytes[part]), B, H, cap, tokens, R, slots, _vp(rows), _vp(index), sb, sh,
+                   n, _stream(dev))
+    return out
+
+
+def keep_tokens(buffers: list[torch.Tensor], index: torch.Tensor, *, first: int, tokens: int) -> None:
+    """In place, in every buffer [B, H, cap, ...]: of the slots [first, first + tokens), slot first + j becomes
+    slot first + index[j] (tq_keep_tokens).  ``index`` int [n], [B, n] or [B, H, n], n <= 256, in any order;
+    an index outside [0, tokens) gives zeros.  The slots from first + n on stay as they were."""
+    B, H, cap, row_bytes = _move_buffers("keep_tokens", buffers)
+    dev = buffers[0].device
+    if first < 0 or tokens < 0 or first + tokens > cap:
+        raise ValueError(f"keep_tokens: slots [{first}, {first + tokens}) of a capacity of {cap}")
+    index, sb, sh, n = _token_index("keep_tokens", index, B, H, dev)
+    if n > min(tokens, MAX_KEEP):
+        raise ValueError(f"keep_tokens: {n} of {tokens} tokens (at most {MAX_KEEP}; gather_tokens takes more)")
+    if n == 0 or B * H == 0:
+        return
+    for a in range(0, len(buffers), _MOVE_BUFFERS):
+        part = slice(a, a + _MOVE_BUFFERS)
+        count = len(buffers[part])
+        _on_device("tq_keep_tokens", dev, count, _pointers(buffers[part]), (ctypes.c_int * count)(*row_bytes[part]), B,
+                   H, cap, first, tokens, _vp(index), sb, sh, n, _stream(dev))
+
+
 def rows16(t: torch.Tensor) -> torch.Tensor:
     """``t`` with rows of its last dimension contiguous and 16-byte aligned (itself when it is)."""
     n = 16 // t.element_size()
