@@ -348,6 +348,35 @@ int tq_prompt_attention(const void* q, const void* k, const void* v, void* out, 
                         void* stream);
 
 /*
+ * Attention of a tree of drafted tokens over the packed cache: `nodes` (1..TQ_MAX_NODES) query tokens per
+ * sequence.  With `parents` the nodes' own keys and values stand packed in the `nodes` slots behind the
+ * history, and node i attends to the history, to its ancestors and to itself; without (NULL) every node
+ * attends to the history alone.  The reference's several-token path decodes all rows instead
+ * (runtime/attention.py:215-304).
+ *
+ *   q        q_type 0: bf16, 1: fp32, 2: fp16; [batch][q_heads][nodes][dim] with element strides, dim contiguous
+ *   parents  int32 (device), node i of row b at b parents_sb + i: the node it follows, < i; anything else: none
+ *   seq_starts, seq_lens  int32 [batch] (device, nullable: 0 and n_tokens - nodes): row b's history is the
+ *            slots [start, len), its nodes the slots [len, len + nodes); slots from n_tokens on are not attended
+ *   n_tokens slots stored per group, nodes included (<= cap)
+ *   packed cache, codecs, scale (> 0), out_f32 / out_bf16 [batch][q_heads][nodes][dim] (at least one) and
+ *   lse_out [batch][q_heads][nodes] as for tq_decode_attention; any number of query heads per KV head
+ *   workspace  device scratch of tq_tree_attention_workspace_bytes() (16-byte aligned), used during the
+ *            call only
+ * A node without tokens gets 0 (lse -inf).
+ */
+#define TQ_MAX_NODES 64
+size_t tq_tree_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int nodes, int dim, int64_t n_tokens);
+int tq_tree_attention(const void* q, int q_type, int batch, int q_heads, int kv_heads, int nodes, int dim, int64_t q_sb,
+                      int64_t q_sh, int64_t q_st, const int32_t* parents, int64_t parents_sb,
+                      const int32_t* seq_starts, const int32_t* seq_lens, int64_t n_tokens, int64_t cap,
+                      const uint8_t* k_codes, const uint16_t* k_norms, const uint8_t* k_signs,
+                      const uint16_t* k_rnorms, const uint8_t* v_codes, const uint16_t* v_norms, int key_bits,
+                      int value_bits, int has_qjl, const float* key_rotation, const float* key_centers, const float* qjl,
+                      const float* value_rotation, const float* value_centers, float scale, float* out_f32,
+                      uint16_t* out_bf16, float* lse_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * A new cache of chosen batch rows and tokens: for every buffer, batch row b, head and j < n
  *   dst[b][head][j] = src[rows[b]][head][index[b][head][j]],   dst[b][head][n..dst_cap) = 0
  * with n = n_index, or tokens (the source's valid slots) without an index.  Replaces the torch

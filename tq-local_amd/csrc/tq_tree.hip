@@ -1,0 +1,673 @@
+// tq_tree.hip -- attention of a tree of drafted tokens over the packed TurboQuant cache (gfx950).
+//
+// T <= 64 drafted tokens (nodes) of each sequence stand packed in the slots behind its history.  Node i
+// attends to the history, to its ancestors and to itself:
+//   logit_t = scale (|k_t| <q R_k^T, C_k[kidx_t]> + sqrt(pi/2)/D |r_t| <q S^T, s_t>)
+//   out     = (sum_t softmax_t |v_t| C_v[vidx_t]) R_v
+// so keys and values are never rotated: the queries are, once, and the sums are rotated back, once.
+//
+//   prep_kernel   32 query rows of a KV head per workgroup: q R_k^T and q S^T, scaled by a power of two per
+//                 row, in fp16, in the order the products below take them
+//   tree_kernel   a token range of one KV head per workgroup, 32 query rows (head x node) per wave.  Tiles of
+//                 64 tokens: all waves turn the packed codes into fp16 rows in LDS, then each forms
+//                 S^T = K Q^T (codes and signs apart: their norms differ) and O^T = V^T P^T with
+//                 v_mfma_f32_32x32x16_f16
+//   merge_kernel  the splits' partials of a row weighed and added, rotated back by R_v
+//
+// Codes to fp16: a byte lookup (v_perm_b32) of the centroid's two halves for four codes at once, from
+// tables in registers.  Which four codes meet in a register follows from the packing (those at the same
+// bits of neighbouring bytes), so each bit width has an order of the 128 dims of its own, which the queries
+// are written in and the sums are read back in (dim_of).
+//
+// Rounding.  Rotated queries and centroids are rounded once to fp16, 2^-12 of each (with |q| = 11 and |k| = 20 the
+// logits move by 3e-4 of their unit), value centroids too (their sum's errors are kept from adding up by the
+// codebook, see tq_value_codebook_f16), weights times norm p |v| once, 2^-12 of each.  Logits, maxima, weights, sums
+// and outputs are fp32.
+
+#include <algorithm>
+
+#include "tq_common.h"
+
+namespace {
+
+constexpr int D = TQ_DIM;
+constexpr int TK = 64;         // tokens per tile
+constexpr int MAX_SPLIT = 64;  // partials a merge wave weighs with one lane each
+constexpr float LOG2E = 1.44269504f;
+constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+union Frag {
+    uint32_t u[4];
+    uint4 q;
+    s16x4 t[2];
+    f16x8 f;
+};
+
+__device__ __forceinline__ f32x16 mfma_f16(const Frag& a, const Frag& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.f, b.f, c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const f32x2 p = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(p, f16x2));
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+    return __builtin_amdgcn_perm(hi, lo, sel);
+}
+__device__ __forceinline__ f32x16 zero16() {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+    return z;
+}
+
+// A row of 128 dims is 16 chunks of 8 elements: chunk 2 s + h is the s-th of dims [64 h, 64 h + 64).  The dim at
+// element e of it for codes of `bits` bits (0: the QJL signs).  Codes of one and of three bits are at the same
+// bits of bytes 8 codes apart, of two bits 4 apart, of four bits 2 apart.
+__host__ __device__ constexpr int dim_of(int bits, int chunk, int e) {
+    const int s = chunk >> 1, h = chunk & 1;
+    if (bits == 0) return 64 * h + 32 * (s >> 2) + 4 * (s & 3) + (e >> 1) + 16 * (e & 1);
+    const int st = bits == 4 ? 2 : bits == 2 ? 4 : 8, per = st / 2;
+    return 64 * h + 4 * st * (s / per) + 2 * (s % per) + (e >> 2) + st * (e & 3);
+}
+
+// ------------------------------------------------------------------ codes to fp16 rows
+
+// The fp16 centroids' high and low bytes, four entries to a register.
+template <int BITS>
+struct Lut {
+    static constexpr int N = BITS == 4 ? 4 : 2;
+    uint32_t hi[N], lo[N];
+    __device__ __forceinline__ void load(const float* centers) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            hi[i] = lo[i] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (4 * i + e < (1 << BITS)) {
+                    const uint32_t x = tq::f32_to_f16(centers[4 * i + e]);
+                    hi[i] |= (x >> 8) << (8 * e);
+                    lo[i] |= (x & 0xFFu) << (8 * e);
+                }
+        }
+    }
+    // four codes, one to a byte: their centroids (0, 1) and (2, 3)
+    __device__ __forceinline__ void four(uint32_t code, uint32_t& a, uint32_t& b) const {
+        uint32_t h, l;
+        if constexpr (BITS < 4) {
+            h = perm(hi[1], hi[0], code), l = perm(lo[1], lo[0], code);
+        } else {
+            const uint32_t sel = code & 0x07070707u, up = perm(0u, 0x0000FF00u, (code >> 3) & 0x01010101u);
+            h = (perm(hi[3], hi[2], sel) & up) | (perm(hi[1], hi[0], sel) & ~up);
+            l = (perm(lo[3], lo[2], sel) & up) | (perm(lo[1], lo[0], sel) & ~up);
+        }
+        a = perm(h, l, 0x05010400u), b = perm(h, l, 0x07030602u);
+    }
+};
+
+// Four chunks of 8 elements from 32 codes (BITS words), in the order of dim_of.
+template <int BITS>
+__device__ __forceinline__ void expand32(const uint32_t* w, const Lut<BITS>& lut, uint4* out) {
+    uint32_t q[8];
+    if constexpr (BITS == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) q[2 * j] = w[j] & 0x0F0F0F0Fu, q[2 * j + 1] = (w[j] >> 4) & 0x0F0F0F0Fu;
+    } else if constexpr (BITS == 3) {
+        const uint32_t b0 = perm(w[2], perm(w[1], w[0], 0x0C060300u), 0x05020100u);
+        const uint32_t b1 = perm(w[2], perm(w[1], w[0], 0x0C070401u), 0x06020100u);
+        const uint32_t b2 = perm(w[2], perm(w[1], w[0], 0x0C0C0502u), 0x07040100u);
+        q[0] = b0 & 0x07070707u;
+        q[1] = (b0 >> 3) & 0x07070707u;
+        q[2] = ((b0 >> 6) & 0x03030303u) | ((b1 << 2) & 0x04040404u);
+        q[3] = (b1 >> 1) & 0x07070707u;
+        q[4] = (b1 >> 4) & 0x07070707u;
+        q[5] = ((b1 >> 7) & 0x01010101u) | ((b2 << 1) & 0x06060606u);
+        q[6] = (b2 >> 2) & 0x07070707u;
+        q[7] = (b2 >> 5) & 0x07070707u;
+    } else if constexpr (BITS == 2) {
+#pragma unroll
+        for (int p = 0; p < 8; ++p) q[p] = (w[p >> 2] >> (2 * (p & 3))) & 0x03030303u;
+    } else {
+#pragma unroll
+        for (int p = 0; p < 8; ++p) q[p] = (w[0] >> p) & 0x01010101u;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        lut.four(q[2 * j], out[j].x, out[j].y);
+        lut.four(q[2 * j + 1], out[j].z, out[j].w);
+    }
+}
+
+// Four chunks of +-1 from 32 sign bits: bits i and i + 16 in one register.
+__device__ __forceinline__ void expand_signs(uint32_t w, uint4* out) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t x[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = ((w << (15 - 4 * j - k)) & 0x80008000u) ^ 0xBC00BC00u;
+        out[j] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+}
+
+__device__ __forceinline__ int swizzle(int token) { return ((token & 3) << 2) | ((token >> 2) & 3); }
+
+__device__ __forceinline__ s16x4 read_tr(const uint8_t* l) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)l);
+}
+// Byte offsets in a tile: the 16 bytes of a key row that a lane takes in step ks (plus 32 rows per block of tokens), and
+// the 8 bytes of dims 32 d + ... of the four tokens e of 16 (plus 16 rows per step).
+__device__ __forceinline__ int key_offset(int ks, int lane) {
+    return (lane & 31) * 256 + (((2 * ks + (lane >> 5)) ^ swizzle(lane & 31)) << 4);
+}
+__device__ __forceinline__ int value_offset(int d, int e, int lane) {
+    const int tok = 8 * e + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    return tok * 256 + ((chunk ^ swizzle(tok)) << 4) + 8 * (lane & 1);
+}
+
+// ------------------------------------------------------------------ queries
+
+struct PrepArgs {
+    const void* q;
+    int q_type;  // 0 bf16, 1 fp32, 2 fp16
+    int q_heads, kv_heads, T, rows;
+    int64_t q_sb, q_sh, q_st;
+    const float *rk, *s;
+    int key_bits;
+    float c2;       // scale log2(e)
+    uint4* frags;   // [kv head][row block][2][8 steps][64 lanes]
+    float* row_c;   // [kv head][row block][32] c2 over the row's power of two
+};
+
+__device__ __forceinline__ float query_element(const PrepArgs& a, int64_t i) {
+    if (a.q_type == 0) return tq::bf16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
+    if (a.q_type == 1) return static_cast<const float*>(a.q)[i];
+    return tq::f16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
+}
+
+// One workgroup: 32 query rows of a KV head against R_k and (grid z = 2) S.  fp32 fma chains.
+__global__ __launch_bounds__(256) void prep_kernel(PrepArgs a) {
+    __shared__ float s_q[32][D + 1];
+    __shared__ float s_o[2][32][D + 1];
+    __shared__ float s_top[32];
+    const int blk = blockIdx.x, kv = blockIdx.y;
+    const int b = kv / a.kv_heads, kvh = kv - b * a.kv_heads, group = a.q_heads / a.kv_heads;
+    for (int i = threadIdx.x; i < 32 * D; i += 256) {
+        const int r = i / D, d = i - r * D, row = 32 * blk + r;
+        float x = 0.0f;
+        if (row < a.rows) {
+            const int g = row / a.T, t = row - g * a.T;
+            x = query_element(a, b * a.q_sb + (int64_t)(kvh * group + g) * a.q_sh + (int64_t)t * a.q_st + d);
+        }
+        s_q[r][d] = x;
+    }
+    __syncthreads();
+    const int mats = a.s ? 2 : 1;
+    // thread: one row of the matrix (dim j), 16 query rows
+    const int j = threadIdx.x & 127, half = threadIdx.x >> 7;
+    for (int m = 0; m < mats; ++m) {
+        const float* mat = (m ? a.s : a.rk) + j * D;
+        float acc[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
+        for (int d = 0; d < D; d += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(mat + d);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float* q = &s_q[16 * half + i][d];
+                acc[i] = __builtin_fmaf(q[0], x.x, acc[i]);
+                acc[i] = __builtin_fmaf(q[1], x.y, acc[i]);
+                acc[i] = __builtin_fmaf(q[2], x.z, acc[i]);
+                acc[i] = __builtin_fmaf(q[3], x.w, acc[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s_o[m][16 * half + i][j] = acc[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        float top = 0.0f;
+        for (int m = 0; m < mats; ++m)
+            for (int d = 0; d < D; ++d) top = fmaxf(top, fabsf(s_o[m][threadIdx.x][d]));
+        // largest element in [2^9, 2^10); rows of zeros, and with an infinity, as they are
+        int e = 0;
+        if (top > 0.0f && top < __builtin_inff()) e = 9 - (int)((__float_as_uint(top) >> 23) & 0xFF) + 127;
+        e = std::min(e, 126);
+        s_top[threadIdx.x] = __uint_as_float((uint32_t)(127 + e) << 23);
+        a.row_c[((int64_t)kv * gridDim.x + blk) * 32 + threadIdx.x] = a.c2 * __uint_as_float((uint32_t)(127 - e) << 23);
+    }
+    __syncthreads();
+    uint4* const frags = a.frags + ((int64_t)kv * gridDim.x + blk) * 2 * 8 * 64;
+    for (int i = threadIdx.x; i < mats * 8 * 64; i += 256) {
+        const int m = i >> 9, s = (i >> 6) & 7, lane = i & 63, r = lane & 31, h = lane >> 5;
+        uint32_t x[4];
+        for (int k = 0; k < 4; ++k) {
+            const int bits = m ? 0 : a.key_bits;
+            x[k] = pack_f16(s_o[m][r][dim_of(bits, 2 * s + h, 2 * k)] * s_top[r],
+                            s_o[m][r][dim_of(bits, 2 * s + h, 2 * k + 1)] * s_top[r]);
+        }
+        frags[i] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+}
+
+// ------------------------------------------------------------------ attention
+
+struct TreeArgs {
+    int kv_heads, T, rows, row_blocks;
+    const int32_t* parents;
+    int64_t parents_sb;
+    const int32_t *starts, *lens;
+    int64_t n_tokens, cap;
+    const uint8_t *k_codes, *k_signs, *v_codes;
+    const uint16_t *k_norms, *k_rnorms, *v_norms;
+    const float *key_centers, *value_centers;
+    const uint4* frags;
+    const float* row_c;
+    int n_split;
+    float* part_o;   // [split][kv head][row][D]
+    float4* part_ms; // [split][kv head][row] (reference of the weights in log2, sum of weights, scale of the output sums)
+};
+
+// Bit j of a node's mask: node j is the node itself or one of its ancestors.  A parent that is not an earlier
+// node is none.  Called by one whole wave, lane = node.
+__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int T, int lane) {
+    int p = lane < T ? parents[lane] : -1;
+    if (p < 0 || p >= lane) p = -1;
+    uint64_t mask = 1ull << lane;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {  // paths of 2^k steps
+        const uint64_t up = __shfl(mask, p < 0 ? 0 : p);
+        const int next = __shfl(p, p < 0 ? 0 : p);
+        if (p >= 0) mask |= up, p = next;
+    }
+    return mask;
+}
+
+// Of one value to each token: those of the tokens 32 t + 8 j + 4 h + (0..3).
+__device__ __forceinline__ f32x4 norms4(const float* n, int t, int j, int h) {
+    return *reinterpret_cast<const f32x4*>(n + 32 * t + 8 * j + 4 * h);
+}
+
+// The tokens of a tile that a node attends to, as bits: those of the history (the first `to_end` of the tile, none
+// if it is negative), the nodes behind it that `sees` names, and none from `left` on.
+__device__ __forceinline__ uint64_t seen_of_tile(uint64_t sees, int to_end, int left) {
+    const uint64_t nodes = to_end >= TK || to_end <= -TK ? 0ull : to_end >= 0 ? sees << to_end : sees >> -to_end;
+    const uint64_t history = to_end >= TK ? ~0ull : to_end <= 0 ? 0ull : (1ull << to_end) - 1;
+    return (nodes | history) & (left >= TK ? ~0ull : (1ull << left) - 1);
+}
+
+template <int KB, int VB, bool QJL>
+__global__ __launch_bounds__(256, 1) void tree_kernel(TreeArgs a) {
+    __shared__ uint4 s_k[TK * 16];
+    __shared__ uint4 s_s[QJL ? TK * 16 : 1];
+    __shared__ uint4 s_v[TK * 16];
+    __shared__ __align__(16) float s_kn[TK], s_rn[TK], s_vn[TK];
+    __shared__ float s_vtop;
+    __shared__ uint64_t s_anc[64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
+    const int kv = blockIdx.x / a.n_split, split = blockIdx.x - kv * a.n_split;
+    const int b = kv / a.kv_heads;
+    const int blk = blockIdx.y * 4 + wave;  // this wave's 32 rows
+    const bool busy = blk < a.row_blocks;
+
+    // history [lo, end) and the nodes behind it, cut into tiles for the splits
+    const int nodes = a.parents ? a.T : 0;
+    int64_t end = a.lens ? a.lens[b] : a.n_tokens - nodes;
+    end = std::min<int64_t>(std::max<int64_t>(end, 0), a.n_tokens);
+    int64_t lo = a.starts ? a.starts[b] : 0;
+    lo = std::min<int64_t>(std::max<int64_t>(lo, 0), end);
+    const int64_t stop = std::min<int64_t>(end + nodes, a.n_tokens);
+    const int64_t tiles = (stop - lo + TK - 1) / TK, per = (tiles + a.n_split - 1) / a.n_split;
+    const int64_t t_begin = lo + std::min<int64_t>(split * per, tiles) * TK;
+    const int64_t t_end = std::min<int64_t>(lo + (split + 1) * per * TK, stop);
+
+    if (nodes && wave == 0) s_anc[lane] = ancestors(a.parents + b * a.parents_sb, a.T, lane);
+    Lut<KB> klut;
+    Lut<VB> vlut;
+    klut.load(a.key_centers);
+    vlut.load(a.value_centers);
+    Frag q[QJL ? 2 : 1][8];
+    float c = 0.0f;
+    if (busy) {
+        const uint4* f = a.frags + ((int64_t)kv * a.row_blocks + blk) * 2 * 8 * 64;
+#pragma unroll
+        for (int m = 0; m < (QJL ? 2 : 1); ++m)
+#pragma unroll
+            for (int s = 0; s < 8; ++s) q[m][s].q = f[(m * 8 + s) * 64 + lane];
+        c = a.row_c[((int64_t)kv * a.row_blocks + blk) * 32 + r];
+    }
+    __syncthreads();
+    uint64_t sees = nodes ? s_anc[(32 * blk + r) % a.T] : 0ull;
+
+    f32x16 o[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] = zero16();
+    float top = -__builtin_inff(), sum = 0.0f;
+    // the output sums are in units of a power of two, 2^-15 of one above the largest |v| so far: weights times norm then
+    // reach up to 2^15, and fp16 keeps its 11 bits for those 2^29 times smaller
+    float unit = 0x1p-39f;
+    const uint8_t *const k8 = reinterpret_cast<const uint8_t*>(s_k), *const s8 = reinterpret_cast<const uint8_t*>(s_s),
+                  *const v8 = reinterpret_cast<const uint8_t*>(s_v);
+    const int64_t first = (int64_t)kv * a.cap;
+
+    for (int64_t t0 = t_begin; t0 < t_end; t0 += TK) {
+        __syncthreads();
+        const int left = (int)std::min<int64_t>(t_end - t0, TK);
+        {  // four threads to a token, 32 codes of each kind
+            const int tok = threadIdx.x >> 2, p = threadIdx.x & 3, u = p & 1, ph = p >> 1;
+            const int64_t slot = first + t0 + std::min(tok, left - 1);
+            uint32_t wk[KB], wv[VB], ws = 0u;
+            uint4 x[4];
+            auto put = [&](uint4* dst) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dst[tok * 16 + ((8 * u + 2 * j + ph) ^ swizzle(tok))] = x[j];
+                __builtin_amdgcn_sched_barrier(0);  // one kind at a time: all three do not fit the registers
+            };
+            __builtin_memcpy(wk, __builtin_assume_aligned(a.k_codes + slot * (16 * KB) + 4 * KB * p, 4), 4 * KB);
+            __builtin_memcpy(wv, __builtin_assume_aligned(a.v_codes + slot * (16 * VB) + 4 * VB * p, 4), 4 * VB);
+            if constexpr (QJL) __builtin_memcpy(&ws, __builtin_assume_aligned(a.k_signs + slot * 16 + 4 * p, 4), 4);
+            expand32<KB>(wk, klut, x);
+            put(s_k);
+            expand32<VB>(wv, vlut, x);
+            put(s_v);
+            if constexpr (QJL) {
+                expand_signs(ws, x);
+                put(s_s);
+            }
+        }
+        if (wave == 0) {
+            const int64_t slot = first + t0 + std::min(lane, left - 1);
+            const float vn = lane < left ? tq::f16_to_f32(a.v_norms[slot]) : 0.0f;
+            s_kn[lane] = tq::f16_to_f32(a.k_norms[slot]);
+            if constexpr (QJL) s_rn[lane] = tq::f16_to_f32(a.k_rnorms[slot]) * QJL_SCALE;
+            s_vn[lane] = vn;
+            float m = fabsf(vn) < __builtin_inff() ? fabsf(vn) : 0.0f;
+#pragma unroll
+            for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
+            if (lane == 0) s_vtop = m;
+        }
+        __syncthreads();
+        if (!busy) continue;
+
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x16 x = zero16();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                Frag kf;
+                kf.q = *reinterpret_cast<const uint4*>(k8 + key_offset(ks, lane) + 32 * 256 * t);
+                x = mfma_f16(kf, q[0][ks], x);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // the reads of all sixteen steps at once do not fit the registers
+            if constexpr (QJL) {
+                f32x16 y = zero16();
+#pragma unroll
+                for (int ks = 0; ks < 8; ++ks) {
+                    Frag kf;
+                    kf.q = *reinterpret_cast<const uint4*>(s8 + key_offset(ks, lane) + 32 * 256 * t);
+                    y = mfma_f16(kf, q[1][ks], y);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 kn = norms4(s_kn, t, j, h), rn = norms4(s_rn, t, j, h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[t][4 * j + e] = __builtin_fmaf(y[4 * j + e], rn[e], x[4 * j + e] * kn[e]);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 kn = norms4(s_kn, t, j, h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[t][4 * j + e] = x[4 * j + e] * kn[e];
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (t0 + TK > end || left < TK) {  // uniform: drafted tokens, or none
+            const uint64_t allowed = seen_of_tile(sees, (int)std::max<int64_t>(std::min<int64_t>(end - t0, TK), -TK), left);
+            const uint32_t word[2] = {(uint32_t)allowed >> (4 * h), (uint32_t)(allowed >> 32) >> (4 * h)};
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(word[t] & (1u << (8 * (i >> 2) + (i & 3))))) s[t][i] = -__builtin_inff();
+        }
+        float mx = top;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float safe = mx == -__builtin_inff() ? 0.0f : mx;
+        float new_unit = unit;
+        if (s_vtop > 0x1p15f * unit)
+            new_unit = 0x1p-15f * __uint_as_float((__float_as_uint(s_vtop) & 0x7F800000u) + 0x00800000u);
+        if (__any(mx > top) || new_unit != unit) {
+            const float corr = exp2_(__builtin_fmaf(top, c, -safe * c));
+            sum *= corr;
+            const float oc = corr * (unit / new_unit);
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= oc;
+            unit = new_unit;
+        }
+        top = mx;
+        const float base = safe * c, inv_unit = 1.0f / unit;
+        Frag pf[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 vn = norms4(s_vn, t, j, h);
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = exp2_(__builtin_fmaf(s[t][4 * j + e], c, -base));
+                    sum += p;
+                    const float x = p * (vn[e] * inv_unit);
+                    w[e] = p == 0.0f ? 0.0f : x;  // a left-out token's norm may be anything
+                }
+                pf[2 * t + (j >> 1)].u[2 * (j & 1)] = pack_f16(w[0], w[1]);
+                pf[2 * t + (j >> 1)].u[2 * (j & 1) + 1] = pack_f16(w[2], w[3]);
+            }
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                Frag vf;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) vf.t[e] = read_tr(v8 + value_offset(d, e, lane) + 16 * 256 * ks);
+                o[d] = mfma_f16(vf, pf[ks], o[d]);
+            }
+    }
+    const int row = 32 * blk + r;
+    sum += __shfl_xor(sum, 32);
+    if (!busy || row >= a.rows) return;
+    const int64_t at = ((int64_t)split * (gridDim.x / a.n_split) + kv) * a.rows + row;
+    if (h == 0) a.part_ms[at] = make_float4(top == -__builtin_inff() ? top : top * c, sum, unit, 0.0f);
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<float4*>(a.part_o + at * D + 32 * d + 8 * j + 4 * h) =
+                make_float4(o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]);
+}
+
+// ------------------------------------------------------------------ merge
+
+struct MergeArgs {
+    int q_heads, kv_heads, T, rows, n_split, value_bits;
+    int64_t all_rows;  // of all KV heads
+    const float* part_o;
+    const float4* part_ms;
+    const float* rv;
+    float* out_f32;
+    uint16_t* out_bf16;
+    float* lse;
+};
+
+// Eight rows per workgroup: their splits weighed and added, then rotated back.
+__global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
+    __shared__ float s_w[8][MAX_SPLIT];
+    __shared__ float s_den[8];
+    __shared__ float s_o[8][D];
+    const int64_t row0 = (int64_t)blockIdx.x * 8;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int k = wave; k < 8; k += 4) {
+        const int64_t row = row0 + k;
+        float4 ms = make_float4(-__builtin_inff(), 0.0f, 0.0f, 0.0f);
+        if (row < a.all_rows && lane < a.n_split) ms = a.part_ms[lane * a.all_rows + row];
+        float top = ms.x;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
+        const float w = exp2_(ms.x - (top == -__builtin_inff() ? 0.0f : top));
+        float den = w * ms.y;
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) den += __shfl_xor(den, x);
+        s_w[k][lane] = w == 0.0f ? 0.0f : w * ms.z;
+        if (lane == 0) {
+            s_den[k] = den;
+            if (a.lse && row < a.all_rows) {
+                const int64_t kv = row / a.rows;
+                const int in = (int)(row - kv * a.rows), g = in / a.T, t = in - g * a.T;
+                const int64_t b = kv / a.kv_heads, hq = (kv % a.kv_heads) * (a.q_heads / a.kv_heads) + g;
+                a.lse[(b * a.q_heads + hq) * a.T + t] =
+                    den == 0.0f ? -__builtin_inff() : top * 0.6931471805599453f + __builtin_logf(den);
+            }
+        }
+    }
+    __syncthreads();
+    const int pos = threadIdx.x & 127;
+    for (int k = threadIdx.x >> 7; k < 8; k += 2) {
+        const int64_t row = row0 + k;
+        float o = 0.0f;
+        if (row < a.all_rows)
+            for (int i = 0; i < a.n_split; ++i)
+                if (s_w[k][i] != 0.0f) o = __builtin_fmaf(s_w[k][i], a.part_o[(i * a.all_rows + row) * D + pos], o);
+        s_o[k][dim_of(a.value_bits, pos >> 3, pos & 7)] = s_den[k] == 0.0f ? 0.0f : o / s_den[k];
+    }
+    __syncthreads();
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int half = threadIdx.x >> 7;
+    for (int d = 0; d < D; ++d) {
+        const float x = a.rv[d * D + pos];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = __builtin_fmaf(s_o[4 * half + k][d], x, acc[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t row = row0 + 4 * half + k;
+        if (row >= a.all_rows) continue;
+        const int64_t kv = row / a.rows;
+        const int in = (int)(row - kv * a.rows), g = in / a.T, t = in - g * a.T;
+        const int64_t b = kv / a.kv_heads, hq = (kv % a.kv_heads) * (a.q_heads / a.kv_heads) + g;
+        const int64_t at = ((b * a.q_heads + hq) * a.T + t) * D + pos;
+        if (a.out_f32) a.out_f32[at] = acc[k];
+        if (a.out_bf16) a.out_bf16[at] = (uint16_t)tq::f32_to_bf16(acc[k]);
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+struct Plan {
+    int rows, row_blocks, n_split;
+    int64_t heads;
+    size_t frag_bytes, row_c_bytes, ms_bytes, o_bytes;
+    size_t total() const { return frag_bytes + row_c_bytes + ms_bytes + o_bytes; }
+};
+
+// Splits: two workgroups for each CU, as long as none is left without a tile.
+bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Plan& p) {
+    p.heads = (int64_t)batch * kv_heads;
+    p.rows = q_heads / kv_heads * T;
+    p.row_blocks = (p.rows + 31) / 32;
+    const int64_t wgs = p.heads * ((p.row_blocks + 3) / 4), tiles = std::max<int64_t>(1, (n_tokens + TK - 1) / TK);
+    int64_t n = std::max<int64_t>(1, std::min<int64_t>({(512 + wgs - 1) / wgs, tiles, MAX_SPLIT}));
+    const int64_t per = (tiles + n - 1) / n;
+    p.n_split = (int)((tiles + per - 1) / per);
+    const int64_t all = p.heads * p.rows;
+    p.frag_bytes = (size_t)(p.heads * p.row_blocks) * 2 * 8 * 64 * 16;
+    p.row_c_bytes = (size_t)(p.heads * p.row_blocks) * 32 * 4;
+    p.ms_bytes = (size_t)all * p.n_split * 16;
+    p.o_bytes = (size_t)all * p.n_split * D * 4;
+    return p.heads * p.n_split < ((int64_t)1 << 24) && all < ((int64_t)1 << 26) && p.heads <= 65535;
+}
+
+template <int KB, int VB, bool QJL>
+void launch_tree(const TreeArgs& a, dim3 grid, hipStream_t s) {
+    hipLaunchKernelGGL((tree_kernel<KB, VB, QJL>), grid, dim3(256), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" size_t tq_tree_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int nodes, int dim,
+                                                    int64_t n_tokens) {
+    Plan p;
+    if (batch < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || nodes < 1 || nodes > TQ_MAX_NODES || dim != D ||
+        n_tokens < 0 || !make_plan(batch, q_heads, kv_heads, nodes, n_tokens, p))
+        return 0;
+    return p.total();
+}
+
+extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_heads, int kv_heads, int nodes, int dim,
+                                 int64_t q_sb, int64_t q_sh, int64_t q_st, const int32_t* parents, int64_t parents_sb,
+                                 const int32_t* seq_starts, const int32_t* seq_lens, int64_t n_tokens, int64_t cap,
+                                 const uint8_t* k_codes, const uint16_t* k_norms, const uint8_t* k_signs,
+                                 const uint16_t* k_rnorms, const uint8_t* v_codes, const uint16_t* v_norms, int key_bits,
+                                 int value_bits, int has_qjl, const float* key_rotation, const float* key_centers,
+                                 const float* qjl, const float* value_rotation, const float* value_centers, float scale,
+                                 float* out_f32, uint16_t* out_bf16, float* lse_out, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+    if (!q || q_type < 0 || q_type > 2 || batch < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || nodes < 1 ||
+        n_tokens < 0 || n_tokens > cap || cap < 1 || !k_codes || !k_norms || !v_codes || !v_norms || !key_rotation ||
+        !key_centers || !value_rotation || !value_centers || (has_qjl && (!k_signs || !k_rnorms || !qjl)) ||
+        (!out_f32 && !out_bf16) || !(scale > 0.0f) || scale == __builtin_inff())
+        return TQ_ERR_INVALID_ARGUMENT;
+    if (dim != D || nodes > TQ_MAX_NODES || value_bits < 1 || value_bits > 4 || key_bits < 1 ||
+        key_bits != value_bits - (has_qjl ? 1 : 0))
+        return TQ_ERR_UNSUPPORTED;
+    if (!aligned16(key_rotation) || !aligned16(k_codes) || !aligned16(v_codes) || (has_qjl && (!aligned16(k_signs) || !aligned16(qjl))))
+        return TQ_ERR_UNSUPPORTED;
+    Plan p;
+    if (!make_plan(batch, q_heads, kv_heads, nodes, n_tokens, p)) return TQ_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < p.total() || !aligned16(workspace)) return TQ_ERR_WORKSPACE;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    uint4* frags = reinterpret_cast<uint4*>(ws);
+    float* part_o = reinterpret_cast<float*>(ws + p.frag_bytes);
+    float4* part_ms = reinterpret_cast<float4*>(ws + p.frag_bytes + p.o_bytes);
+    float* row_c = reinterpret_cast<float*>(ws + p.frag_bytes + p.o_bytes + p.ms_bytes);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const PrepArgs prep{q, q_type, q_heads, kv_heads, nodes, p.rows, q_sb, q_sh, q_st, key_rotation,
+                        has_qjl ? qjl : nullptr, key_bits, scale * LOG2E, frags, row_c};
+    hipLaunchKernelGGL(prep_kernel, dim3((unsigned)p.row_blocks, (unsigned)p.heads), dim3(256), 0, s, prep);
+    TQ_CHECK_LAUNCH();
+    const TreeArgs a{kv_heads, nodes, p.rows, p.row_blocks, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
+                     k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, frags, row_c,
+                     p.n_split, part_o, part_ms};
+    const dim3 grid((unsigned)(p.heads * p.n_split), (unsigned)((p.row_blocks + 3) / 4));
+    if (has_qjl) {
+        if (value_bits == 4) launch_tree<3, 4, true>(a, grid, s);
+        else if (value_bits == 3) launch_tree<2, 3, true>(a, grid, s);
+        else launch_tree<1, 2, true>(a, grid, s);
+    } else {
+        if (value_bits == 4) launch_tree<4, 4, false>(a, grid, s);
+        else if (value_bits == 3) launch_tree<3, 3, false>(a, grid, s);
+        else if (value_bits == 2) launch_tree<2, 2, false>(a, grid, s);
+        else launch_tree<1, 1, false>(a, grid, s);
+    }
+    TQ_CHECK_LAUNCH();
+    const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, value_bits, p.heads * p.rows, part_o, part_ms,
+                      value_rotation, out_f32, out_bf16, lse_out};
+    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((p.heads * p.rows + 7) / 8)), dim3(256), 0, s, m);
+    TQ_CHECK_LAUNCH();
+    return TQ_OK;
+}

@@ -4,7 +4,9 @@ from turboquant.runtime.attention import (
     chunked_turboquant_attention,
     fused_attention,
     prompt_attention,
+    tree_attention,
     triton_available,
 )
 
-__all__ = ["fused_attention", "triton_available", "chunked_turboquant_attention", "prompt_attention"]
+__all__ = ["fused_attention", "triton_available", "chunked_turboquant_attention", "prompt_attention",
+           "tree_attention"]

@@ -350,6 +350,81 @@ def chunked_turboquant_attention(query_states: torch.Tensor, packed_layer: "Pack
     return (o / s.clamp(min=1e-8)).to(query_states.dtype)
 
 
+def _tree_mask(parents: torch.Tensor, total: int, starts: torch.Tensor | None, ends: torch.Tensor) -> torch.Tensor:
+    """bool [B, 1, T, total]: the slots each node of a tree attends to; ``parents`` [B, T], ``ends`` [B] each
+    row's history end, where its nodes begin."""
+    T = parents.shape[1]
+    i = torch.arange(T, device=parents.device)
+    p = torch.where((parents >= 0) & (parents < i), parents, -1).long()
+    sees = torch.eye(T, dtype=torch.bool, device=p.device).expand(p.shape[0], T, T).clone()
+    for _ in range(max(1, (T - 1).bit_length())):  # paths of 1, 2, 4, ... steps
+        at, live = p.clamp(min=0), p >= 0
+        sees |= live[..., None] & sees.gather(1, at[..., None].expand_as(sees))
+        p = torch.where(live, p.gather(1, at), -1)
+    slot = torch.arange(total, device=p.device)[None, :]
+    node = slot - ends[:, None]
+    mine = (node >= 0) & (node < T)
+    seen = sees.gather(2, node.clamp(0, T - 1)[:, None].expand(-1, T, -1)) & mine[:, None]
+    history = node < 0
+    if starts is not None:
+        history = history & (slot >= starts[:, None])
+    return (seen | history[:, None])[:, None]
+
+
+def tree_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", parents: torch.Tensor,
+                   n_kv_groups: int = 1, seq_starts: torch.Tensor | None = None,
+                   seq_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a tree of drafted tokens, [B, Hq, T, D] over a packed layer -> [B, Hq, T, D].
+
+    The T drafted tokens are the layer's last ones (``update`` has stored them, packed or dense as the layer keeps
+    generated tokens).  ``parents`` int [T] or [B, T]: the node each follows, an earlier one, or -1; a
+    node attends to the history, to its ancestors and to itself (a chain -1, 0, 1, ... is causal).
+    ``seq_starts`` / ``seq_lens`` int [B]: row b's history is the tokens [start, len) and its nodes the T
+    tokens from len on (packed nodes only).  After the drafts are checked, ``keep_tokens`` of the layer closes
+    up the accepted path.
+
+    One-group layers with up to 64 nodes run on the packed codes (``kernels.tree_attention``), tokens kept
+    dense merged by log-sum-exp; others take ``chunked_turboquant_attention`` with the tree as its mask.
+    """
+    B, Hq, T, D = query_states.shape
+    if parents.dim() not in (1, 2) or tuple(parents.shape) not in ((T,), (B, T)):
+        raise ValueError(f"parents must be [{T}] or [{B}, {T}], got {tuple(parents.shape)}")
+    K._no_gradient("tree_attention", query_states)
+    n_packed, n_dense = packed_layer.packed_seq_length(), packed_layer._dense_len
+    total = n_packed + n_dense
+    if T > (n_dense if n_dense else n_packed):
+        raise ValueError(f"{T} drafted tokens, but the layer holds {n_dense or n_packed} of their kind")
+    if n_dense and seq_lens is not None:
+        raise ValueError("seq_lens needs the drafted tokens packed (quantize_decode=True)")
+    dev = query_states.device
+    seq_starts = K._int32_on(seq_starts, dev, "seq_starts", (B,))
+    seq_lens = K._int32_on(seq_lens, dev, "seq_lens", (B,))
+    store = packed_layer._store
+    fused = (store is not None and not packed_layer._outlier_enabled and T <= K.MAX_NODES
+             and query_states.dtype in K._QUERY_TYPES)
+    if fused:
+        c = packed_layer.codecs
+        kw = dict(k_codes=store.kc, k_norms=store.kn, v_codes=store.vc, v_norms=store.vn, n_tokens=n_packed, key=c.key,
+                  value=c.value, k_signs=store.ks, k_rnorms=store.kr, qjl=c.qjl, seq_starts=seq_starts)
+        if n_dense == 0:
+            return K.tree_attention(query_states, parents, seq_lens=seq_lens, **kw)
+    own = parents.to(dev)
+    own = own[None].expand(B, -1) if own.dim() == 1 else own
+    ends = torch.full((B,), total - T, dtype=torch.int32, device=dev) if seq_lens is None else seq_lens
+    if fused:
+        dk, dv = packed_layer._dense_buf
+        if _native_rows(query_states, dk, dv) and K.DenseAttention.takes(query_states, dk.shape[1]):
+            _, o_packed, lse = K.tree_attention(query_states, None, want_f32=True, want_lse=True, **kw)
+            starts = None if seq_starts is None else seq_starts - n_packed
+            mask = _tree_mask(own, n_dense, starts, ends - n_packed)
+            q = query_states if query_states.dtype == torch.bfloat16 else query_states.float()
+            n = K.DenseAttention.split_count(q, dk.shape[1], n_dense, K.DENSE_SPLITS)
+            return K.DenseAttention(q, dk.shape[1], n).add(dk, dv, n_dense, 0, n, 1.0 / math.sqrt(D), mask=mask,
+                                                           out=query_states.dtype, prev=o_packed, prev_lse=lse)
+    return chunked_turboquant_attention(query_states, packed_layer, n_kv_groups=n_kv_groups,
+                                        attention_mask=_tree_mask(own, total, seq_starts, ends))
+
+
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *,
                      cu_seqlens: torch.Tensor | None = None, seq_starts: torch.Tensor | None = None,
                      seq_ends: torch.Tensor | None = None, scale: float | None = None,

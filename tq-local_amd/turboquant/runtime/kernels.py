@@ -607,6 +607,83 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
     return (out, lse) if want_lse else out
 
 
+MAX_NODES = 64  # drafted tokens of one sequence the tree kernel takes (TQ_MAX_NODES)
+_QUERY_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+
+
+def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: torch.Tensor, k_norms: torch.Tensor,
+                   v_codes: torch.Tensor, v_norms: torch.Tensor, n_tokens: int, key: CodecParams, value: CodecParams,
+                   k_signs: torch.Tensor | None = None, k_rnorms: torch.Tensor | None = None,
+                   qjl: torch.Tensor | None = None, seq_starts: torch.Tensor | None = None,
+                   seq_lens: torch.Tensor | None = None, scale: float | None = None, want_f32: bool = False,
+                   want_lse: bool = False):
+    """Attention of T <= 64 drafted tokens per sequence over a packed cache (tq_tree_attention).
+
+    q [B, Hq, T, D] (bf16, fp16 or fp32).  ``parents`` int [T] or [B, T]: the node each node follows, an
+    earlier one, or -1 for those that follow the history itself; node i attends to the history, to its
+    ancestors and to itself.  Packed buffers are [B, Hkv, cap, ...] with ``n_tokens`` valid slots, the nodes'
+    the last T of them.  ``seq_starts`` / ``seq_lens`` int [B]: row b's history is the slots [start, len) and
+    its nodes the T slots from len on.  Without ``parents`` (None) there are no nodes in the cache and
+    every row of q attends to the history alone, up to n_tokens.  Returns [B, Hq, T, D] in q's dtype, then fp32
+    with ``want_f32``, then the fp32 log-sum-exp [B, Hq, T] of the scaled logits with ``want_lse``.
+    """
+    if q.dim() != 4 or q.shape[-1] != HEAD_DIM:
+        raise ValueError(f"expected q [B, Hq, T, {HEAD_DIM}], got {tuple(q.shape)}")
+    B, Hq, T, D = q.shape
+    if q.dtype not in _QUERY_TYPES:
+        raise ValueError(f"q must be bf16, fp16 or fp32, got {q.dtype}")
+    if not 1 <= T <= MAX_NODES:
+        raise ValueError(f"{T} drafted tokens: 1 to {MAX_NODES} are taken")
+    if k_codes.dim() != 4 or k_codes.shape[0] != B or k_codes.shape[1] == 0 or Hq % k_codes.shape[1]:
+        raise ValueError(f"k_codes {tuple(k_codes.shape)} do not match q {tuple(q.shape)}")
+    Hkv, cap = int(k_codes.shape[1]), int(k_codes.shape[2])
+    has_qjl = k_signs is not None
+    if (k_rnorms is not None) != has_qjl or (qjl is not None) != has_qjl:
+        raise ValueError("Q_prod keys need k_signs, k_rnorms and qjl")
+    _no_gradient("tree_attention", q)
+    _require_gpu(q, k_codes, k_norms, v_codes, v_norms, k_signs, k_rnorms)
+    dev = q.device
+    for name, t, row in (("k_codes", k_codes, row_bytes(D, key.bits)), ("v_codes", v_codes, row_bytes(D, value.bits)),
+                         ("k_signs", k_signs, D // 8), ("k_norms", k_norms, 0), ("v_norms", v_norms, 0),
+                         ("k_rnorms", k_rnorms, 0)):
+        if t is None:
+            continue
+        shape, dtype = ((B, Hkv, cap, row), torch.uint8) if row else ((B, Hkv, cap), torch.float16)
+        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{name}: expected a contiguous {dtype} {shape} on {dev}, got {t.dtype} {tuple(t.shape)}")
+    nodes = 0 if parents is None else T
+    if not 0 <= n_tokens <= cap or n_tokens < nodes:
+        raise ValueError(f"{n_tokens} tokens, {nodes} of them drafted, of a capacity of {cap}")
+    psb = 0
+    if parents is not None:
+        if parents.dim() not in (1, 2):
+            raise ValueError("parents must be [T] or [B, T]")
+        psb = T if parents.dim() == 2 else 0
+        parents = _int32_on(parents, dev, "parents", (B, T) if psb else (T,))
+    seq_starts = _int32_on(seq_starts, dev, "seq_starts", (B,))
+    seq_lens = _int32_on(seq_lens, dev, "seq_lens", (B,))
+    bf16 = q.dtype == torch.bfloat16
+    f32 = torch.empty((B, Hq, T, D), dtype=torch.float32, device=dev) if want_f32 or not bf16 else None
+    out = torch.empty((B, Hq, T, D), dtype=torch.bfloat16, device=dev) if bf16 else None
+    lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if want_lse else None
+    if B and Hq:
+        if q.stride(-1) != 1:
+            q = q.contiguous()
+        need = _lib.load().tq_tree_attention_workspace_bytes(B, Hq, Hkv, T, D, n_tokens)
+        ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=dev)
+        s = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+        _on_device("tq_tree_attention", dev, _vp(q), _QUERY_TYPES[q.dtype], B, Hq, Hkv, T, D, *q.stride()[:3],
+                   _vp(parents), psb, _vp(seq_starts), _vp(seq_lens), int(n_tokens), cap, _vp(k_codes), _vp(k_norms),
+                   _vp(k_signs), _vp(k_rnorms), _vp(v_codes), _vp(v_norms), key.bits, value.bits, int(has_qjl),
+                   _vp(key.rotation), _vp(key.centers), _vp(qjl), _vp(value.rotation),
+                   _vp(attention_value_centers(value)), s, _vp(f32), _vp(out), _vp(lse), _vp(ws), ws.numel(),
+                   _stream(dev))
+    if out is None:
+        out = f32 if q.dtype == torch.float32 else f32.to(q.dtype)
+    outs = (out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
+    return outs if len(outs) > 1 else out
+
+
 #: most buffers of one launch, and the limits of TQ_MAX_KEEP and TQ_MAX_ROW_BYTES
 _MOVE_BUFFERS = 16
 MAX_KEEP = 256
