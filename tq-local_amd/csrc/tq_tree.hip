@@ -39,6 +39,7 @@ constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -46,11 +47,15 @@ union Frag {
     uint32_t u[4];
     uint4 q;
     s16x4 t[2];
+    bf16x8 b;
     f16x8 f;
 };
 
 __device__ __forceinline__ f32x16 mfma_f16(const Frag& a, const Frag& b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.f, b.f, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma_bf16(const Frag& a, const Frag& b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.b, b.b, c, 0, 0, 0);
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const f32x2 p = {a, b};
@@ -60,12 +65,13 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
     return __builtin_amdgcn_perm(hi, lo, sel);
 }
-__device__ __forceinline__ f32x16 zero16() {
+__device__ __forceinline__ f32x16 fill16(float x) {
     f32x16 z;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+    for (int i = 0; i < 16; ++i) z[i] = x;
     return z;
 }
+__device__ __forceinline__ f32x16 zero16() { return fill16(0.0f); }
 
 // A row of 128 dims is 16 chunks of 8 elements: chunk 2 s + h is the s-th of dims [64 h, 64 h + 64).  The dim at
 // element e of it for codes of `bits` bits (0: the QJL signs).  Codes of one and of three bits are at the same
@@ -144,13 +150,17 @@ __device__ __forceinline__ void expand32(const uint32_t* w, const Lut<BITS>& lut
     }
 }
 
-// Four chunks of +-1 from 32 sign bits: bits i and i + 16 in one register.
+// Four chunks from 32 sign bits, left where they are: bits i and i + 16 of the word (or of the word moved down by 8,
+// for i = 8..15) as the lowest mantissa bits of two fp16 numbers, 2^(p - 24) with p = i mod 8 for a set bit and 0 for a
+// clear one (the matrix cores keep subnormals).  The queries carry the 2^(7 - p), and sum_i s_i x_i = 2 sum_i bit_i x_i -
+// sum_i x_i.
 __device__ __forceinline__ void expand_signs(uint32_t w, uint4* out) {
+    const uint32_t v = w >> 8;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         uint32_t x[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = ((w << (15 - 4 * j - k)) & 0x80008000u) ^ 0xBC00BC00u;
+        for (int k = 0; k < 4; ++k) x[k] = (j < 2 ? w : v) & (0x00010001u << ((4 * j + k) & 7));
         out[j] = make_uint4(x[0], x[1], x[2], x[3]);
     }
 }
@@ -182,7 +192,7 @@ struct PrepArgs {
     int key_bits;
     float c2;       // scale log2(e)
     uint4* frags;   // [kv head][row block][2][8 steps][64 lanes]
-    float* row_c;   // [kv head][row block][32] c2 over the row's power of two
+    float* row_c;   // [kv head][row block][2][32] c2 over the row's power of two, and what a row's sign products start from
 };
 
 __device__ __forceinline__ float query_element(const PrepArgs& a, int64_t i) {
@@ -191,68 +201,124 @@ __device__ __forceinline__ float query_element(const PrepArgs& a, int64_t i) {
     return tq::f16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
 }
 
-// One workgroup: 32 query rows of a KV head against R_k and (grid z = 2) S.  fp32 fma chains.
+// fp32 pairs to bf16 terms, truncated: x - hi and (x - hi) - mid are exact, and three terms hold all 24 bits
+__device__ __forceinline__ uint32_t high_halves(float a, float b) {
+    return perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float drop_high(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
+template <int N>
+__device__ __forceinline__ void split_terms(const float* x, Frag* t) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float a = x[2 * k], b = x[2 * k + 1];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            t[n].u[k] = high_halves(a, b);
+            a = drop_high(a), b = drop_high(b);
+        }
+    }
+}
+
+// Where dim j stands in a row ordered by dim_of.
+__device__ __forceinline__ int position_of(int bits, int j) {
+    const int h = j >> 6, x = j & 63;
+    if (bits == 0) {
+        const int n = x & 15;
+        return (2 * (4 * (x >> 5) + (n >> 2)) + h) * 8 + 2 * (n & 3) + ((x >> 4) & 1);
+    }
+    const int st = bits == 4 ? 2 : bits == 2 ? 4 : 8, per = st / 2;
+    const int y = x % (4 * st), z = y % st;
+    return (2 * ((x / (4 * st)) * per + (z >> 1)) + h) * 8 + 4 * (z & 1) + y / st;
+}
+
+// One workgroup: 32 query rows of a KV head against R_k and S, wave w their rows [32 w, 32 w + 32), as products of bf16
+// terms: a bf16 query is one, any other three, the matrices three; what is left out is 2^-24 of a product.
+template <int NQ>
 __global__ __launch_bounds__(256) void prep_kernel(PrepArgs a) {
-    __shared__ float s_q[32][D + 1];
-    __shared__ float s_o[2][32][D + 1];
-    __shared__ float s_top[32];
-    const int blk = blockIdx.x, kv = blockIdx.y;
+    __shared__ uint4 s_f[2][32 * 16];  // [row][chunk], chunks xor-swizzled by the row
+    __shared__ float s_top[4][32], s_sum[4][32];
+    const int blk = blockIdx.x, kv = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int r = lane & 31, h = lane >> 5;
     const int b = kv / a.kv_heads, kvh = kv - b * a.kv_heads, group = a.q_heads / a.kv_heads;
-    for (int i = threadIdx.x; i < 32 * D; i += 256) {
-        const int r = i / D, d = i - r * D, row = 32 * blk + r;
-        float x = 0.0f;
-        if (row < a.rows) {
-            const int g = row / a.T, t = row - g * a.T;
-            x = query_element(a, b * a.q_sb + (int64_t)(kvh * group + g) * a.q_sh + (int64_t)t * a.q_st + d);
-        }
-        s_q[r][d] = x;
-    }
-    __syncthreads();
-    const int mats = a.s ? 2 : 1;
-    // thread: one row of the matrix (dim j), 16 query rows
-    const int j = threadIdx.x & 127, half = threadIdx.x >> 7;
-    for (int m = 0; m < mats; ++m) {
-        const float* mat = (m ? a.s : a.rk) + j * D;
-        float acc[16];
+    const int row = 32 * blk + r;
+    const bool live = row < a.rows;
+    const int g = live ? row / a.T : 0, t = live ? row - g * a.T : 0;
+    const int64_t at = b * a.q_sb + (int64_t)(kvh * group + g) * a.q_sh + (int64_t)t * a.q_st + 8 * h;
+    const float* const m0 = a.rk + (32 * wave + r) * D + 8 * h;
+    const float* const m1 = a.s ? a.s + (32 * wave + r) * D + 8 * h : m0;
+
+    f32x16 acc[2] = {zero16(), zero16()};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-        for (int d = 0; d < D; d += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(mat + d);
+    for (int s = 0; s < 8; ++s) {
+        float x[8];
+        Frag q[NQ], m[3];
+        if constexpr (NQ == 1) {
+            __builtin_memcpy(&q[0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);
+            if (!live) q[0].q = make_uint4(0u, 0u, 0u, 0u);
+        } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float* q = &s_q[16 * half + i][d];
-                acc[i] = __builtin_fmaf(q[0], x.x, acc[i]);
-                acc[i] = __builtin_fmaf(q[1], x.y, acc[i]);
-                acc[i] = __builtin_fmaf(q[2], x.z, acc[i]);
-                acc[i] = __builtin_fmaf(q[3], x.w, acc[i]);
-            }
+            for (int e = 0; e < 8; ++e) x[e] = live ? query_element(a, at + 16 * s + e) : 0.0f;
+            split_terms<NQ>(x, q);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_o[m][16 * half + i][j] = acc[i];
+        for (int k = 0; k < 2; ++k) {
+            if (k == 1 && !a.s) break;
+            const float4* p = reinterpret_cast<const float4*>((k ? m1 : m0) + 16 * s);
+            const float4 u = p[0], v = p[1];
+            const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+            split_terms<3>(e, m);
+#pragma unroll
+            for (int i = 2; i >= 0; --i)
+#pragma unroll
+                for (int j = NQ - 1; j >= 0; --j)
+                    if (i + j <= 2) acc[k] = mfma_bf16(m[i], q[j], acc[k]);
+        }
     }
+    // this lane: row r's dims 32 wave + 8 j + 4 h + (0..3)
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        acc[1][i] *= QJL_SCALE;
+        top = fmaxf(top, fmaxf(fabsf(acc[0][i]), a.s ? fabsf(acc[1][i]) : 0.0f));
+    }
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (h == 0) s_top[wave][r] = top;
     __syncthreads();
+    top = fmaxf(fmaxf(s_top[0][r], s_top[1][r]), fmaxf(s_top[2][r], s_top[3][r]));
+    // largest element in [2^7, 2^8); rows of zeros, and with an infinity, as they are
+    int e = 0;
+    if (top > 0.0f && top < __builtin_inff()) e = std::min(126, 7 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFF));
+    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+    uint16_t* const f0 = reinterpret_cast<uint16_t*>(s_f[0]);
+    uint16_t* const f1 = reinterpret_cast<uint16_t*>(s_f[1]);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int j = 32 * wave + 8 * (i >> 2) + 4 * h + (i & 3);
+        int p = position_of(a.key_bits, j);
+        f0[r * 128 + (((p >> 3) ^ (r & 15)) << 3) + (p & 7)] = (uint16_t)tq::f32_to_f16(acc[0][i] * up);
+        if (a.s) {
+            const uint32_t x = tq::f32_to_f16(acc[1][i] * up);
+            sum += tq::f16_to_f32(x);
+            p = position_of(0, j);
+            f1[r * 128 + (((p >> 3) ^ (r & 15)) << 3) + (p & 7)] =
+                (uint16_t)tq::f32_to_f16(tq::f16_to_f32(x) * (float)(128 >> (j & 7)));
+        }
+    }
+    sum += __shfl_xor(sum, 32);
+    if (h == 0) s_sum[wave][r] = sum;
+    __syncthreads();
+    const int64_t out = (int64_t)kv * gridDim.x + blk;
     if (threadIdx.x < 32) {
-        float top = 0.0f;
-        for (int m = 0; m < mats; ++m)
-            for (int d = 0; d < D; ++d) top = fmaxf(top, fabsf(s_o[m][threadIdx.x][d]));
-        // largest element in [2^9, 2^10); rows of zeros, and with an infinity, as they are
-        int e = 0;
-        if (top > 0.0f && top < __builtin_inff()) e = 9 - (int)((__float_as_uint(top) >> 23) & 0xFF) + 127;
-        e = std::min(e, 126);
-        s_top[threadIdx.x] = __uint_as_float((uint32_t)(127 + e) << 23);
-        a.row_c[((int64_t)kv * gridDim.x + blk) * 32 + threadIdx.x] = a.c2 * __uint_as_float((uint32_t)(127 - e) << 23);
+        // what the scores' fma takes from a set-bit product in units of 2^-17 to a sign's
+        const float all = s_sum[0][r] + s_sum[1][r] + s_sum[2][r] + s_sum[3][r];
+        a.row_c[out * 64 + r] = a.c2 * __uint_as_float((uint32_t)(127 - e) << 23);
+        a.row_c[out * 64 + 32 + r] = -0x1p-18f * all;
     }
-    __syncthreads();
-    uint4* const frags = a.frags + ((int64_t)kv * gridDim.x + blk) * 2 * 8 * 64;
-    for (int i = threadIdx.x; i < mats * 8 * 64; i += 256) {
-        const int m = i >> 9, s = (i >> 6) & 7, lane = i & 63, r = lane & 31, h = lane >> 5;
-        uint32_t x[4];
-        for (int k = 0; k < 4; ++k) {
-            const int bits = m ? 0 : a.key_bits;
-            x[k] = pack_f16(s_o[m][r][dim_of(bits, 2 * s + h, 2 * k)] * s_top[r],
-                            s_o[m][r][dim_of(bits, 2 * s + h, 2 * k + 1)] * s_top[r]);
-        }
-        frags[i] = make_uint4(x[0], x[1], x[2], x[3]);
+    uint4* const frags = a.frags + out * 2 * 8 * 64;
+    for (int i = threadIdx.x; i < (a.s ? 2 : 1) * 512; i += 256) {
+        const int m = i >> 9, s = (i >> 6) & 7, l = i & 63;
+        frags[i] = s_f[m][(l & 31) * 16 + ((2 * s + (l >> 5)) ^ (l & 15))];
     }
 }
 
@@ -271,7 +337,7 @@ struct TreeArgs {
     const float* row_c;
     int n_split;
     float* part_o;   // [split][kv head][row][D]
-    float4* part_ms; // [split][kv head][row] (reference of the weights in log2, sum of weights, scale of the output sums)
+    float2* part_ms; // [split][kv head][row] (reference of the weights in log2, sum of weights)
 };
 
 // Bit j of a node's mask: node j is the node itself or one of its ancestors.  A parent that is not an earlier
@@ -303,7 +369,7 @@ __device__ __forceinline__ uint64_t seen_of_tile(uint64_t sees, int to_end, int 
 }
 
 template <int KB, int VB, bool QJL>
-__global__ __launch_bounds__(256, 1) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(256, QJL ? 1 : 2) void tree_kernel(TreeArgs a) {
     __shared__ uint4 s_k[TK * 16];
     __shared__ uint4 s_s[QJL ? TK * 16 : 1];
     __shared__ uint4 s_v[TK * 16];
@@ -333,14 +399,15 @@ __global__ __launch_bounds__(256, 1) void tree_kernel(TreeArgs a) {
     klut.load(a.key_centers);
     vlut.load(a.value_centers);
     Frag q[QJL ? 2 : 1][8];
-    float c = 0.0f;
+    float c = 0.0f, sign0 = 0.0f;
     if (busy) {
         const uint4* f = a.frags + ((int64_t)kv * a.row_blocks + blk) * 2 * 8 * 64;
 #pragma unroll
         for (int m = 0; m < (QJL ? 2 : 1); ++m)
 #pragma unroll
             for (int s = 0; s < 8; ++s) q[m][s].q = f[(m * 8 + s) * 64 + lane];
-        c = a.row_c[((int64_t)kv * a.row_blocks + blk) * 32 + r];
+        c = a.row_c[((int64_t)kv * a.row_blocks + blk) * 64 + r];
+        sign0 = a.row_c[((int64_t)kv * a.row_blocks + blk) * 64 + 32 + r];
     }
     __syncthreads();
     uint64_t sees = nodes ? s_anc[(32 * blk + r) % a.T] : 0ull;
@@ -385,7 +452,7 @@ __global__ __launch_bounds__(256, 1) void tree_kernel(TreeArgs a) {
             const int64_t slot = first + t0 + std::min(lane, left - 1);
             const float vn = lane < left ? tq::f16_to_f32(a.v_norms[slot]) : 0.0f;
             s_kn[lane] = tq::f16_to_f32(a.k_norms[slot]);
-            if constexpr (QJL) s_rn[lane] = tq::f16_to_f32(a.k_rnorms[slot]) * QJL_SCALE;
+            if constexpr (QJL) s_rn[lane] = tq::f16_to_f32(a.k_rnorms[slot]) * 0x1p18f;
             s_vn[lane] = vn;
             float m = fabsf(vn) < __builtin_inff() ? fabsf(vn) : 0.0f;
 #pragma unroll
@@ -407,7 +474,7 @@ __global__ __launch_bounds__(256, 1) void tree_kernel(TreeArgs a) {
             }
             __builtin_amdgcn_sched_barrier(0);  // the reads of all sixteen steps at once do not fit the registers
             if constexpr (QJL) {
-                f32x16 y = zero16();
+                f32x16 y = fill16(sign0);
 #pragma unroll
                 for (int ks = 0; ks < 8; ++ks) {
                     Frag kf;
@@ -493,38 +560,51 @@ __global__ __launch_bounds__(256, 1) void tree_kernel(TreeArgs a) {
     sum += __shfl_xor(sum, 32);
     if (!busy || row >= a.rows) return;
     const int64_t at = ((int64_t)split * (gridDim.x / a.n_split) + kv) * a.rows + row;
-    if (h == 0) a.part_ms[at] = make_float4(top == -__builtin_inff() ? top : top * c, sum, unit, 0.0f);
+    if (h == 0) a.part_ms[at] = make_float2(top == -__builtin_inff() ? top : top * c, sum);
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             *reinterpret_cast<float4*>(a.part_o + at * D + 32 * d + 8 * j + 4 * h) =
-                make_float4(o[d][4 * j], o[d][4 * j + 1], o[d][4 * j + 2], o[d][4 * j + 3]);
+                make_float4(o[d][4 * j] * unit, o[d][4 * j + 1] * unit, o[d][4 * j + 2] * unit, o[d][4 * j + 3] * unit);
 }
 
 // ------------------------------------------------------------------ merge
 
 struct MergeArgs {
-    int q_heads, kv_heads, T, rows, n_split, value_bits;
+    int q_heads, kv_heads, T, rows, n_split, value_bits;  // value_bits: the order of the partials' dims, 0 their own
     int64_t all_rows;  // of all KV heads
     const float* part_o;
-    const float4* part_ms;
+    const float2* part_ms;
     const float* rv;
     float* out_f32;
     uint16_t* out_bf16;
     float* lse;
 };
 
-// Eight rows per workgroup: their splits weighed and added, then rotated back.
+// Eight rows per workgroup: their splits weighed and added, then rotated back.  The matrix is read ahead of the partials,
+// half of its rows by a thread for its output dim.
 __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     __shared__ float s_w[8][MAX_SPLIT];
     __shared__ float s_den[8];
-    __shared__ float s_o[8][D];
+    __shared__ __align__(16) float s_o[8][D];
+    __shared__ float s_half[8][D];
     const int64_t row0 = (int64_t)blockIdx.x * 8;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int j = threadIdx.x & 127, half = threadIdx.x >> 7;
+    float m[64];
+#pragma unroll
+    for (int d = 0; d < 64; ++d) m[d] = a.rv[(64 * half + d) * D + j];
+    auto place = [&](int64_t row) {  // of a row in [batch][q heads][T]
+        const int64_t kv = row / a.rows;
+        const int in = (int)(row - kv * a.rows), g = in / a.T, t = in - g * a.T;
+        const int64_t b = kv / a.kv_heads, hq = (kv - b * a.kv_heads) * (a.q_heads / a.kv_heads) + g;
+        return (b * a.q_heads + hq) * a.T + t;
+    };
+#pragma unroll
     for (int k = wave; k < 8; k += 4) {
         const int64_t row = row0 + k;
-        float4 ms = make_float4(-__builtin_inff(), 0.0f, 0.0f, 0.0f);
+        float2 ms = make_float2(-__builtin_inff(), 0.0f);
         if (row < a.all_rows && lane < a.n_split) ms = a.part_ms[lane * a.all_rows + row];
         float top = ms.x;
 #pragma unroll
@@ -533,46 +613,61 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
         float den = w * ms.y;
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) den += __shfl_xor(den, x);
-        s_w[k][lane] = w == 0.0f ? 0.0f : w * ms.z;
+        s_w[k][lane] = w;
         if (lane == 0) {
             s_den[k] = den;
-            if (a.lse && row < a.all_rows) {
-                const int64_t kv = row / a.rows;
-                const int in = (int)(row - kv * a.rows), g = in / a.T, t = in - g * a.T;
-                const int64_t b = kv / a.kv_heads, hq = (kv % a.kv_heads) * (a.q_heads / a.kv_heads) + g;
-                a.lse[(b * a.q_heads + hq) * a.T + t] =
-                    den == 0.0f ? -__builtin_inff() : top * 0.6931471805599453f + __builtin_logf(den);
-            }
+            if (a.lse && row < a.all_rows)
+                a.lse[place(row)] = den == 0.0f ? -__builtin_inff() : top * 0.6931471805599453f + __builtin_logf(den);
         }
     }
     __syncthreads();
-    const int pos = threadIdx.x & 127;
-    for (int k = threadIdx.x >> 7; k < 8; k += 2) {
-        const int64_t row = row0 + k;
-        float o = 0.0f;
-        if (row < a.all_rows)
-            for (int i = 0; i < a.n_split; ++i)
-                if (s_w[k][i] != 0.0f) o = __builtin_fmaf(s_w[k][i], a.part_o[(i * a.all_rows + row) * D + pos], o);
-        s_o[k][dim_of(a.value_bits, pos >> 3, pos & 7)] = s_den[k] == 0.0f ? 0.0f : o / s_den[k];
+    {  // 32 threads to a row, four dims each
+        const int k = threadIdx.x >> 5, c = threadIdx.x & 31;
+        const int64_t row = std::min(row0 + k, a.all_rows - 1);
+        const float4* p = reinterpret_cast<const float4*>(a.part_o + row * D) + c;
+        const int64_t step = a.all_rows * (D / 4);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int i = 0; i < a.n_split; ++i) {
+            const float w = s_w[k][i];
+            const float4 x = p[i * step];
+            o.x = __builtin_fmaf(w, x.x, o.x), o.y = __builtin_fmaf(w, x.y, o.y);
+            o.z = __builtin_fmaf(w, x.z, o.z), o.w = __builtin_fmaf(w, x.w, o.w);
+        }
+        const float den = s_den[k] == 0.0f ? 1.0f : s_den[k];
+        const float v[4] = {o.x / den, o.y / den, o.z / den, o.w / den};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int pos = 4 * c + e;
+            s_o[k][a.value_bits ? dim_of(a.value_bits, pos >> 3, pos & 7) : pos] = v[e];
+        }
     }
     __syncthreads();
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int half = threadIdx.x >> 7;
-    for (int d = 0; d < D; ++d) {
-        const float x = a.rv[d * D + pos];
+    float acc[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] = __builtin_fmaf(s_o[4 * half + k][d], x, acc[k]);
+    for (int k = 0; k < 8; ++k) {
+        acc[k] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 64; d += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(&s_o[k][64 * half + d]);
+            acc[k] = __builtin_fmaf(o.x, m[d], acc[k]);
+            acc[k] = __builtin_fmaf(o.y, m[d + 1], acc[k]);
+            acc[k] = __builtin_fmaf(o.z, m[d + 2], acc[k]);
+            acc[k] = __builtin_fmaf(o.w, m[d + 3], acc[k]);
+        }
     }
+    // the halves are exchanged: thread (j, half) finishes rows 4 half + (0..3)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s_half[4 * (1 - half) + k][j] = half ? acc[k] : acc[4 + k];
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const int64_t row = row0 + 4 * half + k;
         if (row >= a.all_rows) continue;
-        const int64_t kv = row / a.rows;
-        const int in = (int)(row - kv * a.rows), g = in / a.T, t = in - g * a.T;
-        const int64_t b = kv / a.kv_heads, hq = (kv % a.kv_heads) * (a.q_heads / a.kv_heads) + g;
-        const int64_t at = ((b * a.q_heads + hq) * a.T + t) * D + pos;
-        if (a.out_f32) a.out_f32[at] = acc[k];
-        if (a.out_bf16) a.out_bf16[at] = (uint16_t)tq::f32_to_bf16(acc[k]);
+        const float x = (half ? acc[4 + k] : acc[k]) + s_half[4 * half + k][j];
+        const int64_t at = place(row) * D + j;
+        if (a.out_f32) a.out_f32[at] = x;
+        if (a.out_bf16) a.out_bf16[at] = (uint16_t)tq::f32_to_bf16(x);
     }
 }
 
@@ -596,8 +691,8 @@ bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Pl
     p.n_split = (int)((tiles + per - 1) / per);
     const int64_t all = p.heads * p.rows;
     p.frag_bytes = (size_t)(p.heads * p.row_blocks) * 2 * 8 * 64 * 16;
-    p.row_c_bytes = (size_t)(p.heads * p.row_blocks) * 32 * 4;
-    p.ms_bytes = (size_t)all * p.n_split * 16;
+    p.row_c_bytes = (size_t)(p.heads * p.row_blocks) * 64 * 4;
+    p.ms_bytes = ((size_t)all * p.n_split * 8 + 15) / 16 * 16;
     p.o_bytes = (size_t)all * p.n_split * D * 4;
     return p.heads * p.n_split < ((int64_t)1 << 24) && all < ((int64_t)1 << 26) && p.heads <= 65535;
 }
@@ -643,12 +738,14 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint4* frags = reinterpret_cast<uint4*>(ws);
     float* part_o = reinterpret_cast<float*>(ws + p.frag_bytes);
-    float4* part_ms = reinterpret_cast<float4*>(ws + p.frag_bytes + p.o_bytes);
+    float2* part_ms = reinterpret_cast<float2*>(ws + p.frag_bytes + p.o_bytes);
     float* row_c = reinterpret_cast<float*>(ws + p.frag_bytes + p.o_bytes + p.ms_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const PrepArgs prep{q, q_type, q_heads, kv_heads, nodes, p.rows, q_sb, q_sh, q_st, key_rotation,
                         has_qjl ? qjl : nullptr, key_bits, scale * LOG2E, frags, row_c};
-    hipLaunchKernelGGL(prep_kernel, dim3((unsigned)p.row_blocks, (unsigned)p.heads), dim3(256), 0, s, prep);
+    const dim3 prep_grid((unsigned)p.row_blocks, (unsigned)p.heads);
+    if (q_type == 0) hipLaunchKernelGGL(prep_kernel<1>, prep_grid, dim3(256), 0, s, prep);
+    else hipLaunchKernelGGL(prep_kernel<3>, prep_grid, dim3(256), 0, s, prep);
     TQ_CHECK_LAUNCH();
     const TreeArgs a{kv_heads, nodes, p.rows, p.row_blocks, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
                      k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, frags, row_c,
