@@ -25,6 +25,7 @@
 // and outputs are fp32.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tq_common.h"
 
@@ -34,6 +35,8 @@ constexpr int D = TQ_DIM;
 constexpr int TK = 64;         // tokens per tile
 constexpr int MAX_SPLIT = 64;  // partials a merge wave weighs with one lane each
 constexpr float LOG2E = 1.44269504f;
+constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's reference by
+constexpr int TOP_BIT = 7;    // largest weight times norm at the reference: 2^TOP_BIT
 constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -42,6 +45,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 union Frag {
     uint32_t u[4];
@@ -569,6 +573,335 @@ __global__ __launch_bounds__(256, QJL ? 1 : 2) void tree_kernel(TreeArgs a) {
                 make_float4(o[d][4 * j] * unit, o[d][4 * j + 1] * unit, o[d][4 * j + 2] * unit, o[d][4 * j + 3] * unit);
 }
 
+// ---- few rows: a wave's tile is its own
+
+// Pairs of value codes looked up in LDS: entry e of the table is the pair (or the two pairs) that the byte e of the
+// packed codes holds, 256 bytes to an entry: 32 copies of the first pair, one for each lane of a half wave, so that no two
+// lanes meet in a bank, then 32 of the second.  A byte of 3-bit codes is taken as 6-bit windows: bits 0-5, and 2-7.
+template <int VB>
+struct PairTable {
+    static constexpr int SECOND = 128;  // bytes from an entry's first pair to its second
+    // `centers` in LDS
+    static __device__ __forceinline__ void build(uint32_t* table, const float* centers, int threads) {
+        constexpr uint32_t m = (1u << VB) - 1;
+        constexpr int sh = VB == 2 ? 4 : 2;
+        for (int i = threadIdx.x; i < 256 * 16; i += threads) {
+            const uint32_t e = i >> 4, x = e >> ((i & 15) < 8 || VB == 4 ? 0 : sh);
+            const uint32_t pair = pack_f16(centers[x & m], centers[(x >> VB) & m]);
+            reinterpret_cast<uint4*>(table)[i] = make_uint4(pair, pair, pair, pair);
+        }
+    }
+    // byte k of w as a table address
+    static __device__ __forceinline__ uint32_t at(const uint8_t* table, uint32_t w, int k, uint32_t lane4, int second) {
+        const uint32_t off = perm(w, lane4, 0x0C0C0000u | (uint32_t)(4 + k) << 8);
+        return *reinterpret_cast<const uint32_t*>(table + off + (second ? SECOND : 0));
+    }
+    // pairs 8 g + (0..7) of 64 codes (2 VB words), in the order of their dims
+    static __device__ __forceinline__ void look_up(const uint8_t* t, const uint32_t* w, uint32_t lane4, int g, uint32_t* out) {
+        if constexpr (VB == 3) {
+            auto moved = [&](int i) { return i < 5 ? __builtin_amdgcn_alignbit(w[i + 1], w[i], 4) : w[i] >> 4; };
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {  // 8 codes in 3 bytes
+                const int at0 = 3 * (2 * g + k);
+                out[4 * k] = at(t, w[at0 >> 2], at0 & 3, lane4, 0);
+                out[4 * k + 1] = at(t, moved(at0 >> 2), at0 & 3, lane4, 1);
+                out[4 * k + 2] = at(t, moved((at0 + 1) >> 2), (at0 + 1) & 3, lane4, 0);
+                out[4 * k + 3] = at(t, w[(at0 + 2) >> 2], (at0 + 2) & 3, lane4, 1);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int n = 8 * g + k;
+                if constexpr (VB == 4) out[k] = at(t, w[n >> 2], n & 3, lane4, 0);
+                else if constexpr (VB == 2) out[k] = at(t, w[n >> 3], (n >> 1) & 3, lane4, n & 1);
+                else out[k] = at(t, n & 2 ? w[n >> 4] >> 4 : w[n >> 4], (n >> 2) & 3, lane4, n & 1);
+            }
+        }
+    }
+};
+
+// Up to 32 RB rows of a KV head, all of them in every wave; the waves take the tiles of 32 tokens in turn.  A lane is a
+// token and half of its dims: the keys' codes and signs become its A operands in registers, the values' go through 8 KB of
+// LDS of the wave's own.  No barrier until the waves' sums meet at the end.
+template <int RB>
+struct Narrow {
+    static constexpr int W = RB == 1 ? 8 : 4;
+    static constexpr int T = 64 * W;
+    struct Tiles {
+        uint32_t table[256 * 64];
+        uint4 v[W][32 * 16];
+        uint4 qs[8 * 64];  // the rows' sign operands: beside those of the codes they do not fit the registers
+        uint16_t kn[W][32], vn[W][32];
+        float rn[W][32];
+    };
+    struct Sums {
+        float4 o[W][32 * RB][32];  // chunks xor-swizzled by the row
+        float2 ms[W][32 * RB];
+        float unit[W];
+    };
+    union Lds {
+        Tiles t;
+        Sums s;
+    };
+};
+
+template <int KB, int VB, bool QJL, int RB>
+__global__ __launch_bounds__(Narrow<RB>::T, RB == 1 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
+    using N = Narrow<RB>;
+    constexpr int W = N::W, NT = 32;  // tokens of a tile
+    __shared__ typename N::Lds lds;
+    __shared__ uint64_t s_anc[64];
+    __shared__ float s_centers[1 << VB];
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // in a scalar register, and what follows from it
+    const int kv = blockIdx.x / a.n_split, split = blockIdx.x - kv * a.n_split;
+    const int b = kv / a.kv_heads;
+
+    const int nodes = a.parents ? a.T : 0;
+    int64_t end = a.lens ? a.lens[b] : a.n_tokens - nodes;
+    end = std::min<int64_t>(std::max<int64_t>(end, 0), a.n_tokens);
+    int64_t lo = a.starts ? a.starts[b] : 0;
+    lo = std::min<int64_t>(std::max<int64_t>(lo, 0), end);
+    const int64_t stop = std::min<int64_t>(end + nodes, a.n_tokens);
+    const int64_t tiles = (stop - lo + NT - 1) / NT;
+    const int64_t first_tile = tiles * split / a.n_split, last_tile = tiles * (split + 1) / a.n_split;
+
+    if (threadIdx.x < (1 << VB)) s_centers[threadIdx.x] = a.value_centers[threadIdx.x];
+    if (nodes && wave == 0) s_anc[lane] = ancestors(a.parents + b * a.parents_sb, a.T, lane);
+
+    // a lane's part of a tile, on its way
+    struct Raw {
+        uint32_t k[2 * KB], v[2 * VB], s[2];
+        uint16_t kn, rn, vn;
+    };
+    // a tile's arrays at scalar addresses, a lane's place in them as 32-bit offsets
+    auto load = [&](Raw& w, int64_t tile) {
+        const int64_t t0 = lo + tile * NT, slot = (int64_t)kv * a.cap + t0;
+        const uint32_t tok = std::min<uint32_t>(r, (uint32_t)std::min<int64_t>(stop - t0, NT) - 1);
+        __builtin_memcpy(w.k, __builtin_assume_aligned(a.k_codes + slot * (16 * KB) + (tok * (16 * KB) + 8 * KB * h), 8), 8 * KB);
+        __builtin_memcpy(w.v, __builtin_assume_aligned(a.v_codes + slot * (16 * VB) + (tok * (16 * VB) + 8 * VB * h), 8), 8 * VB);
+        if constexpr (QJL) {
+            __builtin_memcpy(w.s, __builtin_assume_aligned(a.k_signs + slot * 16 + (tok * 16 + 8 * h), 8), 8);
+            w.rn = (a.k_rnorms + slot)[tok];
+        }
+        w.kn = (a.k_norms + slot)[tok], w.vn = (a.v_norms + slot)[tok];
+    };
+    Raw raw;
+    int64_t tile = first_tile + wave;
+    if (tile < last_tile) load(raw, tile);
+
+    Lut<KB> klut;
+    klut.load(a.key_centers);
+    Frag q[RB][8];
+    float c[RB], sign0[RB];
+#pragma unroll
+    for (int m = 0; m < RB; ++m) {
+        const int blk = std::min((int)blockIdx.y * RB + m, a.row_blocks - 1);
+        const int64_t at = (int64_t)kv * a.row_blocks + blk;
+        const uint4* f = a.frags + at * 2 * 8 * 64;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) q[m][s].q = f[s * 64 + lane];
+        if constexpr (QJL)
+            for (int i = threadIdx.x; i < 8 * 64; i += N::T) lds.t.qs[i] = f[8 * 64 + i];
+        c[m] = a.row_c[at * 64 + r];
+        sign0[m] = QJL ? a.row_c[at * 64 + 32 + r] : 0.0f;
+    }
+    __syncthreads();
+    PairTable<VB>::build(lds.t.table, s_centers, N::T);
+    uint64_t sees[RB];
+#pragma unroll
+    for (int m = 0; m < RB; ++m) sees[m] = nodes ? s_anc[(32 * ((int)blockIdx.y * RB + m) + r) % a.T] : 0ull;
+    __syncthreads();
+
+    f32x16 o[RB][4];
+    float top[RB], sum[RB];  // `top` is a weight's reference, raised when a score is more than 2^LAZY above it
+#pragma unroll
+    for (int m = 0; m < RB; ++m) {
+        top[m] = -__builtin_inff(), sum[m] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[m][d] = zero16();
+    }
+    // weights and output sums are in units of 2^-shift, 2^-TOP_BIT of a power of two above the largest |v| so far: weights
+    // times norm then reach up to 2^(TOP_BIT + LAZY), and fp16 keeps its 11 bits down to 2^-14
+    int shift = TOP_BIT + 24;
+    const uint32_t lane4 = (lane & 31) * 4;
+    const uint8_t* const table = reinterpret_cast<const uint8_t*>(lds.t.table);
+    uint8_t* const v8 = reinterpret_cast<uint8_t*>(lds.t.v[wave]);
+
+    auto step = [&](Raw& w, int64_t tile, auto nodes_here) {
+        const int64_t t0 = lo + tile * NT;
+        const int left = (int)std::min<int64_t>(stop - t0, NT);
+        // ---- values to LDS, eight dims at a time
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint32_t x[8];
+            PairTable<VB>::look_up(table, w.v, lane4, g, x);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                *reinterpret_cast<uint4*>(v8 + r * 256 + (((8 * h + 2 * g + j) ^ swizzle(r)) << 4)) =
+                    make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+        }
+        const uint32_t norm = !nodes_here || r < left ? w.vn : 0u;  // tokens past the last weigh nothing
+        if (h == 0) {
+            lds.t.kn[wave][r] = w.kn;
+            lds.t.vn[wave][r] = (uint16_t)norm;
+            if constexpr (QJL) lds.t.rn[wave][r] = tq::f16_to_f32(w.rn) * 0x1p18f;
+        }
+        // ---- scores
+        f32x16 x[RB], y[RB];
+#pragma unroll
+        for (int m = 0; m < RB; ++m) x[m] = zero16(), y[m] = fill16(sign0[m]);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            uint4 f[4];
+            expand32<KB>(w.k + KB * u, klut, f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                Frag kf;
+                kf.q = f[j];
+#pragma unroll
+                for (int m = 0; m < RB; ++m) x[m] = mfma_f16(kf, q[m][4 * u + j], x[m]);
+            }
+            if constexpr (QJL) {
+                expand_signs(w.s[u], f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    Frag kf, qf;
+                    kf.q = f[j];
+                    qf.q = lds.t.qs[(4 * u + j) * 64 + lane];
+#pragma unroll
+                    for (int m = 0; m < RB; ++m) y[m] = mfma_f16(kf, qf, y[m]);
+                }
+            }
+        }
+        // the largest finite |v| of the tile: its exponent decides the unit (2^(e + 1) is above it)
+        const int e5 = (norm >> 10) & 31, ve = e5 == 31 ? 0 : e5;
+        int need = 0;  // uniform: a token whose exponent the unit does not cover
+        if (__any(ve > 14 + TOP_BIT - shift)) {
+            int e = ve;
+#pragma unroll
+            for (int k = 1; k < 32; k <<= 1) e = std::max(e, __shfl_xor(e, k));
+            need = shift - (14 + TOP_BIT - std::max(__builtin_amdgcn_readfirstlane(e), 1));
+        }
+        shift -= need;
+        if (tile + W < last_tile) load(w, tile + W);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        Frag pf[RB][2];
+#pragma unroll
+        for (int m = 0; m < RB; ++m) {
+            f32x16 s;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f16x4 k4 = *reinterpret_cast<const f16x4*>(&lds.t.kn[wave][8 * j + 4 * h]);
+                if constexpr (QJL) {
+                    const f32x4 r4 = *reinterpret_cast<const f32x4*>(&lds.t.rn[wave][8 * j + 4 * h]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[4 * j + e] = __builtin_fmaf((float)k4[e], x[m][4 * j + e], r4[e] * y[m][4 * j + e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[4 * j + e] = (float)k4[e] * x[m][4 * j + e];
+                }
+            }
+            if constexpr (nodes_here) {
+                const int to_end = (int)std::max<int64_t>(std::min<int64_t>(end - t0, TK), -TK);
+                const uint32_t word = (uint32_t)seen_of_tile(sees[m], to_end, left) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (!(word & (1u << (8 * (i >> 2) + (i & 3))))) s[i] = -__builtin_inff();
+            }
+            float mx = s[0];
+#pragma unroll
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+            // both halves of the row see the same, and neither -inf nor NaN raises the reference
+            if (__any(__builtin_fmaf(mx, c[m], -top[m]) > LAZY) || need) {
+                mx = fmaxf(mx, __shfl_xor(mx, 32)) * c[m];
+                const float ref = mx > top[m] ? mx : top[m];
+                const float corr = exp2_(top[m] == ref ? -(float)need : top[m] - ref - (float)need);
+                top[m] = ref;
+                sum[m] *= corr;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[m][d][i] *= corr;
+            }
+            const float base = (float)shift - (top[m] == -__builtin_inff() ? 0.0f : top[m]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f16x4 v4 = *reinterpret_cast<const f16x4*>(&lds.t.vn[wave][8 * j + 4 * h]);
+                float p[4], wt[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = exp2_(__builtin_fmaf(s[4 * j + e], c[m], base));
+                    sum[m] += p[e];
+                    wt[e] = p[e] * (float)v4[e];
+                    if constexpr (nodes_here) wt[e] = p[e] == 0.0f ? 0.0f : wt[e];  // a left-out token's norm may be anything
+                }
+                pf[m][j >> 1].u[2 * (j & 1)] = pack_f16(wt[0], wt[1]);
+                pf[m][j >> 1].u[2 * (j & 1) + 1] = pack_f16(wt[2], wt[3]);
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                Frag vf;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) vf.t[e] = read_tr(v8 + value_offset(d, e, lane) + 16 * 256 * ks);
+#pragma unroll
+                for (int m = 0; m < RB; ++m) o[m][d] = mfma_f16(vf, pf[m][ks], o[m][d]);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    // whole tiles of the history, then those with the end of it or drafted tokens in them
+    const int64_t whole = std::min(last_tile, (end - lo) / NT);
+    for (; tile < whole; tile += W) step(raw, tile, std::false_type{});
+    for (; tile < last_tile; tile += W) step(raw, tile, std::true_type{});
+
+    // ---- the waves' sums
+    __syncthreads();
+    const float unit = __uint_as_float((uint32_t)(127 - shift) << 23);
+#pragma unroll
+    for (int m = 0; m < RB; ++m) {
+        const float all = sum[m] + __shfl_xor(sum[m], 32);
+        if (h == 0)
+            lds.s.ms[wave][32 * m + r] = make_float2(top[m], all * unit);
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                lds.s.o[wave][32 * m + r][(8 * d + 2 * j + h) ^ r] =
+                    make_float4(o[m][d][4 * j], o[m][d][4 * j + 1], o[m][d][4 * j + 2], o[m][d][4 * j + 3]);
+    }
+    if (lane == 0) lds.s.unit[wave] = unit;
+    __syncthreads();
+    const int64_t heads = gridDim.x / a.n_split;
+    for (int i = threadIdx.x; i < 32 * RB * 32; i += N::T) {
+        const int row = i >> 5, ch = i & 31, out_row = (int)blockIdx.y * 32 * RB + row;
+        if (out_row >= a.rows) continue;
+        float best = -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < W; ++k) best = fmaxf(best, lds.s.ms[k][row].x);
+        const float safe = best == -__builtin_inff() ? 0.0f : best;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float den = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float2 ms = lds.s.ms[k][row];
+            const float w = exp2_(ms.x - safe), wu = w * lds.s.unit[k];
+            const float4 y = lds.s.o[k][row][ch ^ (row & 31)];
+            den = __builtin_fmaf(w, ms.y, den);
+            x.x = __builtin_fmaf(wu, y.x, x.x), x.y = __builtin_fmaf(wu, y.y, x.y);
+            x.z = __builtin_fmaf(wu, y.z, x.z), x.w = __builtin_fmaf(wu, y.w, x.w);
+        }
+        const int64_t at = ((int64_t)split * heads + kv) * a.rows + out_row;
+        reinterpret_cast<float4*>(a.part_o + at * D)[ch] = x;
+        if (ch == 0) a.part_ms[at] = make_float2(best, den);
+    }
+}
+
 // ------------------------------------------------------------------ merge
 
 struct MergeArgs {
@@ -675,31 +1008,43 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 struct Plan {
     int rows, row_blocks, n_split;
+    bool narrow;
     int64_t heads;
     size_t frag_bytes, row_c_bytes, ms_bytes, o_bytes;
     size_t total() const { return frag_bytes + row_c_bytes + ms_bytes + o_bytes; }
 };
 
-// Splits: two workgroups for each CU, as long as none is left without a tile.
+// Up to 64 rows of a KV head are one workgroup's, a CU's worth of waves; more are dealt to the waves of several, two to a
+// CU.  As many splits as fill the CUs, as long as none is left without a tile.
 bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Plan& p) {
     p.heads = (int64_t)batch * kv_heads;
     p.rows = q_heads / kv_heads * T;
     p.row_blocks = (p.rows + 31) / 32;
-    const int64_t wgs = p.heads * ((p.row_blocks + 3) / 4), tiles = std::max<int64_t>(1, (n_tokens + TK - 1) / TK);
-    int64_t n = std::max<int64_t>(1, std::min<int64_t>({(512 + wgs - 1) / wgs, tiles, MAX_SPLIT}));
-    const int64_t per = (tiles + n - 1) / n;
-    p.n_split = (int)((tiles + per - 1) / per);
+    p.narrow = p.row_blocks <= 2;
+    const int64_t wgs = p.narrow ? p.heads * p.row_blocks : p.heads * ((p.row_blocks + 3) / 4);
+    const int64_t per_tile = p.narrow ? 32 : TK, tiles = std::max<int64_t>(1, (n_tokens + per_tile - 1) / per_tile);
+    const int64_t fill = p.narrow ? 256 / wgs : (512 + wgs - 1) / wgs;
+    int64_t n = std::max<int64_t>(1, std::min<int64_t>({fill, tiles, MAX_SPLIT}));
+    if (!p.narrow) {
+        const int64_t per = (tiles + n - 1) / n;
+        n = (tiles + per - 1) / per;
+    }
+    p.n_split = (int)n;
     const int64_t all = p.heads * p.rows;
     p.frag_bytes = (size_t)(p.heads * p.row_blocks) * 2 * 8 * 64 * 16;
     p.row_c_bytes = (size_t)(p.heads * p.row_blocks) * 64 * 4;
     p.ms_bytes = ((size_t)all * p.n_split * 8 + 15) / 16 * 16;
     p.o_bytes = (size_t)all * p.n_split * D * 4;
-    return p.heads * p.n_split < ((int64_t)1 << 24) && all < ((int64_t)1 << 26) && p.heads <= 65535;
+    return p.heads * p.n_split < ((int64_t)1 << 22) && all < ((int64_t)1 << 26) && p.heads <= 65535;
 }
 
 template <int KB, int VB, bool QJL>
-void launch_tree(const TreeArgs& a, dim3 grid, hipStream_t s) {
-    hipLaunchKernelGGL((tree_kernel<KB, VB, QJL>), grid, dim3(256), 0, s, a);
+void launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
+    const unsigned x = (unsigned)(p.heads * p.n_split);
+    if (!p.narrow)
+        hipLaunchKernelGGL((tree_kernel<KB, VB, QJL>), dim3(x, (unsigned)((p.row_blocks + 3) / 4)), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((tree_narrow_kernel<KB, VB, QJL, 1>), dim3(x, (unsigned)p.row_blocks), dim3(Narrow<1>::T), 0, s, a);
 }
 
 }  // namespace
@@ -750,19 +1095,18 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
     const TreeArgs a{kv_heads, nodes, p.rows, p.row_blocks, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
                      k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, frags, row_c,
                      p.n_split, part_o, part_ms};
-    const dim3 grid((unsigned)(p.heads * p.n_split), (unsigned)((p.row_blocks + 3) / 4));
     if (has_qjl) {
-        if (value_bits == 4) launch_tree<3, 4, true>(a, grid, s);
-        else if (value_bits == 3) launch_tree<2, 3, true>(a, grid, s);
-        else launch_tree<1, 2, true>(a, grid, s);
+        if (value_bits == 4) launch_tree<3, 4, true>(a, p, s);
+        else if (value_bits == 3) launch_tree<2, 3, true>(a, p, s);
+        else launch_tree<1, 2, true>(a, p, s);
     } else {
-        if (value_bits == 4) launch_tree<4, 4, false>(a, grid, s);
-        else if (value_bits == 3) launch_tree<3, 3, false>(a, grid, s);
-        else if (value_bits == 2) launch_tree<2, 2, false>(a, grid, s);
-        else launch_tree<1, 1, false>(a, grid, s);
+        if (value_bits == 4) launch_tree<4, 4, false>(a, p, s);
+        else if (value_bits == 3) launch_tree<3, 3, false>(a, p, s);
+        else if (value_bits == 2) launch_tree<2, 2, false>(a, p, s);
+        else launch_tree<1, 1, false>(a, p, s);
     }
     TQ_CHECK_LAUNCH();
-    const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, value_bits, p.heads * p.rows, part_o, part_ms,
+    const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, p.narrow ? 0 : value_bits, p.heads * p.rows, part_o, part_ms,
                       value_rotation, out_f32, out_bf16, lse_out};
     hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((p.heads * p.rows + 7) / 8)), dim3(256), 0, s, m);
     TQ_CHECK_LAUNCH();
