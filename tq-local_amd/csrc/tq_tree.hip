@@ -32,7 +32,7 @@
 namespace {
 
 constexpr int D = TQ_DIM;
-constexpr int TK = 64;         // tokens per tile
+constexpr int TK = 32;         // tokens per tile
 constexpr int MAX_SPLIT = 64;  // partials a merge wave weighs with one lane each
 constexpr float LOG2E = 1.44269504f;
 constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's reference by
@@ -77,16 +77,6 @@ __device__ __forceinline__ f32x16 fill16(float x) {
 }
 __device__ __forceinline__ f32x16 zero16() { return fill16(0.0f); }
 
-// A row of 128 dims is 16 chunks of 8 elements: chunk 2 s + h is the s-th of dims [64 h, 64 h + 64).  The dim at
-// element e of it for codes of `bits` bits (0: the QJL signs).  Codes of one and of three bits are at the same
-// bits of bytes 8 codes apart, of two bits 4 apart, of four bits 2 apart.
-__host__ __device__ constexpr int dim_of(int bits, int chunk, int e) {
-    const int s = chunk >> 1, h = chunk & 1;
-    if (bits == 0) return 64 * h + 32 * (s >> 2) + 4 * (s & 3) + (e >> 1) + 16 * (e & 1);
-    const int st = bits == 4 ? 2 : bits == 2 ? 4 : 8, per = st / 2;
-    return 64 * h + 4 * st * (s / per) + 2 * (s % per) + (e >> 2) + st * (e & 3);
-}
-
 // ------------------------------------------------------------------ codes to fp16 rows
 
 // The fp16 centroids' high and low bytes, four entries to a register.
@@ -121,7 +111,7 @@ struct Lut {
     }
 };
 
-// Four chunks of 8 elements from 32 codes (BITS words), in the order of dim_of.
+// Four chunks of 8 elements from 32 codes (BITS words), in the order of position_of.
 template <int BITS>
 __device__ __forceinline__ void expand32(const uint32_t* w, const Lut<BITS>& lut, uint4* out) {
     uint32_t q[8];
@@ -171,14 +161,15 @@ __device__ __forceinline__ void expand_signs(uint32_t w, uint4* out) {
 
 __device__ __forceinline__ int swizzle(int token) { return ((token & 3) << 2) | ((token >> 2) & 3); }
 
+__device__ __forceinline__ void load_lds16(const void* g, void* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g,
+                                     (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
+}
 __device__ __forceinline__ s16x4 read_tr(const uint8_t* l) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)l);
 }
-// Byte offsets in a tile: the 16 bytes of a key row that a lane takes in step ks (plus 32 rows per block of tokens), and
-// the 8 bytes of dims 32 d + ... of the four tokens e of 16 (plus 16 rows per step).
-__device__ __forceinline__ int key_offset(int ks, int lane) {
-    return (lane & 31) * 256 + (((2 * ks + (lane >> 5)) ^ swizzle(lane & 31)) << 4);
-}
+// Byte offset of what a lane gives ds_read_b64_tr_b16 for dims 32 d + (0..31) of the tokens 8 e + 4 h + (0..3) of 16
+// value rows: 16 lanes read 4 tokens x 16 dims, and each ends with one dim's 4 tokens.
 __device__ __forceinline__ int value_offset(int d, int e, int lane) {
     const int tok = 8 * e + 4 * (lane >> 5) + ((lane & 15) >> 2);
     const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
@@ -223,67 +214,83 @@ __device__ __forceinline__ void split_terms(const float* x, Frag* t) {
     }
 }
 
-// Where dim j stands in a row ordered by dim_of.
-__device__ __forceinline__ int position_of(int bits, int j) {
-    const int h = j >> 6, x = j & 63;
-    if (bits == 0) {
-        const int n = x & 15;
-        return (2 * (4 * (x >> 5) + (n >> 2)) + h) * 8 + 2 * (n & 3) + ((x >> 4) & 1);
-    }
-    const int st = bits == 4 ? 2 : bits == 2 ? 4 : 8, per = st / 2;
-    const int y = x % (4 * st), z = y % st;
-    return (2 * ((x / (4 * st)) * per + (z >> 1)) + h) * 8 + 4 * (z & 1) + y / st;
+// Where dim j stands among a key's 128 operands: 16 chunks of 8 elements, chunk 2 s + h the lanes' operand of step s for
+// dims [64 h, 64 h + 64).  What meets in a register follows from the packing: codes of one and of three bits are at the same
+// bits of bytes 8 codes apart, of two bits 4 apart, of four bits 2 apart (2^log_st); signs are taken 16 apart.
+__device__ __forceinline__ int position_of(int log_st, int j) {
+    const int st = 1 << log_st, x = j & 63, y = x & (4 * st - 1), z = y & (st - 1);
+    const int s = ((x >> (log_st + 2)) << (log_st - 1)) + (z >> 1);
+    return (2 * s + (j >> 6)) * 8 + 4 * (z & 1) + (y >> log_st);
+}
+__device__ __forceinline__ int sign_position_of(int j) {
+    const int x = j & 63, n = x & 15, s = 4 * (x >> 5) + (n >> 2);
+    return (2 * s + (j >> 6)) * 8 + 2 * (n & 3) + ((x >> 4) & 1);
 }
 
 // One workgroup: 32 query rows of a KV head against R_k and S, wave w their rows [32 w, 32 w + 32), as products of bf16
 // terms: a bf16 query is one, any other three, the matrices three; what is left out is 2^-24 of a product.
+//
+// A few workgroups that run once: what they wait for is memory and their own instructions, so the matrices come in all
+// at once, past the registers, and the loops stay rolled (unrolled, each of ~2500 instructions was a trip to memory: 11 us).
 template <int NQ>
 __global__ __launch_bounds__(256) void prep_kernel(PrepArgs a) {
-    __shared__ uint4 s_f[2][32 * 16];  // [row][chunk], chunks xor-swizzled by the row
+    // the matrices' 16-byte chunks are xor-swizzled by the row, those of the operands too
+    __shared__ uint4 s_m[2][128 * 32];
+    __shared__ uint4 s_f[2][32 * 16];  // [row][chunk]
     __shared__ float s_top[4][32], s_sum[4][32];
-    const int blk = blockIdx.x, kv = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = lane & 31, h = lane >> 5;
+    const int blk = blockIdx.x, kv = blockIdx.y, lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mats = a.s ? 2 : 1;
+#pragma unroll 1
+    for (int i = wave; i < mats * 64; i += 4) {  // 64 chunks, two rows, a time
+        const int at = (i & 63) * 64 + lane, row = at >> 5;
+        const float* const m = i < 64 ? a.rk : a.s;
+        load_lds16(m + row * D + 4 * ((at & 31) ^ (row & 31)), &s_m[i >> 6][(i & 63) * 64]);
+    }
     const int b = kv / a.kv_heads, kvh = kv - b * a.kv_heads, group = a.q_heads / a.kv_heads;
     const int row = 32 * blk + r;
     const bool live = row < a.rows;
     const int g = live ? row / a.T : 0, t = live ? row - g * a.T : 0;
     const int64_t at = b * a.q_sb + (int64_t)(kvh * group + g) * a.q_sh + (int64_t)t * a.q_st + 8 * h;
-    const float* const m0 = a.rk + (32 * wave + r) * D + 8 * h;
-    const float* const m1 = a.s ? a.s + (32 * wave + r) * D + 8 * h : m0;
-
-    f32x16 acc[2] = {zero16(), zero16()};
+    Frag q[8][NQ];
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-        float x[8];
-        Frag q[NQ], m[3];
         if constexpr (NQ == 1) {
-            __builtin_memcpy(&q[0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);
-            if (!live) q[0].q = make_uint4(0u, 0u, 0u, 0u);
+            __builtin_memcpy(&q[s][0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);
+            if (!live) q[s][0].q = make_uint4(0u, 0u, 0u, 0u);
         } else {
+            float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = live ? query_element(a, at + 16 * s + e) : 0.0f;
-            split_terms<NQ>(x, q);
+            split_terms<NQ>(x, q[s]);
         }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the matrices, ahead of the barrier
+    __syncthreads();
+    // this lane: row r's dims 32 wave + 8 j + 4 h + (0..3) of both
+    f32x16 acc[2] = {zero16(), zero16()};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (k == 1 && !a.s) break;
-            const float4* p = reinterpret_cast<const float4*>((k ? m1 : m0) + 16 * s);
-            const float4 u = p[0], v = p[1];
-            const float e[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    for (int k = 0; k < 2; ++k) {
+        if (k == 1 && mats == 1) break;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            float e[8];
+            __builtin_memcpy(e, &s_m[k][(32 * wave + r) * 32 + ((4 * s + 2 * h) ^ r)], 16);
+            __builtin_memcpy(e + 4, &s_m[k][(32 * wave + r) * 32 + ((4 * s + 2 * h + 1) ^ r)], 16);
+            Frag m[3];
             split_terms<3>(e, m);
 #pragma unroll
             for (int i = 2; i >= 0; --i)
 #pragma unroll
                 for (int j = NQ - 1; j >= 0; --j)
-                    if (i + j <= 2) acc[k] = mfma_bf16(m[i], q[j], acc[k]);
+                    if (i + j <= 2) acc[k] = mfma_bf16(m[i], q[s][j], acc[k]);
         }
     }
-    // this lane: row r's dims 32 wave + 8 j + 4 h + (0..3)
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         acc[1][i] *= QJL_SCALE;
-        top = fmaxf(top, fmaxf(fabsf(acc[0][i]), a.s ? fabsf(acc[1][i]) : 0.0f));
+        top = fmaxf(top, fmaxf(fabsf(acc[0][i]), fabsf(acc[1][i])));
     }
     top = fmaxf(top, __shfl_xor(top, 32));
     if (h == 0) s_top[wave][r] = top;
@@ -293,34 +300,32 @@ __global__ __launch_bounds__(256) void prep_kernel(PrepArgs a) {
     int e = 0;
     if (top > 0.0f && top < __builtin_inff()) e = std::min(126, 7 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFF));
     const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    uint16_t* const f0 = reinterpret_cast<uint16_t*>(s_f[0]);
-    uint16_t* const f1 = reinterpret_cast<uint16_t*>(s_f[1]);
     float sum = 0.0f;
+    const int log_st = a.key_bits == 4 ? 1 : a.key_bits == 2 ? 2 : 3;
+    auto put = [&](int m, int p, uint32_t x) {
+        reinterpret_cast<uint16_t*>(s_f[m])[r * 128 + (((p >> 3) ^ (r & 15)) << 3) + (p & 7)] = (uint16_t)x;
+    };
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int j = 32 * wave + 8 * (i >> 2) + 4 * h + (i & 3);
-        int p = position_of(a.key_bits, j);
-        f0[r * 128 + (((p >> 3) ^ (r & 15)) << 3) + (p & 7)] = (uint16_t)tq::f32_to_f16(acc[0][i] * up);
-        if (a.s) {
-            const uint32_t x = tq::f32_to_f16(acc[1][i] * up);
-            sum += tq::f16_to_f32(x);
-            p = position_of(0, j);
-            f1[r * 128 + (((p >> 3) ^ (r & 15)) << 3) + (p & 7)] =
-                (uint16_t)tq::f32_to_f16(tq::f16_to_f32(x) * (float)(128 >> (j & 7)));
-        }
+        put(0, position_of(log_st, j), tq::f32_to_f16(acc[0][i] * up));
+        const float x = tq::f16_to_f32(tq::f32_to_f16(acc[1][i] * up));
+        sum += x;
+        put(1, sign_position_of(j), tq::f32_to_f16(x * (float)(128 >> (j & 7))));
     }
     sum += __shfl_xor(sum, 32);
     if (h == 0) s_sum[wave][r] = sum;
     __syncthreads();
     const int64_t out = (int64_t)kv * gridDim.x + blk;
     if (threadIdx.x < 32) {
-        // what the scores' fma takes from a set-bit product in units of 2^-17 to a sign's
+        // what the scores take from the set bits' products, in units of 2^-17, to the signs'
         const float all = s_sum[0][r] + s_sum[1][r] + s_sum[2][r] + s_sum[3][r];
         a.row_c[out * 64 + r] = a.c2 * __uint_as_float((uint32_t)(127 - e) << 23);
         a.row_c[out * 64 + 32 + r] = -0x1p-18f * all;
     }
     uint4* const frags = a.frags + out * 2 * 8 * 64;
-    for (int i = threadIdx.x; i < (a.s ? 2 : 1) * 512; i += 256) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < mats * 512; i += 256) {
         const int m = i >> 9, s = (i >> 6) & 7, l = i & 63;
         frags[i] = s_f[m][(l & 31) * 16 + ((2 * s + (l >> 5)) ^ (l & 15))];
     }
@@ -359,221 +364,13 @@ __device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int T, int
     return mask;
 }
 
-// Of one value to each token: those of the tokens 32 t + 8 j + 4 h + (0..3).
-__device__ __forceinline__ f32x4 norms4(const float* n, int t, int j, int h) {
-    return *reinterpret_cast<const f32x4*>(n + 32 * t + 8 * j + 4 * h);
-}
-
 // The tokens of a tile that a node attends to, as bits: those of the history (the first `to_end` of the tile, none
 // if it is negative), the nodes behind it that `sees` names, and none from `left` on.
-__device__ __forceinline__ uint64_t seen_of_tile(uint64_t sees, int to_end, int left) {
-    const uint64_t nodes = to_end >= TK || to_end <= -TK ? 0ull : to_end >= 0 ? sees << to_end : sees >> -to_end;
-    const uint64_t history = to_end >= TK ? ~0ull : to_end <= 0 ? 0ull : (1ull << to_end) - 1;
-    return (nodes | history) & (left >= TK ? ~0ull : (1ull << left) - 1);
+__device__ __forceinline__ uint32_t seen_of_tile(uint64_t sees, int to_end, int left) {
+    const uint64_t nodes = to_end >= TK || to_end <= -64 ? 0ull : to_end >= 0 ? sees << to_end : sees >> -to_end;
+    const uint64_t history = to_end <= 0 ? 0ull : (1ull << std::min(to_end, TK)) - 1;
+    return (uint32_t)((nodes | history) & ((1ull << std::min(left, TK)) - 1));
 }
-
-template <int KB, int VB, bool QJL>
-__global__ __launch_bounds__(256, QJL ? 1 : 2) void tree_kernel(TreeArgs a) {
-    __shared__ uint4 s_k[TK * 16];
-    __shared__ uint4 s_s[QJL ? TK * 16 : 1];
-    __shared__ uint4 s_v[TK * 16];
-    __shared__ __align__(16) float s_kn[TK], s_rn[TK], s_vn[TK];
-    __shared__ float s_vtop;
-    __shared__ uint64_t s_anc[64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 31, h = lane >> 5;
-    const int kv = blockIdx.x / a.n_split, split = blockIdx.x - kv * a.n_split;
-    const int b = kv / a.kv_heads;
-    const int blk = blockIdx.y * 4 + wave;  // this wave's 32 rows
-    const bool busy = blk < a.row_blocks;
-
-    // history [lo, end) and the nodes behind it, cut into tiles for the splits
-    const int nodes = a.parents ? a.T : 0;
-    int64_t end = a.lens ? a.lens[b] : a.n_tokens - nodes;
-    end = std::min<int64_t>(std::max<int64_t>(end, 0), a.n_tokens);
-    int64_t lo = a.starts ? a.starts[b] : 0;
-    lo = std::min<int64_t>(std::max<int64_t>(lo, 0), end);
-    const int64_t stop = std::min<int64_t>(end + nodes, a.n_tokens);
-    const int64_t tiles = (stop - lo + TK - 1) / TK, per = (tiles + a.n_split - 1) / a.n_split;
-    const int64_t t_begin = lo + std::min<int64_t>(split * per, tiles) * TK;
-    const int64_t t_end = std::min<int64_t>(lo + (split + 1) * per * TK, stop);
-
-    if (nodes && wave == 0) s_anc[lane] = ancestors(a.parents + b * a.parents_sb, a.T, lane);
-    Lut<KB> klut;
-    Lut<VB> vlut;
-    klut.load(a.key_centers);
-    vlut.load(a.value_centers);
-    Frag q[QJL ? 2 : 1][8];
-    float c = 0.0f, sign0 = 0.0f;
-    if (busy) {
-        const uint4* f = a.frags + ((int64_t)kv * a.row_blocks + blk) * 2 * 8 * 64;
-#pragma unroll
-        for (int m = 0; m < (QJL ? 2 : 1); ++m)
-#pragma unroll
-            for (int s = 0; s < 8; ++s) q[m][s].q = f[(m * 8 + s) * 64 + lane];
-        c = a.row_c[((int64_t)kv * a.row_blocks + blk) * 64 + r];
-        sign0 = a.row_c[((int64_t)kv * a.row_blocks + blk) * 64 + 32 + r];
-    }
-    __syncthreads();
-    uint64_t sees = nodes ? s_anc[(32 * blk + r) % a.T] : 0ull;
-
-    f32x16 o[4];
-#pragma unroll
-    for (int d = 0; d < 4; ++d) o[d] = zero16();
-    float top = -__builtin_inff(), sum = 0.0f;
-    // the output sums are in units of a power of two, 2^-15 of one above the largest |v| so far: weights times norm then
-    // reach up to 2^15, and fp16 keeps its 11 bits for those 2^29 times smaller
-    float unit = 0x1p-39f;
-    const uint8_t *const k8 = reinterpret_cast<const uint8_t*>(s_k), *const s8 = reinterpret_cast<const uint8_t*>(s_s),
-                  *const v8 = reinterpret_cast<const uint8_t*>(s_v);
-    const int64_t first = (int64_t)kv * a.cap;
-
-    for (int64_t t0 = t_begin; t0 < t_end; t0 += TK) {
-        __syncthreads();
-        const int left = (int)std::min<int64_t>(t_end - t0, TK);
-        {  // four threads to a token, 32 codes of each kind
-            const int tok = threadIdx.x >> 2, p = threadIdx.x & 3, u = p & 1, ph = p >> 1;
-            const int64_t slot = first + t0 + std::min(tok, left - 1);
-            uint32_t wk[KB], wv[VB], ws = 0u;
-            uint4 x[4];
-            auto put = [&](uint4* dst) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) dst[tok * 16 + ((8 * u + 2 * j + ph) ^ swizzle(tok))] = x[j];
-                __builtin_amdgcn_sched_barrier(0);  // one kind at a time: all three do not fit the registers
-            };
-            __builtin_memcpy(wk, __builtin_assume_aligned(a.k_codes + slot * (16 * KB) + 4 * KB * p, 4), 4 * KB);
-            __builtin_memcpy(wv, __builtin_assume_aligned(a.v_codes + slot * (16 * VB) + 4 * VB * p, 4), 4 * VB);
-            if constexpr (QJL) __builtin_memcpy(&ws, __builtin_assume_aligned(a.k_signs + slot * 16 + 4 * p, 4), 4);
-            expand32<KB>(wk, klut, x);
-            put(s_k);
-            expand32<VB>(wv, vlut, x);
-            put(s_v);
-            if constexpr (QJL) {
-                expand_signs(ws, x);
-                put(s_s);
-            }
-        }
-        if (wave == 0) {
-            const int64_t slot = first + t0 + std::min(lane, left - 1);
-            const float vn = lane < left ? tq::f16_to_f32(a.v_norms[slot]) : 0.0f;
-            s_kn[lane] = tq::f16_to_f32(a.k_norms[slot]);
-            if constexpr (QJL) s_rn[lane] = tq::f16_to_f32(a.k_rnorms[slot]) * 0x1p18f;
-            s_vn[lane] = vn;
-            float m = fabsf(vn) < __builtin_inff() ? fabsf(vn) : 0.0f;
-#pragma unroll
-            for (int k = 1; k < 64; k <<= 1) m = fmaxf(m, __shfl_xor(m, k));
-            if (lane == 0) s_vtop = m;
-        }
-        __syncthreads();
-        if (!busy) continue;
-
-        f32x16 s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x16 x = zero16();
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                Frag kf;
-                kf.q = *reinterpret_cast<const uint4*>(k8 + key_offset(ks, lane) + 32 * 256 * t);
-                x = mfma_f16(kf, q[0][ks], x);
-            }
-            __builtin_amdgcn_sched_barrier(0);  // the reads of all sixteen steps at once do not fit the registers
-            if constexpr (QJL) {
-                f32x16 y = fill16(sign0);
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {
-                    Frag kf;
-                    kf.q = *reinterpret_cast<const uint4*>(s8 + key_offset(ks, lane) + 32 * 256 * t);
-                    y = mfma_f16(kf, q[1][ks], y);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x4 kn = norms4(s_kn, t, j, h), rn = norms4(s_rn, t, j, h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[t][4 * j + e] = __builtin_fmaf(y[4 * j + e], rn[e], x[4 * j + e] * kn[e]);
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x4 kn = norms4(s_kn, t, j, h);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[t][4 * j + e] = x[4 * j + e] * kn[e];
-                }
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (t0 + TK > end || left < TK) {  // uniform: drafted tokens, or none
-            const uint64_t allowed = seen_of_tile(sees, (int)std::max<int64_t>(std::min<int64_t>(end - t0, TK), -TK), left);
-            const uint32_t word[2] = {(uint32_t)allowed >> (4 * h), (uint32_t)(allowed >> 32) >> (4 * h)};
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (!(word[t] & (1u << (8 * (i >> 2) + (i & 3))))) s[t][i] = -__builtin_inff();
-        }
-        float mx = top;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float safe = mx == -__builtin_inff() ? 0.0f : mx;
-        float new_unit = unit;
-        if (s_vtop > 0x1p15f * unit)
-            new_unit = 0x1p-15f * __uint_as_float((__float_as_uint(s_vtop) & 0x7F800000u) + 0x00800000u);
-        if (__any(mx > top) || new_unit != unit) {
-            const float corr = exp2_(__builtin_fmaf(top, c, -safe * c));
-            sum *= corr;
-            const float oc = corr * (unit / new_unit);
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= oc;
-            unit = new_unit;
-        }
-        top = mx;
-        const float base = safe * c, inv_unit = 1.0f / unit;
-        Frag pf[4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 vn = norms4(s_vn, t, j, h);
-                float w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = exp2_(__builtin_fmaf(s[t][4 * j + e], c, -base));
-                    sum += p;
-                    const float x = p * (vn[e] * inv_unit);
-                    w[e] = p == 0.0f ? 0.0f : x;  // a left-out token's norm may be anything
-                }
-                pf[2 * t + (j >> 1)].u[2 * (j & 1)] = pack_f16(w[0], w[1]);
-                pf[2 * t + (j >> 1)].u[2 * (j & 1) + 1] = pack_f16(w[2], w[3]);
-            }
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                Frag vf;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) vf.t[e] = read_tr(v8 + value_offset(d, e, lane) + 16 * 256 * ks);
-                o[d] = mfma_f16(vf, pf[ks], o[d]);
-            }
-    }
-    const int row = 32 * blk + r;
-    sum += __shfl_xor(sum, 32);
-    if (!busy || row >= a.rows) return;
-    const int64_t at = ((int64_t)split * (gridDim.x / a.n_split) + kv) * a.rows + row;
-    if (h == 0) a.part_ms[at] = make_float2(top == -__builtin_inff() ? top : top * c, sum);
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<float4*>(a.part_o + at * D + 32 * d + 8 * j + 4 * h) =
-                make_float4(o[d][4 * j] * unit, o[d][4 * j + 1] * unit, o[d][4 * j + 2] * unit, o[d][4 * j + 3] * unit);
-}
-
-// ---- few rows: a wave's tile is its own
 
 // Pairs of value codes looked up in LDS: entry e of the table is the pair (or the two pairs) that the byte e of the
 // packed codes holds, 256 bytes to an entry: 32 copies of the first pair, one for each lane of a half wave, so that no two
@@ -596,10 +393,10 @@ struct PairTable {
         const uint32_t off = perm(w, lane4, 0x0C0C0000u | (uint32_t)(4 + k) << 8);
         return *reinterpret_cast<const uint32_t*>(table + off + (second ? SECOND : 0));
     }
-    // pairs 8 g + (0..7) of 64 codes (2 VB words), in the order of their dims
+    // pairs 8 g + (0..7) of 32 codes (VB words), in the order of their dims
     static __device__ __forceinline__ void look_up(const uint8_t* t, const uint32_t* w, uint32_t lane4, int g, uint32_t* out) {
         if constexpr (VB == 3) {
-            auto moved = [&](int i) { return i < 5 ? __builtin_amdgcn_alignbit(w[i + 1], w[i], 4) : w[i] >> 4; };
+            auto moved = [&](int i) { return i + 1 < VB ? __builtin_amdgcn_alignbit(w[i + 1], w[i], 4) : w[i] >> 4; };
 #pragma unroll
             for (int k = 0; k < 2; ++k) {  // 8 codes in 3 bytes
                 const int at0 = 3 * (2 * g + k);
@@ -620,23 +417,24 @@ struct PairTable {
     }
 };
 
-// Up to 32 RB rows of a KV head, all of them in every wave; the waves take the tiles of 32 tokens in turn.  A lane is a
-// token and half of its dims: the keys' codes and signs become its A operands in registers, the values' go through 8 KB of
-// LDS of the wave's own.  No barrier until the waves' sums meet at the end.
+// 32 RB rows of a KV head to a workgroup, all of them in every wave; the waves take the tiles of 32 tokens in turn.  A lane
+// is a token and half of its dims: the keys' codes and signs become its A operands in registers; the values' codes go,
+// 16 tokens at a time, through 4 KB of LDS of the wave's own.  No barrier until the waves' sums meet at the end.
 template <int RB>
-struct Narrow {
-    static constexpr int W = RB == 1 ? 8 : 4;
+struct Tree {
+    static constexpr int W = 8;
     static constexpr int T = 64 * W;
     struct Tiles {
         uint32_t table[256 * 64];
-        uint4 v[W][32 * 16];
-        uint4 qs[8 * 64];  // the rows' sign operands: beside those of the codes they do not fit the registers
+        uint4 v[W][16 * 16];
+        // the rows' operands for the signs, and with two blocks of rows those for the codes: they do not fit the registers
+        uint4 qs[RB][8 * 64], qc[RB == 1 ? 1 : RB][RB == 1 ? 1 : 8 * 64];
         uint16_t kn[W][32], vn[W][32];
-        float rn[W][32];
+        float ratio[W][32];
     };
     struct Sums {
-        float4 o[W][32 * RB][32];  // chunks xor-swizzled by the row
-        float2 ms[W][32 * RB];
+        float4 o[W][32][32];  // chunks xor-swizzled by the row
+        float2 ms[W][32];
         float unit[W];
     };
     union Lds {
@@ -646,9 +444,9 @@ struct Narrow {
 };
 
 template <int KB, int VB, bool QJL, int RB>
-__global__ __launch_bounds__(Narrow<RB>::T, RB == 1 ? 2 : 1) void tree_narrow_kernel(TreeArgs a) {
-    using N = Narrow<RB>;
-    constexpr int W = N::W, NT = 32;  // tokens of a tile
+__global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
+    using N = Tree<RB>;
+    constexpr int W = N::W;
     __shared__ typename N::Lds lds;
     __shared__ uint64_t s_anc[64];
     __shared__ float s_centers[1 << VB];
@@ -663,49 +461,60 @@ __global__ __launch_bounds__(Narrow<RB>::T, RB == 1 ? 2 : 1) void tree_narrow_ke
     int64_t lo = a.starts ? a.starts[b] : 0;
     lo = std::min<int64_t>(std::max<int64_t>(lo, 0), end);
     const int64_t stop = std::min<int64_t>(end + nodes, a.n_tokens);
-    const int64_t tiles = (stop - lo + NT - 1) / NT;
-    const int64_t first_tile = tiles * split / a.n_split, last_tile = tiles * (split + 1) / a.n_split;
+    const uint32_t tiles = (uint32_t)((stop - lo + TK - 1) / TK), each = tiles / a.n_split, more = tiles - each * a.n_split;
+    const int64_t first_tile = split * each + std::min<uint32_t>(split, more), last_tile = first_tile + each + ((uint32_t)split < more);
 
     if (threadIdx.x < (1 << VB)) s_centers[threadIdx.x] = a.value_centers[threadIdx.x];
     if (nodes && wave == 0) s_anc[lane] = ancestors(a.parents + b * a.parents_sb, a.T, lane);
 
-    // a lane's part of a tile, on its way
-    struct Raw {
-        uint32_t k[2 * KB], v[2 * VB], s[2];
-        uint16_t kn, rn, vn;
-    };
-    // a tile's arrays at scalar addresses, a lane's place in them as 32-bit offsets
-    auto load = [&](Raw& w, int64_t tile) {
-        const int64_t t0 = lo + tile * NT, slot = (int64_t)kv * a.cap + t0;
-        const uint32_t tok = std::min<uint32_t>(r, (uint32_t)std::min<int64_t>(stop - t0, NT) - 1);
-        __builtin_memcpy(w.k, __builtin_assume_aligned(a.k_codes + slot * (16 * KB) + (tok * (16 * KB) + 8 * KB * h), 8), 8 * KB);
-        __builtin_memcpy(w.v, __builtin_assume_aligned(a.v_codes + slot * (16 * VB) + (tok * (16 * VB) + 8 * VB * h), 8), 8 * VB);
+    // a lane's part of a tile, on its way: half of token r's key codes and signs and its norms, and a quarter of the value
+    // codes of tokens lane % 16 and lane % 16 + 16.  The arrays are at scalar addresses, a lane's place in them 32-bit
+    // offsets; tokens past the last are copies of it, left out by the mask
+    uint32_t wk[2 * KB], ws[2], wv[2][VB];
+    uint16_t kn, rn = 0, vn;
+    auto load_keys = [&](int64_t tile) {
+        const int64_t t0 = lo + tile * TK, slot = (int64_t)kv * a.cap + t0;
+        const uint32_t tok = std::min<uint32_t>(r, (uint32_t)std::min<int64_t>(stop - t0, TK) - 1);
+        __builtin_memcpy(wk, __builtin_assume_aligned(a.k_codes + slot * (16 * KB) + (tok * (16 * KB) + 8 * KB * h), 8), 8 * KB);
         if constexpr (QJL) {
-            __builtin_memcpy(w.s, __builtin_assume_aligned(a.k_signs + slot * 16 + (tok * 16 + 8 * h), 8), 8);
-            w.rn = (a.k_rnorms + slot)[tok];
+            __builtin_memcpy(ws, __builtin_assume_aligned(a.k_signs + slot * 16 + (tok * 16 + 8 * h), 8), 8);
+            rn = (a.k_rnorms + slot)[tok];
         }
-        w.kn = (a.k_norms + slot)[tok], w.vn = (a.v_norms + slot)[tok];
+        kn = (a.k_norms + slot)[tok], vn = (a.v_norms + slot)[tok];
     };
-    Raw raw;
+    auto load_values = [&](int64_t tile) {
+        const int64_t t0 = lo + tile * TK, slot = (int64_t)kv * a.cap + t0;
+        const uint32_t last = (uint32_t)std::min<int64_t>(stop - t0, TK) - 1;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t tok = std::min<uint32_t>((lane & 15) + 16 * x, last);
+            __builtin_memcpy(wv[x], __builtin_assume_aligned(a.v_codes + slot * (16 * VB) + (tok * (16 * VB) + 4 * VB * (lane >> 4)), 4),
+                             4 * VB);
+        }
+    };
     int64_t tile = first_tile + wave;
-    if (tile < last_tile) load(raw, tile);
+    if (tile < last_tile) load_keys(tile), load_values(tile);
 
     Lut<KB> klut;
     klut.load(a.key_centers);
-    Frag q[RB][8];
+    Frag q[8];  // with one block of rows
     float c[RB], sign0[RB];
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
         const int blk = std::min((int)blockIdx.y * RB + m, a.row_blocks - 1);
         const int64_t at = (int64_t)kv * a.row_blocks + blk;
         const uint4* f = a.frags + at * 2 * 8 * 64;
+        if constexpr (RB == 1) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s) q[m][s].q = f[s * 64 + lane];
-        if constexpr (QJL)
-            for (int i = threadIdx.x; i < 8 * 64; i += N::T) lds.t.qs[i] = f[8 * 64 + i];
+            for (int s = 0; s < 8; ++s) q[s].q = f[s * 64 + lane];
+        } else {
+            lds.t.qc[m][threadIdx.x] = f[threadIdx.x];
+        }
+        if constexpr (QJL) lds.t.qs[m][threadIdx.x] = f[8 * 64 + threadIdx.x];
         c[m] = a.row_c[at * 64 + r];
         sign0[m] = QJL ? a.row_c[at * 64 + 32 + r] : 0.0f;
     }
+    static_assert(N::T == 8 * 64, "a thread copies one fragment of each kind");
     __syncthreads();
     PairTable<VB>::build(lds.t.table, s_centers, N::T);
     uint64_t sees[RB];
@@ -728,55 +537,69 @@ __global__ __launch_bounds__(Narrow<RB>::T, RB == 1 ? 2 : 1) void tree_narrow_ke
     const uint8_t* const table = reinterpret_cast<const uint8_t*>(lds.t.table);
     uint8_t* const v8 = reinterpret_cast<uint8_t*>(lds.t.v[wave]);
 
-    auto step = [&](Raw& w, int64_t tile, auto nodes_here) {
-        const int64_t t0 = lo + tile * NT;
-        const int left = (int)std::min<int64_t>(stop - t0, NT);
-        // ---- values to LDS, eight dims at a time
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            uint32_t x[8];
-            PairTable<VB>::look_up(table, w.v, lane4, g, x);
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                *reinterpret_cast<uint4*>(v8 + r * 256 + (((8 * h + 2 * g + j) ^ swizzle(r)) << 4)) =
-                    make_uint4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
-        }
-        const uint32_t norm = !nodes_here || r < left ? w.vn : 0u;  // tokens past the last weigh nothing
+    auto step = [&](int64_t tile, auto nodes_here) {
+        const int64_t t0 = lo + tile * TK;
+        const int left = (int)std::min<int64_t>(stop - t0, TK);
+        const uint32_t norm = !nodes_here || r < left ? vn : 0u;  // tokens past the last weigh nothing
         if (h == 0) {
-            lds.t.kn[wave][r] = w.kn;
+            // a key's norm that fp16 holds as 0 counts as 2^-24, its least
+            const uint16_t k = QJL && (kn & 0x7FFFu) == 0 ? 1 : kn;
+            lds.t.kn[wave][r] = k;
             lds.t.vn[wave][r] = (uint16_t)norm;
-            if constexpr (QJL) lds.t.rn[wave][r] = tq::f16_to_f32(w.rn) * 0x1p18f;
+            // |r| / |k|, in the units of the sign products
+            if constexpr (QJL) lds.t.ratio[wave][r] = tq::f16_to_f32(rn) * 0x1p18f / tq::f16_to_f32(k);
         }
-        // ---- scores
-        f32x16 x[RB], y[RB];
+        // ---- scores: |k| (<codes> + |r| / |k| <signs>), the sign products' sums going into the codes'
+        f32x16 x[RB];
 #pragma unroll
-        for (int m = 0; m < RB; ++m) x[m] = zero16(), y[m] = fill16(sign0[m]);
+        for (int m = 0; m < RB; ++m) x[m] = zero16();
+        if constexpr (QJL) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            uint4 f[4];
-            expand32<KB>(w.k + KB * u, klut, f);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                Frag kf;
-                kf.q = f[j];
-#pragma unroll
-                for (int m = 0; m < RB; ++m) x[m] = mfma_f16(kf, q[m][4 * u + j], x[m]);
-            }
-            if constexpr (QJL) {
-                expand_signs(w.s[u], f);
+            for (int u = 0; u < 2; ++u) {
+                uint4 f[4];
+                expand_signs(ws[u], f);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     Frag kf, qf;
                     kf.q = f[j];
-                    qf.q = lds.t.qs[(4 * u + j) * 64 + lane];
 #pragma unroll
-                    for (int m = 0; m < RB; ++m) y[m] = mfma_f16(kf, qf, y[m]);
+                    for (int m = 0; m < RB; ++m) {
+                        qf.q = lds.t.qs[m][(4 * u + j) * 64 + lane];
+                        x[m] = mfma_f16(kf, qf, x[m]);
+                    }
+                }
+                if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);  // the registers hold a few operands at a time
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const f32x4 r4 = *reinterpret_cast<const f32x4*>(&lds.t.ratio[wave][8 * j + 4 * h]);
+#pragma unroll
+                for (int m = 0; m < RB; ++m)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[m][4 * j + e] = (x[m][4 * j + e] + sign0[m]) * r4[e];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            uint4 f[4];
+            expand32<KB>(wk + KB * u, klut, f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                Frag kf, qf;
+                kf.q = f[j];
+#pragma unroll
+                for (int m = 0; m < RB; ++m) {
+                    if constexpr (RB > 1) qf.q = lds.t.qc[m][(4 * u + j) * 64 + lane];
+                    x[m] = mfma_f16(kf, RB > 1 ? qf : q[4 * u + j], x[m]);
                 }
             }
+            if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);
         }
         // the largest finite |v| of the tile: its exponent decides the unit (2^(e + 1) is above it)
         const int e5 = (norm >> 10) & 31, ve = e5 == 31 ? 0 : e5;
-        int need = 0;  // uniform: a token whose exponent the unit does not cover
+        int need = 0;  // uniform: by how much the unit has to rise
         if (__any(ve > 14 + TOP_BIT - shift)) {
             int e = ve;
 #pragma unroll
@@ -784,37 +607,29 @@ __global__ __launch_bounds__(Narrow<RB>::T, RB == 1 ? 2 : 1) void tree_narrow_ke
             need = shift - (14 + TOP_BIT - std::max(__builtin_amdgcn_readfirstlane(e), 1));
         }
         shift -= need;
-        if (tile + W < last_tile) load(w, tile + W);
+        if (tile + W < last_tile) load_keys(tile + W);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         Frag pf[RB][2];
 #pragma unroll
         for (int m = 0; m < RB; ++m) {
-            f32x16 s;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const f16x4 k4 = *reinterpret_cast<const f16x4*>(&lds.t.kn[wave][8 * j + 4 * h]);
-                if constexpr (QJL) {
-                    const f32x4 r4 = *reinterpret_cast<const f32x4*>(&lds.t.rn[wave][8 * j + 4 * h]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[4 * j + e] = __builtin_fmaf((float)k4[e], x[m][4 * j + e], r4[e] * y[m][4 * j + e]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[4 * j + e] = (float)k4[e] * x[m][4 * j + e];
-                }
+                for (int e = 0; e < 4; ++e) x[m][4 * j + e] = __builtin_fmaf((float)k4[e], x[m][4 * j + e], 0.0f);
             }
             if constexpr (nodes_here) {
-                const int to_end = (int)std::max<int64_t>(std::min<int64_t>(end - t0, TK), -TK);
-                const uint32_t word = (uint32_t)seen_of_tile(sees[m], to_end, left) >> (4 * h);
+                const int to_end = (int)std::max<int64_t>(std::min<int64_t>(end - t0, TK), -64);
+                const uint32_t word = seen_of_tile(sees[m], to_end, left) >> (4 * h);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (!(word & (1u << (8 * (i >> 2) + (i & 3))))) s[i] = -__builtin_inff();
+                    if (!(word & (1u << (8 * (i >> 2) + (i & 3))))) x[m][i] = -__builtin_inff();
             }
-            float mx = s[0];
+            float mx = x[m][0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-            // both halves of the row see the same, and neither -inf nor NaN raises the reference
+            for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[m][i]);
+            // neither -inf nor NaN raises the reference
             if (__any(__builtin_fmaf(mx, c[m], -top[m]) > LAZY) || need) {
                 mx = fmaxf(mx, __shfl_xor(mx, 32)) * c[m];
                 const float ref = mx > top[m] ? mx : top[m];
@@ -833,79 +648,93 @@ __global__ __launch_bounds__(Narrow<RB>::T, RB == 1 ? 2 : 1) void tree_narrow_ke
                 float p[4], wt[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    p[e] = exp2_(__builtin_fmaf(s[4 * j + e], c[m], base));
+                    p[e] = exp2_(__builtin_fmaf(x[m][4 * j + e], c[m], base));
                     sum[m] += p[e];
-                    wt[e] = p[e] * (float)v4[e];
+                    wt[e] = __builtin_fmaf((float)v4[e], p[e], 0.0f);
                     if constexpr (nodes_here) wt[e] = p[e] == 0.0f ? 0.0f : wt[e];  // a left-out token's norm may be anything
                 }
                 pf[m][j >> 1].u[2 * (j & 1)] = pack_f16(wt[0], wt[1]);
                 pf[m][j >> 1].u[2 * (j & 1) + 1] = pack_f16(wt[2], wt[3]);
             }
+            if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);
         }
+        // ---- values, 16 tokens at a time: lane (token lane % 16, quarter lane / 16 of its dims), then V^T
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
+        for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                uint32_t y[8];
+                PairTable<VB>::look_up(table, wv[ks], lane4, g, y);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    *reinterpret_cast<uint4*>(v8 + (lane & 15) * 256 + (((4 * (lane >> 4) + 2 * g + j) ^ swizzle(lane & 15)) << 4)) =
+                        make_uint4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (ks == 1 && tile + W < last_tile) load_values(tile + W);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 Frag vf;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) vf.t[e] = read_tr(v8 + value_offset(d, e, lane) + 16 * 256 * ks);
+                for (int e = 0; e < 2; ++e) vf.t[e] = read_tr(v8 + value_offset(d, e, lane));
 #pragma unroll
                 for (int m = 0; m < RB; ++m) o[m][d] = mfma_f16(vf, pf[m][ks], o[m][d]);
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
     };
     // whole tiles of the history, then those with the end of it or drafted tokens in them
-    const int64_t whole = std::min(last_tile, (end - lo) / NT);
-    for (; tile < whole; tile += W) step(raw, tile, std::false_type{});
-    for (; tile < last_tile; tile += W) step(raw, tile, std::true_type{});
+    const int64_t whole = std::min(last_tile, (end - lo) / TK);
+    for (; tile < whole; tile += W) step(tile, std::false_type{});
+    for (; tile < last_tile; tile += W) step(tile, std::true_type{});
 
-    // ---- the waves' sums
-    __syncthreads();
+    // ---- the waves' sums, one block of rows at a time
     const float unit = __uint_as_float((uint32_t)(127 - shift) << 23);
+    const int64_t heads = gridDim.x / a.n_split;
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
+        __syncthreads();
         const float all = sum[m] + __shfl_xor(sum[m], 32);
-        if (h == 0)
-            lds.s.ms[wave][32 * m + r] = make_float2(top[m], all * unit);
+        if (h == 0) lds.s.ms[wave][r] = make_float2(top[m], all * unit);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                lds.s.o[wave][32 * m + r][(8 * d + 2 * j + h) ^ r] =
+                lds.s.o[wave][r][(8 * d + 2 * j + h) ^ r] =
                     make_float4(o[m][d][4 * j], o[m][d][4 * j + 1], o[m][d][4 * j + 2], o[m][d][4 * j + 3]);
-    }
-    if (lane == 0) lds.s.unit[wave] = unit;
-    __syncthreads();
-    const int64_t heads = gridDim.x / a.n_split;
-    for (int i = threadIdx.x; i < 32 * RB * 32; i += N::T) {
-        const int row = i >> 5, ch = i & 31, out_row = (int)blockIdx.y * 32 * RB + row;
-        if (out_row >= a.rows) continue;
-        float best = -__builtin_inff();
+        if (lane == 0) lds.s.unit[wave] = unit;
+        __syncthreads();
+        for (int i = threadIdx.x; i < 32 * 32; i += N::T) {
+            const int row = i >> 5, ch = i & 31, out_row = 32 * ((int)blockIdx.y * RB + m) + row;
+            if (out_row >= a.rows) continue;
+            float best = -__builtin_inff();
 #pragma unroll
-        for (int k = 0; k < W; ++k) best = fmaxf(best, lds.s.ms[k][row].x);
-        const float safe = best == -__builtin_inff() ? 0.0f : best;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float den = 0.0f;
+            for (int k = 0; k < W; ++k) best = fmaxf(best, lds.s.ms[k][row].x);
+            const float safe = best == -__builtin_inff() ? 0.0f : best;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float den = 0.0f;
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-            const float2 ms = lds.s.ms[k][row];
-            const float w = exp2_(ms.x - safe), wu = w * lds.s.unit[k];
-            const float4 y = lds.s.o[k][row][ch ^ (row & 31)];
-            den = __builtin_fmaf(w, ms.y, den);
-            x.x = __builtin_fmaf(wu, y.x, x.x), x.y = __builtin_fmaf(wu, y.y, x.y);
-            x.z = __builtin_fmaf(wu, y.z, x.z), x.w = __builtin_fmaf(wu, y.w, x.w);
+            for (int k = 0; k < W; ++k) {
+                const float2 ms = lds.s.ms[k][row];
+                const float w = exp2_(ms.x - safe), wu = w * lds.s.unit[k];
+                const float4 y = lds.s.o[k][row][ch ^ row];
+                den = __builtin_fmaf(w, ms.y, den);
+                x.x = __builtin_fmaf(wu, y.x, x.x), x.y = __builtin_fmaf(wu, y.y, x.y);
+                x.z = __builtin_fmaf(wu, y.z, x.z), x.w = __builtin_fmaf(wu, y.w, x.w);
+            }
+            const int64_t at = ((int64_t)split * heads + kv) * a.rows + out_row;
+            reinterpret_cast<float4*>(a.part_o + at * D)[ch] = x;
+            if (ch == 0) a.part_ms[at] = make_float2(best, den);
         }
-        const int64_t at = ((int64_t)split * heads + kv) * a.rows + out_row;
-        reinterpret_cast<float4*>(a.part_o + at * D)[ch] = x;
-        if (ch == 0) a.part_ms[at] = make_float2(best, den);
     }
 }
 
 // ------------------------------------------------------------------ merge
 
 struct MergeArgs {
-    int q_heads, kv_heads, T, rows, n_split, value_bits;  // value_bits: the order of the partials' dims, 0 their own
+    int q_heads, kv_heads, T, rows, n_split;
     int64_t all_rows;  // of all KV heads
     const float* part_o;
     const float2* part_ms;
@@ -921,20 +750,27 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     __shared__ float s_w[8][MAX_SPLIT];
     __shared__ float s_den[8];
     __shared__ __align__(16) float s_o[8][D];
-    __shared__ float s_half[8][D];
+    __shared__ float s_half[2][8][D];
     const int64_t row0 = (int64_t)blockIdx.x * 8;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int j = threadIdx.x & 127, half = threadIdx.x >> 7;
     float m[64];
 #pragma unroll
     for (int d = 0; d < 64; ++d) m[d] = a.rv[(64 * half + d) * D + j];
-    auto place = [&](int64_t row) {  // of a row in [batch][q heads][T]
-        const int64_t kv = row / a.rows;
-        const int in = (int)(row - kv * a.rows), g = in / a.T, t = in - g * a.T;
-        const int64_t b = kv / a.kv_heads, hq = (kv - b * a.kv_heads) * (a.q_heads / a.kv_heads) + g;
-        return (b * a.q_heads + hq) * a.T + t;
-    };
+    // 32 threads to a row, four dims each: the first splits' partials are on their way before the weights are known
+    constexpr int AHEAD = 8;
+    const int pk = threadIdx.x >> 5, pc = threadIdx.x & 31;
+    const float4* const part = reinterpret_cast<const float4*>(a.part_o + std::min(row0 + pk, a.all_rows - 1) * D) + pc;
+    const int64_t step = a.all_rows * (D / 4);
+    float4 ahead[AHEAD];
 #pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = i < a.n_split ? part[i * step] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto place = [&](int64_t row) {  // of a row in [batch][q heads][T]
+        const uint32_t n = (uint32_t)row, kv = n / (uint32_t)a.rows, in = n - kv * a.rows, g = in / (uint32_t)a.T;
+        const uint32_t b = kv / (uint32_t)a.kv_heads, hq = (kv - b * a.kv_heads) * (a.q_heads / a.kv_heads) + g;
+        return ((int64_t)b * a.q_heads + hq) * a.T + (in - g * a.T);
+    };
+#pragma unroll 1
     for (int k = wave; k < 8; k += 4) {
         const int64_t row = row0 + k;
         float2 ms = make_float2(-__builtin_inff(), 0.0f);
@@ -954,50 +790,37 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
         }
     }
     __syncthreads();
-    {  // 32 threads to a row, four dims each
-        const int k = threadIdx.x >> 5, c = threadIdx.x & 31;
-        const int64_t row = std::min(row0 + k, a.all_rows - 1);
-        const float4* p = reinterpret_cast<const float4*>(a.part_o + row * D) + c;
-        const int64_t step = a.all_rows * (D / 4);
+    {
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int i = 0; i < a.n_split; ++i) {
-            const float w = s_w[k][i];
-            const float4 x = p[i * step];
+        auto add = [&](float w, float4 x) {
             o.x = __builtin_fmaf(w, x.x, o.x), o.y = __builtin_fmaf(w, x.y, o.y);
             o.z = __builtin_fmaf(w, x.z, o.z), o.w = __builtin_fmaf(w, x.w, o.w);
-        }
-        const float den = s_den[k] == 0.0f ? 1.0f : s_den[k];
-        const float v[4] = {o.x / den, o.y / den, o.z / den, o.w / den};
+        };
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int pos = 4 * c + e;
-            s_o[k][a.value_bits ? dim_of(a.value_bits, pos >> 3, pos & 7) : pos] = v[e];
-        }
+        for (int i = 0; i < AHEAD; ++i) add(s_w[pk][i], ahead[i]);  // splits that there are not: 0 times 0
+#pragma unroll 8
+        for (int i = AHEAD; i < a.n_split; ++i) add(s_w[pk][i], part[i * step]);
+        const float den = s_den[pk] == 0.0f ? 1.0f : s_den[pk];
+        *reinterpret_cast<float4*>(&s_o[pk][4 * pc]) = make_float4(o.x / den, o.y / den, o.z / den, o.w / den);
     }
     __syncthreads();
-    float acc[8];
-#pragma unroll
+#pragma unroll 1
     for (int k = 0; k < 8; ++k) {
-        acc[k] = 0.0f;
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int d = 0; d < 64; d += 4) {
             const float4 o = *reinterpret_cast<const float4*>(&s_o[k][64 * half + d]);
-            acc[k] = __builtin_fmaf(o.x, m[d], acc[k]);
-            acc[k] = __builtin_fmaf(o.y, m[d + 1], acc[k]);
-            acc[k] = __builtin_fmaf(o.z, m[d + 2], acc[k]);
-            acc[k] = __builtin_fmaf(o.w, m[d + 3], acc[k]);
+            x[0] = __builtin_fmaf(o.x, m[d], x[0]), x[1] = __builtin_fmaf(o.y, m[d + 1], x[1]);
+            x[2] = __builtin_fmaf(o.z, m[d + 2], x[2]), x[3] = __builtin_fmaf(o.w, m[d + 3], x[3]);
         }
+        s_half[half][k][j] = (x[0] + x[1]) + (x[2] + x[3]);
     }
-    // the halves are exchanged: thread (j, half) finishes rows 4 half + (0..3)
-#pragma unroll
-    for (int k = 0; k < 4; ++k) s_half[4 * (1 - half) + k][j] = half ? acc[k] : acc[4 + k];
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t row = row0 + 4 * half + k;
-        if (row >= a.all_rows) continue;
-        const float x = (half ? acc[4 + k] : acc[k]) + s_half[4 * half + k][j];
+#pragma unroll 1
+    for (int k = half; k < 8; k += 2) {
+        const int64_t row = row0 + k;
+        if (row >= a.all_rows) break;
+        const float x = s_half[0][k][j] + s_half[1][k][j];
         const int64_t at = place(row) * D + j;
         if (a.out_f32) a.out_f32[at] = x;
         if (a.out_bf16) a.out_bf16[at] = (uint16_t)tq::f32_to_bf16(x);
@@ -1008,43 +831,35 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 struct Plan {
     int rows, row_blocks, n_split;
-    bool narrow;
+    unsigned row_groups;
     int64_t heads;
     size_t frag_bytes, row_c_bytes, ms_bytes, o_bytes;
     size_t total() const { return frag_bytes + row_c_bytes + ms_bytes + o_bytes; }
 };
 
-// Up to 64 rows of a KV head are one workgroup's, a CU's worth of waves; more are dealt to the waves of several, two to a
-// CU.  As many splits as fill the CUs, as long as none is left without a tile.
+// A workgroup fills a CU.  As many splits as fill the CUs, as long as none is left without a tile.
 bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Plan& p) {
+    const int64_t rows = (int64_t)(q_heads / kv_heads) * T;
     p.heads = (int64_t)batch * kv_heads;
-    p.rows = q_heads / kv_heads * T;
+    if (p.heads > 65535 || p.heads * rows >= (int64_t)1 << 26 || rows > 65535 * 32) return false;
+    p.rows = (int)rows;
     p.row_blocks = (p.rows + 31) / 32;
-    p.narrow = p.row_blocks <= 2;
-    const int64_t wgs = p.narrow ? p.heads * p.row_blocks : p.heads * ((p.row_blocks + 3) / 4);
-    const int64_t per_tile = p.narrow ? 32 : TK, tiles = std::max<int64_t>(1, (n_tokens + per_tile - 1) / per_tile);
-    const int64_t fill = p.narrow ? 256 / wgs : (512 + wgs - 1) / wgs;
-    int64_t n = std::max<int64_t>(1, std::min<int64_t>({fill, tiles, MAX_SPLIT}));
-    if (!p.narrow) {
-        const int64_t per = (tiles + n - 1) / n;
-        n = (tiles + per - 1) / per;
-    }
-    p.n_split = (int)n;
+    p.row_groups = p.row_blocks == 1 ? 1 : (unsigned)(p.row_blocks + 1) / 2;
+    const int64_t tiles = std::max<int64_t>(1, (n_tokens + TK - 1) / TK);
+    p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({256 / (p.heads * p.row_groups), tiles, MAX_SPLIT}));
     const int64_t all = p.heads * p.rows;
     p.frag_bytes = (size_t)(p.heads * p.row_blocks) * 2 * 8 * 64 * 16;
     p.row_c_bytes = (size_t)(p.heads * p.row_blocks) * 64 * 4;
     p.ms_bytes = ((size_t)all * p.n_split * 8 + 15) / 16 * 16;
     p.o_bytes = (size_t)all * p.n_split * D * 4;
-    return p.heads * p.n_split < ((int64_t)1 << 22) && all < ((int64_t)1 << 26) && p.heads <= 65535;
+    return true;
 }
 
 template <int KB, int VB, bool QJL>
 void launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
-    const unsigned x = (unsigned)(p.heads * p.n_split);
-    if (!p.narrow)
-        hipLaunchKernelGGL((tree_kernel<KB, VB, QJL>), dim3(x, (unsigned)((p.row_blocks + 3) / 4)), dim3(256), 0, s, a);
-    else
-        hipLaunchKernelGGL((tree_narrow_kernel<KB, VB, QJL, 1>), dim3(x, (unsigned)p.row_blocks), dim3(Narrow<1>::T), 0, s, a);
+    const dim3 grid((unsigned)(p.heads * p.n_split), p.row_groups);
+    if (p.row_blocks == 1) hipLaunchKernelGGL((tree_kernel<KB, VB, QJL, 1>), grid, dim3(Tree<1>::T), 0, s, a);
+    else hipLaunchKernelGGL((tree_kernel<KB, VB, QJL, 2>), grid, dim3(Tree<2>::T), 0, s, a);
 }
 
 }  // namespace
@@ -1072,7 +887,7 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
         !key_centers || !value_rotation || !value_centers || (has_qjl && (!k_signs || !k_rnorms || !qjl)) ||
         (!out_f32 && !out_bf16) || !(scale > 0.0f) || scale == __builtin_inff())
         return TQ_ERR_INVALID_ARGUMENT;
-    if (dim != D || nodes > TQ_MAX_NODES || value_bits < 1 || value_bits > 4 || key_bits < 1 ||
+    if (dim != D || nodes > TQ_MAX_NODES || n_tokens >= (int64_t)1 << 31 || value_bits < 1 || value_bits > 4 || key_bits < 1 ||
         key_bits != value_bits - (has_qjl ? 1 : 0))
         return TQ_ERR_UNSUPPORTED;
     if (!aligned16(key_rotation) || !aligned16(k_codes) || !aligned16(v_codes) || (has_qjl && (!aligned16(k_signs) || !aligned16(qjl))))
@@ -1106,7 +921,7 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
         else launch_tree<1, 1, false>(a, p, s);
     }
     TQ_CHECK_LAUNCH();
-    const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, p.narrow ? 0 : value_bits, p.heads * p.rows, part_o, part_ms,
+    const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, p.heads * p.rows, part_o, part_ms,
                       value_rotation, out_f32, out_bf16, lse_out};
     hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((p.heads * p.rows + 7) / 8)), dim3(256), 0, s, m);
     TQ_CHECK_LAUNCH();
