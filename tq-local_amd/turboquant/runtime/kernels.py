@@ -529,25 +529,34 @@ class DenseAttention:
 
 
 def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise ValueError(f"{name} has no backward pass: call it under torch.no_grad()")
 
 
-def _on_device(fn: str, device: torch.device, *args) -> None:
-    """The C call, made with ``device`` as the current one (a stream belongs to its device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        _lib.call(fn, *args)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _on_device(fn: str, index: int, *args) -> None:
+    """The C call with device ``index`` as the current one (a stream belongs to its device)."""
+    if index == _get_device():
+        st = getattr(_lib.load(), fn)(*args)
     else:
-        with torch.cuda.device(device):
-            _lib.call(fn, *args)
+        with torch.cuda.device(index):
+            st = getattr(_lib.load(), fn)(*args)
+    if st != _lib.TQ_OK:
+        _lib.check(fn, st)
 
 
 def _int32_on(t: torch.Tensor | None, device: torch.device, name: str, shape: tuple) -> torch.Tensor | None:
     """``t`` as a contiguous int32 tensor of ``shape`` on ``device`` (itself when it is one)."""
     if t is None:
         return None
-    if t.dtype not in (torch.int32, torch.int64) or tuple(t.shape) != shape:
+    if (t.dtype != torch.int32 and t.dtype != torch.int64) or t.shape != shape:
         raise ValueError(f"{name} must be int32 or int64 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype == torch.int32 and t.device == device and t.is_contiguous():
+        return t
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
@@ -601,9 +610,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
         lse.fill_(float("-inf"))
     q, k, v = rows16(q), rows16(k), rows16(v)
     s = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    _on_device("tq_prompt_attention", dev, _vp(q), _vp(k), _vp(v), _vp(out), _vp(lse), int(q.dtype == torch.float16), B,
-               Hq, Hkv, S, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], _vp(cu_seqlens),
-               n_seqs, _vp(seq_starts), _vp(seq_ends), int(zero_outside), s, _stream(dev))
+    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
+    _on_device("tq_prompt_attention", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
+               int(q.dtype == torch.float16), B, Hq, Hkv, S, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
+               vs[2], os[0], os[1], os[2], _ptr(cu_seqlens), n_seqs, _ptr(seq_starts), _ptr(seq_ends), int(zero_outside),
+               s, _stream_handle(dev))
     return (out, lse) if want_lse else out
 
 
@@ -643,14 +654,14 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: to
     _no_gradient("tree_attention", q)
     _require_gpu(q, k_codes, k_norms, v_codes, v_norms, k_signs, k_rnorms)
     dev = q.device
+    lead = (B, Hkv, cap)
     for name, t, row in (("k_codes", k_codes, row_bytes(D, key.bits)), ("v_codes", v_codes, row_bytes(D, value.bits)),
                          ("k_signs", k_signs, D // 8), ("k_norms", k_norms, 0), ("v_norms", v_norms, 0),
                          ("k_rnorms", k_rnorms, 0)):
-        if t is None:
-            continue
-        shape, dtype = ((B, Hkv, cap, row), torch.uint8) if row else ((B, Hkv, cap), torch.float16)
-        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"{name}: expected a contiguous {dtype} {shape} on {dev}, got {t.dtype} {tuple(t.shape)}")
+        if t is not None and (t.shape != ((*lead, row) if row else lead) or t.dtype != (torch.uint8 if row else torch.float16)
+                              or not t.is_contiguous() or t.device != dev):
+            raise ValueError(f"{name}: expected a contiguous tensor of {(*lead, row) if row else lead} on {dev}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
     nodes = 0 if parents is None else T
     if not 0 <= n_tokens <= cap or n_tokens < nodes:
         raise ValueError(f"{n_tokens} tokens, {nodes} of them drafted, of a capacity of {cap}")
@@ -672,12 +683,13 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: to
         need = _lib.load().tq_tree_attention_workspace_bytes(B, Hq, Hkv, T, D, n_tokens)
         ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=dev)
         s = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-        _on_device("tq_tree_attention", dev, _vp(q), _QUERY_TYPES[q.dtype], B, Hq, Hkv, T, D, *q.stride()[:3],
-                   _vp(parents), psb, _vp(seq_starts), _vp(seq_lens), int(n_tokens), cap, _vp(k_codes), _vp(k_norms),
-                   _vp(k_signs), _vp(k_rnorms), _vp(v_codes), _vp(v_norms), key.bits, value.bits, int(has_qjl),
-                   _vp(key.rotation), _vp(key.centers), _vp(qjl), _vp(value.rotation),
-                   _vp(attention_value_centers(value)), s, _vp(f32), _vp(out), _vp(lse), _vp(ws), ws.numel(),
-                   _stream(dev))
+        qs = q.stride()
+        _on_device("tq_tree_attention", q.get_device(), q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, T, D, qs[0], qs[1],
+                   qs[2], _ptr(parents), psb, _ptr(seq_starts), _ptr(seq_lens), int(n_tokens), cap, k_codes.data_ptr(),
+                   k_norms.data_ptr(), _ptr(k_signs), _ptr(k_rnorms), v_codes.data_ptr(), v_norms.data_ptr(), key.bits,
+                   value.bits, int(has_qjl), key.rotation.data_ptr(), key.centers.data_ptr(), _ptr(qjl),
+                   value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s, _ptr(f32), _ptr(out),
+                   _ptr(lse), ws.data_ptr(), ws.numel(), _stream_handle(dev))
     if out is None:
         out = f32 if q.dtype == torch.float32 else f32.to(q.dtype)
     outs = (out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
@@ -694,33 +706,31 @@ def _move_buffers(name: str, buffers: list[torch.Tensor]) -> tuple[int, int, int
     """(batch, heads, cap, row bytes) of a layer's [B, H, cap, ...] buffers."""
     if not buffers:
         raise ValueError(f"{name}: no buffers")
-    first = buffers[0]
-    rows = []
+    lead, dev, rows = buffers[0].shape[:3], buffers[0].get_device(), []
     for b in buffers:
-        if b.dim() < 3 or b.shape[:3] != first.shape[:3] or not b.is_contiguous() or b.device != first.device:
+        if b.shape[:3] != lead or len(lead) != 3 or b.get_device() != dev or not b.is_contiguous():
             raise ValueError(f"{name}: expected contiguous [B, H, cap, ...] buffers of one shape and device, got "
                              f"{tuple(b.shape)}")
-        rows.append(math.prod(b.shape[3:]) * b.element_size())
+        rows.append((1 if b.dim() == 3 else b.shape[3] if b.dim() == 4 else math.prod(b.shape[3:])) * b.element_size())
         if not 1 <= rows[-1] <= _MAX_ROW_BYTES:
             raise ValueError(f"{name}: {rows[-1]} bytes to a token ({_MAX_ROW_BYTES} at most)")
-    _require_gpu(*buffers)
-    return int(first.shape[0]), int(first.shape[1]), int(first.shape[2]), rows
+    if dev < 0:
+        _require_gpu(buffers[0])
+    return lead[0], lead[1], lead[2], rows
 
 
 def _token_index(name: str, index: torch.Tensor, batch: int, heads: int, device: torch.device):
     """``index`` [n], [B, n] or [B, H, n] as int32, with its strides over batch and heads."""
-    if index.dtype not in (torch.int32, torch.int64) or not 1 <= index.dim() <= 3:
-        raise ValueError(f"{name}: index must be int32 or int64 [n], [B, n] or [B, H, n]")
-    lead = (batch, heads)[:index.dim() - 1]
-    if tuple(index.shape[:-1]) != lead:
-        raise ValueError(f"{name}: index {tuple(index.shape)} does not match batch {batch}, heads {heads}")
-    index = index.to(device=device, dtype=torch.int32).contiguous()
-    n = int(index.shape[-1])
-    return index, (n * heads if index.dim() == 3 else n if index.dim() == 2 else 0), (n if index.dim() == 3 else 0), n
+    dims = index.dim()
+    if not 1 <= dims <= 3:
+        raise ValueError(f"{name}: index must be [n], [B, n] or [B, H, n]")
+    n = index.shape[-1]
+    index = _int32_on(index, device, f"{name}: index", (batch, heads)[:dims - 1] + (n,))
+    return index, (n * heads if dims == 3 else n if dims == 2 else 0), (n if dims == 3 else 0), n
 
 
 def _pointers(tensors) -> ctypes.Array:
-    return (ctypes.c_void_p * len(tensors))(*(t.data_ptr() for t in tensors))
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
 
 
 def gather_tokens(buffers: list[torch.Tensor], *, tokens: int, rows: torch.Tensor | None = None,
@@ -748,17 +758,17 @@ def gather_tokens(buffers: list[torch.Tensor], *, tokens: int, rows: torch.Tenso
     slots = n if capacity is None else int(capacity)
     if slots < n:
         raise ValueError(f"gather_tokens: {n} tokens do not fit a capacity of {slots}")
-    out = [torch.empty(R, H, slots, *b.shape[3:], dtype=b.dtype, device=dev) for b in buffers]
+    out = [b.new_empty((R, H, slots, *b.shape[3:])) for b in buffers]
     if R == 0 or H == 0 or slots == 0:
         return out
     if B == 0 or n == 0:
         return [o.zero_() for o in out]
     for a in range(0, len(buffers), _MOVE_BUFFERS):
         part = slice(a, a + _MOVE_BUFFERS)
-        count = len(buffers[part])
-        _on_device("tq_gather_tokens", dev, count, _pointers(buffers[part]), _pointers(out[part]),
-                   (ctypes.c_int * count)(*row_bytes[part]), B, H, cap, tokens, R, slots, _vp(rows), _vp(index), sb, sh,
-                   n, _stream(dev))
+        count = len(row_bytes[part])
+        _on_device("tq_gather_tokens", buffers[0].get_device(), count, _pointers(buffers[part]), _pointers(out[part]),
+                   (ctypes.c_int * count)(*row_bytes[part]), B, H, cap, tokens, R, slots, _ptr(rows), _ptr(index), sb, sh,
+                   n, _stream_handle(dev))
     return out
 
 
@@ -777,9 +787,10 @@ def keep_tokens(buffers: list[torch.Tensor], index: torch.Tensor, *, first: int,
         return
     for a in range(0, len(buffers), _MOVE_BUFFERS):
         part = slice(a, a + _MOVE_BUFFERS)
-        count = len(buffers[part])
-        _on_device("tq_keep_tokens", dev, count, _pointers(buffers[part]), (ctypes.c_int * count)(*row_bytes[part]), B,
-                   H, cap, first, tokens, _vp(index), sb, sh, n, _stream(dev))
+        count = len(row_bytes[part])
+        _on_device("tq_keep_tokens", buffers[0].get_device(), count, _pointers(buffers[part]),
+                   (ctypes.c_int * count)(*row_bytes[part]), B, H, cap, first, tokens, index.data_ptr(), sb, sh, n,
+                   _stream_handle(dev))
 
 
 def rows16(t: torch.Tensor) -> torch.Tensor:
