@@ -22,6 +22,7 @@
 // independent from weight to weight.  The sum of a row's weights is of the unrounded ones.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tq_common.h"
 
@@ -30,6 +31,9 @@ namespace {
 constexpr int D = TQ_DIM;
 constexpr int TK = 64;  // tokens per tile
 constexpr float LOG2E = 1.44269504f;
+constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's reference by
+
+constexpr int MFMA = 0x8, DS_READ = 0x100;  // kinds of instructions for the scheduler
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -67,8 +71,18 @@ __device__ __forceinline__ void load_lds16(const void* g, void* l) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g,
                                      (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
 }
-__device__ __forceinline__ s16x4 read_tr(const uint16_t* l) {
+__device__ __forceinline__ s16x4 read_tr(const uint8_t* l) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)l);
+}
+// Byte offsets in a tile: a lane's 16 bytes of key row r in step ks (plus 32 rows for the second block of tokens), and what it
+// gives ds_read_b64_tr_b16 for dims 32 d + (0..31) of the tokens 8 e + 4 h + (0..3) (plus 16 rows per step).
+__device__ __forceinline__ int key_offset(int ks, int lane) {
+    return (lane & 31) * 256 + (((2 * ks + (lane >> 5)) ^ swizzle(lane & 31)) << 4);
+}
+__device__ __forceinline__ int value_offset(int d, int e, int lane) {
+    const int tok = 8 * e + 4 * (lane >> 5) + ((lane & 15) >> 2);
+    const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    return tok * 256 + ((chunk ^ swizzle(tok)) << 4) + 8 * (lane & 1);
 }
 
 struct PromptArgs {
@@ -128,14 +142,23 @@ __device__ __forceinline__ Block find_packed(const PromptArgs& a, int blk, int B
     return {0, 0, 0, (int)row0, (int)row0, (int)std::min<int64_t>(row0 + BM, a.tokens)};
 }
 
-template <bool F16, int RB, int W>
-__global__ __launch_bounds__(64 * W, RB == 1 ? 2 : 1) void prompt_kernel(PromptArgs a) {
-    constexpr int T = 64 * W, BM = 32 * RB * W;
+// Waits of a wave for its own loads to LDS, and the barrier, with nothing moved across either.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_barrier" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <bool F16, int W>
+__global__ __launch_bounds__(64 * W, 2) void prompt_kernel(PromptArgs a) {
+    constexpr int T = 64 * W, BM = 32 * W;
     constexpr int CH = TK * 16 / T;  // 16-byte chunks of K, and of V, a thread brings in per tile
-    __shared__ uint4 s_k[TK * 16];
-    __shared__ uint4 s_v[TK * 16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = lane & 31, h = lane >> 5;
+    constexpr int BUF = W == 8 ? 2 : 1;
+    __shared__ uint4 s_k[BUF][TK * 16];
+    __shared__ uint4 s_v[BUF][TK * 16];
+    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // in a scalar register, and what follows from it
     // workgroups of one KV head share an XCD's L2 where their number divides by the eight XCDs
     const int n_kv = (a.cu ? 1 : a.batch) * a.kv_heads, group = a.q_heads / a.kv_heads;
     const int kv = blockIdx.x % n_kv, item = blockIdx.x / n_kv;
@@ -164,61 +187,203 @@ __global__ __launch_bounds__(64 * W, RB == 1 ? 2 : 1) void prompt_kernel(PromptA
         return;
     }
 
-    // ---- the wave's query rows: dims 16 s + 8 h + (0..7) of row r of each block of 32
-    const int wrow = w.row0 + wave * 32 * RB;
-    Frag q[RB][8];
-#pragma unroll
-    for (int m = 0; m < RB; ++m) {
-        const int row = wrow + 32 * m + r;
-        const bool live = row >= w.lo && row < w.hi;
+    // ---- the wave's query rows: dims 16 s + 8 h + (0..7) of row r
+    const int wrow = w.row0 + 32 * wave, row = wrow + r;
+    const bool live = row >= w.lo && row < w.hi;
+    Frag q[8];
+    {
         const uint16_t* p = a.q + w.b * a.q_sb + hq * a.q_sh + (int64_t)(live ? row : w.lo) * a.q_st;
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
-            q[m][s].q = reinterpret_cast<const uint4*>(p)[2 * s + h];
-            if (!live) q[m][s].q = make_uint4(0u, 0u, 0u, 0u);
+            q[s].q = reinterpret_cast<const uint4*>(p)[2 * s + h];
+            if (!live) q[s].q = make_uint4(0u, 0u, 0u, 0u);
         }
     }
     const uint16_t* const kb = a.k + w.b * a.k_sb + kvh * a.k_sh;
     const uint16_t* const vb = a.v + w.b * a.v_sb + kvh * a.v_sh;
     const int k_end = (int)std::min<int64_t>(w.hi, (int64_t)w.row0 + BM);
 
-    // a tile to LDS; tokens past the last are copies of it, left out by the mask
-    auto load_tile = [&](int t0) {
+    // a tile's rows to LDS; tokens past the last are copies of it, left out by the mask
+    auto load_rows = [&](const uint16_t* base, int64_t st, uint4* dst, int t0) {
+        const uint16_t* const tile = base + (int64_t)t0 * st;  // scalar
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
             const int id = i * T + threadIdx.x, tok = id >> 4, c = (id & 15) ^ swizzle(tok);
-            const int64_t t = std::min(t0 + tok, k_end - 1);
-            load_lds16(kb + t * a.k_st + 8 * c, s_k + i * T + wave * 64);
-            load_lds16(vb + t * a.v_st + 8 * c, s_v + i * T + wave * 64);
+            load_lds16(tile + std::min(tok, k_end - 1 - t0) * st + 8 * c, dst + i * T + wave * 64);
         }
     };
 
     const float c2 = a.scale * LOG2E;
-    f32x16 o[RB][4];
-    float top[RB], sum[RB];  // reference of a row's weights, in units of q . k, and this lane's share of their sum
+    f32x16 o[4], s[2];
+    Frag p[4];
+    float top = -__builtin_inff(), sum = 0.0f;  // reference of the row's weights in log2, this lane's share of their sum
 #pragma unroll
-    for (int m = 0; m < RB; ++m) {
-        top[m] = -__builtin_inff(), sum[m] = 0.0f;
+    for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[m][d][i] = 0.0f;
-    }
-    const uint16_t* const v16 = reinterpret_cast<const uint16_t*>(s_v);
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
 
-    for (int t0 = w.lo; t0 < k_end; t0 += TK) {
+    auto products_qk = [&](const uint4* k) {
+        const uint8_t* const k8 = reinterpret_cast<const uint8_t*>(k);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                Frag kf;
+                kf.q = *reinterpret_cast<const uint4*>(k8 + key_offset(ks, lane) + 32 * 256 * t);
+                s[t] = mfma_32<F16>(kf, q[ks], s[t]);
+            }
+        // operands on their way six products ahead
+        __builtin_amdgcn_sched_group_barrier(DS_READ, 6, 0);
+#pragma unroll
+        for (int i = 0; i < 10; ++i) {
+            __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(MFMA, 6, 0);
+    };
+    auto products_pv = [&](const uint4* v, const Frag* weights, f32x16* out) {
+        const uint8_t* const v8 = reinterpret_cast<const uint8_t*>(v);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                Frag vf;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) vf.t[e] = read_tr(v8 + value_offset(d, e, lane) + 16 * 256 * ks);
+                out[d] = mfma_32<F16>(vf, weights[ks], out[d]);
+            }
+        __builtin_amdgcn_sched_group_barrier(DS_READ, 8, 0);
+#pragma unroll
+        for (int i = 0; i < 12; ++i) {
+            __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(DS_READ, 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(MFMA, 4, 0);
+    };
+    // weights of the scores of tile t0, in their B-operand order
+    auto softmax = [&](int t0, auto edge) {
+        if constexpr (edge) {
+            if (t0 + TK > wrow + 1) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (t0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > row) s[t][i] = -__builtin_inff();
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
+        // the reference is raised when some score is more than 2^LAZY above it; -inf and NaN do not raise it
+        if (__any(__builtin_fmaf(mx, c2, -top) > LAZY)) {
+            mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2;
+            const float ref = mx > top ? mx : top;
+            const float corr = top == ref ? 1.0f : exp2_(top - ref);
+            top = ref;
+            sum *= corr;
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= corr;
+        }
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i = 8 * x + 2 * k;
+                    s[t][i] = exp2_(__builtin_fmaf(s[t][i], c2, -base));
+                    s[t][i + 1] = exp2_(__builtin_fmaf(s[t][i + 1], c2, -base));
+                    sum += s[t][i];
+                    sum += s[t][i + 1];
+                    p[2 * t + x].u[k] = pack2<F16>(s[t][i], s[t][i + 1]);
+                }
+    };
+
+    int t0 = w.lo;
+    if constexpr (W == 8) {
+        // ---- tiles that every row attends to whole.  Waves 0-3 and 4-7 share the SIMDs two by two and take turns: while the
+        // one half does its products, QK of tile j and PV of tile j - 1, the other does the softmax of its scores.  In time
+        // slots with a barrier between them:
+        //   slot 2 j      first half: products of j      second half: softmax of j - 1
+        //   slot 2 j + 1  first half: softmax of j       second half: products of j
+        // K of tile j and V of tile j - 1 are read in slots 2 j and 2 j + 1, those of the next step come in meanwhile.
+        const int n = w.row0 >= w.lo ? (w.row0 + 1 - w.lo) / TK : 0;
+        if (n > 0) {
+            const bool second = wave >= 4;
+            // this thread's chunks of the next K and V tile
+            const uint16_t *kp[CH], *vp[CH];
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int id = i * T + threadIdx.x, tok = id >> 4, c = (id & 15) ^ swizzle(tok);
+                kp[i] = kb + (int64_t)(w.lo + tok) * a.k_st + 8 * c;
+                vp[i] = vb + (int64_t)(w.lo + tok) * a.v_st + 8 * c;
+            }
+            const int64_t k_step = TK * a.k_st, v_step = TK * a.v_st;
+            auto load_k = [&](int j) {
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    load_lds16(kp[i], s_k[j & 1] + i * T + wave * 64);
+                    kp[i] += k_step;
+                }
+            };
+            auto load = [&](int j) {  // K of tile j + 1 and V of tile j
+                if (j + 1 < n) load_k(j + 1);
+                if (j < n) {
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        load_lds16(vp[i], s_v[j & 1] + i * T + wave * 64);
+                        vp[i] += v_step;
+                    }
+                }
+            };
+            load_k(0);
+            wait_loads();
+            barrier();
+            if (second) {
+                load(0);
+                barrier();
+            }
+            for (int j = 0; j <= n; ++j) {
+                if (!second) load(j);
+                __builtin_amdgcn_s_setprio(1);
+                if (j > 0) products_pv(s_v[(j - 1) & 1], p, o);
+                if (j < n) products_qk(s_k[j & 1]);
+                __builtin_amdgcn_s_setprio(0);
+                if (second) wait_loads();
+                barrier();
+                if (second) load(j + 1);
+                if (j < n) softmax(w.lo + j * TK, std::false_type{});
+                if (!second) wait_loads();
+                barrier();
+            }
+            if (!second) barrier();
+            t0 = w.lo + n * TK;
+        }
+    }
+
+    // ---- tiles with tokens that some row leaves out
+    for (; t0 < k_end; t0 += TK) {
         __syncthreads();
-        load_tile(t0);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // of this wave's part, ahead of the barrier
+        load_rows(kb, a.k_st, s_k[0], t0);
+        load_rows(vb, a.v_st, s_v[0], t0);
+        wait_loads();
         __syncthreads();
-        const bool edge = t0 + TK > w.row0 + 1;  // some row leaves out some token
         bool special = false;
-        if (edge) {
+        if (t0 + TK > w.row0 + 1) {
             // a left-out token's weight is 0, which makes NaN of a value that is not finite: such values
             // are taken out of the tile and added apart
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                const uint4 x = s_v[i * T + threadIdx.x];
+                const uint4 x = s_v[0][i * T + threadIdx.x];
                 const uint32_t e = F16 ? 0x7C00u : 0x7F80u;
                 for (uint32_t u : {x.x, x.y, x.z, x.w})
                     special |= (u & e) == e || ((u >> 16) & e) == e;
@@ -228,96 +393,22 @@ __global__ __launch_bounds__(64 * W, RB == 1 ? 2 : 1) void prompt_kernel(PromptA
         if (special) {
 #pragma unroll 1
             for (int i = 0; i < CH; ++i) {
-                uint4 x = s_v[i * T + threadIdx.x];
+                uint4 x = s_v[0][i * T + threadIdx.x];
                 const uint32_t e = F16 ? 0x7C00u : 0x7F80u;
                 for (uint32_t* u : {&x.x, &x.y, &x.z, &x.w}) {
                     if ((*u & e) == e) *u &= 0xFFFF0000u;
                     if (((*u >> 16) & e) == e) *u &= 0x0000FFFFu;
                 }
-                s_v[i * T + threadIdx.x] = x;
+                s_v[0][i * T + threadIdx.x] = x;
             }
             __syncthreads();
         }
-
-        f32x16 s[RB][2];
-#pragma unroll
-        for (int m = 0; m < RB; ++m)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[m][t][i] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks) {
-                Frag kf;
-                const int tok = 32 * t + r;
-                kf.q = s_k[tok * 16 + ((2 * ks + h) ^ swizzle(tok))];
-#pragma unroll
-                for (int m = 0; m < RB; ++m) s[m][t] = mfma_32<F16>(kf, q[m][ks], s[m][t]);
-            }
-        Frag p[RB][4];
-#pragma unroll
-        for (int m = 0; m < RB; ++m) {
-            const int row = wrow + 32 * m + r;
-            if (edge) {
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (t0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > row) s[m][t][i] = -__builtin_inff();
-            }
-            float mx = top[m];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[m][t][i]);
-            mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float safe = mx == -__builtin_inff() ? 0.0f : mx;
-            if (__any(mx > top[m])) {
-                const float corr = exp2_(__builtin_fmaf(top[m], c2, -safe * c2));
-                sum[m] *= corr;
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[m][d][i] *= corr;
-            }
-            top[m] = mx;
-            const float base = safe * c2;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[m][t][i] = exp2_(__builtin_fmaf(s[m][t][i], c2, -base));
-                    sum[m] += s[m][t][i];
-                }
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        p[m][2 * t + x].u[k] = pack2<F16>(s[m][t][8 * x + 2 * k], s[m][t][8 * x + 2 * k + 1]);
+        const bool some = t0 < wrow + 32;  // the wave's rows attend to some token of the tile
+        if (some) {
+            products_qk(s_k[0]);
+            softmax(t0, std::true_type{});
+            products_pv(s_v[0], p, o);
         }
-        // V^T of 16 tokens: lane (r, h) takes dim 32 d + r of tokens 4 h + (0..3) and 8 + 4 h + (0..3)
-        auto v_frag = [&](int ks, int d) {
-            Frag vf;
-            const int cl = 4 * d + 2 * (r >> 4) + ((lane & 3) >> 1);  // 16-byte chunk of this lane's 4 dims
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int tok = 16 * ks + 8 * e + 4 * h + ((lane & 15) >> 2);
-                vf.t[e] = read_tr(v16 + (tok * 16 + (cl ^ swizzle(tok))) * 8 + 4 * (lane & 1));
-            }
-            return vf;
-        };
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                const Frag vf = v_frag(ks, d);
-#pragma unroll
-                for (int m = 0; m < RB; ++m) o[m][d] = mfma_32<F16>(vf, p[m][ks], o[m][d]);
-            }
         if (special) {
             // what was taken out, counted apart for every row and dim that gives it weight: +inf as 1, -inf as
             // 128, NaN as 16384, at most 64 of each
@@ -337,76 +428,68 @@ __global__ __launch_bounds__(64 * W, RB == 1 ? 2 : 1) void prompt_kernel(PromptA
                     }
                     *u = f[0] | f[1] << 16;
                 }
-                s_v[id] = x;
+                s_v[0][id] = x;
             }
             __syncthreads();
+            if (some) {
+                f32x16 n[4];
 #pragma unroll
-            for (int m = 0; m < RB; ++m) {
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) n[d][i] = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        p[m][ks].u[k] = pack2<F16>(s[m][ks >> 1][8 * (ks & 1) + 2 * k] > 0.0f ? 1.0f : 0.0f,
-                                                   s[m][ks >> 1][8 * (ks & 1) + 2 * k + 1] > 0.0f ? 1.0f : 0.0f);
+                        p[ks].u[k] = pack2<F16>(s[ks >> 1][8 * (ks & 1) + 2 * k] > 0.0f ? 1.0f : 0.0f,
+                                                s[ks >> 1][8 * (ks & 1) + 2 * k + 1] > 0.0f ? 1.0f : 0.0f);
+                products_pv(s_v[0], p, n);
 #pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    f32x16 n;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) n[i] = 0.0f;
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) n = mfma_32<F16>(v_frag(ks, d), p[m][ks], n);
+                for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int x = (int)n[i];
-                        if (x & 127) o[m][d][i] += __builtin_inff();
-                        if (x >> 7 & 127) o[m][d][i] -= __builtin_inff();
-                        if (x >> 14) o[m][d][i] = __builtin_nanf("");
+                        const int x = (int)n[d][i];
+                        if (x & 127) o[d][i] += __builtin_inff();
+                        if (x >> 7 & 127) o[d][i] -= __builtin_inff();
+                        if (x >> 14) o[d][i] = __builtin_nanf("");
                     }
-                }
             }
         }
     }
 
     // ---- rows out: two lanes hold a row's dims 8 j + 4 h + (0..3); pairs of j are exchanged for 16-byte stores
+    const float total = sum + __shfl_xor(sum, 32);
+    const float inv = live ? 1.0f / (total == 0.0f ? 1.0f : total) : 0.0f;
+    const bool mine = row >= w.w_lo && row < w.w_hi;
+    if (a.lse && mine && h == 0)
+        a.lse[lse_row + row] = !live || total == 0.0f ? -__builtin_inff() : top / LOG2E + __builtin_logf(total);
 #pragma unroll
-    for (int m = 0; m < RB; ++m) {
-        const int row = wrow + 32 * m + r;
-        float total = sum[m] + __shfl_xor(sum[m], 32);
-        const bool live = row >= w.lo && row < w.hi;
-        const float inv = live ? 1.0f / (total == 0.0f ? 1.0f : total) : 0.0f;
-        const bool mine = row >= w.w_lo && row < w.w_hi;
-        if (a.lse && mine && h == 0) {
-            a.lse[lse_row + row] = !live || total == 0.0f ? -__builtin_inff()
-                                                          : top[m] * a.scale + __builtin_logf(total);
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+            uint32_t x[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int i = 4 * (2 * jj + e) + 2 * k;
+                    x[e][k] = live ? pack2<F16>(o[d][i] * inv, o[d][i + 1] * inv) : 0u;
+                }
+            const auto lo = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
+            const auto hi = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+            if (mine)
+                *reinterpret_cast<uint4*>(ob + row * a.o_st + 32 * d + 8 * (2 * jj + h)) =
+                    make_uint4(lo[0], hi[0], lo[1], hi[1]);
         }
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int jj = 0; jj < 2; ++jj) {
-                uint32_t x[2][2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int i = 4 * (2 * jj + e) + 2 * k;
-                        x[e][k] = live ? pack2<F16>(o[m][d][i] * inv, o[m][d][i + 1] * inv) : 0u;
-                    }
-                const auto lo = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
-                const auto hi = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
-                if (mine)
-                    *reinterpret_cast<uint4*>(ob + row * a.o_st + 32 * d + 8 * (2 * jj + h)) =
-                        make_uint4(lo[0], hi[0], lo[1], hi[1]);
-            }
-    }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <bool F16, int RB, int W>
+template <bool F16, int W>
 void launch(PromptArgs& a, unsigned grid_kv, hipStream_t s) {
-    constexpr int BM = 32 * RB * W;
+    constexpr int BM = 32 * W;
     a.row_blocks = (a.tokens + BM - 1) / BM + (a.cu ? a.n_seqs + 2 : 0);
-    hipLaunchKernelGGL((prompt_kernel<F16, RB, W>), dim3(grid_kv * (unsigned)a.row_blocks), dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((prompt_kernel<F16, W>), dim3(grid_kv * (unsigned)a.row_blocks), dim3(64 * W), 0, s, a);
 }
 
 }  // namespace
@@ -434,8 +517,9 @@ extern "C" int tq_prompt_attention(const void* q, const void* k, const void* v, 
                  scale, 0};
     const unsigned grid_kv = (unsigned)(batch * q_heads);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (is_f16) launch<true, 1, 4>(a, grid_kv, s);
-    else launch<false, 1, 4>(a, grid_kv, s);
+    const bool wide = tokens * batch * q_heads >= (int64_t)256 * 256;
+    if (is_f16) wide ? launch<true, 8>(a, grid_kv, s) : launch<true, 4>(a, grid_kv, s);
+    else wide ? launch<false, 8>(a, grid_kv, s) : launch<false, 4>(a, grid_kv, s);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
 }
