@@ -220,3 +220,56 @@ def test_refusals_and_empty_calls(cuda):
         prompt_attention(q, k, k, out=torch.empty(2, 4, 8, D, device="cuda"))
     assert prompt_attention(q[:, :, :0], k[:, :, :0], k[:, :, :0]).shape == (2, 4, 0, D)
     assert prompt_attention(q[:0], k[:0], k[:0]).shape == (0, 4, 8, D)
+
+
+# calls of more than 512 blocks of 128 rows take blocks of 256
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hkv,g,S", [(130, 4, 1), (130, 4, 65), (66, 4, 129), (1, 176, 257), (28, 4, 600), (15, 4, 1100)])
+def test_many_blocks_match_fp64(cuda, dtype, Hkv, g, S):
+    q, k, v = (randn((1, S, h, D), i, dtype).transpose(1, 2) for i, h in ((1, Hkv * g), (2, Hkv), (3, Hkv)))
+    got, lse = prompt_attention(q, k, v, return_lse=True)
+    ref, ref_lse, size = oracle(q, k, v)
+    check(got, ref, size)
+    assert (lse.double().cpu() - ref_lse).abs().max() <= 4e-5
+
+
+def test_many_blocks_of_padded_batches(cuda):
+    S = 300
+    q, k, v = (randn((5, S, h, D), i, torch.bfloat16).transpose(1, 2) for i, h in ((1, 36), (2, 9), (3, 9)))
+    starts, ends = [0, 1, 130, 299, 300], [300, 299, 290, 300, 300]
+    for b in range(5):
+        for x in (k, v):
+            x[b, :, :starts[b]] = float("nan")
+            x[b, :, ends[b]:] = float("inf")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = prompt_attention(q, k, v, seq_starts=i32(starts), seq_ends=i32(ends))
+    ref, _, size = oracle(q, k, v, [(b, starts[b], ends[b]) for b in range(5)])
+    check(got, ref, size)
+
+
+def test_many_blocks_of_packed_sequences(cuda):
+    lens, tail = [300, 0, 5, 129, 1, 256, 0, 513], 40
+    total = sum(lens) + tail
+    q, k, v = (randn((1, total, h, D), i, torch.float16).transpose(1, 2) for i, h in ((1, 60), (2, 10), (3, 10)))
+    for x in (k, v):
+        x[:, :, total - tail:] = float("nan")
+    at = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    cu = torch.tensor(at, dtype=torch.int32, device="cuda")
+    mine = torch.full((1, 60, total, D), 7.0, dtype=torch.float16, device="cuda")
+    prompt_attention(q, k, v, cu_seqlens=cu, out=mine)
+    ref, _, size = oracle(q, k, v, [(0, a, b) for a, b in zip(at, at[1:])])
+    check(mine[:, :, :total - tail], ref[:, :, :total - tail], size[:, :, :total - tail])
+    assert (mine[:, :, total - tail:] == 7.0).all()
+
+
+@pytest.mark.parametrize("at", [0, 63, 200, 299])
+def test_values_that_are_not_finite_in_many_blocks(cuda, at):
+    q, k, v = (randn((1, h, 300, D), i, torch.bfloat16) for i, h in ((1, 176), (2, 2), (3, 2)))
+    ref, _, size = oracle(q, k, v)
+    v[0, 0, at, 3], v[0, 0, at, 7] = float("-inf"), float("nan")
+    got = prompt_attention(q, k, v)
+    check(got[:, :88, :at], ref[:, :88, :at], size[:, :88, :at])
+    check(got[:, 88:], ref[:, 88:], size[:, 88:])
+    assert (got[:, :88, at:, 3] == float("-inf")).all() and got[:, :88, at:, 7].isnan().all()
+    rest = [d for d in range(D) if d not in (3, 7)]
+    check(got[..., rest], ref[..., rest], size[..., rest])

@@ -5,21 +5,29 @@
 //
 // j over the sequence of row i.  One pass over the keys with a running reference m_i of each row.
 //
-// Layout.  A workgroup owns 32 RB W consecutive rows of one sequence and query head, a wave 32 RB of
-// them, and all waves walk the keys in tiles of 64 tokens.
+// Layout.  A workgroup of eight waves owns 256 consecutive rows of one sequence and query head (KS = 1), or 128 (KS = 2),
+// a wave 32 of them, and the waves walk the keys in tiles of 64 tokens.
 //   S^T = K Q^T   v_mfma_f32_32x32x16, A = 32 tokens x 16 dims, B = 16 dims x 32 rows: lane (r = l % 32,
 //                 h = l / 32) ends with row r's scores of the tokens 8 j + 4 h + (0..3) of a block of 32
 //   O^T = V^T P^T A = 32 dims x 16 tokens, B = 16 tokens x 32 rows.  The order of the 16 tokens along k
 //                 is free: it is the order the scores come back in, so a lane's weights become its B
 //                 operand as they are, and ds_read_b64_tr_b16 takes V^T out of row-major rows in that
 //                 order (16 lanes read 4 tokens x 16 dims and each ends with one dim's 4 tokens).
-// K and V go from memory to LDS without passing registers (16 bytes a lane); a row's 16-byte chunk c is at
-// slot c ^ f(token), f taking the token's low four bits to the slot with the bits 0-1 on top, so that
+// K and V go from memory to LDS without passing registers (16 bytes a lane), double-buffered; a row's 16-byte chunk c
+// is at slot c ^ f(token), f taking the token's low four bits to the slot with the bits 0-1 on top, so that
 // the 16 rows of a K read and the 4 x 2 rows of a V read both meet every bank once.
 //
+// Cost.  Bound by the matrix pipe and the softmax beside it: a tile of 64 tokens and 32 rows is 32 products of 32 cycles
+// and about 430 cycles of exponentials, maxima, sums and roundings, on a SIMD that holds two waves.  The waves' halves therefore
+// take turns (below): 1 x 32/8 heads of 8192 tokens take 584 us = 940 TFLOP/s of counted work, where a large
+// product of matrices reaches 1326; four waves that each do one thing after the other took 662, eight without the
+// operands read ahead 595 at the time they took 544 with them.  The clock gives way under this load (1.6 to 1.9
+// GHz of 2.4), so cycles won come back in part only.  64 rows to a wave (512 registers) took longer: its sums move
+// between the two register files.  Small prompts are bound by latency, 13 us at 300 tokens.
+//
 // Rounding.  Scores, weights, sums and outputs are fp32; the weights are rounded to the values' type for
-// their product, once and to nearest: relative 2^-9 (bf16), as much as the output's own rounding, and
-// independent from weight to weight.  The sum of a row's weights is of the unrounded ones.
+// their product, once and to nearest: off by at most half a step (relative 2^-8 in bf16), as much as the
+// output's own rounding, and independently from weight to weight.  The sum of a row's weights is of the unrounded ones.
 
 #include <algorithm>
 #include <type_traits>
@@ -33,7 +41,9 @@ constexpr int TK = 64;  // tokens per tile
 constexpr float LOG2E = 1.44269504f;
 constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's reference by
 
+#define INLINE __attribute__((always_inline))
 constexpr int MFMA = 0x8, DS_READ = 0x100;  // kinds of instructions for the scheduler
+constexpr int AHEAD = 4;                    // products whose operands are on their way
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -142,7 +152,8 @@ __device__ __forceinline__ Block find_packed(const PromptArgs& a, int blk, int B
     return {0, 0, 0, (int)row0, (int)row0, (int)std::min<int64_t>(row0 + BM, a.tokens)};
 }
 
-// Waits of a wave for its own loads to LDS, and the barrier, with nothing moved across either.
+// Waits of a wave for its own loads to LDS and reads of it, and the barrier, with nothing moved across any.
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() {
     __builtin_amdgcn_sched_barrier(0);
@@ -150,15 +161,20 @@ __device__ __forceinline__ void barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-template <bool F16, int W>
-__global__ __launch_bounds__(64 * W, 2) void prompt_kernel(PromptArgs a) {
-    constexpr int T = 64 * W, BM = 32 * W;
-    constexpr int CH = TK * 16 / T;  // 16-byte chunks of K, and of V, a thread brings in per tile
-    constexpr int BUF = W == 8 ? 2 : 1;
-    __shared__ uint4 s_k[BUF][TK * 16];
-    __shared__ uint4 s_v[BUF][TK * 16];
+// Eight waves, two to a SIMD, in two halves of four.  KS = 1: 256 rows, 32 to a wave, and every wave walks all tiles.
+// KS = 2: 128 rows, and the halves walk every other tile of the same rows, their sums meet at the end: half the steps where
+// there are few blocks.
+template <bool F16, int KS>
+__global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
+    constexpr int T = 512, BM = 256 / KS;
+    constexpr int TL = T / KS;           // threads that bring in a tile
+    constexpr int CH = TK * 16 / TL;     // 16-byte chunks of K, and of V, each of them
+    __shared__ uint4 s_k[KS][2][TK * 16];
+    __shared__ uint4 s_v[KS][2][TK * 16];
     const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // in a scalar register, and what follows from it
+    const bool second = wave >= 4;
+    const int part = KS == 2 && second ? 1 : 0;
     // workgroups of one KV head share an XCD's L2 where their number divides by the eight XCDs
     const int n_kv = (a.cu ? 1 : a.batch) * a.kv_heads, group = a.q_heads / a.kv_heads;
     const int kv = blockIdx.x % n_kv, item = blockIdx.x / n_kv;
@@ -175,6 +191,9 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_kernel(PromptArgs a) {
         const int hi = a.ends ? std::min(std::max(a.ends[b], lo), a.tokens) : a.tokens;
         w = {b, lo, hi, blk * BM, blk * BM, (int)std::min<int64_t>((int64_t)blk * BM + BM, a.tokens)};
     }
+    // the same in every lane
+    w.lo = __builtin_amdgcn_readfirstlane(w.lo), w.hi = __builtin_amdgcn_readfirstlane(w.hi);
+    w.row0 = __builtin_amdgcn_readfirstlane(w.row0), w.b = __builtin_amdgcn_readfirstlane(w.b);
     uint16_t* const ob = a.out + w.b * a.o_sb + hq * a.o_sh;
     const int64_t lse_row = ((int64_t)w.b * a.q_heads + hq) * a.tokens;
     if (w.lo >= w.hi || w.row0 >= w.hi || w.row0 + BM <= w.lo) {  // no row of a sequence
@@ -187,8 +206,32 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_kernel(PromptArgs a) {
         return;
     }
 
+    const uint16_t* const kb = a.k + w.b * a.k_sb + kvh * a.k_sh;
+    const uint16_t* const vb = a.v + w.b * a.v_sb + kvh * a.v_sh;
+    const int k_end = (int)std::min<int64_t>(w.hi, (int64_t)w.row0 + BM);
+    const int n = (k_end - w.lo + TK - 1) / TK, steps = (n + KS - 1) / KS, last = KS * steps;  // tiles, and each half's
+
+    // ---- tiles to LDS; those of a half of KS = 2 are part, part + 2, ...
+    // (a thread has a chunk of every TL / 16-th row, at the same place of its row: TL / 16 is a multiple of the swizzle's 16;
+    // tokens past the last are copies of it, left out by the mask)
+    const int tid = threadIdx.x % TL, lds_wave = KS == 2 ? wave & 3 : wave;
+    const uint32_t in_row = 16 * ((tid & 15) ^ swizzle(tid >> 4));
+    const uint32_t k_st2 = (uint32_t)a.k_st * 2, v_st2 = (uint32_t)a.v_st * 2, k_off = (tid >> 4) * k_st2, v_off = (tid >> 4) * v_st2;
+    auto load = [&](const uint16_t* base, int64_t st, uint32_t st2, uint32_t off, int tile, uint4* dst) INLINE {
+        if (tile >= last) return;
+        const int t0 = std::min(w.lo + tile * TK, k_end - 1);
+        const char* const rows = reinterpret_cast<const char*>(base + (int64_t)t0 * st);
+        const uint32_t most = (uint32_t)(k_end - 1 - t0) * st2;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            load_lds16(rows + (std::min(off + i * (TL / 16) * st2, most) + in_row), dst + i * TL + lds_wave * 64);
+    };
+    auto load_k = [&](int j) INLINE { load(kb, a.k_st, k_st2, k_off, KS * j + part, s_k[part][j & 1]); };
+    auto load_v = [&](int j) INLINE { load(vb, a.v_st, v_st2, v_off, KS * j + part, s_v[part][j & 1]); };
+    load_k(0);
+
     // ---- the wave's query rows: dims 16 s + 8 h + (0..7) of row r
-    const int wrow = w.row0 + 32 * wave, row = wrow + r;
+    const int wrow = w.row0 + 32 * (KS == 2 ? wave & 3 : wave), row = wrow + r;
     const bool live = row >= w.lo && row < w.hi;
     Frag q[8];
     {
@@ -199,81 +242,89 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_kernel(PromptArgs a) {
             if (!live) q[s].q = make_uint4(0u, 0u, 0u, 0u);
         }
     }
-    const uint16_t* const kb = a.k + w.b * a.k_sb + kvh * a.k_sh;
-    const uint16_t* const vb = a.v + w.b * a.v_sb + kvh * a.v_sh;
-    const int k_end = (int)std::min<int64_t>(w.hi, (int64_t)w.row0 + BM);
-
-    // a tile's rows to LDS; tokens past the last are copies of it, left out by the mask
-    auto load_rows = [&](const uint16_t* base, int64_t st, uint4* dst, int t0) {
-        const uint16_t* const tile = base + (int64_t)t0 * st;  // scalar
-#pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int id = i * T + threadIdx.x, tok = id >> 4, c = (id & 15) ^ swizzle(tok);
-            load_lds16(tile + std::min(tok, k_end - 1 - t0) * st + 8 * c, dst + i * T + wave * 64);
-        }
-    };
-
     const float c2 = a.scale * LOG2E;
     f32x16 o[4], s[2];
     Frag p[4];
-    float top = -__builtin_inff(), sum = 0.0f;  // reference of the row's weights in log2, this lane's share of their sum
+    float top, sum;  // reference of the row's weights in log2, this lane's share of their sum
+    auto start = [&]() INLINE {
+        top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
-
-    auto products_qk = [&](const uint4* k) {
-        const uint8_t* const k8 = reinterpret_cast<const uint8_t*>(k);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                Frag kf;
-                kf.q = *reinterpret_cast<const uint4*>(k8 + key_offset(ks, lane) + 32 * 256 * t);
-                s[t] = mfma_32<F16>(kf, q[ks], s[t]);
-            }
-        // operands on their way six products ahead
-        __builtin_amdgcn_sched_group_barrier(DS_READ, 6, 0);
-#pragma unroll
-        for (int i = 0; i < 10; ++i) {
-            __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(MFMA, 6, 0);
+            for (int i = 0; i < 16; ++i) o[d][i] = 0.0f;
     };
-    auto products_pv = [&](const uint4* v, const Frag* weights, f32x16* out) {
-        const uint8_t* const v8 = reinterpret_cast<const uint8_t*>(v);
+    start();
+
+    // S^T of a tile of keys and (or) the last weights' sums of a tile of values.  The operands are asked for some products
+    // ahead: left to itself the compiler reads two, waits and multiplies (595 us against 544 at 8192 tokens).  `between`
+    // is called when all operands are read and AHEAD products are left.
+    auto products = [&](const uint4* k, const uint4* v, f32x16* out, auto qk, auto pv, auto between) INLINE {
+        const uint8_t *const k8 = reinterpret_cast<const uint8_t*>(k), *const v8 = reinterpret_cast<const uint8_t*>(v);
+        Frag last[AHEAD];
+        auto value_operand = [&](int i) INLINE {
+            Frag f;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
+            for (int e = 0; e < 2; ++e) f.t[e] = read_tr(v8 + value_offset(i & 3, e, lane) + 16 * 256 * (i >> 2));
+            return f;
+        };
+        auto key_operand = [&](int i) INLINE {
+            Frag f;
+            f.q = *reinterpret_cast<const uint4*>(k8 + key_offset(i >> 1, lane) + 32 * 256 * (i & 1));
+            return f;
+        };
+        if constexpr (pv) {
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                Frag vf;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) vf.t[e] = read_tr(v8 + value_offset(d, e, lane) + 16 * 256 * ks);
-                out[d] = mfma_32<F16>(vf, weights[ks], out[d]);
+            for (int i = 0; i < 16; ++i) {
+                const Frag f = value_operand(i);
+                if (!qk && i >= 16 - AHEAD) last[i - (16 - AHEAD)] = f;
+                else out[i & 3] = mfma_32<F16>(f, p[i >> 2], out[i & 3]);
             }
-        __builtin_amdgcn_sched_group_barrier(DS_READ, 8, 0);
-#pragma unroll
-        for (int i = 0; i < 12; ++i) {
-            __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(DS_READ, 2, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(MFMA, 4, 0);
+        if constexpr (qk) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[t][i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const Frag f = key_operand(i);
+                if (i >= 16 - AHEAD) last[i - (16 - AHEAD)] = f;
+                else s[i & 1] = mfma_32<F16>(f, q[i >> 1], s[i & 1]);
+            }
+        }
+        if constexpr (pv) {
+            __builtin_amdgcn_sched_group_barrier(DS_READ, 2 * AHEAD, 0);
+#pragma unroll
+            for (int i = 0; i < 16 - AHEAD; ++i) {
+                __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(DS_READ, 2, 0);
+            }
+        } else {
+            __builtin_amdgcn_sched_group_barrier(DS_READ, AHEAD, 0);
+        }
+        if constexpr (qk) {
+#pragma unroll
+            for (int i = 0; i < (pv ? 16 : 16 - AHEAD); ++i) {
+                __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
+            }
+        }
+        between();
+#pragma unroll
+        for (int i = 16 - AHEAD; i < 16; ++i) {
+            const Frag f = last[i - (16 - AHEAD)];
+            if constexpr (qk) s[i & 1] = mfma_32<F16>(f, q[i >> 1], s[i & 1]);
+            else out[i & 3] = mfma_32<F16>(f, p[i >> 2], out[i & 3]);
+        }
     };
     // weights of the scores of tile t0, in their B-operand order
-    auto softmax = [&](int t0, auto edge) {
-        if constexpr (edge) {
-            if (t0 + TK > wrow + 1) {
+    auto softmax = [&](int t0) INLINE {
+        if (t0 + TK > wrow + 1) {  // some row leaves out some token
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (t0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > row) s[t][i] = -__builtin_inff();
-            }
+                for (int i = 0; i < 16; ++i)
+                    if (t0 + 32 * t + 8 * (i >> 2) + 4 * h + (i & 3) > row) s[t][i] = -__builtin_inff();
         }
         float mx = s[0][0];
 #pragma unroll
@@ -307,158 +358,152 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_kernel(PromptArgs a) {
                     p[2 * t + x].u[k] = pack2<F16>(s[t][i], s[t][i + 1]);
                 }
     };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
 
-    int t0 = w.lo;
-    if constexpr (W == 8) {
-        // ---- tiles that every row attends to whole.  Waves 0-3 and 4-7 share the SIMDs two by two and take turns: while the
-        // one half does its products, QK of tile j and PV of tile j - 1, the other does the softmax of its scores.  In time
-        // slots with a barrier between them:
-        //   slot 2 j      first half: products of j      second half: softmax of j - 1
-        //   slot 2 j + 1  first half: softmax of j       second half: products of j
-        // K of tile j and V of tile j - 1 are read in slots 2 j and 2 j + 1, those of the next step come in meanwhile.
-        const int n = w.row0 >= w.lo ? (w.row0 + 1 - w.lo) / TK : 0;
-        if (n > 0) {
-            const bool second = wave >= 4;
-            // this thread's chunks of the next K and V tile
-            const uint16_t *kp[CH], *vp[CH];
-#pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const int id = i * T + threadIdx.x, tok = id >> 4, c = (id & 15) ^ swizzle(tok);
-                kp[i] = kb + (int64_t)(w.lo + tok) * a.k_st + 8 * c;
-                vp[i] = vb + (int64_t)(w.lo + tok) * a.v_st + 8 * c;
-            }
-            const int64_t k_step = TK * a.k_st, v_step = TK * a.v_st;
-            auto load_k = [&](int j) {
-#pragma unroll
-                for (int i = 0; i < CH; ++i) {
-                    load_lds16(kp[i], s_k[j & 1] + i * T + wave * 64);
-                    kp[i] += k_step;
-                }
-            };
-            auto load = [&](int j) {  // K of tile j + 1 and V of tile j
-                if (j + 1 < n) load_k(j + 1);
-                if (j < n) {
-#pragma unroll
-                    for (int i = 0; i < CH; ++i) {
-                        load_lds16(vp[i], s_v[j & 1] + i * T + wave * 64);
-                        vp[i] += v_step;
-                    }
-                }
-            };
-            load_k(0);
-            wait_loads();
+    // ---- The halves take turns: while one does its products, QK of its tile j and PV of its tile j - 1, the other does the
+    // softmax of its scores.  In time slots with a barrier between them:
+    //   slot 2 j      first half: products of j      second half: softmax of j - 1
+    //   slot 2 j + 1  first half: softmax of j       second half: products of j
+    // With KS = 1, K of tile j and V of tile j - 1 are read in slots 2 j and 2 j + 1, and those of the next step come in
+    // meanwhile.  Tiles that leave a wave's rows out whole take their turns like the others, with weights of 0.
+    {
+        wait_loads();
+        barrier();
+        if (second) {
+            load_k(1);
+            load_v(0);
             barrier();
-            if (second) {
-                load(0);
+        }
+        auto turn = [&](int j, auto qk, auto pv) INLINE {
+            int half = wave >> 2;
+            asm volatile("" : "+s"(half));  // one copy of the loop, not one for each half
+            const bool later = half != 0;
+            // the other half may begin when the operands are read: it has its own to wait for.  The loads come behind the
+            // reads, since the compiler has every read of LDS wait for the loads to it ahead of it
+            auto between = [&]() INLINE {
+                wait_reads();
+                if (later) {
+                    wait_loads();
+                } else {
+                    load_k(j + 1);
+                    load_v(j);
+                }
                 barrier();
+            };
+            __builtin_amdgcn_s_setprio(1);
+            products(s_k[part][j & 1], s_v[part][(j - 1) & 1], o, qk, pv, between);
+            __builtin_amdgcn_s_setprio(0);
+            if (later) {
+                load_k(j + 2);
+                load_v(j + 1);
             }
-            for (int j = 0; j <= n; ++j) {
-                if (!second) load(j);
-                __builtin_amdgcn_s_setprio(1);
-                if (j > 0) products_pv(s_v[(j - 1) & 1], p, o);
-                if (j < n) products_qk(s_k[j & 1]);
-                __builtin_amdgcn_s_setprio(0);
-                if (second) wait_loads();
-                barrier();
-                if (second) load(j + 1);
-                if (j < n) softmax(w.lo + j * TK, std::false_type{});
-                if (!second) wait_loads();
-                barrier();
+            if constexpr (qk) softmax(w.lo + (KS * j + part) * TK);
+            if (!later) wait_loads();
+            barrier();
+        };
+        turn(0, yes, no);
+        for (int j = 1; j < steps; ++j) turn(j, yes, yes);
+        turn(steps, no, yes);
+        if (!second) barrier();
+    }
+
+    // ---- A left-out token's weight is 0, which makes NaN of a value that is not finite.  A workgroup that ends with a sum
+    // that is not finite walks its tiles once more, with care: such values are taken out of the tile and added apart.
+    uint32_t most = 0u;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = std::max(most, __float_as_uint(o[d][i]) & 0x7FFFFFFFu);
+    if (__syncthreads_or(most >= 0x7F800000u)) {
+        start();
+        uint4 *const ck = s_k[0][0], *const cv = s_v[0][0];
+        constexpr int CC = TK * 16 / T;
+#pragma unroll 1
+        for (int t0 = w.lo; t0 < k_end; t0 += TK) {
+            const bool some = part == 0 && t0 < wrow + 32;  // the wave's rows attend to some token of the tile
+            __syncthreads();
+            // values that are not finite as 0, and again as counts: +inf 1, -inf 128, NaN 16384, at most 64 of each
+#pragma unroll 1
+            for (int round = 0; round < 2; ++round) {
+#pragma unroll 1
+                for (int i = 0; i < CC; ++i) {
+                    const int id = i * T + threadIdx.x, tok = id >> 4, c = (id & 15) ^ swizzle(tok);
+                    const int64_t t = std::min(t0 + tok, k_end - 1);
+                    if (round == 0) ck[id] = *reinterpret_cast<const uint4*>(kb + t * a.k_st + 8 * c);
+                    uint4 x = *reinterpret_cast<const uint4*>(vb + t * a.v_st + 8 * c);
+                    const uint32_t inf = F16 ? 0x7C00u : 0x7F80u;
+                    for (uint32_t* u : {&x.x, &x.y, &x.z, &x.w}) {
+                        uint32_t f[2];
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t y = (*u >> (16 * e)) & 0xFFFFu, z = y & 0x7FFFu;
+                            const float count = z < inf ? 0.0f : z > inf ? 16384.0f : y == inf ? 1.0f : 128.0f;
+                            f[e] = round ? pack2<F16>(count, 0.0f) : z < inf ? y : 0u;
+                        }
+                        *u = f[0] | f[1] << 16;
+                    }
+                    cv[id] = x;
+                }
+                __syncthreads();
+                if (some && round == 0) {
+                    products(ck, nullptr, nullptr, yes, no, [] {});
+                    softmax(t0);
+                    products(nullptr, cv, o, no, yes, [] {});
+                } else if (some) {
+                    f32x16 counts[4];
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) counts[d][i] = 0.0f;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            p[ks].u[k] = pack2<F16>(s[ks >> 1][8 * (ks & 1) + 2 * k] > 0.0f ? 1.0f : 0.0f,
+                                                    s[ks >> 1][8 * (ks & 1) + 2 * k + 1] > 0.0f ? 1.0f : 0.0f);
+                    products(nullptr, cv, counts, no, yes, [] {});
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int x = (int)counts[d][i];
+                            if (x & 127) o[d][i] += __builtin_inff();
+                            if (x >> 7 & 127) o[d][i] -= __builtin_inff();
+                            if (x >> 14) o[d][i] = __builtin_nanf("");
+                        }
+                }
+                __syncthreads();
             }
-            if (!second) barrier();
-            t0 = w.lo + n * TK;
         }
     }
 
-    // ---- tiles with tokens that some row leaves out
-    for (; t0 < k_end; t0 += TK) {
+    float total = sum + __shfl_xor(sum, 32);
+    if constexpr (KS == 2) {  // the halves' sums meet
+        float* const meet = reinterpret_cast<float*>(s_k);
+        float2* const ms = reinterpret_cast<float2*>(s_v);
         __syncthreads();
-        load_rows(kb, a.k_st, s_k[0], t0);
-        load_rows(vb, a.v_st, s_v[0], t0);
-        wait_loads();
+        if (second) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) meet[((wave & 3) * 64 + 16 * d + i) * 64 + lane] = o[d][i];
+            ms[(wave & 3) * 64 + lane] = make_float2(top, total);
+        }
         __syncthreads();
-        bool special = false;
-        if (t0 + TK > w.row0 + 1) {
-            // a left-out token's weight is 0, which makes NaN of a value that is not finite: such values
-            // are taken out of the tile and added apart
+        if (second) return;
+        const float2 m = ms[wave * 64 + lane];
+        const float best = fmaxf(top, m.x), safe = best == -__builtin_inff() ? 0.0f : best;
+        const float w0 = exp2_(top - safe), w1 = exp2_(m.x - safe);
+        total = total * w0 + m.y * w1;
+        top = best;
 #pragma unroll
-            for (int i = 0; i < CH; ++i) {
-                const uint4 x = s_v[0][i * T + threadIdx.x];
-                const uint32_t e = F16 ? 0x7C00u : 0x7F80u;
-                for (uint32_t u : {x.x, x.y, x.z, x.w})
-                    special |= (u & e) == e || ((u >> 16) & e) == e;
-            }
-            special = __syncthreads_or(special);
-        }
-        if (special) {
-#pragma unroll 1
-            for (int i = 0; i < CH; ++i) {
-                uint4 x = s_v[0][i * T + threadIdx.x];
-                const uint32_t e = F16 ? 0x7C00u : 0x7F80u;
-                for (uint32_t* u : {&x.x, &x.y, &x.z, &x.w}) {
-                    if ((*u & e) == e) *u &= 0xFFFF0000u;
-                    if (((*u >> 16) & e) == e) *u &= 0x0000FFFFu;
-                }
-                s_v[0][i * T + threadIdx.x] = x;
-            }
-            __syncthreads();
-        }
-        const bool some = t0 < wrow + 32;  // the wave's rows attend to some token of the tile
-        if (some) {
-            products_qk(s_k[0]);
-            softmax(t0, std::true_type{});
-            products_pv(s_v[0], p, o);
-        }
-        if (special) {
-            // what was taken out, counted apart for every row and dim that gives it weight: +inf as 1, -inf as
-            // 128, NaN as 16384, at most 64 of each
-            __syncthreads();
-#pragma unroll 1
-            for (int i = 0; i < CH; ++i) {
-                const int id = i * T + threadIdx.x, tok = id >> 4, c = (id & 15) ^ swizzle(tok);
-                const int64_t t = std::min(t0 + tok, k_end - 1);
-                uint4 x = *reinterpret_cast<const uint4*>(vb + t * a.v_st + 8 * c);
-                const uint32_t inf = F16 ? 0x7C00u : 0x7F80u;
-                for (uint32_t* u : {&x.x, &x.y, &x.z, &x.w}) {
-                    uint32_t f[2];
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t y = (*u >> (16 * e)) & 0xFFFFu;
-                        const float n = (y & 0x7FFFu) < inf ? 0.0f : (y & 0x7FFFu) > inf ? 16384.0f : y == inf ? 1.0f : 128.0f;
-                        f[e] = pack2<F16>(n, 0.0f);
-                    }
-                    *u = f[0] | f[1] << 16;
-                }
-                s_v[0][id] = x;
-            }
-            __syncthreads();
-            if (some) {
-                f32x16 n[4];
+        for (int d = 0; d < 4; ++d)
 #pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) n[d][i] = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        p[ks].u[k] = pack2<F16>(s[ks >> 1][8 * (ks & 1) + 2 * k] > 0.0f ? 1.0f : 0.0f,
-                                                s[ks >> 1][8 * (ks & 1) + 2 * k + 1] > 0.0f ? 1.0f : 0.0f);
-                products_pv(s_v[0], p, n);
-#pragma unroll
-                for (int d = 0; d < 4; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int x = (int)n[d][i];
-                        if (x & 127) o[d][i] += __builtin_inff();
-                        if (x >> 7 & 127) o[d][i] -= __builtin_inff();
-                        if (x >> 14) o[d][i] = __builtin_nanf("");
-                    }
-            }
-        }
+            for (int i = 0; i < 16; ++i)
+                o[d][i] = o[d][i] * w0 + (w1 == 0.0f ? 0.0f : meet[(wave * 64 + 16 * d + i) * 64 + lane] * w1);
     }
 
     // ---- rows out: two lanes hold a row's dims 8 j + 4 h + (0..3); pairs of j are exchanged for 16-byte stores
-    const float total = sum + __shfl_xor(sum, 32);
     const float inv = live ? 1.0f / (total == 0.0f ? 1.0f : total) : 0.0f;
     const bool mine = row >= w.w_lo && row < w.w_hi;
     if (a.lse && mine && h == 0)
@@ -485,11 +530,11 @@ __global__ __launch_bounds__(64 * W, 2) void prompt_kernel(PromptArgs a) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <bool F16, int W>
+template <bool F16, int KS>
 void launch(PromptArgs& a, unsigned grid_kv, hipStream_t s) {
-    constexpr int BM = 32 * W;
+    constexpr int BM = 256 / KS;
     a.row_blocks = (a.tokens + BM - 1) / BM + (a.cu ? a.n_seqs + 2 : 0);
-    hipLaunchKernelGGL((prompt_kernel<F16, W>), dim3(grid_kv * (unsigned)a.row_blocks), dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((prompt_kernel<F16, KS>), dim3(grid_kv * (unsigned)a.row_blocks), dim3(512), 0, s, a);
 }
 
 }  // namespace
@@ -507,6 +552,9 @@ extern "C" int tq_prompt_attention(const void* q, const void* k, const void* v, 
     if (dim != D) return TQ_ERR_UNSUPPORTED;
     for (int64_t s : {q_sb, q_sh, q_st, k_sb, k_sh, k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st})
         if (s % 8) return TQ_ERR_UNSUPPORTED;
+    // offsets inside a tile of 64 keys are 32 bits wide
+    for (int64_t s : {k_st, v_st})
+        if (s < 0 || s >= (int64_t)1 << 25) return TQ_ERR_UNSUPPORTED;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return TQ_ERR_UNSUPPORTED;
     // rows and blocks are counted in 32 bits
     const int64_t blocks = (tokens + 127) / 128 + (cu_seqlens ? (int64_t)n_seqs + 2 : 0);
@@ -517,9 +565,12 @@ extern "C" int tq_prompt_attention(const void* q, const void* k, const void* v, 
                  scale, 0};
     const unsigned grid_kv = (unsigned)(batch * q_heads);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const bool wide = tokens * batch * q_heads >= (int64_t)256 * 256;
-    if (is_f16) wide ? launch<true, 8>(a, grid_kv, s) : launch<true, 4>(a, grid_kv, s);
-    else wide ? launch<false, 8>(a, grid_kv, s) : launch<false, 4>(a, grid_kv, s);
+    // KS = 2 while its blocks of 128 rows are at most two for each of the 256 CUs (one fits a CU at a time): 1 x 32 heads of 1024
+    // tokens take 24 us with it and 32 with KS = 1, of 2048 54 and 61; past that a CU has blocks to go on with, and its merge
+    // and its smaller blocks cost more than they save: 2400 tokens take 81 and 77 us, 8192 625 and 584.
+    const bool wide = blocks * batch * q_heads > 512;
+    if (is_f16) wide ? launch<true, 1>(a, grid_kv, s) : launch<true, 2>(a, grid_kv, s);
+    else wide ? launch<false, 1>(a, grid_kv, s) : launch<false, 2>(a, grid_kv, s);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
 }
