@@ -387,7 +387,7 @@ int tq_tree_attention(const void* q, int q_type, int batch, int q_heads, int kv_
  *   index      int32 (device, nullable), element (b, head, j) at b index_sb + head index_sh + j
  * A row outside [0, src_batch), or an index outside [0, tokens), gives zeros.
  */
-#define TQ_MAX_ROW_BYTES 256
+#define TQ_MAX_ROW_BYTES 1024
 int tq_gather_tokens(int n_buffers, const void* const* src, void* const* dst, const int* row_bytes, int src_batch,
                      int heads, int64_t src_cap, int64_t tokens, int dst_batch, int64_t dst_cap, const int32_t* rows,
                      const int32_t* index, int64_t index_sb, int64_t index_sh, int64_t n_index, void* stream);
@@ -395,11 +395,12 @@ int tq_gather_tokens(int n_buffers, const void* const* src, void* const* dst, co
 /*
  * In place: of the slots [first, first + tokens) of every buffer, batch row and head, slot first + j becomes
  * slot first + index[b][head][j] for j < n_index <= TQ_MAX_KEEP (an accepted path of drafted tokens closed
- * up).  All are read before any is written: the index may have any order and name a slot more than once; an
+ * up; n_index rows of the widest buffer hold at most TQ_MAX_KEEP_BYTES).  All are read before any is written: the index may have any order and name a slot more than once; an
  * index outside [0, tokens) gives zeros.  The slots from first + n_index on stay as they were.  Arguments as
  * for tq_gather_tokens.
  */
 #define TQ_MAX_KEEP 256
+#define TQ_MAX_KEEP_BYTES 65536
 int tq_keep_tokens(int n_buffers, void* const* buffers, const int* row_bytes, int batch, int heads, int64_t cap,
                    int64_t first, int64_t tokens, const int32_t* index, int64_t index_sb, int64_t index_sh,
                    int n_index, void* stream);

@@ -16,7 +16,6 @@ constexpr int MAX_BUFFERS = 16;
 constexpr int T = 256;
 constexpr int UNITS = 4;              // 16-byte pieces a thread moves
 constexpr int CHUNK = 16 * T * UNITS; // bytes of a workgroup
-constexpr int KEEP_LDS = 64 << 10;
 
 struct Moves {
     const uint8_t* src[MAX_BUFFERS];
@@ -185,9 +184,10 @@ extern "C" int tq_keep_tokens(int n_buffers, void* const* buffers, const int* ro
         return TQ_ERR_INVALID_ARGUMENT;
     int widest = 0;
     for (int i = 0; i < n_buffers; ++i) widest = std::max(widest, row_bytes[i]);
-    if (n_index > TQ_MAX_KEEP || (int64_t)batch * heads >= (int64_t)1 << 24) return TQ_ERR_UNSUPPORTED;
+    if (n_index > TQ_MAX_KEEP || (int64_t)n_index * widest > TQ_MAX_KEEP_BYTES ||
+        (int64_t)batch * heads >= (int64_t)1 << 24)
+        return TQ_ERR_UNSUPPORTED;
     if (n_index == 0) return TQ_OK;
-    static_assert(TQ_MAX_KEEP * TQ_MAX_ROW_BYTES <= KEEP_LDS, "a region's rows fit in LDS");
     Moves m{};
     for (int i = 0; i < n_buffers; ++i) {
         m.row[i] = row_bytes[i];

@@ -696,10 +696,11 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: to
     return outs if len(outs) > 1 else out
 
 
-#: most buffers of one launch, and the limits of TQ_MAX_KEEP and TQ_MAX_ROW_BYTES
+#: most buffers of one launch, and the limits TQ_MAX_KEEP, TQ_MAX_KEEP_BYTES and TQ_MAX_ROW_BYTES
 _MOVE_BUFFERS = 16
 MAX_KEEP = 256
-_MAX_ROW_BYTES = 256
+MAX_KEEP_BYTES = 65536
+_MAX_ROW_BYTES = 1024
 
 
 def _move_buffers(name: str, buffers: list[torch.Tensor]) -> tuple[int, int, int, list[int]]:
@@ -803,15 +804,16 @@ def gather_tokens(buffers: list[torch.Tensor], *, tokens: int, rows: torch.Tenso
 
 def keep_tokens(buffers: list[torch.Tensor], index: torch.Tensor, *, first: int, tokens: int) -> None:
     """In place, in every buffer [B, H, cap, ...]: of the slots [first, first + tokens), slot first + j becomes
-    slot first + index[j] (tq_keep_tokens).  ``index`` int [n], [B, n] or [B, H, n], n <= 256, in any order;
-    an index outside [0, tokens) gives zeros.  The slots from first + n on stay as they were."""
+    slot first + index[j] (tq_keep_tokens).  ``index`` int [n], [B, n] or [B, H, n], n <= 256 and at most 64 KB
+    of the widest rows, in any order; an index outside [0, tokens) gives zeros.  The slots from first + n on stay as they were."""
     B, H, cap, row_bytes = _move_buffers("keep_tokens", buffers)
     dev = buffers[0].device
     if first < 0 or tokens < 0 or first + tokens > cap:
         raise ValueError(f"keep_tokens: slots [{first}, {first + tokens}) of a capacity of {cap}")
     index, sb, sh, n = _token_index("keep_tokens", index, B, H, dev)
-    if n > min(tokens, MAX_KEEP):
-        raise ValueError(f"keep_tokens: {n} of {tokens} tokens (at most {MAX_KEEP}; gather_tokens takes more)")
+    if n > min(tokens, MAX_KEEP) or n * max(row_bytes) > MAX_KEEP_BYTES:
+        raise ValueError(f"keep_tokens: {n} of {tokens} tokens (at most {MAX_KEEP}, and {MAX_KEEP_BYTES} bytes of a "
+                         "buffer; gather_tokens takes more)")
     if n == 0 or B * H == 0:
         return
     for a in range(0, len(buffers), _MOVE_BUFFERS):

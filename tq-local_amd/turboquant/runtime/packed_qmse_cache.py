@@ -180,6 +180,19 @@ class _Store:
         if need > self.cap:
             self._alloc(max(need + reserve_tokens, 2 * self.cap))
 
+    def buffers(self) -> list[torch.Tensor]:
+        return [getattr(self, name) for name, entry in self.spec.items() if entry is not None]
+
+    def take(self, rows: torch.Tensor | None = None, index: torch.Tensor | None = None) -> None:
+        """These batch rows, or these tokens of every row, instead of what the store holds: new buffers of the
+        same capacity, one launch."""
+        new = K.gather_tokens(self.buffers(), tokens=self.length, rows=rows, index=index, capacity=self.cap)
+        for name, buf in zip((name for name, entry in self.spec.items() if entry is not None), new):
+            setattr(self, name, buf)
+        self.B = int(new[0].shape[0])
+        if index is not None:
+            self.length = int(index.shape[-1])
+
 
 def _flat_spec(D: int, c: LayerCodecs) -> dict[str, tuple[tuple, torch.dtype] | None]:
     spec = {"kc": ((K.row_bytes(D, c.key_bits),), torch.uint8), "kn": ((), torch.float16),
@@ -606,6 +619,75 @@ class PackedMSELayer(CacheLayerMixin):
     def get_seq_length(self) -> int:
         dense = 0 if self._dense_keys is None else int(self._dense_keys.shape[-2])
         return self.packed_seq_length() + dense
+
+    # ------------------------------------------- rows and tokens chosen and moved
+    def _take_rows(self, rows: torch.Tensor) -> None:
+        if self.get_seq_length() == 0:
+            return
+        if self._store is not None:
+            self._store.take(rows=rows)
+            self._shape = (self._store.B, *self._shape[1:])
+        if self._dense_buf is not None:
+            dense = list(self._dense_buf)
+            self._dense_buf = tuple(K.gather_tokens(dense, tokens=self._dense_len, rows=rows, capacity=dense[0].shape[2]))
+
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        """Batch row r becomes row beam_idx[r] (one launch for the packed buffers and one for the dense; a row
+        that there is not becomes zeros)."""
+        self._take_rows(beam_idx)
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        """Only these batch rows (numbers, or a bool for each row)."""
+        self._take_rows(indices.nonzero().flatten() if indices.dtype == torch.bool else indices)
+
+    def batch_repeat_interleave(self, repeats: int) -> None:
+        """Every batch row ``repeats`` times."""
+        if self.get_seq_length():
+            batch = self._store.B if self._store is not None else self._dense_buf[0].shape[0]
+            self._take_rows(torch.arange(batch, device=self.device).repeat_interleave(repeats))
+
+    def crop(self, tokens_to_remove: int) -> None:
+        """Takes the last -n tokens off for n < 0, and all past the first n for n > 0 (none for 0)."""
+        n, total = int(tokens_to_remove), self.get_seq_length()
+        drop = min(-n, total) if n < 0 else max(total - n, 0) if n else 0
+        dense = min(drop, self._dense_len)
+        self._dense_len -= dense
+        if drop > dense:
+            self._store.length -= drop - dense
+
+    def keep_tokens(self, index: torch.Tensor, tokens: int | None = None) -> None:
+        """Of the last ``tokens`` tokens (all without) only those of ``index`` [n], [B, n] or [B, H, n], counted from the
+        first of them, in that order: the accepted path of a tree of drafted tokens, or the tokens that a
+        history keeps.  They have to be all packed or all dense.  An index outside [0, tokens) gives a token
+        of zeros."""
+        total, n = self.get_seq_length(), int(index.shape[-1])
+        tokens = total if tokens is None else int(tokens)
+        if not 0 <= n <= tokens <= total:
+            raise ValueError(f"keep_tokens: {n} of the last {tokens} of {total} tokens")
+        if tokens == 0:
+            return
+        dense = self._dense_len > 0
+        length = self._dense_len if dense else self._store.length
+        if tokens > length:
+            raise ValueError(f"keep_tokens: {tokens} tokens, but the last {length} are dense and those before packed")
+        first = length - tokens
+        buffers = list(self._dense_buf) if dense else self._store.buffers()
+        widest = max(b.stride(2) * b.element_size() for b in buffers)
+        if n <= K.MAX_KEEP and n * widest <= K.MAX_KEEP_BYTES:
+            K.keep_tokens(buffers, index, first=first, tokens=tokens)
+        else:
+            # too many for the move in place: new buffers, with the tokens before them
+            index = torch.where((index < 0) | (index >= tokens), -1, index + first).to(self.device)
+            before = torch.arange(first, dtype=index.dtype, device=index.device).expand(*index.shape[:-1], first)
+            index = torch.cat((before, index), dim=-1)
+            if dense:
+                self._dense_buf = tuple(K.gather_tokens(buffers, tokens=length, index=index, capacity=buffers[0].shape[2]))
+            else:
+                self._store.take(index=index)
+        if dense:
+            self._dense_len = first + n
+        else:
+            self._store.length = first + n
 
     def get_max_length(self) -> int:
         return -1
