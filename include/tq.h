@@ -328,7 +328,7 @@ int tq_dense_attention(const void* q, int q_is_f32, int batch, int q_heads, int 
  *
  *   q, k, v  bf16, or fp16 with is_f16, [batch][heads][tokens][dim] with element strides (multiples of 8;
  *            dim contiguous, rows 16-byte aligned); q_heads a multiple of kv_heads
- *   out      the same type, likewise strided
+ *   out      the same type, likewise strided; no row of it in k, v or other rows of q
  *   lse      fp32 [batch][q_heads][tokens] log-sum-exp of the scaled logits (nullable; -inf for a row
  *            without tokens), for merging with attention over other tokens
  *   cu_seqlens  int32 [n_seqs + 1] (device, nullable), ascending: packed sequences, sequence i the rows

@@ -568,8 +568,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
     q [B, Hq, S, D], k and v [B, Hkv, S, D], bf16 or fp16, any strides with D contiguous; Hq a multiple of
     Hkv.  ``seq_starts`` / ``seq_ends`` int [B] bound each row's sequence in a padded batch (the other
     rows get 0).  ``cu_seqlens`` int [n + 1], ascending from 0: sequences packed behind one another (B = 1);
-    rows behind the last one stay as they were in a given ``out``, and are 0 otherwise.  Returns
-    [B, Hq, S, D] laid out token by token ([B, S, Hq, D] in memory), and with ``want_lse`` the fp32
+    rows behind the last one stay as they were in a given ``out``, and are 0 otherwise; ``out`` must not overlap
+    k, v or another head's q.  Returns [B, Hq, S, D] laid out token by token ([B, S, Hq, D] in memory), and with ``want_lse`` the fp32
     log-sum-exp [B, Hq, S] of the scaled logits (-inf for a row without tokens).
     """
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
@@ -601,8 +601,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
     zero_outside = out is None
     if out is None:
         out = torch.empty(B, S, Hq, D, dtype=q.dtype, device=dev).transpose(1, 2)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or rows16(out) is not out:
-        raise ValueError("out must have q's shape, dtype and device, with 16-byte aligned rows")
+    elif (out.shape != q.shape or out.dtype != q.dtype or out.device != dev or rows16(out) is not out
+          or any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape))):
+        raise ValueError("out must have q's shape, dtype and device, with 16-byte aligned rows of its own")
     lse = torch.empty(B, Hq, S, dtype=torch.float32, device=dev) if want_lse else None
     if q.numel() == 0:
         return (out, lse) if want_lse else out
