@@ -273,3 +273,50 @@ def test_values_that_are_not_finite_in_many_blocks(cuda, at):
     assert (got[:, :88, at:, 3] == float("-inf")).all() and got[:, :88, at:, 7].isnan().all()
     rest = [d for d in range(D) if d not in (3, 7)]
     check(got[..., rest], ref[..., rest], size[..., rest])
+
+
+class Module(torch.nn.Module):
+    is_causal, num_key_value_groups = True, 4
+
+
+def test_attention_interface(cuda):
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+    forward, m = ALL_ATTENTION_FUNCTIONS["turboquant_prompt"], Module()
+    q, k, v = (randn((1, h, 150, D), i, torch.bfloat16) for i, h in ((1, 8), (2, 2), (3, 2)))
+    got, _ = forward(m, q, k, v, None, scaling=0.05)
+    assert torch.equal(got, prompt_attention(q, k, v, scale=0.05).transpose(1, 2))
+    cu = torch.tensor([0, 60, 150], dtype=torch.int32, device="cuda")
+    for other in (cu, cu.clone()):
+        got, _ = forward(m, q, k, v, None, scaling=0.05, cu_seq_lens_q=cu, cu_seq_lens_k=other)
+        assert torch.equal(got, prompt_attention(q, k, v, scale=0.05, cu_seqlens=cu).transpose(1, 2))
+    # what the kernel does not take goes the other way, with the same result as there
+    other = ALL_ATTENTION_FUNCTIONS["turboquant"]
+    mask = torch.ones(1, 1, 150, 150, dtype=torch.bool, device="cuda").tril()
+    mask[..., :9] = False
+    mask[..., 0] = True
+    for args in ((q, k, v, mask), (q.float(), k.float(), v.float(), None), (q[:, :, -1:], k, v, None),
+                 (q[..., :64], k[..., :64], v[..., :64], None)):
+        assert torch.equal(forward(m, *args, scaling=0.05)[0], other(m, *args, scaling=0.05)[0])
+
+
+def test_a_models_prompt_takes_it(cuda, monkeypatch):
+    import turboquant
+    from turboquant.runtime import attention as A
+
+    from ._tiny_model import CharTokenizer, tiny_llama
+
+    calls = []
+    monkeypatch.setattr(A, "prompt_attention", lambda *a, **kw: calls.append(a[0].shape) or prompt_attention(*a, **kw))
+    model = tiny_llama(device=cuda, dtype=torch.bfloat16)
+    ids = torch.randint(0, 94, (1, 300), generator=torch.Generator().manual_seed(0)).to(cuda)
+    with torch.no_grad():
+        ref = model(ids).logits.float()
+        model.set_attn_implementation("turboquant_prompt")
+        got = model(ids).logits.float()
+    assert calls == [(1, 8, 300, D)] * 2
+    # two layers, each with a few bf16 roundings (2^-8) of activations that both sides round at other places
+    assert (got - ref).abs().max() <= 16 * 2 ** -8 * ref.abs().max()
+    turboquant.activate(model, CharTokenizer(), bits=4, use_qjl_keys=True, quiet=True)
+    assert model.generate(ids, max_new_tokens=5).shape == (1, 305)
+    assert len(calls) >= 4

@@ -6,7 +6,8 @@ the module (``module._tq_cache_layer``) a decode step runs the fused libtq
 kernel over the packed history, and several query tokens at once run
 ``chunked_turboquant_attention`` (libtq decoding, fp32 online softmax); without a
 packed layer (prefill, norm-guarded dense layers) it is plain SDPA, as in the
-reference.
+reference.  "turboquant_prompt" is the same with whole causal prompts on libtq's own
+kernel (``prompt_attention``); ``tree_attention`` is the call for drafted tokens.
 
 ``fused_attention`` replaces the reference's Triton host wrapper
 (``runtime/triton_kernels.py:238-368``) with its contract (None = not applicable,
@@ -460,19 +461,44 @@ def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, k
     return out.transpose(1, 2).contiguous(), None
 
 
+def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                              attention_mask: torch.Tensor | None, dropout: float = 0.0,
+                              scaling: float | None = None, is_causal: bool | None = None, **kwargs):
+    """HF attention-interface function "turboquant_prompt": whole causal prompts without a mask, alone or packed
+    (``cu_seq_lens_q``), go through ``prompt_attention``; what it does not take (a mask, dropout, a gradient, other
+    types, head sizes and keys than the prompt's own) and layers that hold packed tokens go the way of "turboquant".
+    One tensor as ``cu_seq_lens_q`` and ``cu_seq_lens_k`` spares a host sync that compares them."""
+    causal = getattr(module, "is_causal", True) if is_causal is None else is_causal
+    window = kwargs.get("sliding_window")
+    cu, cu_k = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
+    S = query.shape[-2]
+    if (attention_mask is None and causal and not dropout and S > 1 and query.shape[-1] == K.HEAD_DIM
+            and key.shape == value.shape and key.shape[-2:] == query.shape[-2:] and query.is_cuda
+            and query.dtype in (torch.bfloat16, torch.float16) and key.dtype == value.dtype == query.dtype
+            and (window is None or window >= S) and kwargs.get("softcap") is None and kwargs.get("s_aux") is None
+            and (cu is None or (query.shape[0] == 1 and (cu_k is None or cu_k is cu or torch.equal(cu_k, cu))))
+            and not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))):
+        layer = getattr(module, "_tq_cache_layer", None)
+        if layer is None or layer._force_dense or layer.packed_seq_length() == 0:
+            return prompt_attention(query, key, value, cu_seqlens=cu, scale=scaling).transpose(1, 2), None
+    return turboquant_attention_forward(module, query, key, value, attention_mask, dropout, scaling, is_causal, **kwargs)
+
+
 def _register_attention_backend() -> None:
-    """Register "turboquant" with HF's attention and mask interfaces (idempotent)."""
+    """Register "turboquant" and "turboquant_prompt" with HF's attention and mask interfaces (idempotent)."""
     try:
         from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
     except ImportError:  # pragma: no cover - transformers is a hard dependency of the adapter
         return
-    if "turboquant" not in ALL_ATTENTION_FUNCTIONS:
-        ALL_ATTENTION_FUNCTIONS.register("turboquant", turboquant_attention_forward)
+    for name, forward in (("turboquant", turboquant_attention_forward), ("turboquant_prompt", turboquant_prompt_forward)):
+        if name not in ALL_ATTENTION_FUNCTIONS:
+            ALL_ATTENTION_FUNCTIONS.register(name, forward)
     try:
         from transformers.masking_utils import ALL_MASK_ATTENTION_FUNCTIONS
 
-        if "turboquant" not in ALL_MASK_ATTENTION_FUNCTIONS:
-            ALL_MASK_ATTENTION_FUNCTIONS.register("turboquant", ALL_MASK_ATTENTION_FUNCTIONS["sdpa"])
+        for name in ("turboquant", "turboquant_prompt"):
+            if name not in ALL_MASK_ATTENTION_FUNCTIONS:
+                ALL_MASK_ATTENTION_FUNCTIONS.register(name, ALL_MASK_ATTENTION_FUNCTIONS["sdpa"])
     except (ImportError, KeyError):  # pragma: no cover
         pass
 
