@@ -175,9 +175,13 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // in a scalar register, and what follows from it
     const bool second = wave >= 4;
     const int part = KS == 2 && second ? 1 : 0;
-    // workgroups of one KV head share an XCD's L2 where their number divides by the eight XCDs
+    // workgroups of one KV head share an XCD's L2 where their number divides by the eight XCDs.  Ragged batches move on by a
+    // batch row with every head and block: an XCD hands its workgroups to its four groups of CUs in turn, and one long
+    // row of 1500 tokens among four (40 heads), on one group of CUs all along, took 106 us, and 47 spread over them
     const int n_kv = (a.cu ? 1 : a.batch) * a.kv_heads, group = a.q_heads / a.kv_heads;
-    const int kv = blockIdx.x % n_kv, item = blockIdx.x / n_kv;
+    const int item = blockIdx.x / n_kv;
+    int kv = blockIdx.x % n_kv;
+    if (a.starts || a.ends) kv = (int)((kv + (int64_t)item * a.kv_heads) % n_kv);
     const int kvh = kv % a.kv_heads, hq = kvh * group + item % group;
     int blk = item / group;
     Block w;
