@@ -33,6 +33,7 @@ namespace {
 
 constexpr int D = TQ_DIM;
 constexpr int TK = 32;         // tokens per tile
+constexpr int MIN_TILES = 8;   // tiles of a split
 constexpr int MAX_SPLIT = 64;  // partials a merge wave weighs with one lane each
 constexpr float LOG2E = 1.44269504f;
 constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's reference by
@@ -68,6 +69,15 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
     return __builtin_amdgcn_perm(hi, lo, sel);
+}
+// the values of lanes l and l ^ 32 joined, in both
+__device__ __forceinline__ float max_of_halves(float x) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float x) {
+    const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(y[0]) + __uint_as_float(y[1]);
 }
 __device__ __forceinline__ f32x16 fill16(float x) {
     f32x16 z;
@@ -161,10 +171,6 @@ __device__ __forceinline__ void expand_signs(uint32_t w, uint4* out) {
 
 __device__ __forceinline__ int swizzle(int token) { return ((token & 3) << 2) | ((token >> 2) & 3); }
 
-__device__ __forceinline__ void load_lds16(const void* g, void* l) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g,
-                                     (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
-}
 __device__ __forceinline__ s16x4 read_tr(const uint8_t* l) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)l);
 }
@@ -177,24 +183,6 @@ __device__ __forceinline__ int value_offset(int d, int e, int lane) {
 }
 
 // ------------------------------------------------------------------ queries
-
-struct PrepArgs {
-    const void* q;
-    int q_type;  // 0 bf16, 1 fp32, 2 fp16
-    int q_heads, kv_heads, T, rows;
-    int64_t q_sb, q_sh, q_st;
-    const float *rk, *s;
-    int key_bits;
-    float c2;       // scale log2(e)
-    uint4* frags;   // [kv head][row block][2][8 steps][64 lanes]
-    float* row_c;   // [kv head][row block][2][32] c2 over the row's power of two, and what a row's sign products start from
-};
-
-__device__ __forceinline__ float query_element(const PrepArgs& a, int64_t i) {
-    if (a.q_type == 0) return tq::bf16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
-    if (a.q_type == 1) return static_cast<const float*>(a.q)[i];
-    return tq::f16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
-}
 
 // fp32 pairs to bf16 terms, truncated: x - hi and (x - hi) - mid are exact, and three terms hold all 24 bits
 __device__ __forceinline__ uint32_t high_halves(float a, float b) {
@@ -217,7 +205,9 @@ __device__ __forceinline__ void split_terms(const float* x, Frag* t) {
 // Where dim j stands among a key's 128 operands: 16 chunks of 8 elements, chunk 2 s + h the lanes' operand of step s for
 // dims [64 h, 64 h + 64).  What meets in a register follows from the packing: codes of one and of three bits are at the same
 // bits of bytes 8 codes apart, of two bits 4 apart, of four bits 2 apart (2^log_st); signs are taken 16 apart.
-__device__ __forceinline__ int position_of(int log_st, int j) {
+template <int KB>
+__device__ __forceinline__ int position_of(int j) {
+    constexpr int log_st = KB == 4 ? 1 : KB == 2 ? 2 : 3;
     const int st = 1 << log_st, x = j & 63, y = x & (4 * st - 1), z = y & (st - 1);
     const int s = ((x >> (log_st + 2)) << (log_st - 1)) + (z >> 1);
     return (2 * s + (j >> 6)) * 8 + 4 * (z & 1) + (y >> log_st);
@@ -225,110 +215,6 @@ __device__ __forceinline__ int position_of(int log_st, int j) {
 __device__ __forceinline__ int sign_position_of(int j) {
     const int x = j & 63, n = x & 15, s = 4 * (x >> 5) + (n >> 2);
     return (2 * s + (j >> 6)) * 8 + 2 * (n & 3) + ((x >> 4) & 1);
-}
-
-// One workgroup: 32 query rows of a KV head against R_k and S, wave w their rows [32 w, 32 w + 32), as products of bf16
-// terms: a bf16 query is one, any other three, the matrices three; what is left out is 2^-24 of a product.
-//
-// A few workgroups that run once: what they wait for is memory and their own instructions, so the matrices come in all
-// at once, past the registers, and the loops stay rolled (unrolled, each of ~2500 instructions was a trip to memory: 11 us).
-template <int NQ>
-__global__ __launch_bounds__(256) void prep_kernel(PrepArgs a) {
-    // the matrices' 16-byte chunks are xor-swizzled by the row, those of the operands too
-    __shared__ uint4 s_m[2][128 * 32];
-    __shared__ uint4 s_f[2][32 * 16];  // [row][chunk]
-    __shared__ float s_top[4][32], s_sum[4][32];
-    const int blk = blockIdx.x, kv = blockIdx.y, lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int mats = a.s ? 2 : 1;
-#pragma unroll 1
-    for (int i = wave; i < mats * 64; i += 4) {  // 64 chunks, two rows, a time
-        const int at = (i & 63) * 64 + lane, row = at >> 5;
-        const float* const m = i < 64 ? a.rk : a.s;
-        load_lds16(m + row * D + 4 * ((at & 31) ^ (row & 31)), &s_m[i >> 6][(i & 63) * 64]);
-    }
-    const int b = kv / a.kv_heads, kvh = kv - b * a.kv_heads, group = a.q_heads / a.kv_heads;
-    const int row = 32 * blk + r;
-    const bool live = row < a.rows;
-    const int g = live ? row / a.T : 0, t = live ? row - g * a.T : 0;
-    const int64_t at = b * a.q_sb + (int64_t)(kvh * group + g) * a.q_sh + (int64_t)t * a.q_st + 8 * h;
-    Frag q[8][NQ];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-        if constexpr (NQ == 1) {
-            __builtin_memcpy(&q[s][0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);
-            if (!live) q[s][0].q = make_uint4(0u, 0u, 0u, 0u);
-        } else {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = live ? query_element(a, at + 16 * s + e) : 0.0f;
-            split_terms<NQ>(x, q[s]);
-        }
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's part of the matrices, ahead of the barrier
-    __syncthreads();
-    // this lane: row r's dims 32 wave + 8 j + 4 h + (0..3) of both
-    f32x16 acc[2] = {zero16(), zero16()};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        if (k == 1 && mats == 1) break;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            float e[8];
-            __builtin_memcpy(e, &s_m[k][(32 * wave + r) * 32 + ((4 * s + 2 * h) ^ r)], 16);
-            __builtin_memcpy(e + 4, &s_m[k][(32 * wave + r) * 32 + ((4 * s + 2 * h + 1) ^ r)], 16);
-            Frag m[3];
-            split_terms<3>(e, m);
-#pragma unroll
-            for (int i = 2; i >= 0; --i)
-#pragma unroll
-                for (int j = NQ - 1; j >= 0; --j)
-                    if (i + j <= 2) acc[k] = mfma_bf16(m[i], q[s][j], acc[k]);
-        }
-    }
-    float top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        acc[1][i] *= QJL_SCALE;
-        top = fmaxf(top, fmaxf(fabsf(acc[0][i]), fabsf(acc[1][i])));
-    }
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (h == 0) s_top[wave][r] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_top[0][r], s_top[1][r]), fmaxf(s_top[2][r], s_top[3][r]));
-    // largest element in [2^7, 2^8); rows of zeros, and with an infinity, as they are
-    int e = 0;
-    if (top > 0.0f && top < __builtin_inff()) e = std::min(126, 7 + 127 - (int)((__float_as_uint(top) >> 23) & 0xFF));
-    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-    float sum = 0.0f;
-    const int log_st = a.key_bits == 4 ? 1 : a.key_bits == 2 ? 2 : 3;
-    auto put = [&](int m, int p, uint32_t x) {
-        reinterpret_cast<uint16_t*>(s_f[m])[r * 128 + (((p >> 3) ^ (r & 15)) << 3) + (p & 7)] = (uint16_t)x;
-    };
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int j = 32 * wave + 8 * (i >> 2) + 4 * h + (i & 3);
-        put(0, position_of(log_st, j), tq::f32_to_f16(acc[0][i] * up));
-        const float x = tq::f16_to_f32(tq::f32_to_f16(acc[1][i] * up));
-        sum += x;
-        put(1, sign_position_of(j), tq::f32_to_f16(x * (float)(128 >> (j & 7))));
-    }
-    sum += __shfl_xor(sum, 32);
-    if (h == 0) s_sum[wave][r] = sum;
-    __syncthreads();
-    const int64_t out = (int64_t)kv * gridDim.x + blk;
-    if (threadIdx.x < 32) {
-        // what the scores take from the set bits' products, in units of 2^-17, to the signs'
-        const float all = s_sum[0][r] + s_sum[1][r] + s_sum[2][r] + s_sum[3][r];
-        a.row_c[out * 64 + r] = a.c2 * __uint_as_float((uint32_t)(127 - e) << 23);
-        a.row_c[out * 64 + 32 + r] = -0x1p-18f * all;
-    }
-    uint4* const frags = a.frags + out * 2 * 8 * 64;
-#pragma unroll 1
-    for (int i = threadIdx.x; i < mats * 512; i += 256) {
-        const int m = i >> 9, s = (i >> 6) & 7, l = i & 63;
-        frags[i] = s_f[m][(l & 31) * 16 + ((2 * s + (l >> 5)) ^ (l & 15))];
-    }
 }
 
 // ------------------------------------------------------------------ attention
@@ -342,12 +228,19 @@ struct TreeArgs {
     const uint8_t *k_codes, *k_signs, *v_codes;
     const uint16_t *k_norms, *k_rnorms, *v_norms;
     const float *key_centers, *value_centers;
-    const uint4* frags;
-    const float* row_c;
+    const void* q;
+    int q_type, q_heads;
+    int64_t q_sb, q_sh, q_st;
+    const float *rk, *s;
+    float c2;  // scale log2(e)
     int n_split;
     float* part_o;   // [split][kv head][row][D]
     float2* part_ms; // [split][kv head][row] (reference of the weights in log2, sum of weights)
 };
+
+__device__ __forceinline__ float query_element(const TreeArgs& a, int64_t i) {
+    return a.q_type == 1 ? static_cast<const float*>(a.q)[i] : tq::f16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
+}
 
 // Bit j of a node's mask: node j is the node itself or one of its ancestors.  A parent that is not an earlier
 // node is none.  Called by one whole wave, lane = node.
@@ -428,7 +321,7 @@ struct Tree {
         uint32_t table[256 * 64];
         uint4 v[W][16 * 16];
         // the rows' operands for the signs, and with two blocks of rows those for the codes: they do not fit the registers
-        uint4 qs[RB][8 * 64], qc[RB == 1 ? 1 : RB][RB == 1 ? 1 : 8 * 64];
+        uint4 qs[RB][8 * 64], qc[RB][8 * 64];
         uint16_t kn[W][32], vn[W][32];
         float ratio[W][32];
     };
@@ -443,14 +336,15 @@ struct Tree {
     };
 };
 
-template <int KB, int VB, bool QJL, int RB>
+template <int KB, int VB, bool QJL, int RB, int NQ>
 __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
     using N = Tree<RB>;
     constexpr int W = N::W;
     __shared__ typename N::Lds lds;
     __shared__ uint64_t s_anc[64];
     __shared__ float s_centers[1 << VB];
-    const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+    __shared__ float s_top[W][32], s_sum[RB][4][32], s_c[RB][32];
+    int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // in a scalar register, and what follows from it
     const int kv = blockIdx.x / a.n_split, split = blockIdx.x - kv * a.n_split;
     const int b = kv / a.kv_heads;
@@ -493,29 +387,109 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
         }
     };
     int64_t tile = first_tile + wave;
-    if (tile < last_tile) load_keys(tile), load_values(tile);
+    if (RB == 1 && tile < last_tile) load_keys(tile), load_values(tile);
 
     Lut<KB> klut;
     klut.load(a.key_centers);
+    // ---- the queries: q R_k^T and q S^T as products of bf16 terms, a bf16 query one, any other three, the matrices three (what is left
+    // out is 2^-24 of a product); a wave has 32 output dims of one of the matrices.  Scaled by a power of two per row,
+    // to a largest element in [2^7, 2^8), they go to fp16 operands in LDS
+    {
+        const int mat = wave >> 2, j0 = 32 * (wave & 3), group = a.q_heads / a.kv_heads;
+        const bool works = QJL || mat == 0;
+        float mrow[8][8];
+        if (works) {
+            const float* const src = (mat ? a.s : a.rk) + (j0 + r) * D + 8 * h;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) __builtin_memcpy(mrow[s], __builtin_assume_aligned(src + 16 * s, 16), 32);
+        }
+#pragma unroll 1
+        for (int m = 0; m < RB; ++m) {
+            const int row = 32 * ((int)blockIdx.y * RB + m) + r;
+            const bool live = row < a.rows;
+            const int g = live ? row / a.T : 0, t = live ? row - g * a.T : 0;
+            const int64_t at = b * a.q_sb + (int64_t)((kv - b * a.kv_heads) * group + g) * a.q_sh + (int64_t)t * a.q_st + 8 * h;
+            Frag x[8][NQ];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                if constexpr (NQ == 1) {
+                    __builtin_memcpy(&x[s][0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);
+                    if (!live) x[s][0].q = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = live ? query_element(a, at + 16 * s + e) : 0.0f;
+                    split_terms<NQ>(y, x[s]);
+                }
+            }
+            f32x16 acc = zero16();
+            if (works) {
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    Frag mt[3];
+                    split_terms<3>(mrow[s], mt);
+#pragma unroll
+                    for (int i = 2; i >= 0; --i)
+#pragma unroll
+                        for (int j = NQ - 1; j >= 0; --j)
+                            if (i + j <= 2) acc = mfma_bf16(mt[i], x[s][j], acc);
+                }
+            }
+            // this lane: row r's dims j0 + 8 j + 4 h + (0..3)
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (mat) acc[i] *= QJL_SCALE;
+                most = fmaxf(most, fabsf(acc[i]));
+            }
+            most = max_of_halves(most);
+            if (h == 0) s_top[wave][r] = most;
+            __syncthreads();
+            most = 0.0f;
+#pragma unroll
+            for (int k = 0; k < (QJL ? 8 : 4); ++k) most = fmaxf(most, s_top[k][r]);
+            // rows of zeros, and with an infinity, as they are
+            int e = 0;
+            if (most > 0.0f && most < __builtin_inff()) e = std::min(126, 7 + 127 - (int)((__float_as_uint(most) >> 23) & 0xFF));
+            const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+            auto put = [&](uint4* to, int p, uint32_t y) {  // chunk p / 8 = 2 s + h is what lane 32 h + r takes in step s
+                reinterpret_cast<uint16_t*>(to + (p >> 4) * 64 + ((p >> 3) & 1) * 32 + r)[p & 7] = (uint16_t)y;
+            };
+            if (mat == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    put(lds.t.qc[m], position_of<KB>(j0 + 8 * (i >> 2) + 4 * h + (i & 3)), tq::f32_to_f16(acc[i] * up));
+            } else if (QJL) {
+                float all = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = j0 + 8 * (i >> 2) + 4 * h + (i & 3);
+                    const float y = tq::f16_to_f32(tq::f32_to_f16(acc[i] * up));
+                    all += y;
+                    put(lds.t.qs[m], sign_position_of(j), tq::f32_to_f16(y * (float)(128 >> (j & 7))));
+                }
+                all = sum_of_halves(all);
+                if (h == 0) s_sum[m][wave & 3][r] = all;
+            }
+            if (threadIdx.x < 32) s_c[m][r] = a.c2 * __uint_as_float((uint32_t)(127 - e) << 23);
+            __syncthreads();
+        }
+    }
+    // nothing of the above stays in registers for the loop
+    asm volatile("" : "+v"(lane));
+    r = lane & 31, h = lane >> 5;
+    if (RB > 1 && tile < last_tile) load_keys(tile), load_values(tile);
     Frag q[8];  // with one block of rows
     float c[RB], sign0[RB];
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
-        const int blk = std::min((int)blockIdx.y * RB + m, a.row_blocks - 1);
-        const int64_t at = (int64_t)kv * a.row_blocks + blk;
-        const uint4* f = a.frags + at * 2 * 8 * 64;
-        if constexpr (RB == 1) {
-#pragma unroll
-            for (int s = 0; s < 8; ++s) q[s].q = f[s * 64 + lane];
-        } else {
-            lds.t.qc[m][threadIdx.x] = f[threadIdx.x];
-        }
-        if constexpr (QJL) lds.t.qs[m][threadIdx.x] = f[8 * 64 + threadIdx.x];
-        c[m] = a.row_c[at * 64 + r];
-        sign0[m] = QJL ? a.row_c[at * 64 + 32 + r] : 0.0f;
+        c[m] = s_c[m][r];
+        // what the scores take from the set bits' products, in units of 2^-17, to the signs'
+        sign0[m] = QJL ? -0x1p-18f * (s_sum[m][0][r] + s_sum[m][1][r] + s_sum[m][2][r] + s_sum[m][3][r]) : 0.0f;
     }
-    static_assert(N::T == 8 * 64, "a thread copies one fragment of each kind");
-    __syncthreads();
+    if constexpr (RB == 1)
+#pragma unroll
+        for (int s = 0; s < 8; ++s) q[s].q = lds.t.qc[0][s * 64 + lane];
     PairTable<VB>::build(lds.t.table, s_centers, N::T);
     uint64_t sees[RB];
 #pragma unroll
@@ -601,10 +575,14 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
         const int e5 = (norm >> 10) & 31, ve = e5 == 31 ? 0 : e5;
         int need = 0;  // uniform: by how much the unit has to rise
         if (__any(ve > 14 + TOP_BIT - shift)) {
-            int e = ve;
+            int e = 0;
+            uint64_t largest = ~0ull;
 #pragma unroll
-            for (int k = 1; k < 32; k <<= 1) e = std::max(e, __shfl_xor(e, k));
-            need = shift - (14 + TOP_BIT - std::max(__builtin_amdgcn_readfirstlane(e), 1));
+            for (int k = 4; k >= 0; --k) {
+                const uint64_t set = __ballot(ve >> k & 1) & largest;
+                if (set) largest = set, e |= 1 << k;
+            }
+            need = shift - (14 + TOP_BIT - std::max(e, 1));
         }
         shift -= need;
         if (tile + W < last_tile) load_keys(tile + W);
@@ -631,7 +609,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
             for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[m][i]);
             // neither -inf nor NaN raises the reference
             if (__any(__builtin_fmaf(mx, c[m], -top[m]) > LAZY) || need) {
-                mx = fmaxf(mx, __shfl_xor(mx, 32)) * c[m];
+                mx = max_of_halves(mx) * c[m];
                 const float ref = mx > top[m] ? mx : top[m];
                 const float corr = exp2_(top[m] == ref ? -(float)need : top[m] - ref - (float)need);
                 top[m] = ref;
@@ -696,7 +674,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
         __syncthreads();
-        const float all = sum[m] + __shfl_xor(sum[m], 32);
+        const float all = sum_of_halves(sum[m]);
         if (h == 0) lds.s.ms[wave][r] = make_float2(top[m], all * unit);
 #pragma unroll
         for (int d = 0; d < 4; ++d)
@@ -833,8 +811,8 @@ struct Plan {
     int rows, row_blocks, n_split;
     unsigned row_groups;
     int64_t heads;
-    size_t frag_bytes, row_c_bytes, ms_bytes, o_bytes;
-    size_t total() const { return frag_bytes + row_c_bytes + ms_bytes + o_bytes; }
+    size_t ms_bytes, o_bytes;
+    size_t total() const { return ms_bytes + o_bytes; }
 };
 
 // A workgroup fills a CU.  As many splits as fill the CUs, as long as none is left without a tile.
@@ -846,10 +824,8 @@ bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Pl
     p.row_blocks = (p.rows + 31) / 32;
     p.row_groups = p.row_blocks == 1 ? 1 : (unsigned)(p.row_blocks + 1) / 2;
     const int64_t tiles = std::max<int64_t>(1, (n_tokens + TK - 1) / TK);
-    p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({256 / (p.heads * p.row_groups), tiles, MAX_SPLIT}));
+    p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({256 / (p.heads * p.row_groups), (tiles + MIN_TILES - 1) / MIN_TILES, MAX_SPLIT}));
     const int64_t all = p.heads * p.rows;
-    p.frag_bytes = (size_t)(p.heads * p.row_blocks) * 2 * 8 * 64 * 16;
-    p.row_c_bytes = (size_t)(p.heads * p.row_blocks) * 64 * 4;
     p.ms_bytes = ((size_t)all * p.n_split * 8 + 15) / 16 * 16;
     p.o_bytes = (size_t)all * p.n_split * D * 4;
     return true;
@@ -858,8 +834,14 @@ bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Pl
 template <int KB, int VB, bool QJL>
 void launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
     const dim3 grid((unsigned)(p.heads * p.n_split), p.row_groups);
-    if (p.row_blocks == 1) hipLaunchKernelGGL((tree_kernel<KB, VB, QJL, 1>), grid, dim3(Tree<1>::T), 0, s, a);
-    else hipLaunchKernelGGL((tree_kernel<KB, VB, QJL, 2>), grid, dim3(Tree<2>::T), 0, s, a);
+    auto launch = [&](auto rb, auto nq) {
+        hipLaunchKernelGGL((tree_kernel<KB, VB, QJL, rb, nq>), grid, dim3(Tree<rb>::T), 0, s, a);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    using Three = std::integral_constant<int, 3>;
+    if (p.row_blocks == 1) a.q_type == 0 ? launch(One{}, One{}) : launch(One{}, Three{});
+    else a.q_type == 0 ? launch(Two{}, One{}) : launch(Two{}, Three{});
 }
 
 }  // namespace
@@ -896,20 +878,12 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
     if (!make_plan(batch, q_heads, kv_heads, nodes, n_tokens, p)) return TQ_ERR_UNSUPPORTED;
     if (!workspace || workspace_bytes < p.total() || !aligned16(workspace)) return TQ_ERR_WORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    uint4* frags = reinterpret_cast<uint4*>(ws);
-    float* part_o = reinterpret_cast<float*>(ws + p.frag_bytes);
-    float2* part_ms = reinterpret_cast<float2*>(ws + p.frag_bytes + p.o_bytes);
-    float* row_c = reinterpret_cast<float*>(ws + p.frag_bytes + p.o_bytes + p.ms_bytes);
+    float* part_o = reinterpret_cast<float*>(ws);
+    float2* part_ms = reinterpret_cast<float2*>(ws + p.o_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const PrepArgs prep{q, q_type, q_heads, kv_heads, nodes, p.rows, q_sb, q_sh, q_st, key_rotation,
-                        has_qjl ? qjl : nullptr, key_bits, scale * LOG2E, frags, row_c};
-    const dim3 prep_grid((unsigned)p.row_blocks, (unsigned)p.heads);
-    if (q_type == 0) hipLaunchKernelGGL(prep_kernel<1>, prep_grid, dim3(256), 0, s, prep);
-    else hipLaunchKernelGGL(prep_kernel<3>, prep_grid, dim3(256), 0, s, prep);
-    TQ_CHECK_LAUNCH();
     const TreeArgs a{kv_heads, nodes, p.rows, p.row_blocks, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
-                     k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, frags, row_c,
-                     p.n_split, part_o, part_ms};
+                     k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, q, q_type, q_heads,
+                     q_sb, q_sh, q_st, key_rotation, qjl, scale * LOG2E, p.n_split, part_o, part_ms};
     if (has_qjl) {
         if (value_bits == 4) launch_tree<3, 4, true>(a, p, s);
         else if (value_bits == 3) launch_tree<2, 3, true>(a, p, s);
