@@ -40,9 +40,12 @@ constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's referenc
 constexpr int TOP_BIT = 7;    // largest weight times norm at the reference: 2^TOP_BIT
 constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
 
+#define INLINE __attribute__((always_inline))
+
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -184,11 +187,7 @@ __device__ __forceinline__ int value_offset(int d, int e, int lane) {
 
 // ------------------------------------------------------------------ queries
 
-// fp32 pairs to bf16 terms, truncated: x - hi and (x - hi) - mid are exact, and three terms hold all 24 bits
-__device__ __forceinline__ uint32_t high_halves(float a, float b) {
-    return perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-}
-__device__ __forceinline__ float drop_high(float a) { return a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u); }
+// fp32 pairs to bf16 terms to nearest: two leave out 2^-18 of a number (half a step of each is 2^-9 of what is left)
 template <int N>
 __device__ __forceinline__ void split_terms(const float* x, Frag* t) {
 #pragma unroll
@@ -196,8 +195,9 @@ __device__ __forceinline__ void split_terms(const float* x, Frag* t) {
         float a = x[2 * k], b = x[2 * k + 1];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            t[n].u[k] = high_halves(a, b);
-            a = drop_high(a), b = drop_high(b);
+            const f32x2 p = {a, b};
+            t[n].u[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
+            a -= __uint_as_float(t[n].u[k] << 16), b -= __uint_as_float(t[n].u[k] & 0xFFFF0000u);
         }
     }
 }
@@ -205,16 +205,20 @@ __device__ __forceinline__ void split_terms(const float* x, Frag* t) {
 // Where dim j stands among a key's 128 operands: 16 chunks of 8 elements, chunk 2 s + h the lanes' operand of step s for
 // dims [64 h, 64 h + 64).  What meets in a register follows from the packing: codes of one and of three bits are at the same
 // bits of bytes 8 codes apart, of two bits 4 apart, of four bits 2 apart (2^log_st); signs are taken 16 apart.
+// Both orders permute the bits of j: the place of j is the sum of those of its parts.
 template <int KB>
-__device__ __forceinline__ int position_of(int j) {
-    constexpr int log_st = KB == 4 ? 1 : KB == 2 ? 2 : 3;
-    const int st = 1 << log_st, x = j & 63, y = x & (4 * st - 1), z = y & (st - 1);
+__device__ __forceinline__ constexpr int position_of(int j) {
+    const int log_st = KB == 4 ? 1 : KB == 2 ? 2 : 3, st = 1 << log_st, x = j & 63, y = x & (4 * st - 1), z = y & (st - 1);
     const int s = ((x >> (log_st + 2)) << (log_st - 1)) + (z >> 1);
     return (2 * s + (j >> 6)) * 8 + 4 * (z & 1) + (y >> log_st);
 }
-__device__ __forceinline__ int sign_position_of(int j) {
+__device__ __forceinline__ constexpr int sign_position_of(int j) {
     const int x = j & 63, n = x & 15, s = 4 * (x >> 5) + (n >> 2);
     return (2 * s + (j >> 6)) * 8 + 2 * (n & 3) + ((x >> 4) & 1);
+}
+// byte offset of a place: chunk p / 8 = 2 s + h is what lane 32 h + r takes in step s
+__device__ __forceinline__ constexpr int operand_offset(int p) {
+    return (p >> 4) * 1024 + ((p >> 3) & 1) * 512 + 2 * (p & 7);
 }
 
 // ------------------------------------------------------------------ attention
@@ -391,9 +395,9 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
 
     Lut<KB> klut;
     klut.load(a.key_centers);
-    // ---- the queries: q R_k^T and q S^T as products of bf16 terms, a bf16 query one, any other three, the matrices three (what is left
-    // out is 2^-24 of a product); a wave has 32 output dims of one of the matrices.  Scaled by a power of two per row,
-    // to a largest element in [2^7, 2^8), they go to fp16 operands in LDS
+    // ---- the queries: q R_k^T and q S^T as products of bf16 terms, a bf16 query one, any other two, the matrices two (what is
+    // left out, 2^-17 of a product, is 2^-5 of what the rounding to fp16 below may take); a wave has 32 output dims of one of
+    // the matrices.  Scaled by a power of two per row, to a largest element in [2^7, 2^8), they go to fp16 operands in LDS
     {
         const int mat = wave >> 2, j0 = 32 * (wave & 3), group = a.q_heads / a.kv_heads;
         const bool works = QJL || mat == 0;
@@ -426,13 +430,13 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
             if (works) {
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
-                    Frag mt[3];
-                    split_terms<3>(mrow[s], mt);
+                    Frag mt[2];
+                    split_terms<2>(mrow[s], mt);
 #pragma unroll
-                    for (int i = 2; i >= 0; --i)
+                    for (int i = 1; i >= 0; --i)
 #pragma unroll
                         for (int j = NQ - 1; j >= 0; --j)
-                            if (i + j <= 2) acc = mfma_bf16(mt[i], x[s][j], acc);
+                            if (i + j <= 1) acc = mfma_bf16(mt[i], x[s][j], acc);
                 }
             }
             // this lane: row r's dims j0 + 8 j + 4 h + (0..3)
@@ -452,21 +456,24 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
             int e = 0;
             if (most > 0.0f && most < __builtin_inff()) e = std::min(126, 7 + 127 - (int)((__float_as_uint(most) >> 23) & 0xFF));
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-            auto put = [&](uint4* to, int p, uint32_t y) {  // chunk p / 8 = 2 s + h is what lane 32 h + r takes in step s
-                reinterpret_cast<uint16_t*>(to + (p >> 4) * 64 + ((p >> 3) & 1) * 32 + r)[p & 7] = (uint16_t)y;
+            auto put = [&](uint4* to, int lane_offset, int offset, uint32_t y) INLINE {
+                *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(to) + lane_offset + offset) = (uint16_t)y;
             };
             if (mat == 0) {
+                const int at0 = operand_offset(position_of<KB>(j0 + 4 * h)) + 16 * r;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    put(lds.t.qc[m], position_of<KB>(j0 + 8 * (i >> 2) + 4 * h + (i & 3)), tq::f32_to_f16(acc[i] * up));
+                    put(lds.t.qc[m], at0, operand_offset(position_of<KB>(8 * (i >> 2) + (i & 3))), tq::f32_to_f16(acc[i] * up));
             } else if (QJL) {
+                const int at0 = operand_offset(sign_position_of(j0 + 4 * h)) + 16 * r;
+                const float bit = h ? 8.0f : 128.0f;  // 2^(7 - j mod 8) is this 2^(-i mod 4)
                 float all = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int j = j0 + 8 * (i >> 2) + 4 * h + (i & 3);
                     const float y = tq::f16_to_f32(tq::f32_to_f16(acc[i] * up));
                     all += y;
-                    put(lds.t.qs[m], sign_position_of(j), tq::f32_to_f16(y * (float)(128 >> (j & 7))));
+                    put(lds.t.qs[m], at0, operand_offset(sign_position_of(8 * (i >> 2) + (i & 3))),
+                        tq::f32_to_f16(y * (bit / (1 << (i & 3)))));
                 }
                 all = sum_of_halves(all);
                 if (h == 0) s_sum[m][wave & 3][r] = all;
@@ -839,9 +846,8 @@ void launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
     };
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
-    using Three = std::integral_constant<int, 3>;
-    if (p.row_blocks == 1) a.q_type == 0 ? launch(One{}, One{}) : launch(One{}, Three{});
-    else a.q_type == 0 ? launch(Two{}, One{}) : launch(Two{}, Three{});
+        if (p.row_blocks == 1) a.q_type == 0 ? launch(One{}, One{}) : launch(One{}, Two{});
+    else a.q_type == 0 ? launch(Two{}, One{}) : launch(Two{}, Two{});
 }
 
 }  // namespace
