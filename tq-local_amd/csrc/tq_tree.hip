@@ -174,6 +174,11 @@ __device__ __forceinline__ void expand_signs(uint32_t w, uint4* out) {
 
 __device__ __forceinline__ int swizzle(int token) { return ((token & 3) << 2) | ((token >> 2) & 3); }
 
+__device__ __forceinline__ void load_lds16(const void* g, void* l) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g,
+                                     (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ s16x4 read_tr(const uint8_t* l) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)l);
 }
@@ -224,7 +229,7 @@ __device__ __forceinline__ constexpr int operand_offset(int p) {
 // ------------------------------------------------------------------ attention
 
 struct TreeArgs {
-    int kv_heads, T, rows, row_blocks;
+    int kv_heads, T, rows;
     const int32_t* parents;
     int64_t parents_sb;
     const int32_t *starts, *lens;
@@ -233,7 +238,7 @@ struct TreeArgs {
     const uint16_t *k_norms, *k_rnorms, *v_norms;
     const float *key_centers, *value_centers;
     const void* q;
-    int q_type, q_heads;
+    int q_type, group;  // query heads per KV head
     int64_t q_sb, q_sh, q_st;
     const float *rk, *s;
     float c2;  // scale log2(e)
@@ -247,9 +252,8 @@ __device__ __forceinline__ float query_element(const TreeArgs& a, int64_t i) {
 }
 
 // Bit j of a node's mask: node j is the node itself or one of its ancestors.  A parent that is not an earlier
-// node is none.  Called by one whole wave, lane = node.
-__device__ __forceinline__ uint64_t ancestors(const int32_t* parents, int T, int lane) {
-    int p = lane < T ? parents[lane] : -1;
+// node is none.  Called by one whole wave, lane = node, with the node's parent.
+__device__ __forceinline__ uint64_t ancestors(int p, int lane) {
     if (p < 0 || p >= lane) p = -1;
     uint64_t mask = 1ull << lane;
 #pragma unroll
@@ -335,6 +339,7 @@ struct Tree {
         float unit[W];
     };
     union Lds {
+        uint4 m[2 * 128 * 32];
         Tiles t;
         Sums s;
     };
@@ -350,8 +355,36 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
     __shared__ float s_top[W][32], s_sum[RB][4][32], s_c[RB][32];
     int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // in a scalar register, and what follows from it
-    const int kv = blockIdx.x / a.n_split, split = blockIdx.x - kv * a.n_split;
-    const int b = kv / a.kv_heads;
+    const int kvh = blockIdx.y, b = blockIdx.z, kv = b * a.kv_heads + kvh;
+    const int row_group = RB == 1 ? 0 : blockIdx.x / a.n_split, split = blockIdx.x - row_group * a.n_split;
+
+    // ---- What the queries' rotation takes is asked for first, then a first tile of the cache, then the small things: a workgroup of a
+    // short history waits for memory once.  The matrices come by way of LDS: read straight into operands, 32 rows at a time, they
+    // were 10000 cycles on their way.  Their 16-byte chunks are xor-swizzled by the row
+#pragma unroll
+    for (int i = 0; i < (QJL ? 16 : 8); ++i) {  // 64 chunks, two rows, a time
+        const int at = (8 * i + wave) * 64 + lane, row = (at >> 5) & 127;
+        load_lds16((i < 8 ? a.rk : a.s) + row * D + 4 * ((at & 31) ^ (row & 31)), &lds.m[(8 * i + wave) * 64]);
+    }
+    Frag x[8][NQ];  // a block's queries: lane (r, h) has row r's dims 16 s + 8 h + (0..7)
+    auto load_queries = [&](int m) INLINE {
+        const int row = 32 * (row_group * RB + m) + r;
+        const bool live = row < a.rows;
+        const uint32_t g = live ? (uint32_t)row / (uint32_t)a.T : 0u, t = live ? row - g * a.T : 0u;
+        const int64_t at = b * a.q_sb + (int64_t)(kvh * a.group + g) * a.q_sh + t * a.q_st + 8 * h;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            if constexpr (NQ == 1) {
+                __builtin_memcpy(&x[s][0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);  // rows past the last: some row
+            } else {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = query_element(a, at + 16 * s + e);
+                split_terms<NQ>(y, x[s]);
+            }
+        }
+    };
+    load_queries(0);
 
     const int nodes = a.parents ? a.T : 0;
     int64_t end = a.lens ? a.lens[b] : a.n_tokens - nodes;
@@ -359,11 +392,8 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
     int64_t lo = a.starts ? a.starts[b] : 0;
     lo = std::min<int64_t>(std::max<int64_t>(lo, 0), end);
     const int64_t stop = std::min<int64_t>(end + nodes, a.n_tokens);
-    const uint32_t tiles = (uint32_t)((stop - lo + TK - 1) / TK), each = tiles / a.n_split, more = tiles - each * a.n_split;
-    const int64_t first_tile = split * each + std::min<uint32_t>(split, more), last_tile = first_tile + each + ((uint32_t)split < more);
-
-    if (threadIdx.x < (1 << VB)) s_centers[threadIdx.x] = a.value_centers[threadIdx.x];
-    if (nodes && wave == 0) s_anc[lane] = ancestors(a.parents + b * a.parents_sb, a.T, lane);
+    const int64_t tiles = (stop - lo + TK - 1) / TK;
+    const int step_tiles = a.n_split * W;  // tiles in turn, to the waves of all splits
 
     // a lane's part of a tile, on its way: half of token r's key codes and signs and its norms, and a quarter of the value
     // codes of tokens lane % 16 and lane % 16 + 16.  The arrays are at scalar addresses, a lane's place in them 32-bit
@@ -390,42 +420,37 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
                              4 * VB);
         }
     };
-    int64_t tile = first_tile + wave;
-    if (RB == 1 && tile < last_tile) load_keys(tile), load_values(tile);
-
-    Lut<KB> klut;
-    klut.load(a.key_centers);
-    // ---- the queries: q R_k^T and q S^T as products of bf16 terms, a bf16 query one, any other two, the matrices two (what is
-    // left out, 2^-17 of a product, is 2^-5 of what the rounding to fp16 below may take); a wave has 32 output dims of one of
-    // the matrices.  Scaled by a power of two per row, to a largest element in [2^7, 2^8), they go to fp16 operands in LDS
-    {
-        const int mat = wave >> 2, j0 = 32 * (wave & 3), group = a.q_heads / a.kv_heads;
-        const bool works = QJL || mat == 0;
-        float mrow[8][8];
-        if (works) {
-            const float* const src = (mat ? a.s : a.rk) + (j0 + r) * D + 8 * h;
+    int64_t tile = split * W + wave;
+    if (RB == 1 && tile < tiles) load_keys(tile), load_values(tile);
+    float key_center[1 << KB];
 #pragma unroll
-            for (int s = 0; s < 8; ++s) __builtin_memcpy(mrow[s], __builtin_assume_aligned(src + 16 * s, 16), 32);
-        }
+    for (int i = 0; i < (1 << KB); ++i) key_center[i] = a.key_centers[i];
+    float value_center = 0.0f;
+    if (threadIdx.x < (1 << VB)) value_center = a.value_centers[threadIdx.x];
+    int parent = -1;
+    if (nodes && wave == 0 && lane < a.T) parent = a.parents[b * a.parents_sb + lane];
+    __builtin_amdgcn_sched_barrier(0);
+
+    wait_loads();
+    __syncthreads();
+    // a wave has 32 output dims of one of the matrices
+    const int mat = wave >> 2, j0 = 32 * (wave & 3);
+    const bool works = QJL || mat == 0;
+    float mrow[8][8];
+    if (works) {
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                __builtin_memcpy(&mrow[s][4 * e], &lds.m[(128 * mat + j0 + r) * 32 + ((4 * s + 2 * h + e) ^ r)], 16);
+    }
+
+    // ---- q R_k^T and q S^T as products of bf16 terms, a bf16 query one, any other two, the matrices two (what is left out,
+    // 2^-17 of a product, is 2^-5 of what the rounding to fp16 below may take).  Scaled by a power of two per row, to a largest
+    // element in [2^7, 2^8), they go to fp16 operands in LDS
+    {
 #pragma unroll 1
         for (int m = 0; m < RB; ++m) {
-            const int row = 32 * ((int)blockIdx.y * RB + m) + r;
-            const bool live = row < a.rows;
-            const int g = live ? row / a.T : 0, t = live ? row - g * a.T : 0;
-            const int64_t at = b * a.q_sb + (int64_t)((kv - b * a.kv_heads) * group + g) * a.q_sh + (int64_t)t * a.q_st + 8 * h;
-            Frag x[8][NQ];
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                if constexpr (NQ == 1) {
-                    __builtin_memcpy(&x[s][0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);
-                    if (!live) x[s][0].q = make_uint4(0u, 0u, 0u, 0u);
-                } else {
-                    float y[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = live ? query_element(a, at + 16 * s + e) : 0.0f;
-                    split_terms<NQ>(y, x[s]);
-                }
-            }
             f32x16 acc = zero16();
             if (works) {
 #pragma unroll
@@ -439,6 +464,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
                             if (i + j <= 1) acc = mfma_bf16(mt[i], x[s][j], acc);
                 }
             }
+            if (m + 1 < RB) load_queries(m + 1);
             // this lane: row r's dims j0 + 8 j + 4 h + (0..3)
             float most = 0.0f;
 #pragma unroll
@@ -456,24 +482,42 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
             int e = 0;
             if (most > 0.0f && most < __builtin_inff()) e = std::min(126, 7 + 127 - (int)((__float_as_uint(most) >> 23) & 0xFF));
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-            auto put = [&](uint4* to, int lane_offset, int offset, uint32_t y) INLINE {
-                *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(to) + lane_offset + offset) = (uint16_t)y;
-            };
+            // what is next to one another goes out together
             if (mat == 0) {
-                const int at0 = operand_offset(position_of<KB>(j0 + 4 * h)) + 16 * r;
+                uint8_t* const to = reinterpret_cast<uint8_t*>(lds.t.qc[m]) + operand_offset(position_of<KB>(j0 + 4 * h)) + 16 * r;
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    put(lds.t.qc[m], at0, operand_offset(position_of<KB>(8 * (i >> 2) + (i & 3))), tq::f32_to_f16(acc[i] * up));
+                for (int i = 0; i < 16; ++i) acc[i] *= up;
+                if constexpr (KB == 3 || KB == 1) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<uint2*>(to + operand_offset(position_of<KB>(e))) =
+                            make_uint2(pack_f16(acc[e], acc[4 + e]), pack_f16(acc[8 + e], acc[12 + e]));
+                } else if constexpr (KB == 4) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        *reinterpret_cast<uint32_t*>(to + operand_offset(position_of<KB>(8 * (i >> 1) + (i & 1)))) =
+                            pack_f16(acc[4 * (i >> 1) + (i & 1)], acc[4 * (i >> 1) + (i & 1) + 2]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        *reinterpret_cast<uint16_t*>(to + operand_offset(position_of<KB>(8 * (i >> 2) + (i & 3)))) =
+                            (uint16_t)tq::f32_to_f16(acc[i]);
+                }
             } else if (QJL) {
-                const int at0 = operand_offset(sign_position_of(j0 + 4 * h)) + 16 * r;
-                const float bit = h ? 8.0f : 128.0f;  // 2^(7 - j mod 8) is this 2^(-i mod 4)
+                uint8_t* const to = reinterpret_cast<uint8_t*>(lds.t.qs[m]) + operand_offset(sign_position_of(j0 + 4 * h)) + 16 * r;
+                const _Float16 bit = h ? 8.0f : 128.0f;  // 2^(7 - j mod 8) is this 2^-(i mod 4): the products with it are exact
                 float all = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float y = tq::f16_to_f32(tq::f32_to_f16(acc[i] * up));
-                    all += y;
-                    put(lds.t.qs[m], at0, operand_offset(sign_position_of(8 * (i >> 2) + (i & 3))),
-                        tq::f32_to_f16(y * (bit / (1 << (i & 3)))));
+                for (int n = 0; n < 2; ++n) {
+                    Frag f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const f16x2 y = __builtin_bit_cast(f16x2, pack_f16(acc[4 * n + e] * up, acc[4 * n + 8 + e] * up));
+                        all += (float)y[0] + (float)y[1];
+                        const _Float16 by = bit * (_Float16)(1.0f / (1 << e));
+                        f.u[e] = __builtin_bit_cast(uint32_t, y * f16x2{by, by});
+                    }
+                    *reinterpret_cast<uint4*>(to + operand_offset(sign_position_of(8 * n))) = f.q;
                 }
                 all = sum_of_halves(all);
                 if (h == 0) s_sum[m][wave & 3][r] = all;
@@ -482,10 +526,15 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
             __syncthreads();
         }
     }
+    if (threadIdx.x < (1 << VB)) s_centers[threadIdx.x] = value_center;
+    if (nodes && wave == 0) s_anc[lane] = ancestors(parent, lane);
+    Lut<KB> klut;
+    klut.load(key_center);
+    __syncthreads();
     // nothing of the above stays in registers for the loop
     asm volatile("" : "+v"(lane));
     r = lane & 31, h = lane >> 5;
-    if (RB > 1 && tile < last_tile) load_keys(tile), load_values(tile);
+    if (RB > 1 && tile < tiles) load_keys(tile), load_values(tile);
     Frag q[8];  // with one block of rows
     float c[RB], sign0[RB];
 #pragma unroll
@@ -500,7 +549,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
     PairTable<VB>::build(lds.t.table, s_centers, N::T);
     uint64_t sees[RB];
 #pragma unroll
-    for (int m = 0; m < RB; ++m) sees[m] = nodes ? s_anc[(32 * ((int)blockIdx.y * RB + m) + r) % a.T] : 0ull;
+    for (int m = 0; m < RB; ++m) sees[m] = nodes ? s_anc[(32 * (row_group * RB + m) + r) % a.T] : 0ull;
     __syncthreads();
 
     f32x16 o[RB][4];
@@ -592,7 +641,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
             need = shift - (14 + TOP_BIT - std::max(e, 1));
         }
         shift -= need;
-        if (tile + W < last_tile) load_keys(tile + W);
+        if (tile + step_tiles < tiles) load_keys(tile + step_tiles);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
         Frag pf[RB][2];
@@ -657,7 +706,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
-            if (ks == 1 && tile + W < last_tile) load_values(tile + W);
+            if (ks == 1 && tile + step_tiles < tiles) load_values(tile + step_tiles);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 Frag vf;
@@ -671,13 +720,13 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
         }
     };
     // whole tiles of the history, then those with the end of it or drafted tokens in them
-    const int64_t whole = std::min(last_tile, (end - lo) / TK);
-    for (; tile < whole; tile += W) step(tile, std::false_type{});
-    for (; tile < last_tile; tile += W) step(tile, std::true_type{});
+    const int64_t whole = std::min(tiles, (end - lo) / TK);
+    for (; tile < whole; tile += step_tiles) step(tile, std::false_type{});
+    for (; tile < tiles; tile += step_tiles) step(tile, std::true_type{});
 
     // ---- the waves' sums, one block of rows at a time
     const float unit = __uint_as_float((uint32_t)(127 - shift) << 23);
-    const int64_t heads = gridDim.x / a.n_split;
+    const int64_t heads = (int64_t)gridDim.y * gridDim.z;
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
         __syncthreads();
@@ -692,7 +741,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
         if (lane == 0) lds.s.unit[wave] = unit;
         __syncthreads();
         for (int i = threadIdx.x; i < 32 * 32; i += N::T) {
-            const int row = i >> 5, ch = i & 31, out_row = 32 * ((int)blockIdx.y * RB + m) + row;
+            const int row = i >> 5, ch = i & 31, out_row = 32 * (row_group * RB + m) + row;
             if (out_row >= a.rows) continue;
             float best = -__builtin_inff();
 #pragma unroll
@@ -840,7 +889,7 @@ bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Pl
 
 template <int KB, int VB, bool QJL>
 void launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
-    const dim3 grid((unsigned)(p.heads * p.n_split), p.row_groups);
+    const dim3 grid(p.n_split * p.row_groups, (unsigned)a.kv_heads, (unsigned)(p.heads / a.kv_heads));
     auto launch = [&](auto rb, auto nq) {
         hipLaunchKernelGGL((tree_kernel<KB, VB, QJL, rb, nq>), grid, dim3(Tree<rb>::T), 0, s, a);
     };
@@ -887,8 +936,8 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
     float* part_o = reinterpret_cast<float*>(ws);
     float2* part_ms = reinterpret_cast<float2*>(ws + p.o_bytes);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const TreeArgs a{kv_heads, nodes, p.rows, p.row_blocks, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
-                     k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, q, q_type, q_heads,
+    const TreeArgs a{kv_heads, nodes, p.rows, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
+                     k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, q, q_type, q_heads / kv_heads,
                      q_sb, q_sh, q_st, key_rotation, qjl, scale * LOG2E, p.n_split, part_o, part_ms};
     if (has_qjl) {
         if (value_bits == 4) launch_tree<3, 4, true>(a, p, s);
