@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
 from dataclasses import dataclass
 
 import numpy as np
@@ -646,31 +647,40 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: to
         raise ValueError(f"q must be bf16, fp16 or fp32, got {q.dtype}")
     if not 1 <= T <= MAX_NODES:
         raise ValueError(f"{T} drafted tokens: 1 to {MAX_NODES} are taken")
-    if k_codes.dim() != 4 or k_codes.shape[0] != B or k_codes.shape[1] == 0 or Hq % k_codes.shape[1]:
-        raise ValueError(f"k_codes {tuple(k_codes.shape)} do not match q {tuple(q.shape)}")
-    Hkv, cap = int(k_codes.shape[1]), int(k_codes.shape[2])
+    sh = k_codes.shape
+    if len(sh) != 4 or sh[0] != B or sh[1] == 0 or Hq % sh[1]:
+        raise ValueError(f"k_codes {tuple(sh)} do not match q {tuple(q.shape)}")
+    Hkv, cap = sh[1], sh[2]
     has_qjl = k_signs is not None
     if (k_rnorms is not None) != has_qjl or (qjl is not None) != has_qjl:
         raise ValueError("Q_prod keys need k_signs, k_rnorms and qjl")
     _no_gradient("tree_attention", q)
-    _require_gpu(q, k_codes, k_norms, v_codes, v_norms, k_signs, k_rnorms)
-    dev = q.device
-    lead = (B, Hkv, cap)
-    for name, t, row in (("k_codes", k_codes, row_bytes(D, key.bits)), ("v_codes", v_codes, row_bytes(D, value.bits)),
+    _require_gpu(q)
+    dev, on = q.device, q.get_device()
+    for name, t, row in (("k_codes", k_codes, 16 * key.bits), ("v_codes", v_codes, 16 * value.bits),
                          ("k_signs", k_signs, D // 8), ("k_norms", k_norms, 0), ("v_norms", v_norms, 0),
                          ("k_rnorms", k_rnorms, 0)):
-        if t is not None and (t.shape != ((*lead, row) if row else lead) or t.dtype != (torch.uint8 if row else torch.float16)
-                              or not t.is_contiguous() or t.device != dev):
-            raise ValueError(f"{name}: expected a contiguous tensor of {(*lead, row) if row else lead} on {dev}, got "
-                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        if t is None:
+            continue
+        sh = t.shape
+        if (len(sh) != (4 if row else 3) or sh[0] != B or sh[1] != Hkv or sh[2] != cap or (row and sh[3] != row)
+                or t.dtype is not (torch.uint8 if row else torch.float16) or not t.is_contiguous() or t.get_device() != on):
+            _require_gpu(t)
+            raise ValueError(f"{name}: expected a contiguous tensor of {(B, Hkv, cap, row) if row else (B, Hkv, cap)} on {dev}, "
+                             f"got {t.dtype} {tuple(sh)} on {t.device}")
+    for name, t in (("key.rotation", key.rotation), ("key.centers", key.centers), ("value.rotation", value.rotation),
+                    ("value.centers", value.centers), ("qjl", qjl)):
+        if t is not None and (t.get_device() != on or t.dtype is not torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"{name}: expected contiguous fp32 on {dev}, got {t.dtype} on {t.device}")
     nodes = 0 if parents is None else T
     if not 0 <= n_tokens <= cap or n_tokens < nodes:
         raise ValueError(f"{n_tokens} tokens, {nodes} of them drafted, of a capacity of {cap}")
     psb = 0
     if parents is not None:
-        if parents.dim() not in (1, 2):
+        dims = parents.dim()
+        if dims not in (1, 2):
             raise ValueError("parents must be [T] or [B, T]")
-        psb = T if parents.dim() == 2 else 0
+        psb = T if dims == 2 else 0
         parents = _int32_on(parents, dev, "parents", (B, T) if psb else (T,))
     seq_starts = _int32_on(seq_starts, dev, "seq_starts", (B,))
     seq_lens = _int32_on(seq_lens, dev, "seq_lens", (B,))
@@ -685,7 +695,7 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: to
         ws = torch.empty(max(int(need), 16), dtype=torch.uint8, device=dev)
         s = float(scale) if scale is not None else 1.0 / math.sqrt(D)
         qs = q.stride()
-        _on_device("tq_tree_attention", q.get_device(), q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, T, D, qs[0], qs[1],
+        _on_device("tq_tree_attention", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, T, D, qs[0], qs[1],
                    qs[2], _ptr(parents), psb, _ptr(seq_starts), _ptr(seq_lens), int(n_tokens), cap, k_codes.data_ptr(),
                    k_norms.data_ptr(), _ptr(k_signs), _ptr(k_rnorms), v_codes.data_ptr(), v_norms.data_ptr(), key.bits,
                    value.bits, int(has_qjl), key.rotation.data_ptr(), key.centers.data_ptr(), _ptr(qjl),
@@ -708,31 +718,39 @@ def _move_buffers(name: str, buffers: list[torch.Tensor]) -> tuple[int, int, int
     """(batch, heads, cap, row bytes) of a layer's [B, H, cap, ...] buffers."""
     if not buffers:
         raise ValueError(f"{name}: no buffers")
-    lead, dev, rows = buffers[0].shape[:3], buffers[0].get_device(), []
-    for b in buffers:
-        if b.shape[:3] != lead or len(lead) != 3 or b.get_device() != dev or not b.is_contiguous():
+    first, dev, rows = buffers[0].shape, buffers[0].get_device(), []
+    if len(first) < 3:
+        raise ValueError(f"{name}: expected [B, H, cap, ...] buffers, got {tuple(first)}")
+    B, H, cap = first[:3]
+    for b in buffers:  # (few queries a buffer, each of them some 0.1 us: a layer has up to twelve)
+        sh = b.shape
+        n = len(sh)
+        if n < 3 or sh[0] != B or sh[1] != H or sh[2] != cap or b.get_device() != dev or not b.is_contiguous():
             raise ValueError(f"{name}: expected contiguous [B, H, cap, ...] buffers of one shape and device, got "
-                             f"{tuple(b.shape)}")
-        rows.append((1 if b.dim() == 3 else b.shape[3] if b.dim() == 4 else math.prod(b.shape[3:])) * b.element_size())
-        if not 1 <= rows[-1] <= _MAX_ROW_BYTES:
-            raise ValueError(f"{name}: {rows[-1]} bytes to a token ({_MAX_ROW_BYTES} at most)")
+                             f"{tuple(sh)}")
+        r = (1 if n == 3 else sh[3] if n == 4 else math.prod(sh[3:])) * b.element_size()
+        if not 1 <= r <= _MAX_ROW_BYTES:
+            raise ValueError(f"{name}: {r} bytes to a token ({_MAX_ROW_BYTES} at most)")
+        rows.append(r)
     if dev < 0:
         _require_gpu(buffers[0])
-    return lead[0], lead[1], lead[2], rows
+    return B, H, cap, rows
 
 
 def _token_index(name: str, index: torch.Tensor, batch: int, heads: int, device: torch.device):
     """``index`` [n], [B, n] or [B, H, n] as int32, with its strides over batch and heads."""
-    dims = index.dim()
+    sh = index.shape
+    dims = len(sh)
     if not 1 <= dims <= 3:
         raise ValueError(f"{name}: index must be [n], [B, n] or [B, H, n]")
-    n = index.shape[-1]
+    n = sh[-1]
     index = _int32_on(index, device, f"{name}: index", (batch, heads)[:dims - 1] + (n,))
     return index, (n * heads if dims == 3 else n if dims == 2 else 0), (n if dims == 3 else 0), n
 
 
-def _pointers(tensors) -> ctypes.Array:
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+def _pointers(tensors) -> array:
+    """The tensors' addresses, as a host array (its own address: ``buffer_info()[0]``; a ctypes array takes twice as long)."""
+    return array("Q", [t.data_ptr() for t in tensors])
 
 
 #: up to here a call's new buffers are parts of one allocation: twelve of their own are 18 us of host time, the parts 12 us of
@@ -794,12 +812,12 @@ def gather_tokens(buffers: list[torch.Tensor], *, tokens: int, rows: torch.Tenso
         return out
     if B == 0 or n == 0:
         return [o.zero_() for o in out]
+    src, dst, row = _pointers(buffers), _pointers(out), array("i", row_bytes)
+    a_src, a_dst, a_row = (x.buffer_info()[0] for x in (src, dst, row))
+    at_rows, at_index, stream = _ptr(rows), _ptr(index), _stream_handle(dev)
     for a in range(0, len(buffers), _MOVE_BUFFERS):
-        part = slice(a, a + _MOVE_BUFFERS)
-        count = len(row_bytes[part])
-        _on_device("tq_gather_tokens", buffers[0].get_device(), count, _pointers(buffers[part]), _pointers(out[part]),
-                   (ctypes.c_int * count)(*row_bytes[part]), B, H, cap, tokens, R, slots, _ptr(rows), _ptr(index), sb, sh,
-                   n, _stream_handle(dev))
+        _on_device("tq_gather_tokens", dev.index, min(_MOVE_BUFFERS, len(buffers) - a), a_src + 8 * a, a_dst + 8 * a,
+                   a_row + 4 * a, B, H, cap, tokens, R, slots, at_rows, at_index, sb, sh, n, stream)
     return out
 
 
@@ -817,12 +835,11 @@ def keep_tokens(buffers: list[torch.Tensor], index: torch.Tensor, *, first: int,
                          "buffer; gather_tokens takes more)")
     if n == 0 or B * H == 0:
         return
+    at, row = _pointers(buffers), array("i", row_bytes)
+    a_at, a_row, at_index, stream = at.buffer_info()[0], row.buffer_info()[0], index.data_ptr(), _stream_handle(dev)
     for a in range(0, len(buffers), _MOVE_BUFFERS):
-        part = slice(a, a + _MOVE_BUFFERS)
-        count = len(row_bytes[part])
-        _on_device("tq_keep_tokens", buffers[0].get_device(), count, _pointers(buffers[part]),
-                   (ctypes.c_int * count)(*row_bytes[part]), B, H, cap, first, tokens, index.data_ptr(), sb, sh, n,
-                   _stream_handle(dev))
+        _on_device("tq_keep_tokens", dev.index, min(_MOVE_BUFFERS, len(buffers) - a), a_at + 8 * a, a_row + 4 * a, B, H, cap,
+                   first, tokens, at_index, sb, sh, n, stream)
 
 
 def rows16(t: torch.Tensor) -> torch.Tensor:
