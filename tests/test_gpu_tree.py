@@ -283,3 +283,18 @@ def test_refusals(cuda):
         tree_attention(randn((1, 8, 21, D), 5), layer, torch.full((21,), -1), 4)
     with pytest.raises(ValueError, match="backward"):
         tree_attention(q.requires_grad_(), layer, torch.tensor([-1, 0, 1, 2]), 4)
+
+
+@pytest.mark.parametrize("B,T,lens", [(3, 2, [4000, 5, 900]), (4, 20, [0, 3000, 0, 64]), (70, 3, [300 - 4 * i for i in range(70)]),
+                                      (2, 40, [0, 0]), (5, 1, [33, 0, 5000, 255, 257])])
+def test_batches_of_very_different_lengths(cuda, B, T, lens):
+    """The splits go to the batch rows by what they have to attend to."""
+    layer = make_layer(B, 2, max(lens) + T, 4, True, seed=41)
+    q = randn((B, 6, T, D), 5)
+    starts = [n // 3 for n in lens]
+    parents = [random_tree(T, b) for b in range(B)]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for st in (None, starts):
+        got = tree_attention(q, layer, torch.tensor(parents), 3, seq_lens=i32(lens), seq_starts=None if st is None else i32(st))
+        ref, _ = attend(q, *rows64(layer), tree_mask(parents, max(lens) + T, st or [0] * B, lens))
+        check(got, ref)

@@ -229,7 +229,7 @@ __device__ __forceinline__ constexpr int operand_offset(int p) {
 // ------------------------------------------------------------------ attention
 
 struct TreeArgs {
-    int kv_heads, T, rows;
+    int batch, kv_heads, T, rows;
     const int32_t* parents;
     int64_t parents_sb;
     const int32_t *starts, *lens;
@@ -242,10 +242,50 @@ struct TreeArgs {
     int64_t q_sb, q_sh, q_st;
     const float *rk, *s;
     float c2;  // scale log2(e)
-    int n_split;
-    float* part_o;   // [split][kv head][row][D]
-    float2* part_ms; // [split][kv head][row] (reference of the weights in log2, sum of weights)
+    int n_split, n_slots;  // n_split slots for each batch row, or n_slots dealt out by what the rows have
+    float* part_o;         // [slot][kv head][row][D]
+    float2* part_ms;       // [slot][kv head][row] (reference of the weights in log2, sum of weights)
+    int2* slots;           // [batch] a batch row's first slot and its number of slots, for rows of different lengths
 };
+
+// What a batch row attends to: history [lo, end), drafted tokens up to stop.
+struct Range {
+    int lo, end, stop;
+};
+// of a row's entries in starts and lens (any number where there are none)
+__device__ __forceinline__ Range range_of(const TreeArgs& a, int start, int len) {
+    const int nodes = a.parents ? a.T : 0, n = (int)a.n_tokens;
+    const int end = std::min(std::max(a.lens ? len : n - nodes, 0), n);
+    const int lo = a.starts ? std::min(std::max(start, 0), end) : 0;
+    return {lo, end, (int)std::min<int64_t>((int64_t)end + nodes, n)};
+}
+__device__ __forceinline__ int tiles_of(const Range& r) { return (int)(((int64_t)r.stop - r.lo + TK - 1) / TK); }
+
+// The batch row of a slot, its first slot and its number of slots.  Up to 64 rows of different lengths share the slots in
+// proportion to their tiles, each with one at least; what is left over goes unused (b = -1).
+struct Slot {
+    int b, first, n;
+    Range range;
+};
+// `start`, `len`: the entries of batch row `lane`.
+__device__ __forceinline__ Slot find_slot(const TreeArgs& a, int slot, int start, int len) {
+    const Range mine = range_of(a, start, len);
+    const int tiles = tiles_of(mine);
+    int total = 0;
+    for (int i = 0; i < a.batch; ++i) total += __builtin_amdgcn_readlane(tiles, i);
+    // (the sum of the shares does not pass what there is to share, whatever the roundings: these are far below 1)
+    const int share = (int)((float)(a.n_slots - a.batch) * ((float)tiles / (float)std::max(total, 1)));
+    const int n = std::min(std::min(1 + share, std::max(1, (tiles + MIN_TILES - 1) / MIN_TILES)), MAX_SPLIT);
+    int before = 0;
+    for (int i = 0; i < a.batch; ++i) {
+        const int own = __builtin_amdgcn_readlane(n, i);
+        if (slot < before + own)
+            return {i, before, own, {__builtin_amdgcn_readlane(mine.lo, i), __builtin_amdgcn_readlane(mine.end, i),
+                                     __builtin_amdgcn_readlane(mine.stop, i)}};
+        before += own;
+    }
+    return {-1, 0, 0, {0, 0, 0}};
+}
 
 __device__ __forceinline__ float query_element(const TreeArgs& a, int64_t i) {
     return a.q_type == 1 ? static_cast<const float*>(a.q)[i] : tq::f16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
@@ -355,9 +395,18 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
     __shared__ float s_top[W][32], s_sum[RB][4][32], s_c[RB][32];
     int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // in a scalar register, and what follows from it
-    const int kvh = blockIdx.y, b = blockIdx.z, kv = b * a.kv_heads + kvh;
-    const int row_group = RB == 1 ? 0 : blockIdx.x / a.n_split, split = blockIdx.x - row_group * a.n_split;
-
+    const int kvh = blockIdx.y, row_group = RB == 1 ? 0 : blockIdx.x / a.n_slots, slot = blockIdx.x - row_group * a.n_slots;
+    // (known before the matrices are asked for: a wait for a load ahead of theirs is one for them all)
+    Slot mine;
+    if (a.slots) {
+        const int entry = std::min(lane, a.batch - 1);
+        mine = find_slot(a, slot, a.starts ? a.starts[entry] : 0, a.lens ? a.lens[entry] : 0);
+        if (mine.b < 0) return;
+    } else {
+        using Scalar = const __attribute__((address_space(4))) int32_t*;
+        const int b = slot % a.batch;
+        mine = {b, 0, a.n_split, range_of(a, a.starts ? ((Scalar)a.starts)[b] : 0, a.lens ? ((Scalar)a.lens)[b] : 0)};
+    }
     // ---- What the queries' rotation takes is asked for first, then a first tile of the cache, then the small things: a workgroup of a
     // short history waits for memory once.  The matrices come by way of LDS: read straight into operands, 32 rows at a time, they
     // were 10000 cycles on their way.  Their 16-byte chunks are xor-swizzled by the row
@@ -366,6 +415,9 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
         const int at = (8 * i + wave) * 64 + lane, row = (at >> 5) & 127;
         load_lds16((i < 8 ? a.rk : a.s) + row * D + 4 * ((at & 31) ^ (row & 31)), &lds.m[(8 * i + wave) * 64]);
     }
+    // without slots of its own a batch row has every batch-th
+    const int b = mine.b, kv = b * a.kv_heads + kvh, split = a.slots ? slot - mine.first : slot / a.batch, n_split = mine.n;
+    if (a.slots && split == 0 && row_group == 0 && kvh == 0 && threadIdx.x == 0) a.slots[b] = make_int2(mine.first, mine.n);
     Frag x[8][NQ];  // a block's queries: lane (r, h) has row r's dims 16 s + 8 h + (0..7)
     auto load_queries = [&](int m) INLINE {
         const int row = 32 * (row_group * RB + m) + r;
@@ -387,13 +439,8 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
     load_queries(0);
 
     const int nodes = a.parents ? a.T : 0;
-    int64_t end = a.lens ? a.lens[b] : a.n_tokens - nodes;
-    end = std::min<int64_t>(std::max<int64_t>(end, 0), a.n_tokens);
-    int64_t lo = a.starts ? a.starts[b] : 0;
-    lo = std::min<int64_t>(std::max<int64_t>(lo, 0), end);
-    const int64_t stop = std::min<int64_t>(end + nodes, a.n_tokens);
-    const int64_t tiles = (stop - lo + TK - 1) / TK;
-    const int step_tiles = a.n_split * W;  // tiles in turn, to the waves of all splits
+    const int64_t lo = mine.range.lo, end = mine.range.end, stop = mine.range.stop, tiles = tiles_of(mine.range);
+    const int step_tiles = n_split * W;  // tiles in turn, to the waves of all splits
 
     // a lane's part of a tile, on its way: half of token r's key codes and signs and its norms, and a quarter of the value
     // codes of tokens lane % 16 and lane % 16 + 16.  The arrays are at scalar addresses, a lane's place in them 32-bit
@@ -726,7 +773,6 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
 
     // ---- the waves' sums, one block of rows at a time
     const float unit = __uint_as_float((uint32_t)(127 - shift) << 23);
-    const int64_t heads = (int64_t)gridDim.y * gridDim.z;
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
         __syncthreads();
@@ -758,7 +804,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
                 x.x = __builtin_fmaf(wu, y.x, x.x), x.y = __builtin_fmaf(wu, y.y, x.y);
                 x.z = __builtin_fmaf(wu, y.z, x.z), x.w = __builtin_fmaf(wu, y.w, x.w);
             }
-            const int64_t at = ((int64_t)split * heads + kv) * a.rows + out_row;
+            const int64_t at = ((int64_t)slot * a.kv_heads + kvh) * a.rows + out_row;
             reinterpret_cast<float4*>(a.part_o + at * D)[ch] = x;
             if (ch == 0) a.part_ms[at] = make_float2(best, den);
         }
@@ -772,6 +818,7 @@ struct MergeArgs {
     int64_t all_rows;  // of all KV heads
     const float* part_o;
     const float2* part_ms;
+    const int2* slots;  // or n_split for every batch row
     const float* rv;
     float* out_f32;
     uint16_t* out_bf16;
@@ -779,7 +826,8 @@ struct MergeArgs {
 };
 
 // Eight rows per workgroup: their splits weighed and added, then rotated back.  The matrix is read ahead of the partials,
-// half of its rows by a thread for its output dim.
+// half of its rows by a thread for its output dim.  (More rows to a workgroup, one eight after the other, read the matrix less
+// often and take longer: 26 us against 15 for 7168 rows.)
 __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     __shared__ float s_w[8][MAX_SPLIT];
     __shared__ float s_den[8];
@@ -791,14 +839,27 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     float m[64];
 #pragma unroll
     for (int d = 0; d < 64; ++d) m[d] = a.rv[(64 * half + d) * D + j];
+    // split i of a row is at `at` + i step
+    struct Part {
+        int64_t at;
+        int n;
+    };
+    const int64_t step = a.slots ? (int64_t)a.kv_heads * a.rows : a.all_rows;
+    auto find = [&](int64_t row) INLINE {
+        if (!a.slots) return Part{row, a.n_split};
+        const uint32_t n = (uint32_t)row, b = n / ((uint32_t)a.kv_heads * (uint32_t)a.rows);
+        const int2 slots = a.slots[b];
+        return Part{(slots.x - (int64_t)b) * step + row, slots.y};
+    };
     // 32 threads to a row, four dims each: the first splits' partials are on their way before the weights are known
     constexpr int AHEAD = 8;
     const int pk = threadIdx.x >> 5, pc = threadIdx.x & 31;
-    const float4* const part = reinterpret_cast<const float4*>(a.part_o + std::min(row0 + pk, a.all_rows - 1) * D) + pc;
-    const int64_t step = a.all_rows * (D / 4);
+    const Part mine = find(std::min(row0 + pk, a.all_rows - 1));
+    const float4* const part = reinterpret_cast<const float4*>(a.part_o + mine.at * D) + pc;
+    const int64_t step4 = step * (D / 4);
     float4 ahead[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ahead[i] = i < a.n_split ? part[i * step] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = i < mine.n ? part[i * step4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto place = [&](int64_t row) {  // of a row in [batch][q heads][T]
         const uint32_t n = (uint32_t)row, kv = n / (uint32_t)a.rows, in = n - kv * a.rows, g = in / (uint32_t)a.T;
         const uint32_t b = kv / (uint32_t)a.kv_heads, hq = (kv - b * a.kv_heads) * (a.q_heads / a.kv_heads) + g;
@@ -808,7 +869,10 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     for (int k = wave; k < 8; k += 4) {
         const int64_t row = row0 + k;
         float2 ms = make_float2(-__builtin_inff(), 0.0f);
-        if (row < a.all_rows && lane < a.n_split) ms = a.part_ms[lane * a.all_rows + row];
+        if (row < a.all_rows) {
+            const Part p = find(row);
+            if (lane < p.n) ms = a.part_ms[p.at + lane * step];
+        }
         float top = ms.x;
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
@@ -826,14 +890,14 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     __syncthreads();
     {
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        auto add = [&](float w, float4 x) {
+        auto add = [&](float w, float4 x) INLINE {
             o.x = __builtin_fmaf(w, x.x, o.x), o.y = __builtin_fmaf(w, x.y, o.y);
             o.z = __builtin_fmaf(w, x.z, o.z), o.w = __builtin_fmaf(w, x.w, o.w);
         };
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) add(s_w[pk][i], ahead[i]);  // splits that there are not: 0 times 0
 #pragma unroll 8
-        for (int i = AHEAD; i < a.n_split; ++i) add(s_w[pk][i], part[i * step]);
+        for (int i = AHEAD; i < mine.n; ++i) add(s_w[pk][i], part[i * step4]);
         const float den = s_den[pk] == 0.0f ? 1.0f : s_den[pk];
         *reinterpret_cast<float4*>(&s_o[pk][4 * pc]) = make_float4(o.x / den, o.y / den, o.z / den, o.w / den);
     }
@@ -864,11 +928,11 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 struct Plan {
-    int rows, row_blocks, n_split;
+    int rows, row_blocks, n_split, n_slots;
     unsigned row_groups;
     int64_t heads;
-    size_t ms_bytes, o_bytes;
-    size_t total() const { return ms_bytes + o_bytes; }
+    size_t ms_bytes, o_bytes, slots_bytes;
+    size_t total() const { return ms_bytes + o_bytes + slots_bytes; }
 };
 
 // A workgroup fills a CU.  As many splits as fill the CUs, as long as none is left without a tile.
@@ -881,15 +945,18 @@ bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Pl
     p.row_groups = p.row_blocks == 1 ? 1 : (unsigned)(p.row_blocks + 1) / 2;
     const int64_t tiles = std::max<int64_t>(1, (n_tokens + TK - 1) / TK);
     p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({256 / (p.heads * p.row_groups), (tiles + MIN_TILES - 1) / MIN_TILES, MAX_SPLIT}));
-    const int64_t all = p.heads * p.rows;
-    p.ms_bytes = ((size_t)all * p.n_split * 8 + 15) / 16 * 16;
-    p.o_bytes = (size_t)all * p.n_split * D * 4;
+    // batch rows of different lengths share out what fills the CUs
+    const int64_t most = std::min<int64_t>((tiles + MIN_TILES - 1) / MIN_TILES, MAX_SPLIT) * batch;
+    p.n_slots = (int)std::max<int64_t>((int64_t)p.n_split * batch, std::min<int64_t>(256 / (kv_heads * (int64_t)p.row_groups), most));
+    p.ms_bytes = ((size_t)p.n_slots * kv_heads * rows * 8 + 15) / 16 * 16;
+    p.o_bytes = (size_t)p.n_slots * kv_heads * rows * D * 4;
+    p.slots_bytes = ((size_t)batch * 8 + 15) / 16 * 16;
     return true;
 }
 
 template <int KB, int VB, bool QJL>
 void launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
-    const dim3 grid(p.n_split * p.row_groups, (unsigned)a.kv_heads, (unsigned)(p.heads / a.kv_heads));
+    const dim3 grid((unsigned)a.n_slots * p.row_groups, (unsigned)a.kv_heads);
     auto launch = [&](auto rb, auto nq) {
         hipLaunchKernelGGL((tree_kernel<KB, VB, QJL, rb, nq>), grid, dim3(Tree<rb>::T), 0, s, a);
     };
@@ -935,10 +1002,12 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     float* part_o = reinterpret_cast<float*>(ws);
     float2* part_ms = reinterpret_cast<float2*>(ws + p.o_bytes);
+    int2* const slots = batch > 1 && batch <= 64 && p.n_slots > batch && (seq_starts || seq_lens) ? reinterpret_cast<int2*>(ws + p.o_bytes + p.ms_bytes) : nullptr;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const TreeArgs a{kv_heads, nodes, p.rows, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
+    const TreeArgs a{batch, kv_heads, nodes, p.rows, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
                      k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, q, q_type, q_heads / kv_heads,
-                     q_sb, q_sh, q_st, key_rotation, qjl, scale * LOG2E, p.n_split, part_o, part_ms};
+                     q_sb, q_sh, q_st, key_rotation, qjl, scale * LOG2E, p.n_split, slots ? p.n_slots : p.n_split * batch, part_o, part_ms,
+                     slots};
     if (has_qjl) {
         if (value_bits == 4) launch_tree<3, 4, true>(a, p, s);
         else if (value_bits == 3) launch_tree<2, 3, true>(a, p, s);
@@ -950,9 +1019,10 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
         else launch_tree<1, 1, false>(a, p, s);
     }
     TQ_CHECK_LAUNCH();
-    const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, p.heads * p.rows, part_o, part_ms,
-                      value_rotation, out_f32, out_bf16, lse_out};
-    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((p.heads * p.rows + 7) / 8)), dim3(256), 0, s, m);
+    const int64_t all = p.heads * p.rows;
+    const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, all, part_o, part_ms, slots, value_rotation, out_f32, out_bf16,
+                      lse_out};
+    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((all + 7) / 8)), dim3(256), 0, s, m);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
 }
