@@ -825,20 +825,20 @@ struct MergeArgs {
     float* lse;
 };
 
-// Eight rows per workgroup: their splits weighed and added, then rotated back.  The matrix is read ahead of the partials,
-// half of its rows by a thread for its output dim.  (More rows to a workgroup, one eight after the other, read the matrix less
-// often and take longer: 26 us against 15 for 7168 rows.)
-__global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
-    __shared__ float s_w[8][MAX_SPLIT];
-    __shared__ float s_den[8];
-    __shared__ __align__(16) float s_o[8][D];
-    __shared__ float s_half[2][8][D];
-    const int64_t row0 = (int64_t)blockIdx.x * 8;
+// MERGE_ROWS rows per workgroup: their splits weighed and added, then rotated back.  The matrix is read ahead of the partials,
+// a quarter of its rows by a thread for its output dim.
+constexpr int MERGE_ROWS = 16, MERGE_T = 512, PARTS = MERGE_T / D, PART = D / PARTS;
+__global__ __launch_bounds__(MERGE_T) void merge_kernel(MergeArgs a) {
+    __shared__ float s_w[MERGE_ROWS][MAX_SPLIT];
+    __shared__ float s_den[MERGE_ROWS];
+    __shared__ __align__(16) float s_o[MERGE_ROWS][D];
+    __shared__ float s_part[PARTS][MERGE_ROWS][D];
+    const int64_t row0 = (int64_t)blockIdx.x * MERGE_ROWS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int j = threadIdx.x & 127, half = threadIdx.x >> 7;
-    float m[64];
+    const int j = threadIdx.x & 127, quarter = threadIdx.x >> 7;
+    float m[PART];
 #pragma unroll
-    for (int d = 0; d < 64; ++d) m[d] = a.rv[(64 * half + d) * D + j];
+    for (int d = 0; d < PART; ++d) m[d] = a.rv[(PART * quarter + d) * D + j];
     // split i of a row is at `at` + i step
     struct Part {
         int64_t at;
@@ -866,7 +866,7 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
         return ((int64_t)b * a.q_heads + hq) * a.T + (in - g * a.T);
     };
 #pragma unroll 1
-    for (int k = wave; k < 8; k += 4) {
+    for (int k = wave; k < MERGE_ROWS; k += MERGE_T / 64) {
         const int64_t row = row0 + k;
         float2 ms = make_float2(-__builtin_inff(), 0.0f);
         if (row < a.all_rows) {
@@ -903,22 +903,22 @@ __global__ __launch_bounds__(256) void merge_kernel(MergeArgs a) {
     }
     __syncthreads();
 #pragma unroll 1
-    for (int k = 0; k < 8; ++k) {
+    for (int k = 0; k < MERGE_ROWS; ++k) {
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int d = 0; d < 64; d += 4) {
-            const float4 o = *reinterpret_cast<const float4*>(&s_o[k][64 * half + d]);
+        for (int d = 0; d < PART; d += 4) {
+            const float4 o = *reinterpret_cast<const float4*>(&s_o[k][PART * quarter + d]);
             x[0] = __builtin_fmaf(o.x, m[d], x[0]), x[1] = __builtin_fmaf(o.y, m[d + 1], x[1]);
             x[2] = __builtin_fmaf(o.z, m[d + 2], x[2]), x[3] = __builtin_fmaf(o.w, m[d + 3], x[3]);
         }
-        s_half[half][k][j] = (x[0] + x[1]) + (x[2] + x[3]);
+        s_part[quarter][k][j] = (x[0] + x[1]) + (x[2] + x[3]);
     }
     __syncthreads();
 #pragma unroll 1
-    for (int k = half; k < 8; k += 2) {
+    for (int k = quarter; k < MERGE_ROWS; k += PARTS) {
         const int64_t row = row0 + k;
         if (row >= a.all_rows) break;
-        const float x = s_half[0][k][j] + s_half[1][k][j];
+        const float x = (s_part[0][k][j] + s_part[1][k][j]) + (s_part[2][k][j] + s_part[3][k][j]);
         const int64_t at = place(row) * D + j;
         if (a.out_f32) a.out_f32[at] = x;
         if (a.out_bf16) a.out_bf16[at] = (uint16_t)tq::f32_to_bf16(x);
@@ -1022,7 +1022,7 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
     const int64_t all = p.heads * p.rows;
     const MergeArgs m{q_heads, kv_heads, nodes, p.rows, p.n_split, all, part_o, part_ms, slots, value_rotation, out_f32, out_bf16,
                       lse_out};
-    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((all + 7) / 8)), dim3(256), 0, s, m);
+    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((all + MERGE_ROWS - 1) / MERGE_ROWS)), dim3(MERGE_T), 0, s, m);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
 }
