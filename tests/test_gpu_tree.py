@@ -81,12 +81,12 @@ def random_tree(T, seed):
     return [-1 if i < 3 else int(torch.randint(-1, i, (1,), generator=gen)) for i in range(T)]
 
 
-#: Roundings of the kernel, all independent of each other and of unit 2^-12 (half a step of fp16, relative): a logit is
-#: a sum of 128 products of a rotated query element and a centroid, both rounded: its error is at most of the order
-#: |q| |k| / sqrt(128) * sqrt(2) * 2^-12 / sqrt(128) (|q| 11.3 or less than twice that, |k| about 20 and rarely twice that)
-#: = 11.3 * 20 / 128 * 1.4 * 2.4e-4 = 6e-4, with the QJL part as much again; value centroids and weights 2.4e-4 each.
+#: Roundings of the kernel, all independent of each other, each to fp16: by at most 2^-11 of the number, 2^-11 / sqrt(3) =
+#: 2.8e-4 root mean square.  A logit is a sum of 128 products of a rotated query element and a centroid, both rounded: its error is of the
+#: order |q| |k| / sqrt(128) * sqrt(2) * 2.8e-4 / sqrt(128) (|q| 11.3 or less than twice that, |k| about 20 and rarely twice
+#: that) = 11.3 * 20 / 128 * 1.4 * 2.8e-4 = 7e-4, with the QJL part as much again; value centroids and weights 2.8e-4 each.
 #: Of the output's largest element that is 2e-3 at most, the package's tolerance of its other decode kernels; a bf16
-#: output adds half a step, 2^-9 of the element rounded up to 2^-8.
+#: output adds half a step, 2^-8 of the element.
 TOL = 2e-3
 
 

@@ -6,23 +6,29 @@
 //   out     = (sum_t softmax_t |v_t| C_v[vidx_t]) R_v
 // so keys and values are never rotated: the queries are, once, and the sums are rotated back, once.
 //
-//   prep_kernel   32 query rows of a KV head per workgroup: q R_k^T and q S^T, scaled by a power of two per
-//                 row, in fp16, in the order the products below take them
-//   tree_kernel   a token range of one KV head per workgroup, 32 query rows (head x node) per wave.  Tiles of
-//                 64 tokens: all waves turn the packed codes into fp16 rows in LDS, then each forms
-//                 S^T = K Q^T (codes and signs apart: their norms differ) and O^T = V^T P^T with
-//                 v_mfma_f32_32x32x16_f16
+//   tree_kernel   a share of the tokens of one KV head per workgroup of eight waves, and 32 query rows (head x node) or 64 of
+//                 them, all in every wave.  It rotates its queries first (q R_k^T and q S^T, scaled by a power of two per row, to
+//                 fp16 operands), then the waves take tiles of 32 tokens in turn, on their own until their sums meet:
+//                 S^T = K Q^T (codes and signs apart: their norms differ) and O^T = V^T P^T with v_mfma_f32_32x32x16_f16.
+//                 The splits of a head fill the CUs, with eight tiles at least; batch rows of different lengths share them out
 //   merge_kernel  the splits' partials of a row weighed and added, rotated back by R_v
 //
-// Codes to fp16: a byte lookup (v_perm_b32) of the centroid's two halves for four codes at once, from
-// tables in registers.  Which four codes meet in a register follows from the packing (those at the same
-// bits of neighbouring bytes), so each bit width has an order of the 128 dims of its own, which the queries
-// are written in and the sums are read back in (dim_of).
+// Codes to fp16.  Keys become A operands in registers, a lane's token and half of its dims: a byte lookup (v_perm_b32) of the
+// centroid's two halves for four codes at once.  Which four codes meet in a register follows from the packing (those at the
+// same bits of neighbouring bytes), so each bit width has an order of the 128 dims of its own, which the queries are
+// written in (position_of).  Signs stay where they are, as the lowest mantissa bits of fp16 numbers.  Values are looked up in LDS, two
+// codes at a time (PairTable), and turned around by ds_read_b64_tr_b16.
 //
-// Rounding.  Rotated queries and centroids are rounded once to fp16, 2^-12 of each (with |q| = 11 and |k| = 20 the
-// logits move by 3e-4 of their unit), value centroids too (their sum's errors are kept from adding up by the
-// codebook, see tq_value_codebook_f16), weights times norm p |v| once, 2^-12 of each.  Logits, maxima, weights, sums
-// and outputs are fp32.
+// Cost.  The tiles are bound by their decoding and their softmax beside the matrix instructions: 16 nodes x 4 heads of 8
+// sequences of 32768 tokens (8 KV heads, 4-bit Q_prod) take 149 us, of which the matrix instructions are 78 at the rate of a
+// large product of matrices, the 281 MB of codes 55 at that of a large copy; 64 rows to a workgroup share a tile's decoding
+// (the call took 182 us with 32 and 32 when it took 160 with 64).  64 nodes x 7 heads of 4 sequences of 8192 (4 KV heads, 3-bit Q_mse) take 64 us.
+// Small calls are bound by latency: 8 nodes of one chat of 1037 tokens take 13 us and the merge 7, of which the first bytes
+// from memory are 4, and two launches.  Rotating the queries in a kernel of their own took 9 us more a call and saved 5.
+//
+// Rounding.  Rotated queries and centroids are rounded once to fp16, by at most 2^-11 of each, 2^-11 / sqrt(3) root mean square (with
+// |q| = 11 and |k| = 20 a logit moves by 7e-4), value centroids too (their sum's errors are kept from adding up by the
+// codebook, see tq_value_codebook_f16), weights times norm p |v| once.  Logits, maxima, weights, sums and outputs are fp32.
 
 #include <algorithm>
 #include <type_traits>
@@ -192,7 +198,7 @@ __device__ __forceinline__ int value_offset(int d, int e, int lane) {
 
 // ------------------------------------------------------------------ queries
 
-// fp32 pairs to bf16 terms to nearest: two leave out 2^-18 of a number (half a step of each is 2^-9 of what is left)
+// fp32 pairs to bf16 terms to nearest: two leave out at most 2^-16 of a number (half a step of each is 2^-8 of what is left)
 template <int N>
 __device__ __forceinline__ void split_terms(const float* x, Frag* t) {
 #pragma unroll
@@ -493,7 +499,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
     }
 
     // ---- q R_k^T and q S^T as products of bf16 terms, a bf16 query one, any other two, the matrices two (what is left out,
-    // 2^-17 of a product, is 2^-5 of what the rounding to fp16 below may take).  Scaled by a power of two per row, to a largest
+    // 2^-15 of a product, is 2^-4 of what the rounding to fp16 below may take).  Scaled by a power of two per row, to a largest
     // element in [2^7, 2^8), they go to fp16 operands in LDS
     {
 #pragma unroll 1

@@ -16,6 +16,8 @@ Reference interfaces replaced:
   decode_attention_groups -> the reference's attention over outlier-split layers, which its
                     fused kernel refuses (runtime/triton_kernels.py:252-253) and its chunked
                     path dequantises (runtime/attention.py:215-304)
+Beside the reference's: prompt_attention (whole prompts, runtime/attention.py:75-99), tree_attention (drafted
+tokens, runtime/attention.py:215-304), gather_tokens and keep_tokens (runtime/packed_qmse_cache.py:81-92, 135-140).
 """
 
 from __future__ import annotations
