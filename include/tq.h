@@ -337,7 +337,7 @@ int tq_dense_attention(const void* q, int q_is_f32, int batch, int q_heads, int 
  *   seq_starts, seq_ends  int32 [batch] (device, nullable; not with cu_seqlens): row b's sequence is
  *            [start, end), for padded batches; the other rows get 0 (lse -inf)
  *   scale    logit scale, > 0 and finite
- * Offsets are clamped to [0, tokens].  TQ_ERR_UNSUPPORTED beyond 2^30 tokens, 2^24 blocks of 128 rows
+ * Offsets are clamped to [0, tokens].  TQ_ERR_UNSUPPORTED beyond 2^30 tokens, from 2^23 blocks of 128 rows
  * over all query heads, or with a k_st or v_st outside [0, 2^25).
  */
 int tq_prompt_attention(const void* q, const void* k, const void* v, void* out, float* lse, int is_f16, int batch,

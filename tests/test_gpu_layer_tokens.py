@@ -81,14 +81,16 @@ def test_crop(cuda, kind):
         assert same(layer, [x[:, :, :left - d] for x in packed], [x[:, :, :d] for x in dense])
 
 
-def test_what_crop_leaves_behind_is_not_read(cuda):
-    layer, short = make("qjl", N=64, extra=70), make("qjl", N=64, extra=70)
-    for n in (layer._store.kn, layer._store.kr, layer._store.vn):
-        n[:, :, 70:] = float("nan")
+@pytest.mark.parametrize("kind", ["qjl", "split"])
+def test_what_crop_leaves_behind_is_not_read(cuda, kind):
+    layer, short = make(kind, N=64, extra=70), make(kind, N=64, extra=70)
+    for n in layer._store.buffers():
+        if n.dim() == 3:
+            n[:, :, 70:] = float("nan")
     layer.crop(70)
     short.crop(70)
-    for n in (short._store.kn, short._store.kr, short._store.vn):
-        n[:, :, 70:] = 0.0
+    for n in short._store.buffers():
+        n[:, :, 70:] = 0
     q = torch.randn(3, 8, 5, D, device=cuda).bfloat16()
     assert torch.equal(fused_attention(q[:, :, :1], layer, 4), fused_attention(q[:, :, :1], short, 4))
     parents = torch.arange(-1, 4)
@@ -137,6 +139,27 @@ def test_a_history_thinned_out(cuda, kind, tokens, n, dims):
     assert layer.get_seq_length() == first + n + 1
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_of_a_layer_cropped_to_nothing(cuda, kind):
+    layer = make(kind)
+    layer.crop(-49)
+    layer.batch_repeat_interleave(2)
+    layer.batch_select_indices(torch.tensor([0, 1]))
+    k, v = (kv_bf16((2, 2, 1, D), seed=i).to(layer.dtype) for i in (7, 8))
+    layer.update(k, v)
+    assert layer.get_seq_length() == 1
+
+
+def test_numbers_past_32_bits_name_nothing(cuda):
+    layer = make("qjl")
+    packed, _ = contents(layer)
+    layer.reorder_cache(torch.tensor([2 ** 32 + 1, -2 ** 40, 2], device=cuda))
+    layer.keep_tokens(torch.tensor([2 ** 32, 3], device=cuda), tokens=9)
+    for got, x in zip(contents(layer)[0], packed):
+        assert (got[:2] == 0).all() and (got[2, :, 40] == 0).all()
+        assert torch.equal(got[2, :, :40], x[2, :, :40]) and torch.equal(got[2, :, 41], x[2, :, 43])
+
+
 def test_refusals_and_empty_layers(cuda):
     layer = make("qjl and dense")
     with pytest.raises(ValueError, match="keep_tokens: 3 of the last 2"):
@@ -147,6 +170,9 @@ def test_refusals_and_empty_layers(cuda):
         layer.keep_tokens(torch.tensor([0]), tokens=10)
     with pytest.raises(ValueError, match="index must"):
         layer.keep_tokens(torch.tensor([[0], [1]]), tokens=9)
+    for bad in (torch.tensor(3), torch.zeros(9, dtype=torch.bool), torch.zeros(3)):
+        with pytest.raises(ValueError, match="index must be int"):
+            layer.keep_tokens(bad, tokens=9)
     with pytest.raises(ValueError, match="rows must"):
         layer.reorder_cache(torch.tensor([0.0, 1.0, 2.0]))
     assert layer.get_seq_length() == 49

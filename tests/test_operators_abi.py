@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from turboquant.runtime import _lib, prompt_attention, tree_attention
 from turboquant.runtime import kernels as K
@@ -25,7 +26,8 @@ INF, NAN = float("inf"), float("nan")
     (UNSUPPORTED, dict(k_sh=4)), (UNSUPPORTED, dict(o_sb=12)), (UNSUPPORTED, dict(k_st=-128)),
     (UNSUPPORTED, dict(v_st=1 << 25)), (UNSUPPORTED, dict(q=ODD)), (UNSUPPORTED, dict(k=ODD)), (UNSUPPORTED, dict(v=ODD)),
     (UNSUPPORTED, dict(out=ODD)), (UNSUPPORTED, dict(tokens=(1 << 30) + 1)), (UNSUPPORTED, dict(tokens=1 << 30, q_heads=32)),
-    (UNSUPPORTED, dict(cu=FAKE, n_seqs=(1 << 31) - 1)), (UNSUPPORTED, dict(batch=1 << 22, kv_heads=1, q_heads=4))])
+    (UNSUPPORTED, dict(cu=FAKE, n_seqs=(1 << 31) - 1)), (UNSUPPORTED, dict(batch=1 << 22, kv_heads=1, q_heads=4)),
+    (UNSUPPORTED, dict(tokens=1, batch=1 << 20, kv_heads=1, q_heads=8))])
 def test_prompt_attention_rejects_on_host(status, change):
     args = dict(q=FAKE, k=FAKE, v=FAKE, out=FAKE, lse=None, f16=0, batch=1, q_heads=8, kv_heads=2, tokens=300, dim=128,
                 q_sb=0, q_sh=128, q_st=1024, k_sb=0, k_sh=128, k_st=256, v_sb=0, v_sh=128, v_st=256, o_sb=0, o_sh=128,
@@ -112,6 +114,11 @@ def test_wrappers_refuse_shapes_types_and_cpu_tensors():
         prompt_attention(q, k, k)
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):
         prompt_attention(q.requires_grad_(), k, k)
+    q = q.detach()
+    with pytest.raises(ValueError, match="backward"):
+        prompt_attention(q, k, k, out=torch.zeros_like(q).requires_grad_())
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="tangent"):
+        prompt_attention(q, forward_ad.make_dual(k, k), k)
 
     q = q.detach()
     lc = layer_codecs(128, 4, 0, False, "cpu")

@@ -562,9 +562,9 @@ extern "C" int tq_prompt_attention(const void* q, const void* k, const void* v, 
     for (int64_t s : {k_st, v_st})
         if (s < 0 || s >= (int64_t)1 << 25) return TQ_ERR_UNSUPPORTED;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return TQ_ERR_UNSUPPORTED;
-    // rows and blocks are counted in 32 bits
+    // rows are counted in 32 bits, and threads: 512 to a block
     const int64_t blocks = (tokens + 127) / 128 + (cu_seqlens ? (int64_t)n_seqs + 2 : 0);
-    if (tokens > (int64_t)1 << 30 || blocks * batch * q_heads >= (int64_t)1 << 24) return TQ_ERR_UNSUPPORTED;
+    if (tokens > (int64_t)1 << 30 || blocks * batch * q_heads >= (int64_t)1 << 23) return TQ_ERR_UNSUPPORTED;
     PromptArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                  static_cast<uint16_t*>(out), lse, batch, q_heads, kv_heads, (int)tokens, q_sb, q_sh, q_st, k_sb, k_sh,
                  k_st, v_sb, v_sh, v_st, o_sb, o_sh, o_st, cu_seqlens, n_seqs, seq_starts, seq_ends, zero_outside != 0,

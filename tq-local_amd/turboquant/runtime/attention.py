@@ -465,8 +465,8 @@ def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key:
                               attention_mask: torch.Tensor | None, dropout: float = 0.0,
                               scaling: float | None = None, is_causal: bool | None = None, **kwargs):
     """HF attention-interface function "turboquant_prompt": whole causal prompts without a mask, alone or packed
-    (``cu_seq_lens_q``), go through ``prompt_attention``; what it does not take (a mask, dropout, a gradient, other
-    types, head sizes and keys than the prompt's own) and layers that hold packed tokens go the way of "turboquant".
+    (``cu_seq_lens_q``), go through ``prompt_attention``; what it does not take (a mask, dropout, a gradient, a trace or a
+    transform, other types, head sizes and keys than the prompt's own) and layers that hold packed tokens go the way of "turboquant".
     One tensor as ``cu_seq_lens_q`` and ``cu_seq_lens_k`` spares a host sync that compares them."""
     causal = getattr(module, "is_causal", True) if is_causal is None else is_causal
     window = kwargs.get("sliding_window")
@@ -477,6 +477,7 @@ def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key:
             and query.dtype in (torch.bfloat16, torch.float16) and key.dtype == value.dtype == query.dtype
             and (window is None or window >= S) and kwargs.get("softcap") is None and kwargs.get("s_aux") is None
             and (cu is None or (query.shape[0] == 1 and (cu_k is None or cu_k is cu or torch.equal(cu_k, cu))))
+            and not K.torch_operations_watched()
             and not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))):
         layer = getattr(module, "_tq_cache_layer", None)
         if layer is None or layer._force_dense or layer.packed_seq_length() == 0:

@@ -536,6 +536,8 @@ def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
         for t in tensors:
             if t.requires_grad:
                 raise ValueError(f"{name} has no backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{name} has no derivative: a tensor carries a tangent")
 
 
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -558,9 +560,10 @@ def _int32_on(t: torch.Tensor | None, device: torch.device, name: str, shape: tu
         return None
     if (t.dtype != torch.int32 and t.dtype != torch.int64) or t.shape != shape:
         raise ValueError(f"{name} must be int32 or int64 of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    if t.dtype == torch.int32 and t.device == device and t.is_contiguous():
-        return t
-    return t.to(device=device, dtype=torch.int32).contiguous()
+    if t.dtype == torch.int32:
+        return t if t.device == device and t.is_contiguous() else t.to(device).contiguous()
+    # a number past 32 bits stays past every bound
+    return t.to(device).clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: torch.Tensor | None = None,
@@ -586,7 +589,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
         raise ValueError(f"k, v {tuple(k.shape)} do not match q {tuple(q.shape)}: a whole prompt has as many keys as rows")
     if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"q, k and v must all be bf16 or all fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    _no_gradient("prompt_attention", q, k, v)
+    _no_gradient("prompt_attention", q, k, v, *(() if out is None else (out,)))
     _require_gpu(q, k, v)
     dev = q.device
     if k.device != dev or v.device != dev:
@@ -670,10 +673,11 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: to
             _require_gpu(t)
             raise ValueError(f"{name}: expected a contiguous tensor of {(B, Hkv, cap, row) if row else (B, Hkv, cap)} on {dev}, "
                              f"got {t.dtype} {tuple(sh)} on {t.device}")
-    for name, t in (("key.rotation", key.rotation), ("key.centers", key.centers), ("value.rotation", value.rotation),
-                    ("value.centers", value.centers), ("qjl", qjl)):
-        if t is not None and (t.get_device() != on or t.dtype is not torch.float32 or not t.is_contiguous()):
-            raise ValueError(f"{name}: expected contiguous fp32 on {dev}, got {t.dtype} on {t.device}")
+    for name, t, n in (("key.rotation", key.rotation, D * D), ("key.centers", key.centers, 1 << key.bits),
+                       ("value.rotation", value.rotation, D * D), ("value.centers", value.centers, 1 << value.bits),
+                       ("qjl", qjl, D * D)):
+        if t is not None and (t.get_device() != on or t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"{name}: expected {n} contiguous fp32 on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     nodes = 0 if parents is None else T
     if not 0 <= n_tokens <= cap or n_tokens < nodes:
         raise ValueError(f"{n_tokens} tokens, {nodes} of them drafted, of a capacity of {cap}")

@@ -622,8 +622,6 @@ class PackedMSELayer(CacheLayerMixin):
 
     # ------------------------------------------- rows and tokens chosen and moved
     def _take_rows(self, rows: torch.Tensor) -> None:
-        if self.get_seq_length() == 0:
-            return
         if self._store is not None:
             self._store.take(rows=rows)
             self._shape = (self._store.B, *self._shape[1:])
@@ -642,7 +640,7 @@ class PackedMSELayer(CacheLayerMixin):
 
     def batch_repeat_interleave(self, repeats: int) -> None:
         """Every batch row ``repeats`` times."""
-        if self.get_seq_length():
+        if self._store is not None or self._dense_buf is not None:
             batch = self._store.B if self._store is not None else self._dense_buf[0].shape[0]
             self._take_rows(torch.arange(batch, device=self.device).repeat_interleave(repeats))
 
@@ -660,6 +658,8 @@ class PackedMSELayer(CacheLayerMixin):
         first of them, in that order: the accepted path of a tree of drafted tokens, or the tokens that a
         history keeps.  They have to be all packed or all dense.  An index outside [0, tokens) gives a token
         of zeros."""
+        if not 1 <= index.dim() <= 3 or index.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"keep_tokens: index must be int [n], [B, n] or [B, H, n], got {index.dtype} {tuple(index.shape)}")
         total, n = self.get_seq_length(), int(index.shape[-1])
         tokens = total if tokens is None else int(tokens)
         if not 0 <= n <= tokens <= total:
