@@ -137,3 +137,21 @@ def test_more_buffers_than_one_launch_takes(cuda):
     K.keep_tokens(bufs, index, first=0, tokens=30)
     for b, old in zip(bufs, before):
         assert same(b[:, :, :3], taken(old, index))
+
+
+def test_offsets_past_32_bits(cuda):
+    N = 90_000_000
+    bufs = buffers(1, 1, 64, [48, 62, 1])
+    big = [torch.zeros((1, 2, N, *b.shape[3:]), dtype=b.dtype, device="cuda") for b in bufs]
+    for g, b in zip(big, bufs):
+        g[:, 1, N - 64:] = b[:, 0]
+    index = torch.tensor([60, 3, 3, 0, 63], device="cuda")
+    for got, b in zip(K.gather_tokens(big, tokens=N, index=N - 64 + index), bufs):
+        assert torch.equal(raw(got)[:, 1:], taken(b, index)) and (raw(got)[:, 0] == 0).all()
+    for got, b in zip(K.gather_tokens(big, tokens=N, rows=torch.tensor([0, 0], device="cuda")), bufs):
+        assert torch.equal(raw(got)[1, 1, N - 64:], raw(b)[0, 0]) and not raw(got)[1, 0, -1000:].any()
+        del got
+    K.keep_tokens(big, index, first=N - 64, tokens=64)
+    for g, b in zip(big, bufs):
+        assert torch.equal(raw(g)[0, 1, N - 64:N - 59], taken(b, index)[0, 0])
+        assert torch.equal(raw(g)[0, 1, N - 59:], raw(b)[0, 0, 5:])

@@ -320,3 +320,20 @@ def test_a_models_prompt_takes_it(cuda, monkeypatch):
     turboquant.activate(model, CharTokenizer(), bits=4, use_qjl_keys=True, quiet=True)
     assert model.generate(ids, max_new_tokens=5).shape == (1, 305)
     assert len(calls) >= 4
+
+
+def test_keys_far_apart(cuda):
+    """Token strides up to the limit: offsets inside a tile take all of 32 bits."""
+    S, st = 130, (1 << 25) - 8
+    flat = torch.empty((S - 1) * st + 4 * D, dtype=torch.bfloat16, device="cuda")
+    k, v = (flat.as_strided((1, 2, S, D), (0, D, st, 1), at) for at in (0, 2 * D))
+    k.copy_(randn(k.shape, 2, torch.bfloat16))
+    v.copy_(randn(v.shape, 3, torch.bfloat16))
+    q = randn((1, 8, S, D), 1, torch.bfloat16)
+    got = prompt_attention(q, k, v)
+    ref, _, size = oracle(q, k.contiguous(), v.contiguous())
+    check(got, ref, size)
+    many = prompt_attention(q.repeat(1, 64, 1, 1), k, v)  # blocks of 256 rows: the first 256 heads share KV head 0
+    assert torch.equal(many[:, :256].unflatten(1, (32, 8))[:, :, :4], many[:, :4][:, None].expand(-1, 32, -1, -1, -1))
+    ref, _, size = oracle(q.repeat(1, 64, 1, 1)[:, [0, 300]], k.contiguous(), v.contiguous())
+    check(many[:, [0, 300]], ref, size)

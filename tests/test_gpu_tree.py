@@ -298,3 +298,21 @@ def test_batches_of_very_different_lengths(cuda, B, T, lens):
         got = tree_attention(q, layer, torch.tensor(parents), 3, seq_lens=i32(lens), seq_starts=None if st is None else i32(st))
         ref, _ = attend(q, *rows64(layer), tree_mask(parents, max(lens) + T, st or [0] * B, lens))
         check(got, ref)
+
+
+def test_offsets_past_32_bits(cuda):
+    """A cache of 100 million slots: the tokens attended to are its last ones."""
+    N, T, H = 100_000_000, 5, 1
+    small = make_layer(1, H, 200 + T, 4, True, seed=43)
+    st, c = small._store, small.codecs
+    big = {n: torch.zeros((1, H, N, *getattr(st, n).shape[3:]), dtype=getattr(st, n).dtype, device="cuda")
+           for n in ("kc", "kn", "ks", "kr", "vc", "vn")}
+    for n, b in big.items():
+        b[:, :, N - 200 - T:] = getattr(st, n)[:, :, :200 + T]
+    q = randn((1, 4, T, D), 5)
+    parents = random_tree(T, 1)
+    got = K.tree_attention(q, torch.tensor(parents), k_codes=big["kc"], k_norms=big["kn"], v_codes=big["vc"], v_norms=big["vn"],
+                           n_tokens=N, key=c.key, value=c.value, k_signs=big["ks"], k_rnorms=big["kr"], qjl=c.qjl,
+                           seq_starts=torch.tensor([N - 200 - T]))
+    ref, _ = attend(q, *rows64(small), tree_mask([parents], 200 + T, [0], [200]))
+    check(got, ref)

@@ -227,7 +227,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
         if (tile >= last) return;
         const int t0 = std::min(w.lo + tile * TK, k_end - 1);
         const char* const rows = reinterpret_cast<const char*>(base + (int64_t)t0 * st);
-        const uint32_t most = (uint32_t)(k_end - 1 - t0) * st2;
+        const uint32_t most = (uint32_t)std::min(k_end - 1 - t0, TK - 1) * st2;
 #pragma unroll
         for (int i = 0; i < CH; ++i)
             load_lds16(rows + (std::min(off + i * (TL / 16) * st2, most) + in_row), dst + i * TL + lds_wave * 64);
