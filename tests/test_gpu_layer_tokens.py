@@ -252,3 +252,41 @@ def test_a_copied_layer_stays_as_it_was(cuda):
     layer.reorder_cache(torch.tensor([1, 1, 1]))
     layer.keep_tokens(torch.arange(290))
     assert same(other, packed, dense)
+
+
+def test_beam_search_of_a_model(cuda):
+    """HF's beam search reorders the layers; generated tokens are kept dense here, so it ends with the same beams."""
+    from ._tiny_model import tiny_llama
+
+    model = tiny_llama(device=cuda, dtype=torch.bfloat16)
+    ids = torch.randint(0, 94, (2, 30), generator=torch.Generator().manual_seed(0)).to(cuda)
+    ref = model.generate(ids, num_beams=3, num_return_sequences=3, max_new_tokens=8, do_sample=False)
+    calls = []
+
+    class Layer(PackedMSELayer):
+        def reorder_cache(self, beam_idx):
+            calls.append(beam_idx.tolist())
+            super().reorder_cache(beam_idx)
+
+    cache = Cache(layers=[Layer(bits=4) for _ in range(2)])
+    got = model.generate(ids, num_beams=3, num_return_sequences=3, max_new_tokens=8, do_sample=False, past_key_values=cache)
+    assert torch.equal(got, ref)
+    assert calls and any(c != list(range(6)) for c in calls)
+
+
+@pytest.mark.parametrize("kind", ["all dense", "qjl and dense"])
+def test_trees_over_layers_without_packed_tokens(cuda, kind):
+    layer = make(kind, B=1, extra=12)
+    if kind != "all dense":  # every packed token gone, the dense ones left
+        layer._store.length = 0
+    k, v = layer._dense_keys, layer._dense_values
+    n = k.shape[2]
+    q = torch.randn(1, 8, 5, D, generator=torch.Generator(device="cuda").manual_seed(1), device=cuda).bfloat16()
+    parents = torch.tensor([-1, 0, 0, 2, -1])
+    sees = torch.eye(5, dtype=torch.bool)
+    for i, p in ((1, 0), (2, 0), (3, 2), (3, 0)):
+        sees[i, p] = True
+    mask = torch.cat((torch.ones(5, n - 5, dtype=torch.bool), sees), 1).to(cuda)
+    ref = attend(q, k, v, mask)
+    got = tree_attention(q, layer, parents, 4).double()
+    assert ((got - ref).abs() <= 2e-3 * ref.abs().max() + 2 ** -8 * ref.abs()).all()
