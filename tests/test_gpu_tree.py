@@ -316,3 +316,27 @@ def test_offsets_past_32_bits(cuda):
                            seq_starts=torch.tensor([N - 200 - T]))
     ref, _ = attend(q, *rows64(small), tree_mask([parents], 200 + T, [0], [200]))
     check(got, ref)
+
+
+def test_replays_with_other_lengths(cuda):
+    """The sharing out of splits happens on the device: a captured call goes by the lengths of its replay."""
+    B, T, N = 3, 4, 3000
+    layer = make_layer(B, 2, N + T, 4, True, seed=45)
+    q, parents = randn((B, 8, T, D), 5), torch.tensor(random_tree(T, 0), dtype=torch.int32, device="cuda")
+    lens = torch.tensor([N, 10, 700], dtype=torch.int32, device="cuda")
+    starts = torch.zeros(B, dtype=torch.int32, device="cuda")
+    tree_attention(q, layer, parents, 4, seq_starts=starts, seq_lens=lens)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = tree_attention(q, layer, parents, 4, seq_starts=starts, seq_lens=lens)
+    for st, ln in (([0, 0, 0], [N, 10, 700]), ([5, 100, 0], [5, N, 1]), ([0, 2999, 64], [N, N, N])):
+        starts.copy_(torch.tensor(st, dtype=torch.int32))
+        lens.copy_(torch.tensor(ln, dtype=torch.int32))
+        again = tree_attention(q, layer, parents, 4, seq_starts=starts, seq_lens=lens)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, again)
+        ref, _ = attend(q, *rows64(layer), tree_mask([parents.tolist()] * B, N + T, st, ln))
+        check(out, ref)

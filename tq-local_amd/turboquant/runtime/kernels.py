@@ -566,6 +566,15 @@ def _int32_on(t: torch.Tensor | None, device: torch.device, name: str, shape: tu
     return t.to(device).clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()
 
 
+def _placed16(t: torch.Tensor) -> tuple[torch.Tensor, int, tuple]:
+    """A 4-D tensor of 16-bit elements with rows of 16-byte aligned places (itself or a copy), its address and strides."""
+    at, st = t.data_ptr(), t.stride()
+    if st[3] == 1 and not ((st[0] | st[1] | st[2]) & 7 or at & 15):
+        return t, at, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.data_ptr(), t.stride()
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_seqlens: torch.Tensor | None = None,
                      seq_starts: torch.Tensor | None = None, seq_ends: torch.Tensor | None = None,
                      scale: float | None = None, out: torch.Tensor | None = None, want_lse: bool = False):
@@ -578,21 +587,22 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
     k, v or another head's q.  Returns [B, Hq, S, D] laid out token by token ([B, S, Hq, D] in memory), and with ``want_lse`` the fp32
     log-sum-exp [B, Hq, S] of the scaled logits (-inf for a row without tokens).
     """
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"expected q [B, Hq, S, D] and k, v [B, Hkv, S, D], got {tuple(q.shape)}, {tuple(k.shape)}, "
+    qsh, ksh, dtype = q.shape, k.shape, q.dtype
+    if len(qsh) != 4 or len(ksh) != 4 or ksh != v.shape:
+        raise ValueError(f"expected q [B, Hq, S, D] and k, v [B, Hkv, S, D], got {tuple(qsh)}, {tuple(ksh)}, "
                          f"{tuple(v.shape)}")
-    B, Hq, S, D = q.shape
-    Hkv = k.shape[1]
+    B, Hq, S, D = qsh
+    Hkv = ksh[1]
     if D != HEAD_DIM:
         raise ValueError(f"head_dim {D} unsupported (kernels are built for {HEAD_DIM})")
-    if k.shape[0] != B or k.shape[2] != S or k.shape[3] != D or Hkv == 0 or Hq % Hkv:
-        raise ValueError(f"k, v {tuple(k.shape)} do not match q {tuple(q.shape)}: a whole prompt has as many keys as rows")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"q, k and v must all be bf16 or all fp16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if ksh[0] != B or ksh[2] != S or ksh[3] != D or Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"k, v {tuple(ksh)} do not match q {tuple(qsh)}: a whole prompt has as many keys as rows")
+    if dtype not in (torch.bfloat16, torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
+        raise ValueError(f"q, k and v must all be bf16 or all fp16, got {dtype}, {k.dtype}, {v.dtype}")
     _no_gradient("prompt_attention", q, k, v, *(() if out is None else (out,)))
     _require_gpu(q, k, v)
-    dev = q.device
-    if k.device != dev or v.device != dev:
+    dev, on = q.device, q.get_device()
+    if k.get_device() != on or v.get_device() != on:
         raise ValueError("q, k and v must be on one device")
     n_seqs = 0
     if cu_seqlens is not None:
@@ -606,20 +616,19 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
     seq_ends = _int32_on(seq_ends, dev, "seq_ends", (B,))
     zero_outside = out is None
     if out is None:
-        out = torch.empty(B, S, Hq, D, dtype=q.dtype, device=dev).transpose(1, 2)
+        out = torch.empty((B, S, Hq, D), dtype=dtype, device=dev).transpose(1, 2)
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != dev or rows16(out) is not out
           or any(st == 0 and n > 1 for st, n in zip(out.stride(), out.shape))):
         raise ValueError("out must have q's shape, dtype and device, with 16-byte aligned rows of its own")
     lse = torch.empty(B, Hq, S, dtype=torch.float32, device=dev) if want_lse else None
-    if q.numel() == 0:
+    if B == 0 or Hq == 0 or S == 0:
         return (out, lse) if want_lse else out
     if want_lse and not zero_outside:
         lse.fill_(float("-inf"))
-    q, k, v = rows16(q), rows16(k), rows16(v)
+    (q, qp, qs), (k, kp, ks), (v, vp, vs) = _placed16(q), _placed16(k), _placed16(v)
     s = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    qs, ks, vs, os = q.stride(), k.stride(), v.stride(), out.stride()
-    _on_device("tq_prompt_attention", q.get_device(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(lse),
-               int(q.dtype == torch.float16), B, Hq, Hkv, S, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
+    os = out.stride()
+    _on_device("tq_prompt_attention", on, qp, kp, vp, out.data_ptr(), _ptr(lse), int(dtype is torch.float16), B, Hq, Hkv, S, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
                vs[2], os[0], os[1], os[2], _ptr(cu_seqlens), n_seqs, _ptr(seq_starts), _ptr(seq_ends), int(zero_outside),
                s, _stream_handle(dev))
     return (out, lse) if want_lse else out
