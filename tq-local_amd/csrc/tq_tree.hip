@@ -374,7 +374,7 @@ struct Tree {
     struct Tiles {
         uint32_t table[256 * 64];
         uint4 v[W][16 * 16];
-        // the rows' operands for the signs, and with two blocks of rows those for the codes: they do not fit the registers
+        // the rows' operands for the signs and for the codes (these go on to registers with one block of rows; two do not fit)
         uint4 qs[RB][8 * 64], qc[RB][8 * 64];
         uint16_t kn[W][32], vn[W][32];
         float ratio[W][32];
