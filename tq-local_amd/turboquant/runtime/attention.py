@@ -5,8 +5,8 @@
 the module (``module._tq_cache_layer``) a decode step runs the fused libtq
 kernel over the packed history, and several query tokens at once run
 ``chunked_turboquant_attention`` (libtq decoding, fp32 online softmax); without a
-packed layer (prefill, norm-guarded dense layers) it is plain SDPA, as in the
-reference.  "turboquant_prompt" is the same with whole causal prompts on libtq's own
+packed layer (prefill, norm-guarded dense layers, layers whose tokens are all
+dense) it is plain SDPA, as in the reference.  "turboquant_prompt" is the same with whole causal prompts on libtq's own
 kernel (``prompt_attention``); ``tree_attention`` is the call for drafted tokens.
 
 ``fused_attention`` replaces the reference's Triton host wrapper
@@ -447,13 +447,35 @@ def _sdpa_fallback(module, query, key, value, attention_mask, scaling):
     return out.transpose(1, 2).contiguous(), None
 
 
+def _hands_over_all(layer: "PackedMSELayer", query: torch.Tensor, key: torch.Tensor,
+                    attention_mask: torch.Tensor | None) -> bool:
+    """Whether the call's own keys are all that its rows attend to.
+
+    A layer with the backend wired hands over the new tokens alone.  They are everything where it held nothing
+    before them: at a first prompt, and at the one after ``crop`` or ``keep_tokens`` left nothing.  Where that prompt
+    has been packed, its rows attend to the exact keys, each up to its own token, as those of a prompt that is packed
+    afterwards do; a call with a mask has its rows' ranges there, and takes the packed tokens."""
+    if layer._force_dense:
+        return True
+    held = layer.get_seq_length()
+    if layer.packed_seq_length() == 0:
+        return held <= key.shape[-2]
+    Sq = query.shape[-2]
+    return attention_mask is None and 1 < Sq == held and key is not None and key.shape[-2] == Sq
+
+
 def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor,
                                  value: torch.Tensor, attention_mask: torch.Tensor | None, dropout: float = 0.0,
                                  scaling: float | None = None, is_causal: bool | None = None, **kwargs):
     """HF attention-interface function: returns ([B, Sq, Hq, D], None)."""
     layer = getattr(module, "_tq_cache_layer", None)
-    if layer is None or layer._force_dense or layer.packed_seq_length() == 0:
+    if layer is None or _hands_over_all(layer, query, key, attention_mask):
         return _sdpa_fallback(module, query, key, value, attention_mask, scaling)
+    if layer.packed_seq_length() == 0:  # the tokens before are dense: attended to as a norm-guarded layer's are
+        Sq, held = query.shape[-2], layer.get_seq_length()
+        if attention_mask is None and Sq > 1:
+            attention_mask = torch.ones(Sq, held, dtype=torch.bool, device=query.device).tril(held - Sq)
+        return _sdpa_fallback(module, query, layer._dense_keys, layer._dense_values, attention_mask, scaling)
     n_kv_groups = getattr(module, "num_key_value_groups", 1)
     out = fused_attention(query, layer, n_kv_groups, attention_mask) if query.shape[-2] == 1 else None
     if out is None:  # several query tokens, or a shape / mask the fused kernel does not take
@@ -466,7 +488,7 @@ def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key:
                               scaling: float | None = None, is_causal: bool | None = None, **kwargs):
     """HF attention-interface function "turboquant_prompt": whole causal prompts without a mask, alone or packed
     (``cu_seq_lens_q``), go through ``prompt_attention``; what it does not take (a mask, dropout, a gradient, a trace or a
-    transform, other types, head sizes and keys than the prompt's own) and layers that hold packed tokens go the way of "turboquant".
+    transform, other types, head sizes and keys than the prompt's own) and layers that hold earlier tokens go the way of "turboquant".
     One tensor as ``cu_seq_lens_q`` and ``cu_seq_lens_k`` spares a host sync that compares them."""
     causal = getattr(module, "is_causal", True) if is_causal is None else is_causal
     window = kwargs.get("sliding_window")
@@ -480,7 +502,7 @@ def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key:
             and not K.torch_operations_watched()
             and not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))):
         layer = getattr(module, "_tq_cache_layer", None)
-        if layer is None or layer._force_dense or layer.packed_seq_length() == 0:
+        if layer is None or _hands_over_all(layer, query, key, attention_mask):
             return prompt_attention(query, key, value, cu_seqlens=cu, scale=scaling).transpose(1, 2), None
     return turboquant_attention_forward(module, query, key, value, attention_mask, dropout, scaling, is_causal, **kwargs)
 
