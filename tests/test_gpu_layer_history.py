@@ -89,3 +89,18 @@ def test_dense_again(cuda, forward, how, dtype):
                                           torch.ones(b - a, b, device=cuda).tril(a).bool()))
     got = tree_attention(q[:, :, S + 2:], layer, torch.tensor([-1, 0, 1]), G)
     check(got, attend(q[:, :, S + 2:], k, v, torch.ones(3, S + 5, device=cuda).tril(S + 2).bool()))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("split", [False, True])
+def test_without_the_backend(cuda, packed, split):
+    """A layer that hands its history over goes on from an empty one."""
+    k, v = (kv_bf16((B, H, S + 1, D), seed=i) for i in (0, 1))
+    layer = emptied(make(k[:, :, :S], v[:, :, :S], split, packed, wired=False), "crop")
+    assert layer._decode_keys_full().shape == (B, H, 0, D)
+    got = layer.update(k[:, :, :S], v[:, :, :S])
+    assert torch.equal(got[0], k[:, :, :S]) and torch.equal(got[1], v[:, :, :S])
+    keys, values = layer.update(k[:, :, S:], v[:, :, S:])
+    assert keys.shape == values.shape == (B, H, S + 1, D) and torch.equal(keys[:, :, S:], k[:, :, S:])
+    if not packed:
+        assert torch.equal(keys, k) and torch.equal(values, v)

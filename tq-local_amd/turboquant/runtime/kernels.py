@@ -232,6 +232,8 @@ def dequantize_group(codes: torch.Tensor, norms: torch.Tensor, tokens: int, g: G
         raise ValueError("out must be a contiguous bf16 [B, H, tokens, D] tensor")
     if start < 0 or start + tokens > cap:
         raise ValueError(f"slots [{start}, {start + tokens}) outside the capacity {cap}")
+    if out.numel() == 0:
+        return
     _lib.call("tq_dequantize_group", _at_slot(codes, start), _at_slot(norms, start),
               _at_slot(signs if qjl else None, start), _at_slot(rnorms if qjl else None, start), B * H, tokens,
               cap, out.shape[-1], g.channels.ctypes.data, g.dim,
@@ -248,6 +250,8 @@ def dequantize_mse(codes: torch.Tensor, norms: torch.Tensor, tokens: int, codec:
     if start < 0 or start + tokens > cap:
         raise ValueError(f"slots [{start}, {start + tokens}) outside the capacity {cap}")
     out = torch.empty(B, H, tokens, dim, dtype=torch.bfloat16, device=codes.device)
+    if out.numel() == 0:  # no tokens have no address
+        return out
     _lib.call("tq_dequantize_mse", _at_slot(codes, start), _at_slot(norms, start), B * H, tokens, cap, dim, codec.bits,
               _vp(codec.rotation), _vp(codec.centers), _vp(out), _stream(codes.device))
     return out
@@ -263,6 +267,8 @@ def dequantize_prod(codes: torch.Tensor, norms: torch.Tensor, signs: torch.Tenso
     if start < 0 or start + tokens > cap:
         raise ValueError(f"slots [{start}, {start + tokens}) outside the capacity {cap}")
     out = torch.empty(B, H, tokens, dim, dtype=torch.bfloat16, device=codes.device)
+    if out.numel() == 0:  # no tokens have no address
+        return out
     _lib.call("tq_dequantize_prod", _at_slot(codes, start), _at_slot(norms, start), _at_slot(signs, start),
               _at_slot(rnorms, start), B * H, tokens, cap, dim,
               codec.bits, _vp(codec.rotation), _vp(codec.centers), _vp(qjl), _vp(out), _stream(codes.device))
