@@ -350,6 +350,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
         const float base = top == -__builtin_inff() ? 0.0f : top;
+        float added = 0.0f;  // a tile's weights first: one by one, small ones lose their last bits to a large sum
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -359,10 +360,11 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
                     const int i = 8 * x + 2 * k;
                     s[t][i] = exp2_(__builtin_fmaf(s[t][i], c2, -base));
                     s[t][i + 1] = exp2_(__builtin_fmaf(s[t][i + 1], c2, -base));
-                    sum += s[t][i];
-                    sum += s[t][i + 1];
+                    added += s[t][i];
+                    added += s[t][i + 1];
                     p[2 * t + x].u[k] = pack2<F16>(s[t][i], s[t][i + 1]);
                 }
+        sum += added;
     };
     constexpr std::true_type yes{};
     constexpr std::false_type no{};
