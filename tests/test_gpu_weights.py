@@ -12,6 +12,18 @@ pytestmark = pytest.mark.gpu
 D = 128
 
 
+def randn(shape, seed):
+    return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def causal(q, k, v, rows):
+    """fp64 output and mean absolute value of these rows of one KV head's query heads [Hq, S, D]."""
+    x = q[:, rows].double() @ k.double().T / math.sqrt(D)
+    x = x.masked_fill(torch.arange(k.shape[0], device=x.device) > rows[:, None], float("-inf"))
+    p = torch.softmax(x, -1)
+    return p @ v.double(), p @ v.double().abs()
+
+
 # one query head takes blocks of 128 rows, 18 of them (576 blocks) blocks of 256
 @pytest.mark.parametrize("heads", [1, 18])
 @pytest.mark.parametrize("above", [10.0, 12.0])
@@ -26,3 +38,26 @@ def test_the_log_sum_exp_of_many_small_weights(cuda, heads, above):
     top = 8.0 * k[0, 0, 0, 0].double() / math.sqrt(D)
     ref = top + torch.log1p(torch.arange(S, device="cuda") * torch.exp(-top))
     assert (lse.double() - ref).abs().max() <= 2e-5
+
+
+@pytest.mark.parametrize("heads", [1, 18])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("above", [10.0, 17.0, 18.4, 20.0])
+def test_a_first_token_far_above_the_others_of_a_prompt(cuda, heads, dtype, above):
+    """Its value is zero, so the output is what the small weights, all e^-above, give.
+
+    A weight w of a row whose largest is 1 is rounded by half a step, half w, or in fp16 below 2^-25 by half of 2^-35: 4095 of
+    them, of values up to 2, by 2^-23 in all.  An fp16 output below 2^-14 is rounded by 2^-25.  fp32 logits of 20 are off by
+    128 2^-24 20 / 16 = 1e-5 at most, 2e-5 with the exponentials; the sums of 64 tiles by 64 2^-24 = 4e-6."""
+    S = 4096
+    q = torch.zeros(1, heads, S, D, device="cuda", dtype=dtype)
+    k, v = torch.zeros(1, 1, S, D, device="cuda", dtype=dtype), (1 + randn((1, 1, S, D), 1).sigmoid()).to(dtype)
+    q[..., 0], k[:, :, 0, 0], v[:, :, 0] = 8.0, above * math.sqrt(D) / 8, 0.0
+    got = prompt_attention(q, k, v)
+    rows = torch.tensor([0, 1, 63, 64, 500, 2047, 4000, 4095], device="cuda")
+    ref, size = causal(q[0], k[0, 0], v[0, 0], rows)
+    half = torch.finfo(dtype).eps / 2
+    bound = half * ref.abs() + (half + half * half + 3e-5) * size
+    if dtype == torch.float16:
+        bound = bound + 2 ** -23 + 2 ** -25
+    assert ((got[0][:, rows].double() - ref).abs() <= bound).all()

@@ -28,8 +28,10 @@
 // of which 59 are the products.  The smallest calls are bound by latency, 13 us at 300 tokens.
 //
 // Rounding.  Scores, weights, sums and outputs are fp32; the weights are rounded to the values' type for
-// their product, once and to nearest: off by at most half a step (relative 2^-8 in bf16), as much as the
-// output's own rounding, and independently from weight to weight.  The sum of a row's weights is of the unrounded ones.
+// their product, once and to nearest: off by at most half a step (relative 2^-8 in bf16, 2^-11 in fp16), as much as the
+// output's own rounding, and independently from weight to weight.  Fp16 weights below 2^-25 of their row's reference, which
+// is one of its larger scores, are off by up to 2^-36 of it instead: 16384 of them by 2^-22 of their values, where an fp16 output
+// of that size has steps of 2^-24 and more.  The sum of a row's weights is of the unrounded ones.
 
 #include <algorithm>
 #include <type_traits>
@@ -41,7 +43,14 @@ namespace {
 constexpr int D = TQ_DIM;
 constexpr int TK = 64;  // tokens per tile
 constexpr float LOG2E = 1.44269504f;
-constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's reference by
+// A score may exceed its row's reference by LAZY (log2), and weights are in units of 2^-LIFT.  Fp16 weights reach up to 2^15 and
+// keep their 11 bits down to 2^-25 of the reference's; references that rise more often for it cost nothing with logits of a
+// standard deviation of 1 (1 x 32/8 heads of 8192 tokens take 525 us, and 527 with a LAZY of 8), and 2% with one of 4 (554, 542).  A
+// LAZY of 2 takes 532 and 564
+template <bool F16>
+constexpr float LAZY = F16 ? 4.0f : 8.0f;
+template <bool F16>
+constexpr float LIFT = F16 ? 15.0f - LAZY<F16> : 0.0f;
 
 #define INLINE __attribute__((always_inline))
 constexpr int MFMA = 0x8, DS_READ = 0x100;  // kinds of instructions for the scheduler
@@ -337,8 +346,8 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[t][i]);
-        // the reference is raised when some score is more than 2^LAZY above it; -inf and NaN do not raise it
-        if (__any(__builtin_fmaf(mx, c2, -top) > LAZY)) {
+        // the reference is raised when some score is more than LAZY above it; -inf and NaN do not raise it
+        if (__any(__builtin_fmaf(mx, c2, -top) > LAZY<F16>)) {
             mx = fmaxf(mx, __shfl_xor(mx, 32)) * c2;
             const float ref = mx > top ? mx : top;
             const float corr = top == ref ? 1.0f : exp2_(top - ref);
@@ -349,7 +358,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
-        const float base = top == -__builtin_inff() ? 0.0f : top;
+        const float base = (top == -__builtin_inff() ? 0.0f : top) - LIFT<F16>;
         float added = 0.0f;  // a tile's weights first: one by one, small ones lose their last bits to a large sum
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -515,7 +524,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
     const float inv = live ? 1.0f / (total == 0.0f ? 1.0f : total) : 0.0f;
     const bool mine = row >= w.w_lo && row < w.w_hi;
     if (a.lse && mine && h == 0)
-        a.lse[lse_row + row] = !live || total == 0.0f ? -__builtin_inff() : top / LOG2E + __builtin_logf(total);
+        a.lse[lse_row + row] = !live || total == 0.0f ? -__builtin_inff() : (top - LIFT<F16>) / LOG2E + __builtin_logf(total);
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
