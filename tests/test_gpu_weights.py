@@ -1,4 +1,4 @@
-"""Weights far below their row's largest, against fp64."""
+"""Weights far below their row's largest, and values near the ends of their type's range, against fp64."""
 
 import math
 
@@ -61,3 +61,47 @@ def test_a_first_token_far_above_the_others_of_a_prompt(cuda, heads, dtype, abov
     if dtype == torch.float16:
         bound = bound + 2 ** -23 + 2 ** -25
     assert ((got[0][:, rows].double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("heads", [1, 18])
+@pytest.mark.parametrize("dtype,most", [(torch.bfloat16, 3.3e38), (torch.float16, 65504.0)])
+def test_values_near_the_end_of_their_range(cuda, heads, dtype, most):
+    """A weighted mean of finite values is finite, however many they are, also beside an infinity in another dim.  (Weights'
+    sums of 64 tiles are off by 64 2^-24, products' of 256 times 16 tokens by 256 2^-24 = 2e-5.)"""
+    S = 4096
+    q, k = randn((1, heads, S, D), 1).to(dtype), randn((1, 1, S, D), 2).to(dtype)
+    v = ((0.5 + randn((1, 1, S, D), 3).sigmoid() / 2) * most).to(dtype)
+    v[..., 64:] = -v[..., 64:]
+    rows = torch.tensor([0, 1, 2, 63, 64, 500, 2047, 4000, 4095], device="cuda")
+    ref, size = causal(q[0], k[0, 0], v[0, 0], rows)
+    half = torch.finfo(dtype).eps / 2
+    bound = half * ref.abs() + (half + half * half + 5e-5) * size
+    for infinite in (False, True):
+        if infinite:
+            v[:, :, 70, 5] = float("inf")
+        got = prompt_attention(q, k, v)[0][:, rows].double()
+        if infinite:
+            assert (got[:, 5:, 5] == float("inf")).all()
+            got[:, 5:, 5] = ref[:, 5:, 5]
+        assert torch.isfinite(got).all()
+        assert ((got - ref).abs() <= bound).all()
+
+
+def test_two_tiles_of_one_large_weight_each(cuda):
+    """Two values near the end of bf16's range in tiles of 64 tokens that different waves walk: each sum is finite."""
+    q, k, v = (torch.zeros(1, 1, 128, D, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+    q[..., 0], k[:, :, (5, 70), 0], v[:, :, (5, 70)] = 8.0, 100.0, 3.3e38
+    got = prompt_attention(q, k, v)[0].double()
+    ref = torch.full((128, 1), float(v[0, 0, 5, 0]), dtype=torch.float64, device="cuda")
+    ref[:5] = 0.0
+    assert ((got - ref).abs() <= 2 ** -8 * ref + 1e-5 * ref).all()
+
+
+def test_small_values_beside_nothing_else(cuda):
+    """bf16 values down to 2^-100 keep their digits."""
+    q, k = randn((1, 2, 300, D), 1).bfloat16(), randn((1, 1, 300, D), 2).bfloat16()
+    v = (randn((1, 1, 300, D), 3).bfloat16().float() * 2.0 ** -100).bfloat16()
+    got = prompt_attention(q, k, v)
+    rows = torch.arange(300, device="cuda")
+    ref, size = causal(q[0], k[0, 0], v[0, 0], rows)
+    assert ((got[0].double() - ref).abs() <= 2 ** -8 * ref.abs() + (2 ** -8 + 2 ** -16 + 2e-5) * size).all()

@@ -261,6 +261,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
     f32x16 o[4], s[2];
     Frag p[4];
     float top, sum;  // reference of the row's weights in log2, this lane's share of their sum
+    float lift = LIFT<F16>;
     auto start = [&]() INLINE {
         top = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
@@ -358,7 +359,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[d][i] *= corr;
         }
-        const float base = (top == -__builtin_inff() ? 0.0f : top) - LIFT<F16>;
+        const float base = (top == -__builtin_inff() ? 0.0f : top) - lift;
         float added = 0.0f;  // a tile's weights first: one by one, small ones lose their last bits to a large sum
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -426,7 +427,8 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
     }
 
     // ---- A left-out token's weight is 0, which makes NaN of a value that is not finite.  A workgroup that ends with a sum
-    // that is not finite walks its tiles once more, with care: such values are taken out of the tile and added apart.
+    // that is not finite walks its tiles once more, with care: such values are taken out of the tile and added apart, and
+    // bf16 weights are in units of 2^32, so that no number of finite values adds up to an infinity.
     uint32_t most = 0u;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
@@ -434,6 +436,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
         for (int i = 0; i < 16; ++i) most = std::max(most, __float_as_uint(o[d][i]) & 0x7FFFFFFFu);
     if (__syncthreads_or(most >= 0x7F800000u)) {
         start();
+        if constexpr (!F16) lift = -32.0f;
         uint4 *const ck = s_k[0][0], *const cv = s_v[0][0];
         constexpr int CC = TK * 16 / T;
 #pragma unroll 1
@@ -494,7 +497,7 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
         }
     }
 
-    float total = sum + __shfl_xor(sum, 32);
+    float total = sum + __shfl_xor(sum, 32), inv;
     if constexpr (KS == 2) {  // the halves' sums meet
         float* const meet = reinterpret_cast<float*>(s_k);
         float2* const ms = reinterpret_cast<float2*>(s_v);
@@ -510,21 +513,24 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
         if (second) return;
         const float2 m = ms[wave * 64 + lane];
         const float best = fmaxf(top, m.x), safe = best == -__builtin_inff() ? 0.0f : best;
-        const float w0 = exp2_(top - safe), w1 = exp2_(m.x - safe);
+        float w0 = exp2_(top - safe), w1 = exp2_(m.x - safe);
         total = total * w0 + m.y * w1;
         top = best;
+        // divided first: two finite sums may add up to an infinity
+        w0 /= total == 0.0f ? 1.0f : total, w1 /= total == 0.0f ? 1.0f : total, inv = 1.0f;
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 o[d][i] = o[d][i] * w0 + (w1 == 0.0f ? 0.0f : meet[(wave * 64 + 16 * d + i) * 64 + lane] * w1);
+    } else {
+        inv = 1.0f / (total == 0.0f ? 1.0f : total);
     }
 
     // ---- rows out: two lanes hold a row's dims 8 j + 4 h + (0..3); pairs of j are exchanged for 16-byte stores
-    const float inv = live ? 1.0f / (total == 0.0f ? 1.0f : total) : 0.0f;
     const bool mine = row >= w.w_lo && row < w.w_hi;
     if (a.lse && mine && h == 0)
-        a.lse[lse_row + row] = !live || total == 0.0f ? -__builtin_inff() : (top - LIFT<F16>) / LOG2E + __builtin_logf(total);
+        a.lse[lse_row + row] = !live || total == 0.0f ? -__builtin_inff() : (top - lift) / LOG2E + __builtin_logf(total);
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
