@@ -5,7 +5,12 @@ import math
 import pytest
 import torch
 
+from turboquant.runtime import kernels as K
 from turboquant.runtime import prompt_attention
+from turboquant.runtime.packed_qmse_cache import PackedMSELayer
+from turboquant.runtime.synthetic import kv_bf16
+
+from .test_gpu_tree import attend, rows64
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +110,39 @@ def test_small_values_beside_nothing_else(cuda):
     rows = torch.arange(300, device="cuda")
     ref, size = causal(q[0], k[0, 0], v[0, 0], rows)
     assert ((got[0].double() - ref).abs() <= 2 ** -8 * ref.abs() + (2 ** -8 + 2 ** -16 + 2e-5) * size).all()
+
+
+@pytest.mark.parametrize("qjl", [False, True])
+@pytest.mark.parametrize("nodes", [3, 20])
+@pytest.mark.parametrize("above", [10.0, 17.0, 18.4, 19.7])
+def test_tokens_far_above_the_others_of_a_tree(cuda, qjl, nodes, above):
+    """One token of every 32 far above the others, with a value of next to nothing; the others' keys are zero and their
+    values alike, so that the output is what 31 of 32 small weights give.
+
+    Weights times norms are fp16 numbers w in units of 2^-11 of the reference's times a power of two above the largest norm
+    (20 of 32 here): below 2^-14 they are off by 2^-25.  The large logits are of the size that the package's tolerance of 2e-3
+    is derived for and move all weights alike: the error of 1e-3 root mean square may be four times that."""
+    layer = PackedMSELayer(bits=4, use_qjl_keys=qjl, quantize_decode=True)
+    N = 4096
+    layer.initialize_from_dense(kv_bf16((1, 1, N, D), seed=1), kv_bf16((1, 1, N, D), seed=2))
+    st, c, first = layer._store, layer.codecs, slice(7, N - nodes, 32)
+    for n in (st.kc, st.ks) if qjl else (st.kc,):
+        n[:, :, first] = n[:, :, 7:8].clone()
+    st.vc[:, :, :N], st.vn[:, :, :N] = st.vc[:, :, 5:6].clone(), 20.0
+    st.vn[:, :, first] = 2.0 ** -24
+    for n in (st.kn, st.kr) if qjl else (st.kn,):
+        one = n[:, :, 7:8].clone()
+        n.zero_()
+        n[:, :, first] = one
+    k, v = rows64(layer)
+    row = k[0, 0, 7]
+    q = (row * (above * math.sqrt(D) / (row @ row))).float().expand(1, 4, nodes, D).contiguous()
+    _, f32, lse = K.tree_attention(q, torch.full((nodes,), -1, device="cuda"), k_codes=st.kc, k_norms=st.kn, v_codes=st.vc,
+                                   v_norms=st.vn, n_tokens=N, key=c.key, value=c.value, k_signs=st.ks, k_rnorms=st.kr,
+                                   qjl=c.qjl, want_f32=True, want_lse=True)
+    mask = torch.ones(1, nodes, N, dtype=torch.bool, device="cuda")
+    mask[:, :, N - nodes:] = torch.eye(nodes, device="cuda").bool()
+    ref, ref_lse = attend(q, k, v, mask)
+    assert (lse.double() - ref_lse).abs().max() <= 4e-3
+    w = 2 ** 11 * math.exp(-above) * 20 / 32
+    assert ((f32.double() - ref).abs() <= (6e-3 + 2 ** -25 / w) * ref.abs().max()).all()

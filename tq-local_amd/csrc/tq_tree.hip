@@ -28,7 +28,8 @@
 //
 // Rounding.  Rotated queries and centroids are rounded once to fp16, by at most 2^-11 of each, 2^-11 / sqrt(3) root mean square (with
 // |q| = 11 and |k| = 20 a logit moves by 7e-4), value centroids too (their sum's errors are kept from adding up by the
-// codebook, see tq_value_codebook_f16), weights times norm p |v| once.  Logits, maxima, weights, sums and outputs are fp32.
+// codebook, see tq_value_codebook_f16), weights times norm p |v| once: to 11 bits down to 2^-25 of the largest norm's at the row's
+// reference, and by up to 2^-36 of it below.  Logits, maxima, weights, sums and outputs are fp32.
 
 #include <algorithm>
 #include <type_traits>
@@ -42,8 +43,11 @@ constexpr int TK = 32;         // tokens per tile
 constexpr int MIN_TILES = 8;   // tiles of a split
 constexpr int MAX_SPLIT = 64;  // partials a merge wave weighs with one lane each
 constexpr float LOG2E = 1.44269504f;
-constexpr float LAZY = 8.0f;  // log2 that a score may exceed its row's reference by
-constexpr int TOP_BIT = 7;    // largest weight times norm at the reference: 2^TOP_BIT
+// Log2 that a score may exceed its row's reference by, and of the largest weight times norm at the reference: 15 together, what fp16
+// holds.  The less a score may exceed it the smaller the weights that keep their bits, and the more often references rise: with 4 the
+// calls of the header take 159 and 71 us, with 8 156 and 69, with 2 160 and 72
+constexpr float LAZY = 4.0f;
+constexpr int TOP_BIT = 11;
 constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
 
 #define INLINE __attribute__((always_inline))
@@ -614,7 +618,7 @@ __global__ __launch_bounds__(Tree<RB>::T, 2) void tree_kernel(TreeArgs a) {
         for (int d = 0; d < 4; ++d) o[m][d] = zero16();
     }
     // weights and output sums are in units of 2^-shift, 2^-TOP_BIT of a power of two above the largest |v| so far: weights
-    // times norm then reach up to 2^(TOP_BIT + LAZY), and fp16 keeps its 11 bits down to 2^-14
+    // times norm then reach up to 2^(TOP_BIT + LAZY), and fp16 keeps its 11 bits down to 2^-14, 2^-25 of the reference's
     int shift = TOP_BIT + 24;
     const uint32_t lane4 = (lane & 31) * 4;
     const uint8_t* const table = reinterpret_cast<const uint8_t*>(lds.t.table);
