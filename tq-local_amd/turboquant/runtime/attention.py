@@ -483,17 +483,39 @@ def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, k
     return out.transpose(1, 2).contiguous(), None
 
 
+def _sequences_mask(cu: torch.Tensor, cu_k: torch.Tensor, rows: int, keys: int, causal: bool, window: int | None,
+                    device: torch.device) -> torch.Tensor:
+    """bool [rows, keys]: the keys each row of sequences packed behind one another attends to; a sequence's rows and keys end
+    together."""
+    def ranges(offsets: torch.Tensor, n: int):  # each place's sequence, how far from its end, and whether it is of any
+        offsets, at = offsets.to(device).long(), torch.arange(n, device=device)
+        seq = torch.searchsorted(offsets[1:].contiguous(), at, right=True)
+        left = offsets[1:][seq.clamp(max=offsets.numel() - 2)] - at
+        return seq, left, (at >= offsets[0]) & (at < offsets[-1])
+
+    (seq, left, live), (seq_k, left_k, live_k) = ranges(cu, rows), ranges(cu_k, keys)
+    mask = (seq[:, None] == seq_k[None, :]) & live[:, None] & live_k[None, :]
+    back = left_k[None, :] - left[:, None]  # 0: the row's own token
+    if causal:
+        mask &= back >= 0
+    if window is not None:
+        mask &= back < window
+    return mask
+
+
 def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                               attention_mask: torch.Tensor | None, dropout: float = 0.0,
                               scaling: float | None = None, is_causal: bool | None = None, **kwargs):
     """HF attention-interface function "turboquant_prompt": whole causal prompts without a mask, alone or packed
-    (``cu_seq_lens_q``), go through ``prompt_attention``; what it does not take (a mask, dropout, a gradient, a trace or a
+    (``cu_seq_lens_q``, a batch of 1), go through ``prompt_attention``; what it does not take (a mask, dropout, a gradient, a trace or a
     transform, other types, head sizes and keys than the prompt's own) and layers that hold earlier tokens go the way of "turboquant".
+    Packed sequences keep to themselves there too, by a mask made from their offsets; one that is given counts instead of them.
     One tensor as ``cu_seq_lens_q`` and ``cu_seq_lens_k`` spares a host sync that compares them."""
     causal = getattr(module, "is_causal", True) if is_causal is None else is_causal
     window = kwargs.get("sliding_window")
     cu, cu_k = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
     S = query.shape[-2]
+    layer = getattr(module, "_tq_cache_layer", None)
     if (attention_mask is None and causal and not dropout and S > 1 and query.shape[-1] == K.HEAD_DIM
             and key.shape == value.shape and key.shape[-2:] == query.shape[-2:] and query.is_cuda
             and query.dtype in (torch.bfloat16, torch.float16) and key.dtype == value.dtype == query.dtype
@@ -501,9 +523,21 @@ def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key:
             and (cu is None or (query.shape[0] == 1 and (cu_k is None or cu_k is cu or torch.equal(cu_k, cu))))
             and not K.torch_operations_watched()
             and not (torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad))):
-        layer = getattr(module, "_tq_cache_layer", None)
         if layer is None or _hands_over_all(layer, query, key, attention_mask):
             return prompt_attention(query, key, value, cu_seqlens=cu, scale=scaling).transpose(1, 2), None
+    if cu is not None and attention_mask is None and S > 1:
+        cu_k = cu if cu_k is None else cu_k
+        if query.shape[0] != 1:
+            raise ValueError(f"cu_seq_lens_q takes sequences packed into a batch of 1, got {query.shape[0]}")
+        if cu_k.numel() != cu.numel():
+            raise ValueError("cu_seq_lens_q and cu_seq_lens_k must name as many sequences")
+        if layer is None or _hands_over_all(layer, query, key, None):
+            mask = _sequences_mask(cu, cu_k, S, key.shape[-2], causal, window, query.device)
+            empty = ~mask.any(-1, keepdim=True)  # rows of no sequence, or without keys
+            out, _ = _sdpa_fallback(module, query, key, value, mask | empty, scaling)
+            return out.masked_fill(empty[None, :, None], 0.0), None
+        if cu.numel() > 2:
+            raise ValueError("packed sequences, but the cache layer holds tokens before them")
     return turboquant_attention_forward(module, query, key, value, attention_mask, dropout, scaling, is_causal, **kwargs)
 
 
