@@ -373,7 +373,7 @@ def _tree_mask(parents: torch.Tensor, total: int, starts: torch.Tensor | None, e
 
 
 def tree_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", parents: torch.Tensor,
-                   n_kv_groups: int = 1, seq_starts: torch.Tensor | None = None,
+                   n_kv_groups: int | None = None, seq_starts: torch.Tensor | None = None,
                    seq_lens: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of a tree of drafted tokens, [B, Hq, T, D] over a packed layer -> [B, Hq, T, D].
 
@@ -381,7 +381,8 @@ def tree_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", p
     generated tokens).  ``parents`` int [T] or [B, T]: the node each follows, an earlier one, or -1; a
     node attends to the history, to its ancestors and to itself (a chain -1, 0, 1, ... is causal).
     ``seq_starts`` / ``seq_lens`` int [B]: row b's history is the tokens [start, len) and its nodes the T
-    tokens from len on (packed nodes only).  After the drafts are checked, ``keep_tokens`` of the layer closes
+    tokens from len on (packed nodes only).  ``n_kv_groups`` (query heads per KV head) follows from the shapes; another
+    number is refused.  After the drafts are checked, ``keep_tokens`` of the layer closes
     up the accepted path.
 
     One-group layers with up to 64 nodes run on the packed codes (``kernels.tree_attention``), tokens kept
@@ -397,10 +398,17 @@ def tree_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", p
         raise ValueError(f"{T} drafted tokens, but the layer holds {n_dense or n_packed} of their kind")
     if n_dense and seq_lens is not None:
         raise ValueError("seq_lens needs the drafted tokens packed (quantize_decode=True)")
+    store = packed_layer._store
+    if total == 0:  # no nodes either
+        return torch.empty_like(query_states)
+    batch, kv_heads = (store.B, store.H) if store is not None else packed_layer._dense_buf[0].shape[:2]
+    if batch != B or Hq % kv_heads or n_kv_groups not in (None, Hq // kv_heads):
+        raise ValueError(f"queries {tuple(query_states.shape)} with n_kv_groups {n_kv_groups} do not match a layer of "
+                         f"{batch} rows and {kv_heads} KV heads")
+    n_kv_groups = Hq // kv_heads
     dev = query_states.device
     seq_starts = K._int32_on(seq_starts, dev, "seq_starts", (B,))
     seq_lens = K._int32_on(seq_lens, dev, "seq_lens", (B,))
-    store = packed_layer._store
     fused = (store is not None and not packed_layer._outlier_enabled and T <= K.MAX_NODES
              and query_states.dtype in K._QUERY_TYPES)
     if fused:
