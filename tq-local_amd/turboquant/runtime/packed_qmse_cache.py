@@ -621,6 +621,12 @@ class PackedMSELayer(CacheLayerMixin):
         return self.packed_seq_length() + dense
 
     # ------------------------------------------- rows and tokens chosen and moved
+    def _batch(self) -> int | None:
+        """Batch rows held (None: nothing is)."""
+        if self._store is not None:
+            return self._store.B
+        return None if self._dense_buf is None else int(self._dense_buf[0].shape[0])
+
     def _take_rows(self, rows: torch.Tensor) -> None:
         if self._store is not None:
             self._store.take(rows=rows)
@@ -629,19 +635,38 @@ class PackedMSELayer(CacheLayerMixin):
             dense = list(self._dense_buf)
             self._dense_buf = tuple(K.gather_tokens(dense, tokens=self._dense_len, rows=rows, capacity=dense[0].shape[2]))
 
+    def _check_rows(self, rows: torch.Tensor, first: int) -> None:
+        """Numbers outside [first, batch) are refused where the host has them; to look on the device would wait for it."""
+        batch = self._batch()
+        if batch is not None and not rows.is_cuda and rows.numel() and not rows.is_floating_point():
+            if int(rows.min()) < first or int(rows.max()) >= batch:
+                raise IndexError(f"rows {rows.tolist()} of a batch of {batch}")
+
     def reorder_cache(self, beam_idx: torch.Tensor) -> None:
-        """Batch row r becomes row beam_idx[r] (one launch for the packed buffers and one for the dense; a row
-        that there is not becomes zeros)."""
+        """Batch row r becomes row beam_idx[r] (one launch for the packed buffers and one for the dense).  A row
+        that there is not is refused, or becomes zeros where ``beam_idx`` is on the device."""
+        self._check_rows(beam_idx, 0)
         self._take_rows(beam_idx)
 
     def batch_select_indices(self, indices: torch.Tensor) -> None:
-        """Only these batch rows (numbers, or a bool for each row)."""
-        self._take_rows(indices.nonzero().flatten() if indices.dtype == torch.bool else indices)
+        """Only these batch rows (numbers, negative ones from the last row, or a bool for each row).  A row that there is
+        not as in ``reorder_cache``."""
+        batch = self._batch()
+        if batch is None:
+            return
+        if indices.dtype == torch.bool:
+            if indices.shape != (batch,):
+                raise IndexError(f"a mask of {tuple(indices.shape)} for a batch of {batch}")
+            indices = indices.nonzero().flatten()
+        else:
+            self._check_rows(indices, -batch)
+            indices = torch.where(indices < 0, indices + batch, indices)
+        self._take_rows(indices)
 
     def batch_repeat_interleave(self, repeats: int) -> None:
         """Every batch row ``repeats`` times."""
-        if self._store is not None or self._dense_buf is not None:
-            batch = self._store.B if self._store is not None else self._dense_buf[0].shape[0]
+        batch = self._batch()
+        if batch is not None:
             self._take_rows(torch.arange(batch, device=self.device).repeat_interleave(repeats))
 
     def crop(self, tokens_to_remove: int) -> None:
