@@ -546,6 +546,17 @@ def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
         raise ValueError(f"{name} has no derivative: a tensor carries a tangent")
 
 
+#: the dispatch modes of torch's own tracers; others look on
+_TRACERS = tuple(getattr(torch._C._TorchDispatchModeKey, n) for n in ("PROXY", "FAKE", "FUNCTIONAL"))
+
+
+def _not_traced(name: str) -> None:
+    """A trace would keep the empty outputs and miss what is written into them, as would a transform."""
+    if (torch._C._is_tracing() or torch._C._functorch.peek_interpreter_stack() is not None
+            or (torch._C._len_torch_dispatch_stack() and any(torch._C._get_dispatch_mode(m) is not None for m in _TRACERS))):
+        raise ValueError(f"{name} cannot be traced or transformed: torch does not see what it computes")
+
+
 _get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -606,6 +617,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
     if dtype not in (torch.bfloat16, torch.float16) or k.dtype is not dtype or v.dtype is not dtype:
         raise ValueError(f"q, k and v must all be bf16 or all fp16, got {dtype}, {k.dtype}, {v.dtype}")
     _no_gradient("prompt_attention", q, k, v, *(() if out is None else (out,)))
+    _not_traced("prompt_attention")
     _require_gpu(q, k, v)
     dev, on = q.device, q.get_device()
     if k.get_device() != on or v.get_device() != on:
@@ -675,6 +687,7 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor | None, *, k_codes: to
     if (k_rnorms is not None) != has_qjl or (qjl is not None) != has_qjl:
         raise ValueError("Q_prod keys need k_signs, k_rnorms and qjl")
     _no_gradient("tree_attention", q)
+    _not_traced("tree_attention")
     _require_gpu(q)
     dev, on = q.device, q.get_device()
     for name, t, row in (("k_codes", k_codes, 16 * key.bits), ("v_codes", v_codes, 16 * value.bits),
@@ -739,6 +752,7 @@ def _move_buffers(name: str, buffers: list[torch.Tensor]) -> tuple[int, int, int
     """(batch, heads, cap, row bytes) of a layer's [B, H, cap, ...] buffers."""
     if not buffers:
         raise ValueError(f"{name}: no buffers")
+    _not_traced(name)
     first, dev, rows = buffers[0].shape, buffers[0].get_device(), []
     if len(first) < 3:
         raise ValueError(f"{name}: expected [B, H, cap, ...] buffers, got {tuple(first)}")
