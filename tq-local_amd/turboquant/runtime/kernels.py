@@ -329,6 +329,9 @@ def attention_value_centers(codec: CodecParams | GroupCodec) -> torch.Tensor:
     codec's centers (at the group's dimension for a channel group), on the codec's
     device, computed once per codec."""
     if codec.attn_centers is None:
+        if codec.centers.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a value codec's attention codebook is made on the host: call attention_value_centers(codec) "
+                               "before the graph is captured")
         dim = codec.dim if isinstance(codec, GroupCodec) else HEAD_DIM
         host = value_codebook_f16(codec.centers.detach().cpu().numpy(), codec.bits, dim)
         codec.attn_centers = torch.from_numpy(host).to(codec.centers.device)
