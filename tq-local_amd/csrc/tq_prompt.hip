@@ -13,9 +13,7 @@
 //                 is free: it is the order the scores come back in, so a lane's weights become its B
 //                 operand as they are, and ds_read_b64_tr_b16 takes V^T out of row-major rows in that
 //                 order (16 lanes read 4 tokens x 16 dims and each ends with one dim's 4 tokens).
-// K and V go from memory to LDS without passing registers (16 bytes a lane), double-buffered; a row's 16-byte chunk c
-// is at slot c ^ f(token), f taking the token's low four bits to the slot with the bits 0-1 on top, so that
-// the 16 rows of a K read and the 4 x 2 rows of a V read both meet every bank once.
+// K and V go from memory to LDS without passing registers (16 bytes a lane), double-buffered, their chunks swizzled by the token.
 //
 // Cost.  Bound by the matrix pipe and the softmax beside it: a tile of 64 tokens and 32 rows is 32 products of 32 cycles
 // and about 430 cycles of exponentials, maxima, sums and roundings, on a SIMD that holds two waves.  The waves' halves therefore
@@ -36,9 +34,11 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "tq_common.h"
+#include "tq_rows16.h"
 
 namespace {
+
+using namespace tqr;
 
 constexpr int D = TQ_DIM;
 constexpr int TK = 64;  // tokens per tile
@@ -56,56 +56,22 @@ constexpr float LIFT = F16 ? 15.0f - LAZY<F16> : 0.0f;
 constexpr int MFMA = 0x8, DS_READ = 0x100;  // kinds of instructions for the scheduler
 constexpr int AHEAD = 4;                    // products whose operands are on their way
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-union Frag {
-    uint32_t u[4];
-    uint4 q;
-    s16x4 t[2];
-    bf16x8 b;
-    f16x8 f;
-};
-
 template <bool F16>
 __device__ __forceinline__ f32x16 mfma_32(const Frag& a, const Frag& b, f32x16 c) {
-    if constexpr (F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.f, b.f, c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.b, b.b, c, 0, 0, 0);
+    if constexpr (F16) return mfma_f16(a, b, c);
+    else return mfma_bf16(a, b, c);
 }
-// two fp32 values to the element type, nearest even
+// two fp32 values to the element type
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const f32x2 p = {a, b};
-    if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(p, f16x2));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2));
+    if constexpr (F16) return pack_f16(a, b);
+    else return pack_bf16(a, b);
 }
-// 2^x (v_exp_f32, 1 ulp; 2^-inf = 0)
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-
-__device__ __forceinline__ int swizzle(int token) { return ((token & 3) << 2) | ((token >> 2) & 3); }
-
-__device__ __forceinline__ void load_lds16(const void* g, void* l) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g,
-                                     (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
-}
-__device__ __forceinline__ s16x4 read_tr(const uint8_t* l) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)l);
-}
-// Byte offsets in a tile: a lane's 16 bytes of key row r in step ks (plus 32 rows for the second block of tokens), and what it
-// gives ds_read_b64_tr_b16 for dims 32 d + (0..31) of the tokens 8 e + 4 h + (0..3) (plus 16 rows per step).
+// Byte offset in a tile of a lane's 16 bytes of key row r in step ks (plus 32 rows for the second block of tokens); values'
+// in value_offset, plus 16 rows per step.
 __device__ __forceinline__ int key_offset(int ks, int lane) {
     return (lane & 31) * 256 + (((2 * ks + (lane >> 5)) ^ swizzle(lane & 31)) << 4);
 }
-__device__ __forceinline__ int value_offset(int d, int e, int lane) {
-    const int tok = 8 * e + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    return tok * 256 + ((chunk ^ swizzle(tok)) << 4) + 8 * (lane & 1);
-}
-
 struct PromptArgs {
     const uint16_t *q, *k, *v;
     uint16_t* out;
@@ -163,9 +129,8 @@ __device__ __forceinline__ Block find_packed(const PromptArgs& a, int blk, int B
     return {0, 0, 0, (int)row0, (int)row0, (int)std::min<int64_t>(row0 + BM, a.tokens)};
 }
 
-// Waits of a wave for its own loads to LDS and reads of it, and the barrier, with nothing moved across any.
+// The wait of a wave for its own reads of LDS, and the barrier, with nothing moved across either.
 __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_barrier" ::: "memory");
@@ -550,8 +515,6 @@ __global__ __launch_bounds__(512, 2) void prompt_kernel(PromptArgs a) {
                     make_uint4(lo[0], hi[0], lo[1], hi[1]);
         }
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <bool F16, int KS>
 void launch(PromptArgs& a, unsigned grid_kv, hipStream_t s) {

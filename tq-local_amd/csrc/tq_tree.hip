@@ -34,9 +34,11 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "tq_common.h"
+#include "tq_rows16.h"
 
 namespace {
+
+using namespace tqr;
 
 constexpr int D = TQ_DIM;
 constexpr int TK = 32;         // tokens per tile
@@ -52,34 +54,9 @@ constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
 
 #define INLINE __attribute__((always_inline))
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-union Frag {
-    uint32_t u[4];
-    uint4 q;
-    s16x4 t[2];
-    bf16x8 b;
-    f16x8 f;
-};
 
-__device__ __forceinline__ f32x16 mfma_f16(const Frag& a, const Frag& b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.f, b.f, c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x16 mfma_bf16(const Frag& a, const Frag& b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.b, b.b, c, 0, 0, 0);
-}
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    const f32x2 p = {a, b};
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(p, f16x2));
-}
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
     return __builtin_amdgcn_perm(hi, lo, sel);
 }
@@ -180,24 +157,6 @@ __device__ __forceinline__ void expand_signs(uint32_t w, uint4* out) {
         for (int k = 0; k < 4; ++k) x[k] = (j < 2 ? w : v) & (0x00010001u << ((4 * j + k) & 7));
         out[j] = make_uint4(x[0], x[1], x[2], x[3]);
     }
-}
-
-__device__ __forceinline__ int swizzle(int token) { return ((token & 3) << 2) | ((token >> 2) & 3); }
-
-__device__ __forceinline__ void load_lds16(const void* g, void* l) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)g,
-                                     (__attribute__((address_space(3))) uint32_t*)l, 16, 0, 0);
-}
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ s16x4 read_tr(const uint8_t* l) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)l);
-}
-// Byte offset of what a lane gives ds_read_b64_tr_b16 for dims 32 d + (0..31) of the tokens 8 e + 4 h + (0..3) of 16
-// value rows: 16 lanes read 4 tokens x 16 dims, and each ends with one dim's 4 tokens.
-__device__ __forceinline__ int value_offset(int d, int e, int lane) {
-    const int tok = 8 * e + 4 * (lane >> 5) + ((lane & 15) >> 2);
-    const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    return tok * 256 + ((chunk ^ swizzle(tok)) << 4) + 8 * (lane & 1);
 }
 
 // ------------------------------------------------------------------ queries
@@ -935,8 +894,6 @@ __global__ __launch_bounds__(MERGE_T) void merge_kernel(MergeArgs a) {
     }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 struct Plan {
     int rows, row_blocks, n_split, n_slots;
     unsigned row_groups;
@@ -954,10 +911,11 @@ bool make_plan(int batch, int q_heads, int kv_heads, int T, int64_t n_tokens, Pl
     p.row_blocks = (p.rows + 31) / 32;
     p.row_groups = p.row_blocks == 1 ? 1 : (unsigned)(p.row_blocks + 1) / 2;
     const int64_t tiles = std::max<int64_t>(1, (n_tokens + TK - 1) / TK);
-    p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>({256 / (p.heads * p.row_groups), (tiles + MIN_TILES - 1) / MIN_TILES, MAX_SPLIT}));
+    const int64_t most = std::min<int64_t>((tiles + MIN_TILES - 1) / MIN_TILES, MAX_SPLIT);
+    p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(256 / (p.heads * p.row_groups), most));
     // batch rows of different lengths share out what fills the CUs
-    const int64_t most = std::min<int64_t>((tiles + MIN_TILES - 1) / MIN_TILES, MAX_SPLIT) * batch;
-    p.n_slots = (int)std::max<int64_t>((int64_t)p.n_split * batch, std::min<int64_t>(256 / (kv_heads * (int64_t)p.row_groups), most));
+    p.n_slots = (int)std::max<int64_t>((int64_t)p.n_split * batch,
+                                       std::min<int64_t>(256 / (kv_heads * (int64_t)p.row_groups), most * batch));
     p.ms_bytes = ((size_t)p.n_slots * kv_heads * rows * 8 + 15) / 16 * 16;
     p.o_bytes = (size_t)p.n_slots * kv_heads * rows * D * 4;
     p.slots_bytes = ((size_t)batch * 8 + 15) / 16 * 16;
@@ -972,7 +930,7 @@ void launch_tree(const TreeArgs& a, const Plan& p, hipStream_t s) {
     };
     using One = std::integral_constant<int, 1>;
     using Two = std::integral_constant<int, 2>;
-        if (p.row_blocks == 1) a.q_type == 0 ? launch(One{}, One{}) : launch(One{}, Two{});
+    if (p.row_blocks == 1) a.q_type == 0 ? launch(One{}, One{}) : launch(One{}, Two{});
     else a.q_type == 0 ? launch(Two{}, One{}) : launch(Two{}, Two{});
 }
 
@@ -1012,7 +970,8 @@ extern "C" int tq_tree_attention(const void* q, int q_type, int batch, int q_hea
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     float* part_o = reinterpret_cast<float*>(ws);
     float2* part_ms = reinterpret_cast<float2*>(ws + p.o_bytes);
-    int2* const slots = batch > 1 && batch <= 64 && p.n_slots > batch && (seq_starts || seq_lens) ? reinterpret_cast<int2*>(ws + p.o_bytes + p.ms_bytes) : nullptr;
+    const bool ragged = batch > 1 && batch <= 64 && p.n_slots > batch && (seq_starts || seq_lens);
+    int2* const slots = ragged ? reinterpret_cast<int2*>(ws + p.o_bytes + p.ms_bytes) : nullptr;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const TreeArgs a{batch, kv_heads, nodes, p.rows, parents, parents_sb, seq_starts, seq_lens, n_tokens, cap,
                      k_codes, k_signs, v_codes, k_norms, k_rnorms, v_norms, key_centers, value_centers, q, q_type, q_heads / kv_heads,

@@ -649,9 +649,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, cu_se
     (q, qp, qs), (k, kp, ks), (v, vp, vs) = _placed16(q), _placed16(k), _placed16(v)
     s = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     os = out.stride()
-    _on_device("tq_prompt_attention", on, qp, kp, vp, out.data_ptr(), _ptr(lse), int(dtype is torch.float16), B, Hq, Hkv, S, D, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1],
-               vs[2], os[0], os[1], os[2], _ptr(cu_seqlens), n_seqs, _ptr(seq_starts), _ptr(seq_ends), int(zero_outside),
-               s, _stream_handle(dev))
+    _on_device("tq_prompt_attention", on, qp, kp, vp, out.data_ptr(), _ptr(lse), int(dtype is torch.float16), B, Hq, Hkv, S, D,
+               qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], os[0], os[1], os[2], _ptr(cu_seqlens), n_seqs,
+               _ptr(seq_starts), _ptr(seq_ends), int(zero_outside), s, _stream_handle(dev))
     return (out, lse) if want_lse else out
 
 
