@@ -465,11 +465,11 @@ def _hands_over_all(layer: "PackedMSELayer", query: torch.Tensor, key: torch.Ten
     afterwards do; a call with a mask has its rows' ranges there, and takes the packed tokens."""
     if layer._force_dense:
         return True
-    held = layer.get_seq_length()
-    if layer.packed_seq_length() == 0:
-        return held <= key.shape[-2]
-    Sq = query.shape[-2]
-    return attention_mask is None and 1 < Sq == held and key is not None and key.shape[-2] == Sq
+    packed, Sq = layer.packed_seq_length(), query.shape[-2]
+    if packed == 0:
+        return layer._dense_len <= key.shape[-2]
+    return (Sq > 1 and attention_mask is None and Sq == packed + layer._dense_len and key is not None
+            and key.shape[-2] == Sq)
 
 
 def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor,
@@ -480,7 +480,7 @@ def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, k
     if layer is None or _hands_over_all(layer, query, key, attention_mask):
         return _sdpa_fallback(module, query, key, value, attention_mask, scaling)
     if layer.packed_seq_length() == 0:  # the tokens before are dense: attended to as a norm-guarded layer's are
-        Sq, held = query.shape[-2], layer.get_seq_length()
+        Sq, held = query.shape[-2], layer._dense_len
         if attention_mask is None and Sq > 1:
             attention_mask = torch.ones(Sq, held, dtype=torch.bool, device=query.device).tril(held - Sq)
         return _sdpa_fallback(module, query, layer._dense_keys, layer._dense_values, attention_mask, scaling)
