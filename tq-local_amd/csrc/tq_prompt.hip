@@ -17,13 +17,13 @@
 //
 // Cost.  Bound by the matrix pipe and the softmax beside it: a tile of 64 tokens and 32 rows is 32 products of 32 cycles
 // and about 430 cycles of exponentials, maxima, sums and roundings, on a SIMD that holds two waves.  The waves' halves therefore
-// take turns (below).  1 x 32/8 heads of 8192 tokens take 490 to 585 us by the clock of the card = 1120 to 940 TFLOP/s of
-// counted work, where a large product of matrices reaches 1326, and 16384 tokens 1.9 ms = 1160; four waves that each do one thing
+// take turns (below).  1 x 32/8 heads of 8192 tokens take 480 to 525 us by the clock of the card = 1145 to 1050 TFLOP/s of
+// counted work, where a large product of matrices reaches 1326, and 16384 tokens 1.88 to 1.99 ms = 1170 to 1105; four waves that each do one thing
 // after the other took 662 us when these took 584, and eight without the operands read ahead 595 when they took 544 with
 // them.  The clock gives way under this load (1.6 to 1.9 GHz of 2.4), so cycles won come back in part only.  64 rows to a wave
 // (512 registers) took longer: its sums move between the two register files.  Short sequences are bound by a block's
 // start and end, 4 to 5 us of loads and stores that nothing hides: eight packed prompts of 1 to 2811 tokens take 105 us,
-// of which 59 are the products.  The smallest calls are bound by latency, 13 us at 300 tokens.
+// of which 59 are the products, one of 2048 tokens 49, of which 26.  The smallest calls are bound by latency, 13 us at 300 tokens.
 //
 // Rounding.  Scores, weights, sums and outputs are fp32; the weights are rounded to the values' type for
 // their product, once and to nearest: off by at most half a step (relative 2^-8 in bf16, 2^-11 in fp16), as much as the

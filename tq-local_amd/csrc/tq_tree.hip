@@ -20,9 +20,10 @@
 // codes at a time (PairTable), and turned around by ds_read_b64_tr_b16.
 //
 // Cost.  The tiles are bound by their decoding and their softmax beside the matrix instructions: 16 nodes x 4 heads of 8
-// sequences of 32768 tokens (8 KV heads, 4-bit Q_prod) take 149 us, of which the matrix instructions are 78 at the rate of a
+// sequences of 32768 tokens (8 KV heads, 4-bit Q_prod) take 151 us, of which the matrix instructions are 78 at the rate of a
 // large product of matrices, the 281 MB of codes 55 at that of a large copy; 64 rows to a workgroup share a tile's decoding
-// (the call took 182 us with 32 and 32 when it took 160 with 64).  64 nodes x 7 heads of 4 sequences of 8192 (4 KV heads, 3-bit Q_mse) take 64 us.
+// (the call took 182 us with 32 and 32 when it took 160 with 64).  64 nodes x 7 heads of 4 sequences of 8192 (4 KV heads, 3-bit
+// Q_mse) take 67 us.
 // Small calls are bound by latency: 8 nodes of one chat of 1037 tokens take 13 us and the merge 7, of which the first bytes
 // from memory are 4, and two launches.  Rotating the queries in a kernel of their own took 9 us more a call and saved 5.
 //
@@ -47,7 +48,7 @@ constexpr int MAX_SPLIT = 64;  // partials a merge wave weighs with one lane eac
 constexpr float LOG2E = 1.44269504f;
 // Log2 that a score may exceed its row's reference by, and of the largest weight times norm at the reference: 15 together, what fp16
 // holds.  The less a score may exceed it the smaller the weights that keep their bits, and the more often references rise: with 4 the
-// calls of the header take 159 and 71 us, with 8 156 and 69, with 2 160 and 72
+// calls of the header, with their merges, take 159 and 71 us, with 8 156 and 69, with 2 160 and 72
 constexpr float LAZY = 4.0f;
 constexpr int TOP_BIT = 11;
 constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
