@@ -104,6 +104,23 @@ def test_refusals():
         turboquant_prompt_forward(m, q, k, v, None, cu_seq_lens_q=cu)
 
 
+@pytest.mark.parametrize("history", [None, 0, 4])
+def test_rows_that_are_not_causal(history):
+    """Without packed sequences too: every row attends to all that there is, of the call or of the layer."""
+    q, k, v = tensors(6)
+    m, keys = Module(), (k, v)
+    m.is_causal = False
+    if history is not None:
+        m._tq_cache_layer = layer = PackedMSELayer(bits=4)
+        layer._lazy_update = True
+        if history:
+            layer.update(k[:, :, :history] * 0.5, v[:, :, :history] * 2)
+            keys = torch.cat((k[:, :, :history] * 0.5, k), 2), torch.cat((v[:, :, :history] * 2, v), 2)
+        layer.update(k, v)
+    got, _ = turboquant_prompt_forward(m, q, k, v, None, scaling=SCALE)
+    check(got, alone(q, *keys, causal=False), torch.float32)
+
+
 def test_a_mask_is_what_counts_and_one_row_is_a_step():
     q, k, v = tensors(6)
     cu, m = offsets([3, 3]), Module()

@@ -546,6 +546,9 @@ def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key:
             return out.masked_fill(empty[None, :, None], 0.0), None
         if cu.numel() > 2:
             raise ValueError("packed sequences, but the cache layer holds tokens before them")
+    if not causal and attention_mask is None and S > 1:  # no mask means causal there
+        held = key.shape[-2] if layer is None or _hands_over_all(layer, query, key, None) else layer.get_seq_length()
+        attention_mask = torch.ones(S, held, dtype=torch.bool, device=query.device).expand(query.shape[0], 1, -1, -1)
     return turboquant_attention_forward(module, query, key, value, attention_mask, dropout, scaling, is_causal, **kwargs)
 
 
