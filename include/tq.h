@@ -405,6 +405,88 @@ int tq_keep_tokens(int n_buffers, void* const* buffers, const int* row_bytes, in
                    int64_t first, int64_t tokens, const int32_t* index, int64_t index_sb, int64_t index_sh,
                    int n_index, void* stream);
 
+/*
+ * Attention of one query token per sequence where several sequences continue one packed prompt, which is packed and read once for all
+ * of them.  Sequence b of prompt p attends to the prompt's tokens and to its own behind them.  The reference has one cache row per
+ * sequence (runtime/packed_qmse_cache.py:903-951).
+ *
+ *   q        q_type 0: bf16, 1: fp32, 2: fp16; [batch][q_heads][dim] with element strides, dim contiguous; at most 64 query heads per
+ *            KV head
+ *   cu_rows  int32 [prompts + 1] (device, nullable), ascending from 0 to batch: prompt p's sequences are [cu_rows[p], cu_rows[p + 1]).
+ *            NULL: batch / prompts sequences for each
+ *   max_rows with cu_rows, the most sequences of one prompt (what the kernel's blocks are sized for; any number is right)
+ *   prefix_starts, prefix_lens  int32 [prompts] (device, nullable): prompt p is the slots [start, len) of its row; all n_prefix without
+ *   own_lens int32 [batch] (device, nullable): sequence b's own tokens are the slots [0, own_lens[b]) of its row; all n_own without
+ *   prefix, own  HOST arrays of the device pointers k_codes, k_norms, k_signs, k_rnorms, v_codes, v_norms of the packed caches
+ *            [prompts][kv_heads][cap_prefix] and [batch][kv_heads][cap_own] (NULL where there are no tokens), of one codec
+ *   scale    logit scale, > 0 and finite
+ *   out_f32, out_16  [batch][q_heads][dim], fp32 and the query's 16-bit type (bf16 for fp32 queries); at least one.  lse_out
+ *            [batch][q_heads] (nullable; -inf for a sequence without tokens, whose output is 0)
+ *   workspace  device scratch of tq_prefix_attention_workspace_bytes(); `uneven`: whether cu_rows is given
+ * Offsets that descend or leave [0, batch] are taken as empty prompts and as the ends of the batch.  TQ_ERR_UNSUPPORTED beyond
+ * 2^29 tokens (64 n_own counted), 2^26 query rows or 64 query heads per KV head.
+ */
+size_t tq_prefix_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int dim, int prompts, int uneven, int max_rows,
+                                           int64_t n_prefix, int64_t n_own);
+int tq_prefix_attention(const void* q, int q_type, int batch, int q_heads, int kv_heads, int dim, int64_t q_sb, int64_t q_sh,
+                        int prompts, const int32_t* cu_rows, int max_rows, const int32_t* prefix_starts,
+                        const int32_t* prefix_lens, int64_t n_prefix, int64_t cap_prefix, const void* const* prefix,
+                        const int32_t* own_lens, int64_t n_own, int64_t cap_own, const void* const* own, int key_bits,
+                        int value_bits, int has_qjl, const float* key_rotation, const float* key_centers, const float* qjl,
+                        const float* value_rotation, const float* value_centers, float scale, float* out_f32, uint16_t* out_16,
+                        float* lse_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Blocks of TQ_BLOCK_TOKENS slots (block j: the slots [64 j, 64 j + 64)), by which a long history is read in part.  No counterpart in
+ * the reference, which attends to everything.
+ *
+ * tq_block_bounds: bounds of the keys of every block, channel by channel, in whole numbers of a step of the block's own:
+ *   step = the least 2^e, -100 <= e <= 100, with |k| <= 127 step for every key element of the block (2^100 where there is none)
+ *   lohi[0][d] = floor(min_t k_td / step), lohi[1][d] = ceil(max_t k_td / step), both kept to [-127, 127]
+ * An infinity is kept to +-127 so, and a NaN counts as an infinity of its sign.
+ *   k        bf16 [batch][heads][tokens][dim] with element strides, dim contiguous, rows 16-byte aligned; tokens >= 1.  Token t is of
+ *            block first + t / 64; the last block may have fewer
+ *   lohi     int8 [batch][heads][cap][2][dim], step fp32 [batch][heads][cap] of cap >= first + ceil(tokens / 64) blocks; the other
+ *            blocks stay as they were.  lohi 16-byte aligned
+ */
+#define TQ_BLOCK_TOKENS 64
+#define TQ_MAX_BLOCKS 4096 /* blocks chosen for one KV head */
+int tq_block_bounds(const uint16_t* k, int batch, int heads, int64_t tokens, int dim, int64_t k_sb, int64_t k_sh, int64_t k_st,
+                    int8_t* lohi, float* step, int64_t cap, int64_t first, void* stream);
+
+/*
+ * tq_select_blocks: for each KV head of each row the `keep` blocks that its query heads may give the largest logits, by the bounds of
+ * tq_block_bounds, in whole numbers:
+ *   x    = rint(q / s), kept to [-127, 127], s for the KV head's query heads together as `step` is for a block (NaN: 0)
+ *   u_hj = sum_d max(x_hd lohi_j[0][d], x_hd lohi_j[1][d]),  score_j = max_h u_hj step_j  (exact in fp32)
+ * Of the blocks that hold slots of the row's range, the first `sink` and the last `recent` are always chosen, then the others by
+ * (score descending, number ascending).
+ *   q        q_type as for tq_prefix_attention, [batch][q_heads][dim] with element strides
+ *   n_blocks blocks with bounds (<= cap); a later one that is neither of the first nor of the last comes behind all scored ones
+ *   seq_starts, seq_lens  int32 [batch] (device, nullable): row b's range is the slots [start, len) of [0, n_tokens)
+ *   out      int32 [batch][kv_heads][keep], ascending; -1 in the places left where there are fewer blocks
+ * sink + recent <= keep <= TQ_MAX_BLOCKS.  TQ_ERR_UNSUPPORTED beyond TQ_MAX_SCORED * 64 tokens.
+ */
+#define TQ_MAX_SCORED 32768
+int tq_select_blocks(const void* q, int q_type, int batch, int q_heads, int kv_heads, int dim, int64_t q_sb, int64_t q_sh,
+                     const int8_t* lohi, const float* step, int64_t cap, int64_t n_blocks, int64_t n_tokens,
+                     const int32_t* seq_starts, const int32_t* seq_lens, int keep, int sink, int recent, int32_t* out, void* stream);
+
+/*
+ * tq_block_attention: tq_decode_attention over the named blocks only.  blocks int32 [batch][kv_heads][keep] (device): block numbers in any
+ * order; a slot outside [seq_starts, seq_lens) of a named block is left out, and so is a number that names no slot (-1); a block
+ * named twice counts twice.  The other arguments as for tq_decode_attention (scale > 0 and finite).  TQ_ERR_UNSUPPORTED from 2^24
+ * tokens, beyond TQ_MAX_BLOCKS blocks or 65535 KV heads of the batch.
+ */
+size_t tq_block_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int dim, int keep);
+int tq_block_attention(const uint16_t* q, int batch, int q_heads, int kv_heads, int dim, const int32_t* blocks, int keep,
+                       const int32_t* seq_starts, const int32_t* seq_lens, int64_t n_tokens, int64_t cap, const uint8_t* k_codes,
+                       const uint16_t* k_norms, const uint8_t* k_signs, const uint16_t* k_rnorms, const uint8_t* v_codes,
+                       const uint16_t* v_norms, int key_bits, int value_bits, int has_qjl, const float* key_rotation,
+                       const float* key_centers, const float* qjl, const float* value_rotation, const float* value_centers,
+                       float scale, float* out_f32, uint16_t* out_bf16, float* lse_out, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

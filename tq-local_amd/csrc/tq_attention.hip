@@ -52,6 +52,7 @@
 
 #include "tq_common.h"
 
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -705,9 +706,16 @@ struct Og {
     float cq1;          // the logit scale (log2 units) times sqrt(pi/2) / d1
 };
 
+// Blocks of TQ_BLOCK_TOKENS slots to attend to, instead of every slot of the range (LIST): `keep` numbers for each KV head of each batch row.
+struct BlockList {
+    const int32_t* blocks;
+    int keep;
+};
+struct NoList {};
+
 // X1 > 0: group 1's widths are group 0's plus X1 (the reference's default outlier_extra_bits
 // is 1), compile-time constants; X1 = 0: the widths come from og at run time.
-template <int KB, int VB, bool QJL, int GC, int OD = 0, int X1 = 0>
+template <int KB, int VB, bool QJL, int GC, int OD = 0, int X1 = 0, bool LIST = false>
 __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel(
     const uint16_t* __restrict__ q, int q_heads, int kv_heads, int G, const int32_t* __restrict__ seq_starts,
     const int32_t* __restrict__ seq_lens, int64_t n_tokens, int64_t cap, const uint8_t* __restrict__ kc,
@@ -715,8 +723,10 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
     const uint8_t* __restrict__ vc, const uint16_t* __restrict__ vn, const float* __restrict__ Rk,
     const float* __restrict__ S, float c_mse, float c_qjl,
     const float* __restrict__ Ck, const float* __restrict__ Cv, float scale,
-    int64_t tokens_per_split, int n_split, float* __restrict__ part_o, float* __restrict__ part_ml, Og og) {
+    int64_t tokens_per_split, int n_split, float* __restrict__ part_o, float* __restrict__ part_ml, Og og,
+    std::conditional_t<LIST, BlockList, NoList> list) {
     constexpr bool SPL = OD > 0;
+    static_assert(!(SPL && LIST), "chosen blocks: one-group layers only");
     static_assert(!SPL || OD <= OD1, "two-group layers: at most OD1 outlier dims per lane");
     using Sm = Smem<KB, VB, QJL, GC, OD>;
     using R = Rows<GC>;
@@ -750,8 +760,14 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
     }
     int64_t r0 = (int64_t)split * tokens_per_split;
     int64_t r1 = r0 + tokens_per_split;
-    r0 = r0 > start ? r0 : start;
-    r1 = r1 < len ? r1 : len;
+    if constexpr (LIST) {
+        // the split's numbers are the list's [r0, r1) / TQ_BLOCK_TOKENS: places in the list, not in the cache
+        const int64_t all = (int64_t)list.keep * TQ_BLOCK_TOKENS;
+        r1 = r1 < all ? r1 : all;
+    } else {
+        r0 = r0 > start ? r0 : start;
+        r1 = r1 < len ? r1 : len;
+    }
     // The workgroup streams [t0, t1) in 16-token blocks dealt round-robin to its waves (block
     // i to wave i mod NW), so at any moment the waves read neighbouring blocks of every array:
     // DRAM pages are shared instead of NW separate streams per array (~14% more bandwidth).
@@ -761,7 +777,8 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
     // token offsets within the range are 32-bit: the host keeps the range below 2^24 tokens
     const int nt = (int)ntok;
     constexpr int STEP = NW * BLK;
-    const size_t row0 = (size_t)grp * cap + (size_t)(t0 < n_tokens ? t0 : 0);
+    const size_t row0 = (size_t)grp * cap + (LIST ? (size_t)0 : (size_t)(t0 < n_tokens ? t0 : 0));
+    const int64_t nrows = LIST ? len : ntok;  // rows that the descriptors cover, from row0 on
 
     // row bytes: the full-width rows, or group 0's of a two-group layer
     const int krow = SPL ? og.r0k : KROW, srow = SPL ? og.r0s : D / 8, vrow = SPL ? og.r0v : VROW;
@@ -773,17 +790,17 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
     const auto rs_row = [&](const void* arr, int r, int* A) {
         const size_t b0 = row0 * (size_t)r;
         *A = SPL ? (int)(b0 & 3) : 0;
-        return rsrc(static_cast<const uint8_t*>(arr) + (b0 - (size_t)*A), ((int64_t)*A + ntok * r + 3) & ~(int64_t)3);
+        return rsrc(static_cast<const uint8_t*>(arr) + (b0 - (size_t)*A), ((int64_t)*A + nrows * r + 3) & ~(int64_t)3);
     };
     int Ak = 0, As = 0, Av = 0;
     const __amdgpu_buffer_rsrc_t rk = rs_row(kc, krow, &Ak);
     const __amdgpu_buffer_rsrc_t rv = rs_row(vc, vrow, &Av);
-    const __amdgpu_buffer_rsrc_t rkn = rsrc(kn + row0, ntok * 2);
-    const __amdgpu_buffer_rsrc_t rvn = rsrc(vn + row0, ntok * 2);
+    const __amdgpu_buffer_rsrc_t rkn = rsrc(kn + row0, nrows * 2);
+    const __amdgpu_buffer_rsrc_t rvn = rsrc(vn + row0, nrows * 2);
     __amdgpu_buffer_rsrc_t rs = rkn, rkr = rkn;
     if constexpr (QJL) {
         rs = rs_row(ks, srow, &As);
-        rkr = rsrc(kr + row0, ntok * 2);
+        rkr = rsrc(kr + row0, nrows * 2);
     }
 
     // lane offsets (bytes) into the per-wave buffers.  Rows at any byte alignment (two-group
@@ -836,6 +853,26 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
         o1n = no + 2 * hb;
     }
 
+    // LIST: where the wave's blocks stand in the cache.  Lane i has the first slot of block i (at most 64 of them: the host cuts the
+    // list so), which is a quarter of a named block's; a number that names no block, and places past the list, give the range's
+    // end, from where on nothing is read.
+    int place_of = 0;
+    if constexpr (LIST) {
+        const int i = wave + NW * lane;
+        int64_t slot = len;
+        if (i * BLK < nt) {
+            const int64_t block = list.blocks[(size_t)grp * list.keep + (size_t)(t0 / TQ_BLOCK_TOKENS) + i / (TQ_BLOCK_TOKENS / BLK)];
+            if (block >= 0) slot = block * TQ_BLOCK_TOKENS + i % (TQ_BLOCK_TOKENS / BLK) * BLK;
+        }
+        place_of = (int)(slot < len ? slot : len);
+    }
+    // the slot of the wave's block `rel` tokens into the range, relative to row0
+    const auto place = [&](int rel) {
+        if constexpr (!LIST) return __builtin_amdgcn_readfirstlane(rel);
+        const int i = __builtin_amdgcn_readfirstlane((rel - wave * BLK) / STEP);
+        return i < 64 ? __builtin_amdgcn_readlane(place_of, i) : (int)len;
+    };
+
     // Per-block data of a wave, in the part the score stage reads (key codes, sign bits and
     // the three norms of token n) and the part the value stage reads (value codes of tokens
     // 4 r + g).
@@ -873,7 +910,7 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
         }
     };
     auto load_k = [&](Kd& B, int rel_) {
-        const int rel = __builtin_amdgcn_readfirstlane(rel_);  // scalar block offset
+        const int rel = place(rel_);  // scalar block offset
         if constexpr (SPL) {
             // KB + 1 dwords from the one holding the lane's first byte
             if constexpr (KB == 1) {
@@ -916,7 +953,7 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
         B.vn = __builtin_amdgcn_raw_buffer_load_b16(rvn, no, rel * 2, KV_NT);
     };
     auto load_v = [&](Vd& B, int rel_) {
-        const int rel = __builtin_amdgcn_readfirstlane(rel_);
+        const int rel = place(rel_);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             if constexpr (SPL) {
@@ -1351,9 +1388,16 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
         for (int b = 0; b < NB; ++b) {
             const Kd& B = kset[s0 + b];
             const int rel = rel0 + b * STEP;
-            // valid tokens of the block: a scalar count, one compare per lane
-            const int nvalid = __builtin_amdgcn_readfirstlane(nt - rel < BLK ? nt - rel : BLK);
-            const bool valid = n < nvalid;
+            bool valid;
+            if constexpr (LIST) {
+                // slots of [start, len); the value norms of the others, which are read here, weigh nothing
+                valid = (uint32_t)(place(rel) + n) - (uint32_t)start < (uint32_t)(len > start ? len - start : 0);
+                kset[s0 + b].vn = valid ? kset[s0 + b].vn : 0u;
+            } else {
+                // valid tokens of the block: a scalar count, one compare per lane
+                const int nvalid = __builtin_amdgcn_readfirstlane(nt - rel < BLK ? nt - rel : BLK);
+                valid = n < nvalid;
+            }
             // the f16 norms enter v_fma_mix_f32 as they are (no separate conversions)
             const float knf = tq::f16_to_f32(B.kn);
             const float krf = QJL ? tq::f16_to_f32(B.kr) : 0.0f;
@@ -1663,8 +1707,50 @@ int launch_split(const SplitArgs& a, int groups, hipStream_t s, int* n_split_out
     if (a.po == nullptr) return TQ_OK;  // sizing query only
     hipLaunchKernelGGL((split_kernel<KB, VB, QJL, GC, OD, X1>), dim3(ns, groups), dim3(Cfg<VB, GC, QJL, SPL>::NT), 0, s,
                        a.q, a.q_heads, a.kv_heads, a.G, a.seq_starts, a.seq_lens, a.n_tokens, a.cap, a.kc, a.kn, a.ks,
-                       a.kr, a.vc, a.vn, a.Rk, a.S, a.c_mse, a.c_qjl, a.Ck, a.Cv, a.scale, tps, ns, a.po, a.pml, a.og);
+                       a.kr, a.vc, a.vn, a.Rk, a.S, a.c_mse, a.c_qjl, a.Ck, a.Cv, a.scale, tps, ns, a.po, a.pml, a.og, NoList{});
     return TQ_OK;
+}
+
+// Chosen blocks: the split pass over `keep` blocks of each group.  Splits as for a range of as many tokens, cut at whole blocks, and
+// no more of a wave's 16-token blocks than its lanes hold places for.
+template <int KB, int VB, bool QJL, int GC>
+int launch_blocks(const SplitArgs& a, const BlockList& list, int groups, hipStream_t s, int* n_split) {
+    using C = Cfg<VB, GC, QJL>;
+    const int64_t all = (int64_t)list.keep * TQ_BLOCK_TOKENS;
+    int64_t tps;
+    choose_split(groups, all, cu_count(), C::NW, &tps);
+    tps = std::min<int64_t>((tps + TQ_BLOCK_TOKENS - 1) / TQ_BLOCK_TOKENS * TQ_BLOCK_TOKENS, 64 * C::NW * BLK);
+    const int ns = (int)((all + tps - 1) / tps);
+    *n_split = ns;
+    if (a.po == nullptr) return TQ_OK;  // sizing query only
+    hipLaunchKernelGGL((split_kernel<KB, VB, QJL, GC, 0, 0, true>), dim3(ns, groups), dim3(C::NT), 0, s, a.q, a.q_heads, a.kv_heads,
+                       a.G, a.seq_starts, a.seq_lens, a.n_tokens, a.cap, a.kc, a.kn, a.ks, a.kr, a.vc, a.vn, a.Rk, a.S, a.c_mse,
+                       a.c_qjl, a.Ck, a.Cv, a.scale, tps, ns, a.po, a.pml, a.og, list);
+    return TQ_OK;
+}
+
+int dispatch_blocks(int value_bits, int has_qjl, const SplitArgs& a, const BlockList& list, int groups, hipStream_t s, int* ns) {
+    auto launch = [&](auto kb, auto vb, auto qjl) {
+        return a.G <= 4 ? launch_blocks<kb, vb, qjl, 1>(a, list, groups, s, ns) : launch_blocks<kb, vb, qjl, 2>(a, list, groups, s, ns);
+    };
+    using std::integral_constant;
+    const auto one = integral_constant<int, 1>{};
+    const auto two = integral_constant<int, 2>{};
+    const auto three = integral_constant<int, 3>{};
+    const auto four = integral_constant<int, 4>{};
+    if (has_qjl) {
+        switch (value_bits) {
+            case 2: return launch(one, two, std::true_type{});
+            case 3: return launch(two, three, std::true_type{});
+            default: return launch(three, four, std::true_type{});
+        }
+    }
+    switch (value_bits) {
+        case 1: return launch(one, one, std::false_type{});
+        case 2: return launch(two, two, std::false_type{});
+        case 3: return launch(three, three, std::false_type{});
+        default: return launch(four, four, std::false_type{});
+    }
 }
 
 // Two-group layers on the split kernel (group 1 at most OD1 channels): group 0's bit widths as
@@ -2322,6 +2408,68 @@ extern "C" int tq_decode_attention_groups(const uint16_t* q, int batch, int q_he
     }
     TQ_CHECK_LAUNCH();
     hipLaunchKernelGGL(merge_kernel, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml, n_split, value_matrix,
+                       out_f32, out_bf16, lse_out);
+    TQ_CHECK_LAUNCH();
+    return TQ_OK;
+}
+
+// ------------------------------------------------------------------ chosen blocks
+namespace {
+// The splits' partials of `keep` blocks, at most this many for a group.
+size_t blocks_workspace(int batch, int q_heads, int kv_heads, int64_t keep) {
+    const int64_t groups = (int64_t)batch * kv_heads, all = keep * TQ_BLOCK_TOKENS;
+    // splits that fill the CUs, or that the waves' places ask for (12 waves or more)
+    const int64_t most = std::max<int64_t>((MAX_WGS + groups - 1) / groups, (all + 64 * 12 * BLK - 1) / (64 * 12 * BLK));
+    return ws_layout(batch, q_heads, (int)most).total;
+}
+}  // namespace
+
+extern "C" size_t tq_block_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int dim, int keep) {
+    if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || dim != D || keep < 1 || keep > TQ_MAX_BLOCKS) return 0;
+    return blocks_workspace(batch, q_heads, kv_heads, keep);
+}
+
+extern "C" int tq_block_attention(const uint16_t* q, int batch, int q_heads, int kv_heads, int dim, const int32_t* blocks, int keep,
+                                  const int32_t* seq_starts, const int32_t* seq_lens, int64_t n_tokens, int64_t cap,
+                                  const uint8_t* k_codes, const uint16_t* k_norms, const uint8_t* k_signs,
+                                  const uint16_t* k_rnorms, const uint8_t* v_codes, const uint16_t* v_norms, int key_bits,
+                                  int value_bits, int has_qjl, const float* key_rotation, const float* key_centers,
+                                  const float* qjl, const float* value_rotation, const float* value_centers, float scale,
+                                  float* out_f32, uint16_t* out_bf16, float* lse_out, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    if (!q || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || !blocks || keep < 1 || n_tokens < 0 ||
+        cap < n_tokens || !key_rotation || !key_centers || !value_rotation || !value_centers || (has_qjl && !qjl) ||
+        (!out_f32 && !out_bf16 && !lse_out) || (n_tokens > 0 && (!k_codes || !k_norms || !v_codes || !v_norms)) ||
+        (has_qjl && n_tokens > 0 && (!k_signs || !k_rnorms)) || !(scale > 0.0f) || scale == __builtin_inff())
+        return TQ_ERR_INVALID_ARGUMENT;
+    const int G = q_heads / kv_heads;
+    const bool combo_ok = has_qjl ? (key_bits + 1 == value_bits && value_bits >= 2 && value_bits <= 4)
+                                  : (key_bits == value_bits && key_bits >= 1 && key_bits <= 4);
+    // (a lane's byte offsets within a group's rows fit the 31-bit buffer descriptors)
+    if (dim != D || G > TQ_MAX_GROUP || !combo_ok || keep > TQ_MAX_BLOCKS || n_tokens >= (int64_t)1 << 24 ||
+        (int64_t)batch * kv_heads > 65535)
+        return TQ_ERR_UNSUPPORTED;
+    if (!aligned16(q) || (k_codes && !aligned16(k_codes)) || (k_signs && !aligned16(k_signs)) ||
+        (v_codes && !aligned16(v_codes)) || !aligned16(key_rotation) || !aligned16(value_rotation) || (qjl && !aligned16(qjl)))
+        return TQ_ERR_UNSUPPORTED;
+    if (!workspace || !aligned16(workspace)) return TQ_ERR_WORKSPACE;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int groups = batch * kv_heads;
+    SplitArgs a{q,        q_heads,  kv_heads, G,           seq_starts,    seq_lens,
+                n_tokens, cap,      k_codes,  k_norms,     k_signs,       k_rnorms,
+                v_codes,  v_norms,  key_rotation, qjl,     scale * LOG2E, scale * LOG2E * QJL_SCALE,
+                key_centers, value_centers, scale, 0,      0,             nullptr,
+                nullptr};
+    const BlockList list{blocks, keep};
+    int n_split = 0;
+    (void)dispatch_blocks(value_bits, has_qjl, a, list, groups, s, &n_split);  // sizing
+    const Ws w = ws_layout(batch, q_heads, n_split);
+    if (workspace_bytes < w.total) return TQ_ERR_WORKSPACE;
+    a.po = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.po);
+    a.pml = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.pml);
+    (void)dispatch_blocks(value_bits, has_qjl, a, list, groups, s, &n_split);
+    TQ_CHECK_LAUNCH();
+    hipLaunchKernelGGL(merge_kernel, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml, n_split, value_rotation,
                        out_f32, out_bf16, lse_out);
     TQ_CHECK_LAUNCH();
     return TQ_OK;

@@ -1,0 +1,320 @@
+// tq_prefix.hip -- attention of one query token per sequence where several sequences continue one packed prompt (gfx950).
+//
+// The prompt is packed once for all of them, and every sequence has packed tokens of its own behind it; its query attends to both.
+// The formulas, the codes' way to the matrix cores and the rounding are those of tq_tiles.h.
+//
+//   prefix_kernel  a workgroup has up to 32 or 64 query rows of a KV head: `per` sequences of one prompt (an item), all of a sequence's
+//                  query heads.  Its tiles are the prompt's, which every row attends to, then the own tokens of its sequences, each of
+//                  which only that sequence's rows attend to.  The splits of an item share its tiles
+//   merge_kernel   the splits' partials of a row weighed and added, rotated back by R_v
+
+#include "tq_tiles.h"
+
+namespace {
+
+using namespace tqt;
+
+struct PrefixArgs {
+    int prompts, batch, kv_heads, group;  // query heads per KV head
+    int per, items;                       // sequences of an item, and how many items there may be
+    const int32_t* cu_rows;               // prompt p's sequences are [cu_rows[p], cu_rows[p + 1]); or `each` to a prompt
+    int each;
+    const int32_t *starts, *lens, *own_lens;
+    int64_t n_prefix, cap_prefix, n_own, cap_own;
+    Cache prefix, own;
+    int64_t q_sb, q_sh;
+    int n_split, n_slots;  // n_split slots for each item, or with `shared` n_slots dealt out by what the items have
+    int shared;
+    int4* row_slots;  // [batch] a sequence's first slot, its number of slots, their distance, and its place in the item
+};
+
+__device__ __forceinline__ int clamp_to(int64_t x, int64_t n) { return (int)std::min(std::max<int64_t>(x, 0), n); }
+__device__ __forceinline__ int tiles_of(int tokens) { return (int)(((int64_t)tokens + TK - 1) / TK); }
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Prefix sums and maxima over the lanes of a wave.
+__device__ __forceinline__ int scan_sum(int x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+__device__ __forceinline__ int scan_max(int x, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(x, d);
+        if (lane >= d) x = std::max(x, y);
+    }
+    return x;
+}
+
+// An item's prompt, its first sequence and how many it has (0: there is no such item).
+struct Item {
+    int p, first, count;
+};
+// Item `it` (any lane's own), by a whole wave.  Offsets that descend or leave [0, batch] are taken as empty prompts and as the ends of
+// the batch; the first prompt begins at sequence 0 and the last ends with the batch, so every sequence is of one item.
+__device__ __forceinline__ Item find_item(const PrefixArgs& a, int it, int lane) {
+    if (!a.cu_rows) {
+        const int of_each = (a.each + a.per - 1) / a.per, p = it / of_each, at = (it - p * of_each) * a.per;
+        if (p >= a.prompts) return {0, 0, 0};
+        return {p, p * a.each + at, std::min(a.per, a.each - at)};
+    }
+    Item mine{0, 0, 0};
+    int items = 0, rows = 0;  // before these prompts
+    for (int p0 = 0; p0 < a.prompts; p0 += 64) {
+        const int p = p0 + lane;
+        int end = a.batch;
+        if (p + 1 < a.prompts) end = clamp_to(a.cu_rows[p + 1], a.batch);
+        end = std::max(scan_max(end, lane), rows);
+        const int up = __shfl_up(end, 1), begin = lane == 0 ? rows : up;
+        const int last = scan_sum((end - begin + a.per - 1) / a.per, lane) + items;
+        const int n = std::min(64, a.prompts - p0);
+        for (int i = 0; i < n; ++i) {
+            const int e = __builtin_amdgcn_readlane(last, i), to = __builtin_amdgcn_readlane(end, i);
+            const int at = __builtin_amdgcn_readlane(begin, i) + (it - items) * a.per;
+            if (it >= items && it < e) mine = {p0 + i, at, std::min(a.per, to - at)};
+            items = e, rows = to;
+        }
+    }
+    return mine;
+}
+
+// The prompt's tokens [lo, end).
+struct Range {
+    int lo, end;
+};
+__device__ __forceinline__ Range range_of(const PrefixArgs& a, int p) {
+    const int end = a.lens ? clamp_to(a.lens[p], a.n_prefix) : (int)a.n_prefix;
+    return {a.starts ? clamp_to(a.starts[p], end) : 0, end};
+}
+__device__ __forceinline__ int own_of(const PrefixArgs& a, int row) {
+    return a.own_lens ? clamp_to(a.own_lens[row], a.n_own) : (int)a.n_own;
+}
+
+// A slot's item, the first of the item's slots, their number and distance.
+struct Slot {
+    Item item;
+    int first, n, step;
+};
+// Up to 64 items share the slots in proportion to their tiles, each with one at least; what is left over goes unused (count = 0).
+__device__ __forceinline__ Slot share_slots(const PrefixArgs& a, int slot, int lane) {
+    const Item mine = find_item(a, lane, lane);
+    int tiles = 0;
+    if (mine.count) {
+        const Range range = range_of(a, mine.p);
+        tiles = tiles_of(range.end - range.lo);
+        if (a.own_lens) {
+            for (int m = 0; m < mine.count; ++m) tiles += tiles_of(own_of(a, mine.first + m));
+        } else {
+            tiles += mine.count * tiles_of((int)a.n_own);
+        }
+    }
+    const int total = __builtin_amdgcn_readlane(scan_sum(tiles, lane), 63);
+    // (the sum of the shares does not pass what there is to share, whatever the roundings: these are far below 1)
+    const int share = (int)((float)(a.n_slots - a.items) * ((float)tiles / (float)std::max(total, 1)));
+    const int n = mine.count ? std::min(std::min(1 + share, std::max(1, (tiles + MIN_TILES - 1) / MIN_TILES)), MAX_SPLIT) : 0;
+    const int end = scan_sum(n, lane), i = __popcll(__ballot(end <= slot));
+    if (i >= 64) return {{0, 0, 0}, 0, 0, 0};
+    auto of_item = [&](int x) { return __builtin_amdgcn_readlane(x, i); };
+    return {{of_item(mine.p), of_item(mine.first), of_item(mine.count)}, of_item(end - n), of_item(n), 1};
+}
+
+// Rows sequence by sequence, a sequence's query heads next to one another.
+template <int RB>
+struct PrefixSource {
+    const PrefixArgs& a;
+    const Slot& at;
+    const int slot, kvh, lo, end, shared_tiles, own_lens, own_tiles;  // the last two: of sequence `lane`, and with those before it
+    int member[RB];
+
+    __device__ __forceinline__ PrefixSource(const PrefixArgs& a, const Slot& at, int slot, int kvh, Range range, int own_len, int lane)
+        : a(a), at(at), slot(slot), kvh(kvh), lo(scalar(range.lo)), end(scalar(range.end)), shared_tiles(tiles_of(end - lo)),
+          own_lens(own_len), own_tiles(scan_sum(tiles_of(own_len), lane)) {}
+    __device__ __forceinline__ int64_t query(int r) const {
+        const uint32_t m = (uint32_t)r / (uint32_t)a.group, g = r - m * a.group;
+        const bool live = (int)m < at.item.count;
+        return (int64_t)(at.item.first + (live ? m : 0u)) * a.q_sb + (int64_t)(kvh * a.group + (live ? g : 0u)) * a.q_sh;
+    }
+    __device__ __forceinline__ int64_t tiles() const { return shared_tiles + __builtin_amdgcn_readlane(own_tiles, 63); }
+    __device__ __forceinline__ int64_t whole() const { return (end - lo) / TK; }
+    __device__ __forceinline__ int split() const { return (slot - at.first) / at.step; }
+    __device__ __forceinline__ int splits() const { return at.n; }
+    // whose own tile it is; -1: the prompt's
+    __device__ __forceinline__ int owner(int64_t tile) const {
+        return tile < shared_tiles ? -1 : __popcll(__ballot(own_tiles <= (int)tile - shared_tiles));
+    }
+    __device__ __forceinline__ Place place(int64_t tile) const {
+        const int s = owner(tile);
+        if (s < 0) {
+            const int t0 = lo + (int)tile * TK;
+            return {a.prefix, (int64_t)(at.item.p * a.kv_heads + kvh) * a.cap_prefix + t0, std::min(end - t0, TK)};
+        }
+        const int len = __builtin_amdgcn_readlane(own_lens, s), before = __builtin_amdgcn_readlane(own_tiles, s) - tiles_of(len);
+        const int t0 = ((int)tile - shared_tiles - before) * TK;
+        return {a.own, ((int64_t)(at.item.first + s) * a.kv_heads + kvh) * a.cap_own + t0, std::min(len - t0, TK)};
+    }
+    __device__ __forceinline__ uint32_t seen(int m, int64_t tile) const {
+        const int s = owner(tile), left = place(tile).left;  // by the whole wave, ahead of what differs between lanes
+        return s < 0 || s == member[m] ? (uint32_t)((1ull << left) - 1) : 0u;
+    }
+    __device__ __forceinline__ int rows() const { return at.item.count * a.group; }
+    __device__ __forceinline__ int64_t partial() const { return ((int64_t)slot * a.kv_heads + kvh) * (32 * RB); }
+    __device__ __forceinline__ void prefetch(int, int) {}
+    __device__ __forceinline__ void publish(int, int) const {}
+    __device__ __forceinline__ void take_row(int m, int r) { member[m] = r / a.group; }
+};
+
+template <int KB, int VB, bool QJL, int RB, int NQ>
+__global__ __launch_bounds__(Tiles<RB>::T, 2) void prefix_kernel(PrefixArgs a, Codec codec) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slot = blockIdx.x, kvh = blockIdx.y;
+    Slot at;
+    if (a.shared) {
+        at = share_slots(a, slot, lane);
+    } else {
+        const int it = slot % a.items;
+        const Item item = find_item(a, it, lane);
+        at = {{scalar(item.p), scalar(item.first), scalar(item.count)}, it, a.n_split, a.items};
+    }
+    if (at.item.count == 0) return;
+    int own_len = 0;
+    if (lane < at.item.count) own_len = own_of(a, at.item.first + lane);
+    PrefixSource<RB> src(a, at, slot, kvh, range_of(a, at.item.p), own_len, lane);
+    if (src.split() == 0 && kvh == 0 && (int)threadIdx.x < at.item.count)
+        a.row_slots[at.item.first + threadIdx.x] = make_int4(at.first, at.n, at.step, threadIdx.x);
+    attend_tiles<KB, VB, QJL, RB, NQ>(codec, src, lane, wave);
+}
+
+// Rows of [batch][q head].
+struct PrefixRows {
+    int q_heads, kv_heads, rows;  // rows of an item
+    const int4* slots;
+
+    __device__ __forceinline__ Part find(int64_t row) const {
+        const uint32_t n = (uint32_t)row, b = n / (uint32_t)q_heads, hq = n - b * q_heads;
+        const uint32_t group = (uint32_t)q_heads / (uint32_t)kv_heads, kvh = hq / group;
+        const int4 s = slots[b];
+        return {((int64_t)s.x * kv_heads + kvh) * rows + s.w * group + (hq - kvh * group), (int64_t)s.z * kv_heads * rows, s.y};
+    }
+    __device__ __forceinline__ int64_t place(int64_t row) const { return row; }
+};
+__global__ __launch_bounds__(MERGE_T) void merge_kernel(Merge a, PrefixRows rows) { merge_rows(a, rows); }
+
+struct Plan {
+    int row_blocks, per, items, n_split, n_slots;
+    size_t o_bytes, ms_bytes, slots_bytes;
+    size_t total() const { return o_bytes + ms_bytes + slots_bytes; }
+};
+
+// 32 rows where the sequences of a prompt have no more, 64 else.  A workgroup fills a CU: as many splits as fill the CUs, as long as
+// none is left without a tile.
+bool make_plan(int batch, int q_heads, int kv_heads, int prompts, bool uneven, int max_rows, int64_t n_prefix, int64_t n_own, Plan& p) {
+    const int group = q_heads / kv_heads, each = batch / prompts;
+    const int most = uneven ? std::min(batch, std::max(max_rows, 1)) : each;
+    if (group > 64 || kv_heads > 65535 || (int64_t)batch * q_heads >= (int64_t)1 << 26) return false;
+    if (n_prefix + 64 * n_own >= (int64_t)1 << 29) return false;  // sums of 64 items' tiles fit 32 bits
+    p.row_blocks = (int64_t)most * group <= 32 ? 1 : 2;
+    p.per = 32 * p.row_blocks / group;
+    p.items = uneven ? (int)std::min<int64_t>(batch, (int64_t)batch / p.per + prompts) : prompts * ((each + p.per - 1) / p.per);
+    const int64_t tiles = (n_prefix + TK - 1) / TK + std::min(p.per, batch) * ((n_own + TK - 1) / TK);
+    const int64_t useful = std::min<int64_t>(std::max<int64_t>(1, (tiles + MIN_TILES - 1) / MIN_TILES), MAX_SPLIT);
+    p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)p.items * kv_heads), useful));
+    p.n_slots = (int)std::max<int64_t>((int64_t)p.n_split * p.items, std::min<int64_t>(256 / kv_heads, useful * p.items));
+    const size_t rows = (size_t)p.n_slots * kv_heads * 32 * p.row_blocks;
+    p.o_bytes = rows * D * 4, p.ms_bytes = rows * 8, p.slots_bytes = (size_t)batch * 16;
+    return true;
+}
+
+template <int KB, int VB, bool QJL>
+void launch_prefix(const PrefixArgs& a, const Codec& c, const Plan& p, hipStream_t s) {
+    const dim3 grid((unsigned)a.n_slots, (unsigned)a.kv_heads);
+    auto launch = [&](auto rb, auto nq) {
+        hipLaunchKernelGGL((prefix_kernel<KB, VB, QJL, rb, nq>), grid, dim3(Tiles<rb>::T), 0, s, a, c);
+    };
+    using One = std::integral_constant<int, 1>;
+    using Two = std::integral_constant<int, 2>;
+    if (p.row_blocks == 1) c.q_type == 0 ? launch(One{}, One{}) : launch(One{}, Two{});
+    else c.q_type == 0 ? launch(Two{}, One{}) : launch(Two{}, Two{});
+}
+
+bool good_shape(int batch, int q_heads, int kv_heads, int prompts, bool uneven, int64_t n_prefix, int64_t n_own) {
+    return batch >= 1 && q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0 && prompts >= 1 && (uneven || batch % prompts == 0) &&
+           n_prefix >= 0 && n_own >= 0;
+}
+// `caches`: k_codes, k_norms, k_signs, k_rnorms, v_codes, v_norms
+bool has_arrays(const void* const* c, int64_t n, int has_qjl) {
+    return n == 0 || (c && c[0] && c[1] && c[4] && c[5] && (!has_qjl || (c[2] && c[3])));
+}
+bool has_alignment(const void* const* c, int64_t n, int has_qjl) {
+    return n == 0 || (aligned16(c[0]) && aligned16(c[4]) && (!has_qjl || aligned16(c[2])));
+}
+Cache cache_of(const void* const* c, int64_t n) {
+    if (n == 0) return Cache{};
+    auto u8 = [&](int i) { return static_cast<const uint8_t*>(c[i]); };
+    auto u16 = [&](int i) { return static_cast<const uint16_t*>(c[i]); };
+    return {u8(0), u8(2), u8(4), u16(1), u16(3), u16(5)};
+}
+
+}  // namespace
+
+extern "C" size_t tq_prefix_attention_workspace_bytes(int batch, int q_heads, int kv_heads, int dim, int prompts, int uneven,
+                                                      int max_rows, int64_t n_prefix, int64_t n_own) {
+    Plan p;
+    if (!good_shape(batch, q_heads, kv_heads, prompts, uneven != 0, n_prefix, n_own) || dim != D ||
+        !make_plan(batch, q_heads, kv_heads, prompts, uneven != 0, max_rows, n_prefix, n_own, p))
+        return 0;
+    return p.total();
+}
+
+extern "C" int tq_prefix_attention(const void* q, int q_type, int batch, int q_heads, int kv_heads, int dim, int64_t q_sb, int64_t q_sh,
+                                   int prompts, const int32_t* cu_rows, int max_rows, const int32_t* prefix_starts,
+                                   const int32_t* prefix_lens, int64_t n_prefix, int64_t cap_prefix, const void* const* prefix,
+                                   const int32_t* own_lens, int64_t n_own, int64_t cap_own, const void* const* own, int key_bits,
+                                   int value_bits, int has_qjl, const float* key_rotation, const float* key_centers, const float* qjl,
+                                   const float* value_rotation, const float* value_centers, float scale, float* out_f32,
+                                   uint16_t* out_16, float* lse_out, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || q_type < 0 || q_type > 2 || !good_shape(batch, q_heads, kv_heads, prompts, cu_rows != nullptr, n_prefix, n_own) ||
+        n_prefix > cap_prefix || n_own > cap_own || !has_arrays(prefix, n_prefix, has_qjl) || !has_arrays(own, n_own, has_qjl) ||
+        !key_rotation || !key_centers || !value_rotation || !value_centers || (has_qjl && !qjl) || (!out_f32 && !out_16) ||
+        !(scale > 0.0f) || scale == __builtin_inff())
+        return TQ_ERR_INVALID_ARGUMENT;
+    if (dim != D || n_prefix >= (int64_t)1 << 31 || n_own >= (int64_t)1 << 31 || value_bits < 1 || value_bits > 4 || key_bits < 1 ||
+        key_bits != value_bits - (has_qjl ? 1 : 0))
+        return TQ_ERR_UNSUPPORTED;
+    if (!aligned16(key_rotation) || (has_qjl && !aligned16(qjl)) || !has_alignment(prefix, n_prefix, has_qjl) ||
+        !has_alignment(own, n_own, has_qjl))
+        return TQ_ERR_UNSUPPORTED;
+    Plan p;
+    if (!make_plan(batch, q_heads, kv_heads, prompts, cu_rows != nullptr, max_rows, n_prefix, n_own, p)) return TQ_ERR_UNSUPPORTED;
+    if (!workspace || workspace_bytes < p.total() || !aligned16(workspace)) return TQ_ERR_WORKSPACE;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    int4* const row_slots = reinterpret_cast<int4*>(ws + p.o_bytes + p.ms_bytes);
+    const int shared = (cu_rows || prefix_starts || prefix_lens || own_lens) && p.items <= 64 && p.n_slots > p.items;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const PrefixArgs a{prompts, batch, kv_heads, q_heads / kv_heads, p.per, p.items, cu_rows, batch / prompts,
+                       prefix_starts, prefix_lens, own_lens, n_prefix, cap_prefix, n_own, cap_own,
+                       cache_of(prefix, n_prefix), cache_of(own, n_own), q_sb, q_sh, p.n_split,
+                       shared ? p.n_slots : p.n_split * p.items, shared, row_slots};
+    const Codec c{key_centers, value_centers, key_rotation, qjl, scale * LOG2E, q, q_type, reinterpret_cast<float*>(ws),
+                  reinterpret_cast<float2*>(ws + p.o_bytes)};
+    if (has_qjl) {
+        if (value_bits == 4) launch_prefix<3, 4, true>(a, c, p, s);
+        else if (value_bits == 3) launch_prefix<2, 3, true>(a, c, p, s);
+        else launch_prefix<1, 2, true>(a, c, p, s);
+    } else {
+        if (value_bits == 4) launch_prefix<4, 4, false>(a, c, p, s);
+        else if (value_bits == 3) launch_prefix<3, 3, false>(a, c, p, s);
+        else if (value_bits == 2) launch_prefix<2, 2, false>(a, c, p, s);
+        else launch_prefix<1, 1, false>(a, c, p, s);
+    }
+    TQ_CHECK_LAUNCH();
+    const Merge m{(int64_t)batch * q_heads, c.part_o, c.part_ms, value_rotation, out_f32, out_16, q_type == 2, lse_out};
+    const PrefixRows rows{q_heads, kv_heads, 32 * p.row_blocks, row_slots};
+    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((m.all_rows + MERGE_ROWS - 1) / MERGE_ROWS)), dim3(MERGE_T), 0, s, m, rows);
+    TQ_CHECK_LAUNCH();
+    return TQ_OK;
+}

@@ -17,7 +17,9 @@ Reference interfaces replaced:
                     fused kernel refuses (runtime/triton_kernels.py:252-253) and its chunked
                     path dequantises (runtime/attention.py:215-304)
 Beside the reference's: prompt_attention (whole prompts, runtime/attention.py:75-99), tree_attention (drafted
-tokens, runtime/attention.py:215-304), gather_tokens and keep_tokens (runtime/packed_qmse_cache.py:81-92, 135-140).
+tokens, runtime/attention.py:215-304), gather_tokens and keep_tokens (runtime/packed_qmse_cache.py:81-92, 135-140),
+prefix_attention (sequences behind shared prompts), and block_bounds, select_blocks and block_attention (long histories read in
+part).
 """
 
 from __future__ import annotations
@@ -791,6 +793,10 @@ def _pointers(tensors) -> array:
     return array("Q", [t.data_ptr() for t in tensors])
 
 
+def _pointers_or_0(tensors) -> array:
+    return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
+
+
 #: up to here a call's new buffers are parts of one allocation: twelve of their own are 18 us of host time, the parts 12 us of
 #: a call whose kernel takes 15.  A kept view holds on to the block
 _ONE_BLOCK_BYTES = 64 << 20
@@ -878,6 +884,248 @@ def keep_tokens(buffers: list[torch.Tensor], index: torch.Tensor, *, first: int,
     for a in range(0, len(buffers), _MOVE_BUFFERS):
         _on_device("tq_keep_tokens", dev.index, min(_MOVE_BUFFERS, len(buffers) - a), a_at + 8 * a, a_row + 4 * a, B, H, cap,
                    first, tokens, at_index, sb, sh, n, stream)
+
+
+def _packed_arrays(name: str, cache: dict, batch: int | None, key: CodecParams, value: CodecParams, has_qjl: bool, on: int):
+    """The arrays k_codes, k_norms, k_signs, k_rnorms, v_codes, v_norms of a packed cache, looked over, and its [B, Hkv, cap]."""
+    sh = cache["k_codes"].shape
+    if len(sh) != 4 or (batch is not None and sh[0] != batch):
+        raise ValueError(f"{name}: k_codes {tuple(sh)} do not match a batch of {batch}")
+    sh, out = tuple(sh[:3]), []
+    for what, row in (("k_codes", 16 * key.bits), ("k_norms", 0), ("k_signs", HEAD_DIM // 8), ("k_rnorms", 0),
+                      ("v_codes", 16 * value.bits), ("v_norms", 0)):
+        t = cache.get(what)
+        if what in ("k_signs", "k_rnorms"):
+            if (t is not None) != has_qjl:
+                raise ValueError(f"{name}: Q_prod keys need k_signs, k_rnorms and qjl")
+            if t is None:
+                out.append(None)
+                continue
+        want = sh + (row,) if row else sh
+        if (t.shape != want or t.dtype is not (torch.uint8 if row else torch.float16) or not t.is_contiguous()
+                or t.get_device() != on):
+            _require_gpu(t)
+            raise ValueError(f"{name}: {what}: expected a contiguous tensor of {want} on device {on}, got {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
+        out.append(t)
+    return out, sh
+
+
+def _check_codec(key: CodecParams, value: CodecParams, qjl: torch.Tensor | None, on: int) -> None:
+    for name, t, n in (("key.rotation", key.rotation, HEAD_DIM ** 2), ("key.centers", key.centers, 1 << key.bits),
+                       ("value.rotation", value.rotation, HEAD_DIM ** 2), ("value.centers", value.centers, 1 << value.bits),
+                       ("qjl", qjl, HEAD_DIM ** 2)):
+        if t is not None and (t.get_device() != on or t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous()):
+            raise ValueError(f"{name}: expected {n} contiguous fp32 on device {on}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _one_token(name: str, q: torch.Tensor) -> torch.Tensor:
+    """A query of one token per sequence, [B, Hq, D] or [B, Hq, 1, D], as [B, Hq, D]."""
+    if q.dim() == 4 and q.shape[2] == 1:
+        q = q[:, :, 0]
+    if q.dim() != 3 or q.shape[-1] != HEAD_DIM:
+        raise ValueError(f"{name}: expected q [B, Hq, {HEAD_DIM}] or [B, Hq, 1, {HEAD_DIM}], got {tuple(q.shape)}")
+    if q.dtype not in _QUERY_TYPES:
+        raise ValueError(f"{name}: q must be bf16, fp16 or fp32, got {q.dtype}")
+    return q if q.stride(-1) == 1 else q.contiguous()
+
+
+def _logit_scale(name: str, scale: float | None) -> float:
+    s = float(scale) if scale is not None else 1.0 / math.sqrt(HEAD_DIM)
+    if not 0.0 < s < math.inf:
+        raise ValueError(f"{name}: scale {s}")
+    return s
+
+
+def prefix_attention(q: torch.Tensor, prefix: dict, own: dict | None = None, *, n_prefix: int, n_own: int = 0, key: CodecParams,
+                     value: CodecParams, qjl: torch.Tensor | None = None, cu_rows: torch.Tensor | None = None,
+                     max_rows: int | None = None, prefix_starts: torch.Tensor | None = None,
+                     prefix_lens: torch.Tensor | None = None, own_lens: torch.Tensor | None = None,
+                     scale: float | None = None, want_f32: bool = False, want_lse: bool = False):
+    """Attention of one query token per sequence where several sequences continue one packed prompt (tq_prefix_attention).
+
+    q [B, Hq, D] or [B, Hq, 1, D] (bf16, fp16 or fp32), at most 64 query heads per KV head.  ``prefix``: the packed prompts, a dict of
+    k_codes, k_norms, v_codes, v_norms and with QJL k_signs, k_rnorms, [P, Hkv, cap, ...] with ``n_prefix`` valid slots.  ``own``: the
+    sequences' packed tokens behind their prompts, the same arrays [B, Hkv, cap, ...] of the same codec with ``n_own`` valid
+    slots.  Prompt p is continued by B / P sequences, those of prompt 0 first, or with ``cu_rows`` int [P + 1], ascending from 0 to B,
+    by the sequences [cu_rows[p], cu_rows[p + 1]); ``max_rows``, the most sequences of one prompt where the caller knows it, is what the
+    kernel's blocks are then sized for.  ``prefix_starts`` / ``prefix_lens`` int [P]: prompt p is the slots [start, len) of its row;
+    ``own_lens`` int [B]: a sequence's own tokens are the slots [0, len) of its row.  Returns [B, Hq, D] in q's dtype, then fp32 with
+    ``want_f32``, then the fp32 log-sum-exp [B, Hq] of the scaled logits with ``want_lse``.
+    """
+    q = _one_token("prefix_attention", q)
+    _no_gradient("prefix_attention", q)
+    _not_traced("prefix_attention")
+    _require_gpu(q)
+    dev, on = q.device, q.get_device()
+    B, Hq, D = q.shape
+    has_qjl = qjl is not None
+    shared, (P, Hkv, cap) = _packed_arrays("prefix", prefix, None, key, value, has_qjl, on)
+    mine, own_cap = [None] * 6, 0
+    if own is not None:
+        mine, sh = _packed_arrays("own", own, B, key, value, has_qjl, on)
+        own_cap = sh[2]
+        if sh[1] != Hkv:
+            raise ValueError(f"own: {sh[1]} KV heads, the prompts have {Hkv}")
+    _check_codec(key, value, qjl, on)
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads for {Hkv} KV heads")
+    if not 0 <= n_prefix <= cap or not 0 <= n_own <= own_cap:
+        raise ValueError(f"prefix_attention: {n_prefix} and {n_own} tokens of capacities of {cap} and {own_cap}")
+    if P == 0 or (cu_rows is None and B % P):
+        raise ValueError(f"prefix_attention: {B} sequences of {P} prompts: give cu_rows")
+    cu_rows = _int32_on(cu_rows, dev, "cu_rows", (P + 1,))
+    prefix_starts = _int32_on(prefix_starts, dev, "prefix_starts", (P,))
+    prefix_lens = _int32_on(prefix_lens, dev, "prefix_lens", (P,))
+    own_lens = _int32_on(own_lens, dev, "own_lens", (B,))
+    s = _logit_scale("prefix_attention", scale)
+    f32 = torch.empty((B, Hq, D), dtype=torch.float32, device=dev) if want_f32 or q.dtype == torch.float32 else None
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev) if q.dtype != torch.float32 else None
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if want_lse else None
+    if B and Hq:
+        rows = min(B, int(max_rows)) if max_rows is not None else B
+        need = int(_lib.load().tq_prefix_attention_workspace_bytes(B, Hq, Hkv, D, P, int(cu_rows is not None), rows, n_prefix, n_own))
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        at, at_own = _pointers_or_0(shared), _pointers_or_0(mine)
+        qs = q.stride()
+        _on_device("tq_prefix_attention", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, D, qs[0], qs[1], P, _ptr(cu_rows),
+                   rows, _ptr(prefix_starts), _ptr(prefix_lens), n_prefix, cap, at.buffer_info()[0], _ptr(own_lens), n_own,
+                   own_cap, at_own.buffer_info()[0], key.bits, value.bits, int(has_qjl), key.rotation.data_ptr(),
+                   key.centers.data_ptr(), _ptr(qjl), value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s,
+                   _ptr(f32), _ptr(out), _ptr(lse), ws.data_ptr(), ws.numel(), _stream_handle(dev))
+    outs = (f32 if out is None else out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
+    return outs if len(outs) > 1 else outs[0]
+
+
+BLOCK_TOKENS = 64  # slots of a block (TQ_BLOCK_TOKENS): block j is the slots [64 j, 64 j + 64)
+MAX_BLOCKS = 4096  # blocks chosen for one KV head (TQ_MAX_BLOCKS)
+MAX_SCORED = 32768  # blocks of a history that are chosen from (TQ_MAX_SCORED)
+
+
+def block_bounds(k: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, first: int = 0) -> None:
+    """Bounds of the keys of every 64 tokens of k [B, H, T, D] (bf16; other types are rounded to it), written for the blocks from
+    ``first`` on (tq_block_bounds).
+
+    ``lohi`` int8 [B, H, cap, 2, D] and ``step`` fp32 [B, H, cap]: no element of block j's keys is below lohi[j, 0] step[j] or above
+    lohi[j, 1] step[j], channel by channel, up to 127 2^100.  The last block may have fewer than 64 tokens; the bounds are then of those.
+    """
+    k = k if k.dim() == 4 and k.shape[2] == 0 else _as_encoder_input(k)
+    _no_gradient("block_bounds", k)
+    _not_traced("block_bounds")
+    _require_gpu(k)
+    B, H, T, D = k.shape
+    on = k.get_device()
+    if lohi.dim() != 5 or lohi.shape[:2] != (B, H) or lohi.shape[3:] != (2, D) or lohi.dtype is not torch.int8 \
+            or not lohi.is_contiguous() or lohi.get_device() != on:
+        raise ValueError(f"lohi: expected a contiguous int8 tensor of {(B, H)} + (blocks, 2, {D}) on {k.device}, got {lohi.dtype} "
+                         f"{tuple(lohi.shape)} on {lohi.device}")
+    cap = lohi.shape[2]
+    if step.shape != (B, H, cap) or step.dtype is not torch.float32 or not step.is_contiguous() or step.get_device() != on:
+        raise ValueError(f"step: expected a contiguous fp32 tensor of {(B, H, cap)} on {k.device}, got {step.dtype} "
+                         f"{tuple(step.shape)} on {step.device}")
+    n = -(-T // BLOCK_TOKENS)
+    if first < 0 or first + n > cap:
+        raise ValueError(f"block_bounds: blocks [{first}, {first + n}) of a capacity of {cap}")
+    if k.numel() == 0:
+        return
+    st = k.stride()
+    _on_device("tq_block_bounds", on, k.data_ptr(), B, H, T, D, st[0], st[1], st[2], lohi.data_ptr(), step.data_ptr(), cap, first,
+               _stream_handle(k.device))
+
+
+def select_blocks(q: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, *, n_tokens: int, keep: int, sink: int = 1,
+                  recent: int = 1, n_blocks: int | None = None, seq_starts: torch.Tensor | None = None,
+                  seq_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """For each KV head the ``keep`` blocks of a history of ``n_tokens`` that its query heads may give the largest logits, int32
+    [B, Hkv, keep], ascending (tq_select_blocks).
+
+    q [B, Hq, D] or [B, Hq, 1, D] (bf16, fp16 or fp32); ``lohi`` / ``step`` as ``block_bounds`` writes them, of ``n_blocks`` blocks
+    (all that there is room for without).  Of the blocks with slots in the row's range [``seq_starts``, ``seq_lens``) the first ``sink``
+    and the last ``recent`` are always chosen (these need no bounds), the others by their scores: q in whole numbers against the
+    bounds, the largest of the KV head's query heads; equal scores by their number.  Places left, where there are fewer
+    blocks, hold -1.
+    """
+    q = _one_token("select_blocks", q)
+    _no_gradient("select_blocks", q)
+    _not_traced("select_blocks")
+    _require_gpu(q)
+    dev, on = q.device, q.get_device()
+    B, Hq, D = q.shape
+    if lohi.dim() != 5 or lohi.shape[0] != B or lohi.shape[3:] != (2, D) or lohi.dtype is not torch.int8 or not lohi.is_contiguous() \
+            or lohi.get_device() != on or lohi.shape[1] == 0 or Hq % lohi.shape[1]:
+        raise ValueError(f"lohi {lohi.dtype} {tuple(lohi.shape)} on {lohi.device} does not match q {tuple(q.shape)} on {dev}")
+    Hkv, cap = lohi.shape[1:3]
+    if step.shape != (B, Hkv, cap) or step.dtype is not torch.float32 or not step.is_contiguous() or step.get_device() != on:
+        raise ValueError(f"step {step.dtype} {tuple(step.shape)} on {step.device} does not match lohi {tuple(lohi.shape)}")
+    known = cap if n_blocks is None else int(n_blocks)
+    if not 0 <= known <= cap or n_tokens < 0 or -(-n_tokens // BLOCK_TOKENS) - recent > known:
+        raise ValueError(f"select_blocks: bounds of {known} of {cap} blocks for {n_tokens} tokens, the last {recent} blocks without")
+    if sink < 0 or recent < 0 or not max(sink + recent, 1) <= keep <= MAX_BLOCKS:
+        raise ValueError(f"select_blocks: keep {keep} (at most {MAX_BLOCKS}) with {sink} first and {recent} last blocks")
+    seq_starts = _int32_on(seq_starts, dev, "seq_starts", (B,))
+    seq_lens = _int32_on(seq_lens, dev, "seq_lens", (B,))
+    out = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    if B and Hq:
+        qs = q.stride()
+        _on_device("tq_select_blocks", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, D, qs[0], qs[1], lohi.data_ptr(),
+                   step.data_ptr(), cap, known, n_tokens, _ptr(seq_starts), _ptr(seq_lens), keep, sink, recent, out.data_ptr(),
+                   _stream_handle(dev))
+    return out
+
+
+def block_attention(q: torch.Tensor, blocks: torch.Tensor, *, k_codes: torch.Tensor, k_norms: torch.Tensor, v_codes: torch.Tensor,
+                    v_norms: torch.Tensor, n_tokens: int, key: CodecParams, value: CodecParams,
+                    k_signs: torch.Tensor | None = None, k_rnorms: torch.Tensor | None = None, qjl: torch.Tensor | None = None,
+                    seq_starts: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None, scale: float | None = None,
+                    want_f32: bool = False, want_lse: bool = False):
+    """``decode_attention`` over chosen blocks of 64 slots only (tq_block_attention).
+
+    ``blocks`` int [B, Hkv, n], for each KV head the numbers of its blocks, in any order, n <= 4096.  Slots of a block outside
+    [``seq_starts``, ``seq_lens``) and [0, ``n_tokens``) are left out, so is a number that names no slot (-1 as ``select_blocks`` leaves
+    it); a block named twice counts twice.  At most 8 query heads per KV head.  The rest, and what it returns, as for
+    ``decode_attention``.
+    """
+    q = _one_token("block_attention", q)
+    _no_gradient("block_attention", q)
+    _not_traced("block_attention")
+    _require_gpu(q)
+    dev, on = q.device, q.get_device()
+    q = rows16(q.to(torch.bfloat16).contiguous())
+    B, Hq, D = q.shape
+    has_qjl = qjl is not None
+    cache = {"k_codes": k_codes, "k_norms": k_norms, "k_signs": k_signs, "k_rnorms": k_rnorms, "v_codes": v_codes, "v_norms": v_norms}
+    (kc, kn, ks, kr, vc, vn), (_, Hkv, cap) = _packed_arrays("block_attention", cache, B, key, value, has_qjl, on)
+    _check_codec(key, value, qjl, on)
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{Hq} query heads for {Hkv} KV heads")
+    if not 0 <= n_tokens <= cap:
+        raise ValueError(f"block_attention: {n_tokens} tokens of a capacity of {cap}")
+    keep = blocks.shape[-1] if blocks.dim() else 0
+    blocks = _int32_on(blocks, dev, "blocks", (B, Hkv, keep))
+    if keep > MAX_BLOCKS:
+        raise ValueError(f"block_attention: {keep} blocks (at most {MAX_BLOCKS})")
+    seq_starts = _int32_on(seq_starts, dev, "seq_starts", (B,))
+    seq_lens = _int32_on(seq_lens, dev, "seq_lens", (B,))
+    s = _logit_scale("block_attention", scale)
+    out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=dev)
+    f32 = torch.empty((B, Hq, D), dtype=torch.float32, device=dev) if want_f32 else None
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if want_lse else None
+    if B and Hq and keep:
+        need = int(_lib.load().tq_block_attention_workspace_bytes(B, Hq, Hkv, D, keep))
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+        _on_device("tq_block_attention", on, q.data_ptr(), B, Hq, Hkv, D, blocks.data_ptr(), keep, _ptr(seq_starts), _ptr(seq_lens),
+                   n_tokens, cap, kc.data_ptr(), kn.data_ptr(), _ptr(ks), _ptr(kr), vc.data_ptr(), vn.data_ptr(), key.bits,
+                   value.bits, int(has_qjl), key.rotation.data_ptr(), key.centers.data_ptr(), _ptr(qjl),
+                   value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s, _ptr(f32), out.data_ptr(), _ptr(lse),
+                   ws.data_ptr(), ws.numel(), _stream_handle(dev))
+    else:  # nothing is attended to
+        out.zero_()
+        if f32 is not None:
+            f32.zero_()
+        if lse is not None:
+            lse.fill_(float("-inf"))
+    outs = (out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
+    return outs if len(outs) > 1 else out
 
 
 def rows16(t: torch.Tensor) -> torch.Tensor:
