@@ -1,0 +1,352 @@
+"""Attention behind shared prompts (tq_prefix_attention) against the fp64 formula: every bit width, types, tile and block edges,
+prompts with different numbers of sequences, padded prompts, rows without tokens, norms at the ends of their range, strides, streams
+and captured calls; the shared layer beside a layer that holds the prompt once for each sequence, and a model on both."""
+
+import copy
+import math
+
+import pytest
+import torch
+from transformers.cache_utils import Cache
+
+from turboquant.runtime import SharedPrefixLayer, share_prefix, shared_prefix_attention
+from turboquant.runtime import kernels as K
+from turboquant.runtime.packed_qmse_cache import build_packed_mse_cache
+from turboquant.runtime.synthetic import kv_bf16
+
+from ._packed import BITS, D, TOL, arrays, attend64, check, codec, i32, make_layer, randn, rows64
+from ._tiny_model import tiny_llama
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(q, prompts, own, counts, starts=None, lens=None, own_lens=None, scale=None):
+    """In 64 bits, sequence by sequence."""
+    pk, pv = rows64(prompts)
+    ok, ov = rows64(own) if own is not None else (pk[:, :, :0], pv[:, :, :0])
+    outs, b = [], 0
+    for p, n in enumerate(counts):
+        lo, hi = starts[p] if starts else 0, lens[p] if lens else pk.shape[2]
+        lo, hi = min(max(lo, 0), pk.shape[2]), min(max(hi, 0), pk.shape[2])
+        for _ in range(n):
+            m = ok.shape[2] if own_lens is None else min(max(own_lens[b], 0), ok.shape[2])
+            k = torch.cat((pk[p:p + 1, :, min(lo, hi):hi], ok[b:b + 1, :, :m] if own is not None else ok[:1]), 2)
+            v = torch.cat((pv[p:p + 1, :, min(lo, hi):hi], ov[b:b + 1, :, :m] if own is not None else ov[:1]), 2)
+            outs.append(attend64(q[b:b + 1], k, v, scale=scale))
+            b += 1
+    return torch.cat([o for o, _ in outs]), torch.cat([e for _, e in outs])
+
+
+def setup(counts, H, g, N, M, bits=4, qjl=True, dtype=torch.bfloat16, seed=0):
+    prompts = make_layer(len(counts), H, N, bits, qjl, seed=seed)
+    own = make_layer(sum(counts), H, M, bits, qjl, seed=seed + 2) if M else None
+    q = randn((sum(counts), H * g, D), seed + 9, dtype)
+    kw = dict(n_prefix=N, n_own=M, **codec(prompts))
+    if len(set(counts)) > 1:
+        kw["cu_rows"] = i32([sum(counts[:i]) for i in range(len(counts) + 1)])
+    return prompts, own, q, kw
+
+
+def call(prompts, own, q, kw):
+    return K.prefix_attention(q, arrays(prompts), None if own is None else arrays(own), **kw)
+
+
+@pytest.mark.parametrize("bits,qjl", BITS)
+@pytest.mark.parametrize("counts,H,g,N,M", [((3, 3), 2, 4, 100, 33), ((20, 1), 1, 7, 517, 5)])
+def test_every_bit_width(cuda, bits, qjl, counts, H, g, N, M):
+    prompts, own, q, kw = setup(counts, H, g, N, M, bits, qjl)
+    got = call(prompts, own, q, kw)
+    assert got.shape == q.shape and got.dtype == q.dtype
+    check(got, reference(q, prompts, own, counts)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("counts,H,g,N,M", [((1,), 1, 1, 1, 0), ((1,), 2, 4, 1, 1), ((2,), 2, 4, 31, 32), ((8,), 1, 4, 32, 33),
+                                            ((9,), 1, 4, 33, 1), ((5, 5, 5), 2, 8, 65, 64), ((64,), 1, 1, 300, 40),
+                                            ((70,), 1, 1, 40, 3), ((3,), 1, 64, 129, 31), ((2, 2), 1, 33, 64, 2),
+                                            ((1, 7, 0, 2), 2, 5, 700, 100), ((0, 0, 4), 1, 12, 90, 17), ((33,), 2, 2, 2000, 0)])
+def test_shapes_and_types(cuda, dtype, counts, H, g, N, M):
+    prompts, own, q, kw = setup(counts, H, g, N, M, dtype=dtype, seed=3)
+    got, f32, lse = call(prompts, own, q, dict(kw, want_f32=True, want_lse=True))
+    ref, ref_lse = reference(q, prompts, own, counts)
+    assert got.dtype == dtype
+    check(got, ref)
+    check(f32, ref)
+    assert (lse.double() - ref_lse).abs().max() <= 4e-3
+
+
+@pytest.mark.parametrize("max_rows", [None, 1, 3, 40])
+def test_the_most_rows_are_a_hint(cuda, max_rows):
+    counts = (12, 3, 25)
+    prompts, own, q, kw = setup(counts, 2, 4, 400, 20, seed=5)
+    check(call(prompts, own, q, dict(kw, max_rows=max_rows)), reference(q, prompts, own, counts)[0])
+
+
+def test_a_long_prompt_and_many_splits(cuda):
+    prompts, own, q, kw = setup((6,), 2, 4, 33000, 70, seed=7)
+    check(call(prompts, own, q, kw), reference(q, prompts, own, (6,))[0])
+
+
+@pytest.mark.parametrize("counts", [(4, 4, 4), (2, 9, 1)])
+def test_ranges(cuda, counts):
+    prompts, own, q, kw = setup(counts, 2, 3, 600, 90, 3, False, seed=9)
+    starts, lens = [0, 100, 590], [600, 111, 590]
+    mine = [0, 90, 1, 33, 64, 17, 0, 90, 32, 31, 5, 500]
+    got, lse = call(prompts, own, q, dict(kw, prefix_starts=i32(starts), prefix_lens=i32(lens), own_lens=i32(mine), want_lse=True))
+    ref, ref_lse = reference(q, prompts, own, counts, starts, lens, mine)
+    check(got, ref)
+    assert (lse.double() - ref_lse).abs().max() <= 4e-3
+
+
+def test_rows_without_tokens_are_zero(cuda):
+    prompts, own, q, kw = setup((2, 2), 2, 4, 64, 8, seed=11)
+    got, lse = call(prompts, own, q, dict(kw, prefix_lens=i32([0, 40]), prefix_starts=i32([0, 50]), own_lens=i32([0, 3, -5, 0]),
+                                          want_lse=True))
+    ref, ref_lse = reference(q, prompts, own, (2, 2), [0, 50], [0, 40], [0, 3, -5, 0])
+    assert (got[[0, 2, 3]] == 0).all() and (lse[[0, 2, 3]] == -math.inf).all()
+    check(got[1], ref[1])
+    got = K.prefix_attention(q, arrays(prompts), n_prefix=0, **codec(prompts))
+    assert (got == 0).all()
+
+
+def test_offsets_that_are_none(cuda):
+    """Descending offsets and offsets past the batch are empty prompts and ends of the batch; every sequence has a prompt."""
+    prompts, own, q, kw = setup((3, 3, 3), 1, 4, 50, 4, seed=13)
+    got = call(prompts, own, q, dict(kw, cu_rows=i32([5, 4, 2, 100])))  # prompts 0: [0, 4), 1: none, 2: [4, 9)
+    check(got, reference(q, prompts, own, (4, 0, 5))[0])
+    got = call(prompts, own, q, dict(kw, cu_rows=i32([0, -7, 40, 3])))  # prompts 0: none, 1: all
+    check(got, reference(q, prompts, own, (0, 9, 0))[0])
+
+
+def test_many_prompts(cuda):
+    """More items than a wave has lanes, and more prompts."""
+    counts = tuple((i * 7) % 4 for i in range(90))
+    prompts, own, q, kw = setup(counts, 1, 4, 40, 3, seed=15)
+    check(call(prompts, own, q, kw), reference(q, prompts, own, counts)[0])
+    check(call(prompts, own, q, dict(kw, max_rows=3, own_lens=i32([b % 4 for b in range(sum(counts))]))),
+          reference(q, prompts, own, counts, own_lens=[b % 4 for b in range(sum(counts))])[0])
+
+
+@pytest.mark.parametrize("size", [2.0 ** -20, 1.0, 3e4])
+def test_norms_at_the_ends_of_their_range(cuda, size):
+    prompts, own, q, kw = setup((3,), 2, 4, 400, 40, seed=17)
+    for layer, n in ((prompts, 400), (own, 40)):
+        ramp = torch.linspace(1e-3 if size > 1e-3 else 1.0, 2.0, n, device="cuda")
+        layer._store.vn[:, :, :n] = (size * ramp).half()
+    got, f32 = call(prompts, own, q, dict(kw, want_f32=True))
+    ref = reference(q, prompts, own, (3,))[0]
+    check(f32, ref)
+
+
+def test_what_is_not_attended_to_may_be_anything(cuda):
+    prompts, own, q, kw = setup((2, 5), 2, 4, 130, 40, seed=19)
+    limits = dict(prefix_starts=i32([7, 0]), prefix_lens=i32([129, 100]), own_lens=i32([0, 3, 40, 1, 33, 31, 32]))
+    want = call(prompts, own, q, dict(kw, **limits))
+    for layer, lo, hi in ((prompts, [7, 0], [129, 100]), (own, [0] * 7, [0, 3, 40, 1, 33, 31, 32])):
+        for b in range(len(lo)):
+            for t in (layer._store.kn, layer._store.kr, layer._store.vn):
+                t[b, :, :lo[b]] = math.nan
+                t[b, :, hi[b]:] = math.inf
+    assert torch.equal(call(prompts, own, q, dict(kw, **limits)), want)
+
+
+def test_queries_in_any_layout(cuda):
+    prompts, own, q, kw = setup((3, 4), 2, 4, 70, 9, seed=21)
+    want = call(prompts, own, q, kw)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        wide = torch.zeros(8, 7, D + 3, 7, dtype=dtype, device="cuda")
+        odd = wide.permute(1, 0, 3, 2)[:, :, 0, 1:D + 1]  # element stride 7: a copy is made
+        odd.copy_(q)
+        assert torch.equal(call(prompts, own, odd, kw), call(prompts, own, q.to(dtype), kw))
+        rows = torch.zeros(7, 3, 8, D + 1, dtype=dtype, device="cuda")[:, 1, :, 1:]  # rows at any element
+        rows.copy_(q)
+        assert torch.equal(call(prompts, own, rows, kw), call(prompts, own, q.to(dtype), kw))
+    assert torch.equal(call(prompts, own, q[:, :, None], kw), want)
+
+
+def test_a_scale_of_its_own(cuda):
+    prompts, own, q, kw = setup((3,), 2, 4, 200, 9, seed=23)
+    check(call(prompts, own, q, dict(kw, scale=0.031)), reference(q, prompts, own, (3,), scale=0.031)[0])
+
+
+def test_streams_and_captured_calls(cuda):
+    """Two calls on streams of their own, and a captured call replayed with other queries, offsets and lengths."""
+    prompts, own, q, kw = setup((4, 9), 2, 4, 500, 40, seed=25)
+    cu, mine = i32([0, 4, 13]), i32([40] * 13)
+    kw = dict(kw, cu_rows=cu, own_lens=mine)
+    want = call(prompts, own, q, kw)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(call(prompts, own, q, kw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(prompts, own, q, kw)
+    for counts, lens in (((4, 9), [40] * 13), ((0, 13), list(range(13))), ((11, 2), [0, 40] * 6 + [7])):
+        cu.copy_(i32([0, counts[0], 13]))
+        mine.copy_(i32(lens))
+        q.copy_(randn(q.shape, sum(lens)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, call(prompts, own, q, kw))
+        check(out, reference(q, prompts, own, counts, own_lens=lens)[0])
+
+
+# ---------------------------------------------------------------- the shared layer
+
+
+def append(layer, B, H, T, seed):
+    k, v = kv_bf16((B, H, T, D), seed=seed), kv_bf16((B, H, T, D), seed=seed + 1)
+    layer.update(k, v)
+    return k, v
+
+
+def both(counts, H, N, bits=4, qjl=True, quantize=True, seed=0):
+    """A shared layer, and one with the prompt copied for every sequence."""
+    base = make_layer(len(counts), H, N, bits, qjl, seed=seed)
+    base.quantize_decode = quantize
+    copied = copy.deepcopy(base)
+    copied._take_rows(torch.arange(len(counts)).repeat_interleave(torch.tensor(counts)))
+    shared = share_prefix(Cache(layers=[base]), list(counts)).layers[0]
+    assert isinstance(shared, SharedPrefixLayer)
+    shared._lazy_update = True
+    return shared, copied
+
+
+def fused(q, layer, mask=None):
+    from turboquant.runtime import fused_attention
+
+    return fused_attention(q, layer, q.shape[1] // layer._store.H, mask)
+
+
+@pytest.mark.parametrize("bits,qjl", [(4, True), (3, False)])
+@pytest.mark.parametrize("quantize", [True, False])
+@pytest.mark.parametrize("counts", [(3, 3), (1, 6, 2)])
+def test_shared_and_copied_prompts_agree(cuda, bits, qjl, quantize, counts):
+    B, H = sum(counts), 2
+    shared, copied = both(counts, H, 150, bits, qjl, quantize)
+    q = randn((B, 8, 1, D), 5)
+    check(shared_prefix_attention(q, shared), fused(q, copied).double(), 2 * TOL)  # no tokens of their own yet
+    for i in range(3):
+        for layer in (shared, copied):
+            append(layer, B, H, 1 + 20 * i, 50 + i)
+        assert shared.get_seq_length() == copied.get_seq_length()
+        got, want = shared_prefix_attention(q, shared), fused(q, copied)
+        assert got.shape == want.shape and got.dtype == want.dtype
+        check(got, want.double(), 2 * TOL)
+    mask = torch.ones(B, shared.get_seq_length(), dtype=torch.bool, device="cuda")
+    mask[:counts[0], :30] = False  # the first prompt is padded on the left
+    check(shared_prefix_attention(q, shared, mask), fused(q, copied, mask).double(), 2 * TOL)
+
+
+def test_masks_that_are_no_shared_range_take_the_decoded_rows(cuda):
+    counts, B = (3, 2), 5
+    shared, copied = both(counts, 2, 100)
+    for layer in (shared, copied):
+        append(layer, B, 2, 5, 50)
+    q = randn((B, 8, 1, D), 5)
+    k, v = rows64(copied)
+    hole = torch.ones(B, 105, dtype=torch.bool, device="cuda")
+    hole[1, 40:60] = False
+    apart = torch.ones(B, 105, dtype=torch.bool, device="cuda")
+    apart[1, :30] = False  # one sequence of a prompt alone
+    for mask in (hole, apart):
+        ref, _ = attend64(q[:, :, 0], k, v, mask[:, None])
+        # bf16 rows and weights of torch's attention: 2^-8 of the logits' terms and of the values
+        check(shared_prefix_attention(q, shared, mask), ref[:, :, None], 2e-2)
+    several = randn((B, 8, 4, D), 6)
+    got = shared_prefix_attention(several, shared)
+    for i in range(4):
+        ref, _ = attend64(several[:, :, i], k[:, :, :102 + i], v[:, :, :102 + i])
+        check(got[:, :, i], ref, 2e-2)
+
+
+def test_rows_and_tokens_move_with_their_prompts(cuda):
+    counts = (3, 2)
+    shared, copied = both(counts, 2, 100, seed=4)
+    for layer in (shared, copied):
+        append(layer, 5, 2, 6, 50)
+
+    def agree(B):
+        q = randn((B, 8, 1, D), B)
+        check(shared_prefix_attention(q, shared), fused(q, copied).double(), 2 * TOL)
+
+    for layer in (shared, copied):
+        layer.reorder_cache(torch.tensor([2, 2, 0, 4, 3], device="cuda"))
+    agree(5)
+    with pytest.raises(ValueError):
+        shared.reorder_cache(torch.tensor([3, 1, 2, 0, 4], device="cuda"))
+    with pytest.raises(IndexError):
+        shared.reorder_cache(torch.tensor([0, 1, 2, 3, 5], device="cuda"))
+    for layer in (shared, copied):
+        layer.batch_repeat_interleave(2)
+    agree(10)
+    for layer in (shared, copied):
+        layer.batch_select_indices(torch.tensor([0, 1, 5, 7, -1], device="cuda"))
+    assert shared.counts == [3, 2]
+    agree(5)
+    with pytest.raises(ValueError):
+        shared.batch_select_indices(torch.tensor([4, 0]))
+    for layer in (shared, copied):
+        layer.keep_tokens(torch.tensor([1, 3], device="cuda"), tokens=4)
+    agree(5)
+    for layer in (shared, copied):
+        append(layer, 5, 2, 40, 60)
+    agree(5)
+    for layer in (shared, copied):
+        layer.crop(-50)  # into the prompts
+    assert shared.get_seq_length() == copied.get_seq_length() == 94
+    agree(5)
+    for layer in (shared, copied):
+        layer.batch_select_indices(torch.tensor([False, False, False, True, True], device="cuda"))
+        append(layer, 2, 2, 3, 70)
+    assert shared.counts == [0, 2]
+    agree(2)
+
+
+def test_a_model_on_a_shared_prompt(cuda):
+    """Samples of one prompt: logits of decode steps on the shared cache beside those on a repeated one, by the backend and without."""
+    from turboquant.adapters.transformers import disable_turboquant_attention, enable_turboquant_attention
+
+    model = tiny_llama("cuda", torch.bfloat16, layers=2, heads=8, kv_heads=2)
+    gen = torch.Generator().manual_seed(3)
+    ids = torch.randint(0, 94, (2, 70), generator=gen).cuda()
+    mask = torch.ones_like(ids)
+    mask[1, :20] = 0
+    logits = {}
+    for kind in ("shared", "copied", "plain"):
+        with torch.no_grad():
+            past = model(input_ids=ids, attention_mask=mask, use_cache=True).past_key_values
+            cache = build_packed_mse_cache(past, bits=4, use_qjl_keys=True, quantize_decode=True, norm_guard=False)
+            if kind == "copied":
+                cache.batch_repeat_interleave(3)
+            else:
+                cache = share_prefix(cache, 3)
+            if kind != "plain":
+                old = enable_turboquant_attention(model, cache)
+            step, out = mask.repeat_interleave(3, 0), []
+            for i in range(3):
+                token = torch.randint(0, 94, (6, 1), generator=torch.Generator().manual_seed(i)).cuda()
+                step = torch.cat((step, step.new_ones(6, 1)), 1)
+                out.append(model(input_ids=token, attention_mask=step, past_key_values=cache, use_cache=True).logits.float())
+            if kind != "plain":
+                disable_turboquant_attention(model, cache, old)
+        logits[kind] = torch.cat(out, 1)
+    scale = logits["copied"].abs().max()
+    # bf16 activations: eight roundings of 2^-9 root mean square a layer
+    assert (logits["shared"] - logits["copied"]).abs().max() <= 0.03 * scale
+    assert (logits["plain"] - logits["copied"]).abs().max() <= 0.03 * scale
+
+
+def test_layers_that_cannot_be_shared_are_copied(cuda):
+    for layer in (make_layer(2, 2, 40, 4, True, num_outlier_channels=4), make_layer(2, 2, 40, 4, True, dense=3)):
+        cache = share_prefix(Cache(layers=[layer]), [1, 3])
+        assert cache.layers[0] is layer and layer._batch() == 4
+    with pytest.raises(ValueError):
+        share_prefix(Cache(layers=[make_layer(2, 2, 40, 4, True)]), [1, 2, 3])
+    with pytest.raises(ValueError):
+        share_prefix(Cache(layers=[make_layer(2, 2, 40, 4, True)]), 0)

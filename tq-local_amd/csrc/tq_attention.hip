@@ -873,6 +873,13 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
         return i < 64 ? __builtin_amdgcn_readlane(place_of, i) : (int)len;
     };
 
+    // whether block `rel` has slots of [start, len): a block without any would leave the reference maximum at -inf
+    const auto holds = [&](int rel) {
+        if constexpr (!LIST) return true;
+        const int slot = place(rel);
+        return slot < (int)len && slot + BLK > (int)start;
+    };
+
     // Per-block data of a wave, in the part the score stage reads (key codes, sign bits and
     // the three norms of token n) and the part the value stage reads (value codes of tokens
     // 4 r + g).
@@ -1560,7 +1567,7 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
 #pragma unroll
                 for (int s = 0; s < NSET; s += NB) {
                     const int rel = first + (i + rp * NSET + s) * STEP;
-                    if (rel < nt) process(s, rel, rp);
+                    if (rel < nt && holds(rel)) process(s, rel, rp);
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int b = 0; b < NB; ++b)

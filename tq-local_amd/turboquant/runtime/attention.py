@@ -25,6 +25,7 @@ rotated space; the reference's fused kernel refuses such layers
 
 from __future__ import annotations
 
+import functools
 import math
 import threading
 from typing import TYPE_CHECKING
@@ -36,7 +37,8 @@ from turboquant.runtime import _lib
 from turboquant.runtime import kernels as K
 
 if TYPE_CHECKING:
-    from turboquant.runtime.packed_qmse_cache import PackedMSELayer
+    from turboquant.runtime.packed_qmse_cache import BlockChoice, PackedMSELayer
+    from turboquant.runtime.shared_prefix import SharedPrefixLayer
 
 
 def _attend_mask(attention_mask: torch.Tensor, B: int, total: int) -> torch.Tensor:
@@ -117,7 +119,8 @@ def _group_buffers(layer: "PackedMSELayer") -> list[dict]:
 
 
 def fused_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", n_kv_groups: int,
-                    attention_mask: torch.Tensor | None = None) -> torch.Tensor | None:
+                    attention_mask: torch.Tensor | None = None,
+                    choice: "BlockChoice | None" = None) -> torch.Tensor | None:
     """Decode attention of [B, Hq, 1, D] queries over a packed layer -> [B, Hq, 1, D].
 
     The logit scale is 1/sqrt(D) (reference ``triton_kernels.py:285``).  Tokens
@@ -131,6 +134,8 @@ def fused_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", 
     than the kernels' 8 query heads per KV head, and for a mask whose attended slots are
     not one contiguous range per row.  The cache layer's ``_tq_mask_contiguous`` (set by
     the generation loop from the prompt mask) spares the host sync of that last check.
+
+    A layer told to (``attend_blocks``), or a ``choice`` given here, attends to chosen blocks of the packed tokens.
     """
     B, Hq, Sq, D = query_states.shape
     if Sq != 1:
@@ -161,9 +166,15 @@ def fused_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", 
                                          value_stack=sc.value_stack, qjl_stack=sc.qjl_stack, **kw)
     else:
         c = packed_layer.codecs
-        outs = K.decode_attention(query_states, k_codes=store.kc, k_norms=store.kn, v_codes=store.vc,
-                                  v_norms=store.vn, key=c.key, value=c.value, k_signs=store.ks, k_rnorms=store.kr,
-                                  qjl=c.qjl, **kw)
+        q = query_states
+        choice = packed_layer._choice if choice is None else choice
+        blocks = None
+        if choice is not None:
+            q = q if q.dtype in K._QUERY_TYPES else q.to(torch.bfloat16)
+            blocks = packed_layer.choose_blocks(q, choice, starts, p_ends)
+        attend = K.decode_attention if blocks is None else functools.partial(K.block_attention, blocks=blocks)
+        outs = attend(q, k_codes=store.kc, k_norms=store.kn, v_codes=store.vc, v_norms=store.vn, key=c.key, value=c.value,
+                      k_signs=store.ks, k_rnorms=store.kr, qjl=c.qjl, **kw)
     if n_dense == 0:
         out = outs[1] if f32 else outs
         return out.to(query_states.dtype).view(B, Hq, 1, D)
@@ -434,6 +445,96 @@ def tree_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", p
                                         attention_mask=_tree_mask(own, total, seq_starts, ends))
 
 
+def block_sparse_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", keep: int, sink: int = 1, recent: int = 2,
+                           attention_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """A decode step [B, Hq, 1, D] over ``keep`` blocks of 64 packed tokens for each KV head -> [B, Hq, 1, D].
+
+    The first ``sink`` blocks, the last ``recent`` and those that the query heads may give the largest logits, by bounds of the
+    keys that the layer keeps (``PackedMSELayer.attend_blocks`` has every step of a model do it); tokens kept dense are all attended
+    to.  A history of no more blocks is attended to in full.  One-group layers, up to 8 query heads per KV head, masks of one
+    range per row; others are refused."""
+    from turboquant.runtime.packed_qmse_cache import BlockChoice
+
+    B, Hq, Sq, D = query_states.shape
+    store = packed_layer._store
+    if store is None or packed_layer._outlier_enabled or (B, D) != (store.B, K.HEAD_DIM) or Sq != 1 or Hq % store.H \
+            or Hq // store.H > K.MAX_GROUP:
+        raise ValueError(f"block_sparse_attention takes one query token per row of a packed one-group layer and up to "
+                         f"{K.MAX_GROUP} query heads per KV head, got {tuple(query_states.shape)}")
+    out = fused_attention(query_states, packed_layer, Hq // store.H, attention_mask, BlockChoice(keep, sink, recent))
+    if out is None:
+        raise ValueError("block_sparse_attention: a row's attended tokens must be one range")
+    return out
+
+
+def _shared_ranges(layer: "SharedPrefixLayer", mask: torch.Tensor | None, device):
+    """(prefix starts, prefix ends, own ends) of a step's mask, int32 or None.
+
+    The sequences of one prompt have to share its padding (one host sync to find out, for all layers of a forward);
+    ``_HoleyMask`` where they do not, or where a row's tokens are not one range."""
+    if mask is None:
+        return None, None, None
+    n, total = layer.prefix.packed_seq_length(), layer.get_seq_length()
+    key = (mask._version, n, total, tuple(layer.counts), device)
+    c = getattr(_tls, "last_shared", None)
+    if c is None or c[0] is not mask or c[1] != key:
+        starts, ends = _valid_range(mask, layer.batch, total, device)
+        first, last = starts[layer.first_of], ends.clamp(max=n)[layer.first_of]
+        apart = (starts != first[layer.prompt_of]) | (ends.clamp(max=n) != last[layer.prompt_of]) | (starts > n)
+        c = _tls.last_shared = (mask, key, None if bool(apart.any()) else (first, last, (ends - n).clamp(min=0)))
+    if c[2] is None:
+        raise _HoleyMask
+    return c[2]
+
+
+def shared_prefix_attention(query_states: torch.Tensor, layer: "SharedPrefixLayer",
+                            attention_mask: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of sequences that continue shared packed prompts, [B, Hq, Sq, D] over a ``SharedPrefixLayer`` -> [B, Hq, Sq, D].
+
+    One query token per sequence, up to 64 query heads per KV head and a mask of one range per row (left padding of the
+    prompts) run on the packed codes (``kernels.prefix_attention``), tokens kept dense merged by log-sum-exp; others
+    take the decoded rows and torch's attention, the Sq tokens being the sequences' last ones."""
+    B, Hq, Sq, D = query_states.shape
+    prefix, own = layer.prefix, layer.own
+    store, n_prefix, n_own, n_dense = prefix._store, prefix.packed_seq_length(), own.packed_seq_length(), own._dense_len
+    if B != layer.batch or Hq % store.H:
+        raise ValueError(f"queries {tuple(query_states.shape)} for {layer.batch} sequences and {store.H} KV heads")
+    group, dev = Hq // store.H, query_states.device
+    dense = own._dense_buf if n_dense else ()
+    if (Sq == 1 and group <= 64 and query_states.dtype in K._QUERY_TYPES and _native_rows(query_states, *dense)
+            and (not n_dense or K.DenseAttention.takes(query_states, store.H))):
+        try:
+            starts, ends, own_ends = _shared_ranges(layer, attention_mask, dev)
+        except _HoleyMask:
+            pass
+        else:
+            arrays = lambda s: {"k_codes": s.kc, "k_norms": s.kn, "k_signs": s.ks, "k_rnorms": s.kr,  # noqa: E731
+                                "v_codes": s.vc, "v_norms": s.vn}
+            c = prefix.codecs
+            kw = dict(n_prefix=n_prefix, n_own=n_own, key=c.key, value=c.value, qjl=c.qjl, cu_rows=layer.cu_rows,
+                      max_rows=max(layer.counts), prefix_starts=starts, prefix_lens=ends, own_lens=own_ends)
+            mine = arrays(own._store) if n_own else None
+            if not n_dense:
+                return K.prefix_attention(query_states, arrays(store), mine, **kw).view(B, Hq, 1, D)
+            _, o_packed, lse = K.prefix_attention(query_states, arrays(store), mine, want_f32=True, want_lse=True, **kw)
+            q = query_states if query_states.dtype == torch.bfloat16 else query_states.float()
+            n = K.DenseAttention.split_count(q, store.H, n_dense, K.DENSE_SPLITS)
+            more = {} if own_ends is None else dict(starts=torch.zeros_like(own_ends), ends=own_ends, pos0=n_own)
+            return K.DenseAttention(q, store.H, n).add(*dense, n_dense, 0, n, 1.0 / math.sqrt(D), out=query_states.dtype,
+                                                       prev=o_packed, prev_lse=lse, **more)
+    keys, values = layer.dense_rows()
+    mask = attention_mask
+    if mask is None and Sq > 1:
+        mask = torch.ones(Sq, keys.shape[2], dtype=torch.bool, device=dev).tril(keys.shape[2] - Sq)
+    elif mask is not None:
+        if mask.dim() == 2:
+            mask = mask.bool()[:, None, None]
+        mask = mask[..., :keys.shape[2]]
+        mask = mask if mask.dtype == torch.bool else mask.to(query_states.dtype)
+    return F.scaled_dot_product_attention(query_states, keys.to(query_states.dtype), values.to(query_states.dtype), attn_mask=mask,
+                                          enable_gqa=group > 1)
+
+
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *,
                      cu_seqlens: torch.Tensor | None = None, seq_starts: torch.Tensor | None = None,
                      seq_ends: torch.Tensor | None = None, scale: float | None = None,
@@ -477,6 +578,8 @@ def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, k
                                  scaling: float | None = None, is_causal: bool | None = None, **kwargs):
     """HF attention-interface function: returns ([B, Sq, Hq, D], None)."""
     layer = getattr(module, "_tq_cache_layer", None)
+    if getattr(layer, "shares_prompts", False):
+        return shared_prefix_attention(query, layer, attention_mask).transpose(1, 2).contiguous(), None
     if layer is None or _hands_over_all(layer, query, key, attention_mask):
         return _sdpa_fallback(module, query, key, value, attention_mask, scaling)
     if layer.packed_seq_length() == 0:  # the tokens before are dense: attended to as a norm-guarded layer's are
@@ -524,6 +627,12 @@ def turboquant_prompt_forward(module: torch.nn.Module, query: torch.Tensor, key:
     cu, cu_k = kwargs.get("cu_seq_lens_q"), kwargs.get("cu_seq_lens_k")
     S = query.shape[-2]
     layer = getattr(module, "_tq_cache_layer", None)
+    if getattr(layer, "shares_prompts", False):
+        if cu is not None and cu.numel() > 2 and attention_mask is None and S > 1:
+            raise ValueError("packed sequences, but the cache layer holds tokens before them")
+        if not causal and attention_mask is None and S > 1:  # no mask means causal there
+            attention_mask = torch.ones(S, layer.get_seq_length(), dtype=torch.bool, device=query.device).expand(query.shape[0], 1, -1, -1)
+        return turboquant_attention_forward(module, query, key, value, attention_mask, dropout, scaling, is_causal, **kwargs)
     if (attention_mask is None and causal and not dropout and S > 1 and query.shape[-1] == K.HEAD_DIM
             and key.shape == value.shape and key.shape[-2:] == query.shape[-2:] and query.is_cuda
             and query.dtype in (torch.bfloat16, torch.float16) and key.dtype == value.dtype == query.dtype

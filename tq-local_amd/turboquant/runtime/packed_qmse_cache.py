@@ -38,6 +38,9 @@ from turboquant.runtime.params import LayerCodecs, SplitCodecs, layer_codecs, sp
 #: growth step of the capacity buffers when decode-append runs out of slots
 DEFAULT_RESERVE_TOKENS = 256
 
+#: bytes of key rows decoded at once for their bounds: fills the device, and stays in the last-level cache
+_BOUNDS_BYTES = 64 << 20
+
 
 @dataclass
 class PackedTensorMSE:
@@ -215,6 +218,33 @@ def _split_spec(sc: SplitCodecs) -> dict[str, tuple[tuple, torch.dtype] | None]:
     return spec
 
 
+class _BlockBounds:
+    """Bounds of the keys of a layer's blocks of 64 tokens, the first ``count`` of them known."""
+
+    def __init__(self, B: int, H: int, cap: int, D: int, device: torch.device):
+        self.lohi = torch.empty(B, H, cap, 2, D, dtype=torch.int8, device=device)
+        self.step = torch.empty(B, H, cap, dtype=torch.float32, device=device)
+        self.count = 0
+
+    def take(self, rows: torch.Tensor | None, cap: int) -> None:
+        """These batch rows of it, with room for ``cap`` blocks."""
+        self.lohi, self.step = K.gather_tokens([self.lohi, self.step], tokens=self.count, rows=rows, capacity=cap)
+
+
+@dataclass(frozen=True)
+class BlockChoice:
+    """How many blocks of 64 tokens a step attends to for each KV head, the first ``sink`` and the last ``recent`` among them."""
+
+    keep: int
+    sink: int = 1
+    recent: int = 2
+
+    def __post_init__(self):
+        if self.sink < 0 or self.recent < 1 or not self.sink + self.recent <= self.keep <= K.MAX_BLOCKS:
+            raise ValueError(f"{self.keep} blocks (at most {K.MAX_BLOCKS}) with {self.sink} first and {self.recent} last ones "
+                             "(the last is always attended to)")
+
+
 class PackedMSELayer(CacheLayerMixin):
     """One decoder layer's TurboQuant-compressed KV cache."""
 
@@ -243,6 +273,8 @@ class PackedMSELayer(CacheLayerMixin):
         self._lazy_update = False
         self._dense_buf: tuple[torch.Tensor, torch.Tensor] | None = None  # capacity buffers [B, H, cap, D]
         self._dense_len = 0
+        self._choice: BlockChoice | None = None  # decode steps attend to chosen blocks of the packed tokens
+        self._bounds: _BlockBounds | None = None  # of the whole blocks of packed tokens, as far as they were asked for
 
     # ------------------------------------------------------------- parameters
     def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
@@ -620,6 +652,49 @@ class PackedMSELayer(CacheLayerMixin):
         dense = 0 if self._dense_keys is None else int(self._dense_keys.shape[-2])
         return self.packed_seq_length() + dense
 
+    # ------------------------------------------------------ blocks chosen from
+    def attend_blocks(self, keep: int | None, sink: int = 1, recent: int = 2) -> None:
+        """From now on a decode step of the attention backend attends to ``keep`` blocks of 64 packed tokens for each KV head
+        instead of to all of them: the first ``sink``, the last ``recent`` and those that its query may give the
+        largest logits (``kernels.select_blocks``); dense tokens are attended to beside them.  ``None``: to all tokens again.
+        Steps of several tokens, layers split in channel groups and groups of more than 8 query heads attend to everything."""
+        self._choice = None if keep is None else BlockChoice(int(keep), int(sink), int(recent))
+
+    def block_bounds(self) -> tuple[torch.Tensor, torch.Tensor, int]:
+        """Bounds of the keys of the whole blocks of packed tokens, as decoded: (lohi, step, blocks), see
+        ``kernels.block_bounds``.  Blocks that have become whole since the last call are decoded for it."""
+        if self._store is None or self._split is not None:
+            raise ValueError("block bounds need a one-group layer with packed tokens")
+        B, H, D = self._shape
+        n, b = self._store.length // K.BLOCK_TOKENS, self._bounds
+        if b is None:
+            b = self._bounds = _BlockBounds(B, H, n + max(1, self.reserve_tokens // K.BLOCK_TOKENS), D, self._store.device)
+        elif n > b.lohi.shape[2]:
+            b.take(None, max(n + self.reserve_tokens // K.BLOCK_TOKENS, 2 * b.lohi.shape[2]))
+        most = max(1, _BOUNDS_BYTES // (B * H * D * 2 * K.BLOCK_TOKENS))  # blocks decoded at once
+        for first in range(b.count, n, most):
+            to = min(first + most, n)
+            K.block_bounds(self._key_rows(first * K.BLOCK_TOKENS, to * K.BLOCK_TOKENS), b.lohi, b.step, first=first)
+            b.count = to
+        return b.lohi, b.step, b.count
+
+    def choose_blocks(self, query: torch.Tensor, choice: BlockChoice, seq_starts: torch.Tensor | None = None,
+                      seq_lens: torch.Tensor | None = None) -> torch.Tensor | None:
+        """The blocks of packed tokens that a step with ``query`` [B, Hq, 1, D] attends to, int32 [B, H, keep]; None where there
+        are no more than ``choice.keep`` (or more than are chosen from)."""
+        n = self.packed_seq_length()
+        blocks = -(-n // K.BLOCK_TOKENS)
+        if blocks <= choice.keep or blocks > K.MAX_SCORED:
+            return None
+        lohi, step, known = self.block_bounds()
+        return K.select_blocks(query, lohi, step, n_tokens=n, keep=choice.keep, sink=choice.sink, recent=choice.recent,
+                               n_blocks=known, seq_starts=seq_starts, seq_lens=seq_lens)
+
+    def _forget_bounds(self, tokens: int) -> None:
+        """Packed tokens from ``tokens`` on have changed."""
+        if self._bounds is not None:
+            self._bounds.count = min(self._bounds.count, tokens // K.BLOCK_TOKENS)
+
     # ------------------------------------------- rows and tokens chosen and moved
     def _batch(self) -> int | None:
         """Batch rows held (None: nothing is)."""
@@ -631,6 +706,8 @@ class PackedMSELayer(CacheLayerMixin):
         if self._store is not None:
             self._store.take(rows=rows)
             self._shape = (self._store.B, *self._shape[1:])
+            if self._bounds is not None:
+                self._bounds.take(rows, self._bounds.lohi.shape[2])
         if self._dense_buf is not None:
             dense = list(self._dense_buf)
             self._dense_buf = tuple(K.gather_tokens(dense, tokens=self._dense_len, rows=rows, capacity=dense[0].shape[2]))
@@ -677,6 +754,7 @@ class PackedMSELayer(CacheLayerMixin):
         self._dense_len -= dense
         if drop > dense:
             self._store.length -= drop - dense
+            self._forget_bounds(self._store.length)
 
     def keep_tokens(self, index: torch.Tensor, tokens: int | None = None) -> None:
         """Of the last ``tokens`` tokens (all without) only those of ``index`` [n], [B, n] or [B, H, n], counted from the
@@ -713,6 +791,7 @@ class PackedMSELayer(CacheLayerMixin):
             self._dense_len = first + n
         else:
             self._store.length = first + n
+            self._forget_bounds(first)
 
     def get_max_length(self) -> int:
         return -1
