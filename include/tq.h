@@ -465,12 +465,16 @@ int tq_block_bounds(const uint16_t* k, int batch, int heads, int64_t tokens, int
  *   n_blocks blocks with bounds (<= cap); a later one that is neither of the first nor of the last comes behind all scored ones
  *   seq_starts, seq_lens  int32 [batch] (device, nullable): row b's range is the slots [start, len) of [0, n_tokens)
  *   out      int32 [batch][kv_heads][keep], ascending; -1 in the places left where there are fewer blocks
- * sink + recent <= keep <= TQ_MAX_BLOCKS.  TQ_ERR_UNSUPPORTED beyond TQ_MAX_SCORED * 64 tokens.
+ *   workspace  device scratch of tq_select_blocks_workspace_bytes() (NULL where that is 0), used during the call only
+ * sink + recent <= keep <= TQ_MAX_BLOCKS.  TQ_ERR_UNSUPPORTED beyond TQ_MAX_SCORED * 64 tokens, and with a workspace beyond 65535 KV heads
+ * of the batch.
  */
 #define TQ_MAX_SCORED 32768
+size_t tq_select_blocks_workspace_bytes(int batch, int kv_heads, int64_t n_tokens);
 int tq_select_blocks(const void* q, int q_type, int batch, int q_heads, int kv_heads, int dim, int64_t q_sb, int64_t q_sh,
                      const int8_t* lohi, const float* step, int64_t cap, int64_t n_blocks, int64_t n_tokens,
-                     const int32_t* seq_starts, const int32_t* seq_lens, int keep, int sink, int recent, int32_t* out, void* stream);
+                     const int32_t* seq_starts, const int32_t* seq_lens, int keep, int sink, int recent, int32_t* out,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * tq_block_attention: tq_decode_attention over the named blocks only.  blocks int32 [batch][kv_heads][keep] (device): block numbers in any

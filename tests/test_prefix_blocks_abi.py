@@ -69,7 +69,7 @@ def test_block_bounds_rejects_on_host(status, change):
 
 
 SELECT = dict(q=FAKE, q_type=0, batch=1, q_heads=8, kv_heads=2, dim=128, q_sb=1024, q_sh=128, lohi=FAKE, step=FAKE, cap=40, blocks=40,
-              n=2500, starts=None, lens=None, keep=8, sink=1, recent=2, out=FAKE, stream=None)
+              n=2500, starts=None, lens=None, keep=8, sink=1, recent=2, out=FAKE, ws=None, wsb=0, stream=None)
 
 
 @pytest.mark.parametrize("status,change", [
@@ -77,7 +77,8 @@ SELECT = dict(q=FAKE, q_type=0, batch=1, q_heads=8, kv_heads=2, dim=128, q_sb=10
     (INVALID, dict(q_heads=9)), (INVALID, dict(blocks=41)), (INVALID, dict(blocks=-1)), (INVALID, dict(n=-1)), (INVALID, dict(keep=0)),
     (INVALID, dict(sink=-1)), (INVALID, dict(recent=-1)), (INVALID, dict(sink=7)), (INVALID, dict(sink=1 << 30, recent=1 << 30)),
     (UNSUPPORTED, dict(dim=64)), (UNSUPPORTED, dict(keep=4097)), (UNSUPPORTED, dict(n=32768 * 64 + 1)), (UNSUPPORTED, dict(lohi=ODD)),
-    (UNSUPPORTED, dict(batch=1 << 30, kv_heads=8))])
+    (UNSUPPORTED, dict(batch=1 << 30, kv_heads=8)), (WORKSPACE, dict(n=100000)), (WORKSPACE, dict(n=100000, ws=FAKE, wsb=100)),
+    (WORKSPACE, dict(n=100000, ws=ODD, wsb=1 << 30)), (UNSUPPORTED, dict(n=100000, batch=1 << 16, ws=FAKE, wsb=1 << 60))])
 def test_select_blocks_rejects_on_host(status, change):
     assert _lib.load().tq_select_blocks(*dict(SELECT, **change).values()) == status
 
@@ -98,6 +99,12 @@ BLOCKS = dict(q=FAKE, batch=1, q_heads=8, kv_heads=2, dim=128, blocks=FAKE, keep
     (UNSUPPORTED, dict(s=ODD)), (WORKSPACE, dict(ws=None)), (WORKSPACE, dict(ws=ODD)), (WORKSPACE, dict(wsb=100))])
 def test_block_attention_rejects_on_host(status, change):
     assert _lib.load().tq_block_attention(*dict(BLOCKS, **change).values()) == status
+
+
+def test_select_workspace_is_host_arithmetic():
+    size = _lib.load().tq_select_blocks_workspace_bytes
+    assert size(1, 2, 0) == size(1, 2, 1000) == 0 < size(1, 2, 100000) < size(2, 2, 100000)
+    assert size(0, 2, 100000) == size(1, 0, 100000) == size(1, 2, -1) == size(1, 2, 1 << 40) == 0
 
 
 def test_block_workspace_is_host_arithmetic():

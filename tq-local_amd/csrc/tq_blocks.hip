@@ -124,9 +124,21 @@ struct SelectArgs {
     int32_t* out;
 };
 
-constexpr int ST = 1024, SW = ST / 64;  // threads and waves of a workgroup
-constexpr int TILE = 16;                // blocks of a matrix instruction
+constexpr int ST = 512, SW = ST / 64;  // threads and waves of a workgroup
+constexpr int TILE = 16;               // blocks of a matrix instruction
+constexpr int AHEAD = 4;               // tiles of a wave whose bounds are on their way together
 constexpr uint32_t ALWAYS = 0xFFFFFFFFu;
+
+// The blocks of a row's range: [lo, lo + n).
+struct BlockRange {
+    int lo, n;
+};
+__device__ __forceinline__ BlockRange range_of(const SelectArgs& a, int b) {
+    const int64_t len = a.lens ? std::min(std::max<int64_t>(a.lens[b], 0), a.n_tokens) : a.n_tokens;
+    const int64_t start = a.starts ? std::min(std::max<int64_t>(a.starts[b], 0), len) : 0;
+    const int lo = (int)(start / BT);
+    return {lo, len > start ? (int)((len + BT - 1) / BT) - lo : 0};
+}
 
 // fp32 as an integer whose order is its
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -134,162 +146,233 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return b ^ (b & 0x80000000u ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-// Eight elements of a query row as fp32.
-__device__ __forceinline__ void load_query8(const SelectArgs& a, int64_t at, float* x) {
+// Four elements of a query row as fp32.
+__device__ __forceinline__ void load_query4(const SelectArgs& a, int64_t at, float* x) {
     if (a.q_type == 1) {
-        __builtin_memcpy(x, static_cast<const float*>(a.q) + at, 32);
+        __builtin_memcpy(x, static_cast<const float*>(a.q) + at, 16);
         return;
     }
-    uint32_t w[4];
-    __builtin_memcpy(w, static_cast<const uint16_t*>(a.q) + at, 16);
+    uint32_t w[2];
+    __builtin_memcpy(w, static_cast<const uint16_t*>(a.q) + at, 8);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
         x[2 * i] = a.q_type == 2 ? tq::f16_to_f32(w[i] & 0xFFFFu) : tq::bf16_to_f32(w[i] & 0xFFFFu);
         x[2 * i + 1] = a.q_type == 2 ? tq::f16_to_f32(w[i] >> 16) : tq::bf16_to_f32(w[i] >> 16);
     }
 }
+// The largest of their absolute values, as bits; NaN counts as 0.
+__device__ __forceinline__ uint32_t largest4(const float* v) {
+    uint32_t most = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t bits = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+        most = std::max(most, bits > 0x7F800000u ? 0u : bits);
+    }
+    return most;
+}
 
-__global__ __launch_bounds__(ST) void select_kernel(SelectArgs a) {
+// Scores of the blocks [TILE t, TILE t + TILE) below `known` of a range, for the tiles t0 <= t < tiles, by a workgroup: keys[j] of block j, in
+// the order of the scores.  Ends with a barrier.
+__device__ __forceinline__ void score_blocks(const SelectArgs& a, int b, int kvh, int lo, int known, int t0, int tiles, uint32_t* keys) {
+    __shared__ uint32_t s_most[SW];
+    // heads in whole numbers, their negative and their positive parts: 16-byte pieces, swizzled by the head
+    __shared__ __align__(16) uint32_t s_q[2][16][D / 4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // ---- the queries are asked for, then the first tiles' bounds.  A thread has four dims of one of 16 heads; heads past the last are
+    // earlier ones again, which does not change a maximum
+    const int64_t q0 = b * a.q_sb + (int64_t)kvh * a.group * a.q_sh;
+    const int head = threadIdx.x >> 5, dim = 4 * (threadIdx.x & 31), head_tiles = (a.group + 15) / 16;
+    static_assert(ST == 16 * 32, "a thread has four dims of one of 16 heads");
+    float x[4];
+    auto load_head = [&](int h, float* v) { load_query4(a, q0 + h % a.group * a.q_sh + dim, v); };
+    load_head(head, x);
+
+    // bounds: lane (block r of the tile, g) has bytes 64 i + 16 g + (0..15) of its 256, i = 0..3
+    const int r = lane & 15, g = lane >> 4;
+    const int64_t base = ((int64_t)b * a.kv_heads + kvh) * a.cap + lo;
+    i32x4 w[AHEAD][4];
+    float step[AHEAD];
+    auto load = [&](int tile, int slot) {
+        const int64_t at = base + std::min(tile * TILE + r, known - 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[slot][i] = *reinterpret_cast<const i32x4*>(a.lohi + at * (2 * D) + 64 * i + 16 * g);
+        step[slot] = a.step[at];
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (t0 + wave + i * SW < tiles) load(t0 + wave + i * SW, i);
+
+    // ---- the heads' common step
+    uint32_t most = largest4(x);
+    for (int h = 16; h < a.group; h += 16) {
+        float y[4];
+        load_head(h + head, y);
+        most = std::max(most, largest4(y));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) most = std::max(most, (uint32_t)__shfl_xor((int)most, d));
+    if (lane == 0) s_most[wave] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < SW; ++i) most = std::max(most, s_most[i]);
+    const float down = power_of_two(-step_exponent(most));
+
+    for (int ht = 0; ht < head_tiles; ++ht) {
+        if (ht) {
+            load_head(16 * ht + head, x);
+            __syncthreads();
+        }
+        uint32_t neg = 0u, pos = 0u;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float y = x[e] == x[e] ? x[e] : 0.0f;
+            const int z = (int)fminf(fmaxf(__builtin_rintf(y * down), -127.0f), 127.0f);
+            neg |= ((uint32_t)std::min(z, 0) & 0xFFu) << (8 * e), pos |= (uint32_t)std::max(z, 0) << (8 * e);
+        }
+        const int at = (((dim >> 4) ^ (head & 7)) << 2) + (dim >> 2 & 3);
+        s_q[0][head][at] = neg, s_q[1][head][at] = pos;
+        __syncthreads();
+        // lane (head r, g): dims 64 i + 16 g + (0..15), i = 0, 1
+        i32x4 q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = *reinterpret_cast<const i32x4*>(&s_q[i >> 1][r][((4 * (i & 1) + g) ^ (r & 7)) << 2]);
+        for (int t = t0 + wave; t < tiles; t += AHEAD * SW) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int tile = t + i * SW, next = tile + AHEAD * SW;
+                if (tile < tiles) {
+                    i32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(q[k], w[i][k], acc, 0, 0, 0);
+                    int u = std::max(std::max(acc[0], acc[1]), std::max(acc[2], acc[3]));
+                    u = std::max(u, __shfl_xor(u, 16));
+                    u = std::max(u, __shfl_xor(u, 32));
+                    const int j = tile * TILE + r;
+                    if (g == 0 && j < known) {
+                        const uint32_t key = order_of((float)u * step[i]);
+                        keys[j] = ht ? std::max(keys[j], key) : key;
+                    }
+                }
+                // the next tiles, and the first ones again for the next heads
+                if (next < tiles) load(next, i);
+                else if (ht + 1 < head_tiles && t0 + wave + i * SW < tiles) load(t0 + wave + i * SW, i);
+            }
+        }
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ int tiles_of(int known) { return known > 0 ? (known + TILE - 1) / TILE : 0; }
+
+// `per` tiles of a KV head's range to a workgroup, into keys [KV head of the batch][most].
+__global__ __launch_bounds__(ST) void score_kernel(SelectArgs a, uint32_t* keys, int most, int per) {
+    const int group = blockIdx.y, b = group / a.kv_heads, kvh = group - b * a.kv_heads;
+    const BlockRange range = range_of(a, b);
+    const int known = (int)std::min<int64_t>(a.n_blocks - range.lo, range.n), tiles = tiles_of(known), t0 = blockIdx.x * per;
+    if (range.n <= a.keep || t0 >= tiles) return;
+    score_blocks(a, b, kvh, range.lo, known, t0, std::min(t0 + per, tiles), keys + (int64_t)group * most);
+}
+
+// A KV head's choice.  FUSED: its scores too; else they are in `keys`.
+template <bool FUSED>
+__global__ __launch_bounds__(ST) void select_kernel(SelectArgs a, const uint32_t* keys, int most) {
     extern __shared__ uint32_t s_key[];  // a block's score, by its number in the range
-    __shared__ uint32_t s_hist[256];
-    __shared__ int s_digit, s_above;
+    __shared__ __align__(16) uint32_t s_hist[4][256];
     __shared__ int2 s_wave[SW];
+    __shared__ uint2 s_bits[SW];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int b = blockIdx.x / a.kv_heads, kvh = blockIdx.x - b * a.kv_heads;
-    const int64_t len = a.lens ? std::min(std::max<int64_t>(a.lens[b], 0), a.n_tokens) : a.n_tokens;
-    const int64_t start = a.starts ? std::min(std::max<int64_t>(a.starts[b], 0), len) : 0;
-    const int lo = (int)(start / BT), n = len > start ? (int)((len + BT - 1) / BT) - lo : 0;  // the range's blocks
+    const BlockRange range = range_of(a, b);
+    const int lo = range.lo, n = range.n, known = (int)std::min<int64_t>(a.n_blocks - lo, n);
     int32_t* const out = a.out + (int64_t)blockIdx.x * a.keep;
     if (n <= a.keep) {  // all of them
         for (int i = threadIdx.x; i < a.keep; i += ST) out[i] = i < n ? lo + i : -1;
         return;
     }
+    for (int i = threadIdx.x; i < 4 * 256; i += ST) (&s_hist[0][0])[i] = 0u;
+    if (FUSED) score_blocks(a, b, kvh, lo, known, 0, tiles_of(known), s_key);
 
-    // ---- the queries: lane (r = lane % 16, g = lane / 16) has head r's dims 64 i + 16 g + (0..15), i = 0, 1, as its A operands; heads
-    // past the last are earlier ones again, which does not change a maximum
-    const int r = lane & 15, g = lane >> 4;
-    const int64_t q0 = b * a.q_sb + (int64_t)kvh * a.group * a.q_sh + 16 * g;
-    auto load = [&](int h, float* x) {
-        const int64_t at = q0 + (h % a.group) * a.q_sh;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) load_query8(a, at + 64 * (i >> 1) + 8 * (i & 1), x + 8 * i);
-    };
-    const int head_tiles = (a.group + 15) / 16;
-    uint32_t most = 0u;
-    float x[32];
-    for (int ht = head_tiles - 1; ht >= 0; --ht) {
-        load(16 * ht + r, x);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const uint32_t bits = __float_as_uint(x[i]) & 0x7FFFFFFFu;
-            most = std::max(most, bits > 0x7F800000u ? 0u : bits);  // NaN counts as 0
-        }
+    // ---- in between the first and the last blocks, which are always chosen, the choice is by score; blocks without come last.  What the
+    // keys there have in common needs no looking at
+    const int first = a.sink, last = n - a.recent;
+    uint32_t all = 0xFFFFFFFFu, any = 0u;
+    for (int j = threadIdx.x; j < n; j += ST) {
+        uint32_t key = 0u;
+        if (j < known) key = FUSED ? s_key[j] : keys[(int64_t)blockIdx.x * most + j];
+        if (j < first || j >= last) key = ALWAYS;
+        else all &= key, any |= key;
+        s_key[j] = key;
     }
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = std::max(most, (uint32_t)__shfl_xor((int)most, d));
-    const float down = power_of_two(-step_exponent(most));
-    i32x4 neg[2], pos[2];
-    auto operands = [&]() {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t n4 = 0u, p4 = 0u;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float v = x[16 * i + 4 * w + e], y = v == v ? v : 0.0f;
-                    const int z = (int)fminf(fmaxf(__builtin_rintf(y * down), -127.0f), 127.0f);
-                    n4 |= ((uint32_t)std::min(z, 0) & 0xFFu) << (8 * e), p4 |= (uint32_t)std::max(z, 0) << (8 * e);
-                }
-                neg[i][w] = (int)n4, pos[i][w] = (int)p4;
-            }
-    };
-    operands();  // of the first 16 heads
-
-    // ---- scores: lane (block r of the tile, g) has bytes 64 i + 16 g + (0..15) of its 256
-    const int first = a.sink, last = n - a.recent;  // in between the choice is by score
-    const int64_t base = (int64_t)blockIdx.x * a.cap + lo;
-    for (int ht = 0; ht < head_tiles; ++ht) {
-        if (ht) load(16 * ht + r, x), operands();
-        for (int t0 = wave * TILE; t0 < n; t0 += SW * TILE) {
-            const int j = t0 + r, known = std::min(j, (int)std::min<int64_t>(a.n_blocks - 1 - lo, n - 1));
-            uint32_t key = 0u;
-            if (known >= 0) {
-                const int8_t* const p = a.lohi + (base + known) * (2 * D) + 16 * g;
-                i32x4 w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const i32x4*>(p + 64 * i);
-                const float step = a.step[base + known];
-                i32x4 acc = {0, 0, 0, 0};
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg[0], w[0], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(neg[1], w[1], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos[0], w[2], acc, 0, 0, 0);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(pos[1], w[3], acc, 0, 0, 0);
-                int u = std::max(std::max(acc[0], acc[1]), std::max(acc[2], acc[3]));
-                u = std::max(u, __shfl_xor(u, 16));
-                u = std::max(u, __shfl_xor(u, 32));
-                key = known == j ? order_of((float)u * step) : 0u;
-            }
-            if (j < first || j >= last) key = ALWAYS;
-            if (g == 0 && j < n) s_key[j] = ht ? std::max(s_key[j], key) : key;
-        }
-    }
+    for (int d = 1; d < 64; d <<= 1) all &= (uint32_t)__shfl_xor((int)all, d), any |= (uint32_t)__shfl_xor((int)any, d);
+    if (lane == 0) s_bits[wave] = make_uint2(all, any);
     __syncthreads();
-
-    // ---- the keep-th largest, eight bits at a time
-    uint32_t found = 0u, mask = 0u;
-    int rest = a.keep;  // of the keys that share the bits found, the `rest` largest are chosen
-#pragma unroll 1
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (threadIdx.x < 256) s_hist[threadIdx.x] = 0u;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += ST) {
-            const uint32_t key = s_key[i];
-            if ((key & mask) == found) atomicAdd(&s_hist[(key >> shift) & 255u], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {  // lane l: the four digits from 252 - 4 l on
-            uint32_t c[4], sum = 0u;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = s_hist[255 - 4 * lane - i], sum += c[i];
-            uint32_t up = sum;
+    for (int i = 0; i < SW; ++i) all &= s_bits[i].x, any |= s_bits[i].y;
+    int rest = a.keep - (n - (last - first));  // of the keys that share the bits found, the `rest` largest are chosen
+    int shift = 32 - __builtin_clz((all ^ any) | 1u);  // from the highest bit in which two differ, eight at a time
+    uint32_t mask = shift < 32 ? ~0u << shift : 0u, found = all & mask;
+    if (rest > 0) {
+#pragma unroll 1
+        for (int pass = 0; shift > 0; ++pass) {
+            const int width = std::min(shift, 8);
+            shift -= width;
+            uint32_t* const hist = s_hist[pass];
+            const uint32_t digits = (1u << width) - 1;
+            for (int i = first + threadIdx.x; i < last; i += ST) {
+                const uint32_t key = s_key[i];
+                if ((key & mask) == found) atomicAdd(&hist[(key >> shift) & digits], 1u);
+            }
+            __syncthreads();
+            // every wave for itself; lane l: the four digits from 252 - 4 l on
+            const uint4 c4 = *reinterpret_cast<const uint4*>(&hist[252 - 4 * lane]);
+            const int c[4] = {(int)c4.w, (int)c4.z, (int)c4.y, (int)c4.x}, sum = c[0] + c[1] + c[2] + c[3];
+            int up = sum;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t y = (uint32_t)__shfl_up((int)up, d);
+                const int y = __shfl_up(up, d);
                 if (lane >= d) up += y;
             }
-            int above = (int)(up - sum);  // keys with larger digits
+            int above = up - sum, digit = -1, larger = 0, with = 0;  // keys with larger digits, and with this one
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if (above < rest && above + (int)c[i] >= rest) s_digit = 255 - 4 * lane - i, s_above = above;
-                above += (int)c[i];
+                if (above < rest && above + c[i] >= rest) digit = 255 - 4 * lane - i, larger = above, with = c[i];
+                above += c[i];
             }
+            const int who = __builtin_ctzll(__ballot(digit >= 0));  // one lane has it: there are `rest` keys at least
+            found |= (uint32_t)__builtin_amdgcn_readlane(digit, who) << shift, mask |= digits << shift;
+            rest -= __builtin_amdgcn_readlane(larger, who);
+            if (__builtin_amdgcn_readlane(with, who) == rest) break;  // all of them
         }
-        __syncthreads();
-        found |= (uint32_t)s_digit << shift, mask |= 255u << shift, rest -= s_above;
+    } else {
+        mask = found = 0xFFFFFFFFu;  // none
     }
 
     // ---- what is above it, and the first `rest` of those equal to it, in order
     int before = 0, equal = 0;  // so far
     for (int i0 = 0; i0 < n; i0 += ST) {
         const int i = i0 + threadIdx.x;
-        const uint32_t key = i < n ? s_key[i] : 0u;
-        const bool is_above = i < n && key > found, is_equal = i < n && key == found;
+        const bool always = i < first || i >= last;
+        const uint32_t key = i < n ? s_key[i] & mask : 0u;
+        const bool is_above = i < n && (always || key > found), is_equal = i < n && !always && key == found;
         const uint64_t above = __ballot(is_above), same = __ballot(is_equal), below = (1ull << lane) - 1;
-        __syncthreads();
+        if (i0) __syncthreads();
         if (lane == 0) s_wave[wave] = make_int2(__popcll(above), __popcll(same));
         __syncthreads();
         int a0 = before, e0 = equal;
 #pragma unroll
-        for (int w = 0; w < SW; ++w) {
-            const int2 c = s_wave[w];
-            if (w < wave) a0 += c.x, e0 += c.y;
+        for (int v = 0; v < SW; ++v) {
+            const int2 c = s_wave[v];
+            if (v < wave) a0 += c.x, e0 += c.y;
             before += c.x, equal += c.y;
         }
         a0 += __popcll(above & below), e0 += __popcll(same & below);
-        if (is_above || (is_equal && e0 < rest)) out[a0 + std::min(e0, rest)] = lo + i;
+        if (is_above || (is_equal && e0 < rest)) out[a0 + std::min(e0, std::max(rest, 0))] = lo + i;
     }
 }
+
+// One workgroup for a KV head's whole choice up to here, else its scores in a launch of their own, spread over the CUs: a workgroup takes its
+// bounds at about 36 GB/s.
+constexpr int FUSED_BLOCKS = 512;
 
 }  // namespace
 
@@ -308,22 +391,43 @@ extern "C" int tq_block_bounds(const uint16_t* k, int batch, int heads, int64_t 
     return TQ_OK;
 }
 
+extern "C" size_t tq_select_blocks_workspace_bytes(int batch, int kv_heads, int64_t n_tokens) {
+    if (batch < 1 || kv_heads < 1 || n_tokens < 0 || n_tokens > (int64_t)TQ_MAX_SCORED * BT) return 0;
+    const int64_t most = (n_tokens + BT - 1) / BT;
+    return most <= FUSED_BLOCKS ? 0 : (size_t)batch * kv_heads * most * 4;
+}
+
 extern "C" int tq_select_blocks(const void* q, int q_type, int batch, int q_heads, int kv_heads, int dim, int64_t q_sb, int64_t q_sh,
                                 const int8_t* lohi, const float* step, int64_t cap, int64_t n_blocks, int64_t n_tokens,
                                 const int32_t* seq_starts, const int32_t* seq_lens, int keep, int sink, int recent, int32_t* out,
-                                void* stream) {
+                                void* workspace, size_t workspace_bytes, void* stream) {
     if (!q || q_type < 0 || q_type > 2 || batch < 1 || q_heads < 1 || kv_heads < 1 || q_heads % kv_heads || n_blocks < 0 ||
         n_blocks > cap || n_tokens < 0 || (n_blocks > 0 && (!lohi || !step)) || keep < 1 || sink < 0 || recent < 0 || sink > keep ||
         recent > keep - sink || !out)
         return TQ_ERR_INVALID_ARGUMENT;
+    const int64_t groups = (int64_t)batch * kv_heads;
     if (dim != D || keep > TQ_MAX_BLOCKS || n_tokens > (int64_t)TQ_MAX_SCORED * BT || (lohi && !aligned16(lohi)) ||
-        (int64_t)batch * kv_heads >= (int64_t)1 << 31)
+        groups >= (int64_t)1 << 31)
         return TQ_ERR_UNSUPPORTED;
+    const size_t need = tq_select_blocks_workspace_bytes(batch, kv_heads, n_tokens);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return TQ_ERR_WORKSPACE;
     const SelectArgs a{q, q_type, q_heads, kv_heads, q_heads / kv_heads, q_sb, q_sh, lohi, step, cap, n_blocks, n_tokens,
                        seq_starts, seq_lens, keep, sink, recent, out};
-    const int64_t most = (n_tokens + BT - 1) / BT;  // blocks of a range
-    hipLaunchKernelGGL(select_kernel, dim3((unsigned)(batch * kv_heads)), dim3(ST), (size_t)std::max<int64_t>(most, 1) * 4,
-                       static_cast<hipStream_t>(stream), a);
+    const int most = (int)((n_tokens + BT - 1) / BT);  // blocks of a range
+    const size_t lds = (size_t)std::max(most, 1) * 4;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (!need) {
+        hipLaunchKernelGGL(select_kernel<true>, dim3((unsigned)groups), dim3(ST), lds, s, a, nullptr, most);
+        TQ_CHECK_LAUNCH();
+        return TQ_OK;
+    }
+    if (groups > 65535) return TQ_ERR_UNSUPPORTED;
+    uint32_t* const keys = static_cast<uint32_t*>(workspace);
+    const int64_t tiles = (most + TILE - 1) / TILE;
+    const int per = (int)((tiles * groups + 256 * SW - 1) / (256 * SW) * SW);
+    hipLaunchKernelGGL(score_kernel, dim3((unsigned)((tiles + per - 1) / per), (unsigned)groups), dim3(ST), 0, s, a, keys, most, per);
+    TQ_CHECK_LAUNCH();
+    hipLaunchKernelGGL(select_kernel<false>, dim3((unsigned)groups), dim3(ST), lds, s, a, keys, most);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
 }

@@ -793,10 +793,6 @@ def _pointers(tensors) -> array:
     return array("Q", [t.data_ptr() for t in tensors])
 
 
-def _pointers_or_0(tensors) -> array:
-    return array("Q", [0 if t is None else t.data_ptr() for t in tensors])
-
-
 #: up to here a call's new buffers are parts of one allocation: twelve of their own are 18 us of host time, the parts 12 us of
 #: a call whose kernel takes 15.  A kept view holds on to the block
 _ONE_BLOCK_BYTES = 64 << 20
@@ -886,28 +882,28 @@ def keep_tokens(buffers: list[torch.Tensor], index: torch.Tensor, *, first: int,
                    first, tokens, at_index, sb, sh, n, stream)
 
 
+_ARRAYS = ("k_codes", "k_norms", "k_signs", "k_rnorms", "v_codes", "v_norms")
+
+
 def _packed_arrays(name: str, cache: dict, batch: int | None, key: CodecParams, value: CodecParams, has_qjl: bool, on: int):
-    """The arrays k_codes, k_norms, k_signs, k_rnorms, v_codes, v_norms of a packed cache, looked over, and its [B, Hkv, cap]."""
+    """Addresses of a packed cache's arrays (0 for those that Q_mse keys do not have), looked over, and its [B, Hkv, cap]."""
     sh = cache["k_codes"].shape
     if len(sh) != 4 or (batch is not None and sh[0] != batch):
         raise ValueError(f"{name}: k_codes {tuple(sh)} do not match a batch of {batch}")
-    sh, out = tuple(sh[:3]), []
-    for what, row in (("k_codes", 16 * key.bits), ("k_norms", 0), ("k_signs", HEAD_DIM // 8), ("k_rnorms", 0),
-                      ("v_codes", 16 * value.bits), ("v_norms", 0)):
+    sh, out = sh[:3], []
+    for what, row in zip(_ARRAYS, (16 * key.bits, 0, HEAD_DIM // 8, 0, 16 * value.bits, 0)):
         t = cache.get(what)
-        if what in ("k_signs", "k_rnorms"):
-            if (t is not None) != has_qjl:
-                raise ValueError(f"{name}: Q_prod keys need k_signs, k_rnorms and qjl")
-            if t is None:
-                out.append(None)
-                continue
-        want = sh + (row,) if row else sh
-        if (t.shape != want or t.dtype is not (torch.uint8 if row else torch.float16) or not t.is_contiguous()
-                or t.get_device() != on):
+        if t is None and not has_qjl and (what == "k_signs" or what == "k_rnorms"):
+            out.append(0)
+            continue
+        if t is None or (not has_qjl and (what == "k_signs" or what == "k_rnorms")):
+            raise ValueError(f"{name}: {what}: Q_prod keys come with k_signs, k_rnorms and qjl, Q_mse keys without")
+        if (t.shape != (sh + (row,) if row else sh) or t.dtype is not (torch.uint8 if row else torch.float16)
+                or t.get_device() != on or not t.is_contiguous()):
             _require_gpu(t)
-            raise ValueError(f"{name}: {what}: expected a contiguous tensor of {want} on device {on}, got {t.dtype} "
-                             f"{tuple(t.shape)} on {t.device}")
-        out.append(t)
+            raise ValueError(f"{name}: {what}: expected a contiguous tensor of {(*sh, row) if row else tuple(sh)} on device {on}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        out.append(t.data_ptr())
     return out, sh
 
 
@@ -919,15 +915,18 @@ def _check_codec(key: CodecParams, value: CodecParams, qjl: torch.Tensor | None,
             raise ValueError(f"{name}: expected {n} contiguous fp32 on device {on}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _one_token(name: str, q: torch.Tensor) -> torch.Tensor:
-    """A query of one token per sequence, [B, Hq, D] or [B, Hq, 1, D], as [B, Hq, D]."""
-    if q.dim() == 4 and q.shape[2] == 1:
-        q = q[:, :, 0]
-    if q.dim() != 3 or q.shape[-1] != HEAD_DIM:
-        raise ValueError(f"{name}: expected q [B, Hq, {HEAD_DIM}] or [B, Hq, 1, {HEAD_DIM}], got {tuple(q.shape)}")
+def _one_token(name: str, q: torch.Tensor):
+    """A query of one token per sequence, [B, Hq, D] or [B, Hq, 1, D], with contiguous rows: (q, B, Hq, strides of both)."""
+    sh, st = q.shape, q.stride()
+    n = len(sh)
+    if not (n == 3 or (n == 4 and sh[2] == 1)) or sh[-1] != HEAD_DIM:
+        raise ValueError(f"{name}: expected q [B, Hq, {HEAD_DIM}] or [B, Hq, 1, {HEAD_DIM}], got {tuple(sh)}")
     if q.dtype not in _QUERY_TYPES:
         raise ValueError(f"{name}: q must be bf16, fp16 or fp32, got {q.dtype}")
-    return q if q.stride(-1) == 1 else q.contiguous()
+    if st[-1] != 1:
+        q = q.contiguous()
+        st = q.stride()
+    return q, sh[0], sh[1], st[0], st[1]
 
 
 def _logit_scale(name: str, scale: float | None) -> float:
@@ -953,15 +952,14 @@ def prefix_attention(q: torch.Tensor, prefix: dict, own: dict | None = None, *, 
     ``own_lens`` int [B]: a sequence's own tokens are the slots [0, len) of its row.  Returns [B, Hq, D] in q's dtype, then fp32 with
     ``want_f32``, then the fp32 log-sum-exp [B, Hq] of the scaled logits with ``want_lse``.
     """
-    q = _one_token("prefix_attention", q)
+    q, B, Hq, q_sb, q_sh = _one_token("prefix_attention", q)
     _no_gradient("prefix_attention", q)
     _not_traced("prefix_attention")
     _require_gpu(q)
-    dev, on = q.device, q.get_device()
-    B, Hq, D = q.shape
+    dev, on, dtype, D = q.device, q.get_device(), q.dtype, HEAD_DIM
     has_qjl = qjl is not None
     shared, (P, Hkv, cap) = _packed_arrays("prefix", prefix, None, key, value, has_qjl, on)
-    mine, own_cap = [None] * 6, 0
+    mine, own_cap = [0] * 6, 0
     if own is not None:
         mine, sh = _packed_arrays("own", own, B, key, value, has_qjl, on)
         own_cap = sh[2]
@@ -979,20 +977,19 @@ def prefix_attention(q: torch.Tensor, prefix: dict, own: dict | None = None, *, 
     prefix_lens = _int32_on(prefix_lens, dev, "prefix_lens", (P,))
     own_lens = _int32_on(own_lens, dev, "own_lens", (B,))
     s = _logit_scale("prefix_attention", scale)
-    f32 = torch.empty((B, Hq, D), dtype=torch.float32, device=dev) if want_f32 or q.dtype == torch.float32 else None
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev) if q.dtype != torch.float32 else None
+    f32 = torch.empty((B, Hq, D), dtype=torch.float32, device=dev) if want_f32 or dtype is torch.float32 else None
+    out = torch.empty((B, Hq, D), dtype=dtype, device=dev) if dtype is not torch.float32 else None
     lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if want_lse else None
     if B and Hq:
         rows = min(B, int(max_rows)) if max_rows is not None else B
-        need = int(_lib.load().tq_prefix_attention_workspace_bytes(B, Hq, Hkv, D, P, int(cu_rows is not None), rows, n_prefix, n_own))
+        need = _lib.load().tq_prefix_attention_workspace_bytes(B, Hq, Hkv, D, P, int(cu_rows is not None), rows, n_prefix, n_own)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        at, at_own = _pointers_or_0(shared), _pointers_or_0(mine)
-        qs = q.stride()
-        _on_device("tq_prefix_attention", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, D, qs[0], qs[1], P, _ptr(cu_rows),
-                   rows, _ptr(prefix_starts), _ptr(prefix_lens), n_prefix, cap, at.buffer_info()[0], _ptr(own_lens), n_own,
+        at, at_own = array("Q", shared), array("Q", mine)
+        _on_device("tq_prefix_attention", on, q.data_ptr(), _QUERY_TYPES[dtype], B, Hq, Hkv, D, q_sb, q_sh, P, _ptr(cu_rows), rows,
+                   _ptr(prefix_starts), _ptr(prefix_lens), n_prefix, cap, at.buffer_info()[0], _ptr(own_lens), n_own,
                    own_cap, at_own.buffer_info()[0], key.bits, value.bits, int(has_qjl), key.rotation.data_ptr(),
                    key.centers.data_ptr(), _ptr(qjl), value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s,
-                   _ptr(f32), _ptr(out), _ptr(lse), ws.data_ptr(), ws.numel(), _stream_handle(dev))
+                   _ptr(f32), _ptr(out), _ptr(lse), ws.data_ptr(), max(need, 16), _stream_handle(dev))
     outs = (f32 if out is None else out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
     return outs if len(outs) > 1 else outs[0]
 
@@ -1013,14 +1010,13 @@ def block_bounds(k: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, first:
     _no_gradient("block_bounds", k)
     _not_traced("block_bounds")
     _require_gpu(k)
-    B, H, T, D = k.shape
-    on = k.get_device()
-    if lohi.dim() != 5 or lohi.shape[:2] != (B, H) or lohi.shape[3:] != (2, D) or lohi.dtype is not torch.int8 \
-            or not lohi.is_contiguous() or lohi.get_device() != on:
+    (B, H, T, D), on, sh = k.shape, k.get_device(), lohi.shape
+    if (len(sh) != 5 or sh[0] != B or sh[1] != H or sh[3] != 2 or sh[4] != D or lohi.dtype is not torch.int8
+            or lohi.get_device() != on or not lohi.is_contiguous()):
         raise ValueError(f"lohi: expected a contiguous int8 tensor of {(B, H)} + (blocks, 2, {D}) on {k.device}, got {lohi.dtype} "
                          f"{tuple(lohi.shape)} on {lohi.device}")
-    cap = lohi.shape[2]
-    if step.shape != (B, H, cap) or step.dtype is not torch.float32 or not step.is_contiguous() or step.get_device() != on:
+    cap = sh[2]
+    if step.shape != sh[:3] or step.dtype is not torch.float32 or step.get_device() != on or not step.is_contiguous():
         raise ValueError(f"step: expected a contiguous fp32 tensor of {(B, H, cap)} on {k.device}, got {step.dtype} "
                          f"{tuple(step.shape)} on {step.device}")
     n = -(-T // BLOCK_TOKENS)
@@ -1045,17 +1041,16 @@ def select_blocks(q: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, *, n_
     bounds, the largest of the KV head's query heads; equal scores by their number.  Places left, where there are fewer
     blocks, hold -1.
     """
-    q = _one_token("select_blocks", q)
+    q, B, Hq, q_sb, q_sh = _one_token("select_blocks", q)
     _no_gradient("select_blocks", q)
     _not_traced("select_blocks")
     _require_gpu(q)
-    dev, on = q.device, q.get_device()
-    B, Hq, D = q.shape
-    if lohi.dim() != 5 or lohi.shape[0] != B or lohi.shape[3:] != (2, D) or lohi.dtype is not torch.int8 or not lohi.is_contiguous() \
-            or lohi.get_device() != on or lohi.shape[1] == 0 or Hq % lohi.shape[1]:
+    dev, on, D, sh = q.device, q.get_device(), HEAD_DIM, lohi.shape
+    if (len(sh) != 5 or sh[0] != B or sh[3] != 2 or sh[4] != D or sh[1] == 0 or Hq % sh[1] or lohi.dtype is not torch.int8
+            or lohi.get_device() != on or not lohi.is_contiguous()):
         raise ValueError(f"lohi {lohi.dtype} {tuple(lohi.shape)} on {lohi.device} does not match q {tuple(q.shape)} on {dev}")
-    Hkv, cap = lohi.shape[1:3]
-    if step.shape != (B, Hkv, cap) or step.dtype is not torch.float32 or not step.is_contiguous() or step.get_device() != on:
+    Hkv, cap = sh[1], sh[2]
+    if step.shape != sh[:3] or step.dtype is not torch.float32 or step.get_device() != on or not step.is_contiguous():
         raise ValueError(f"step {step.dtype} {tuple(step.shape)} on {step.device} does not match lohi {tuple(lohi.shape)}")
     known = cap if n_blocks is None else int(n_blocks)
     if not 0 <= known <= cap or n_tokens < 0 or -(-n_tokens // BLOCK_TOKENS) - recent > known:
@@ -1066,10 +1061,11 @@ def select_blocks(q: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, *, n_
     seq_lens = _int32_on(seq_lens, dev, "seq_lens", (B,))
     out = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
     if B and Hq:
-        qs = q.stride()
-        _on_device("tq_select_blocks", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, D, qs[0], qs[1], lohi.data_ptr(),
+        need = _lib.load().tq_select_blocks_workspace_bytes(B, Hkv, n_tokens)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _on_device("tq_select_blocks", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, D, q_sb, q_sh, lohi.data_ptr(),
                    step.data_ptr(), cap, known, n_tokens, _ptr(seq_starts), _ptr(seq_lens), keep, sink, recent, out.data_ptr(),
-                   _stream_handle(dev))
+                   _ptr(ws), need, _stream_handle(dev))
     return out
 
 
@@ -1085,13 +1081,13 @@ def block_attention(q: torch.Tensor, blocks: torch.Tensor, *, k_codes: torch.Ten
     it); a block named twice counts twice.  At most 8 query heads per KV head.  The rest, and what it returns, as for
     ``decode_attention``.
     """
-    q = _one_token("block_attention", q)
+    q, B, Hq, q_sb, q_sh = _one_token("block_attention", q)
     _no_gradient("block_attention", q)
     _not_traced("block_attention")
     _require_gpu(q)
-    dev, on = q.device, q.get_device()
-    q = rows16(q.to(torch.bfloat16).contiguous())
-    B, Hq, D = q.shape
+    dev, on, D = q.device, q.get_device(), HEAD_DIM
+    if q.dtype is not torch.bfloat16 or (q_sh != D and Hq != 1) or (q_sb != Hq * D and B != 1) or q.data_ptr() % 16:
+        q = q.to(torch.bfloat16, copy=True, memory_format=torch.contiguous_format)
     has_qjl = qjl is not None
     cache = {"k_codes": k_codes, "k_norms": k_norms, "k_signs": k_signs, "k_rnorms": k_rnorms, "v_codes": v_codes, "v_norms": v_norms}
     (kc, kn, ks, kr, vc, vn), (_, Hkv, cap) = _packed_arrays("block_attention", cache, B, key, value, has_qjl, on)
@@ -1111,13 +1107,12 @@ def block_attention(q: torch.Tensor, blocks: torch.Tensor, *, k_codes: torch.Ten
     f32 = torch.empty((B, Hq, D), dtype=torch.float32, device=dev) if want_f32 else None
     lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if want_lse else None
     if B and Hq and keep:
-        need = int(_lib.load().tq_block_attention_workspace_bytes(B, Hq, Hkv, D, keep))
+        need = _lib.load().tq_block_attention_workspace_bytes(B, Hq, Hkv, D, keep)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         _on_device("tq_block_attention", on, q.data_ptr(), B, Hq, Hkv, D, blocks.data_ptr(), keep, _ptr(seq_starts), _ptr(seq_lens),
-                   n_tokens, cap, kc.data_ptr(), kn.data_ptr(), _ptr(ks), _ptr(kr), vc.data_ptr(), vn.data_ptr(), key.bits,
-                   value.bits, int(has_qjl), key.rotation.data_ptr(), key.centers.data_ptr(), _ptr(qjl),
-                   value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s, _ptr(f32), out.data_ptr(), _ptr(lse),
-                   ws.data_ptr(), ws.numel(), _stream_handle(dev))
+                   n_tokens, cap, kc, kn, ks, kr, vc, vn, key.bits, value.bits, int(has_qjl), key.rotation.data_ptr(),
+                   key.centers.data_ptr(), _ptr(qjl), value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s,
+                   _ptr(f32), out.data_ptr(), _ptr(lse), ws.data_ptr(), max(need, 16), _stream_handle(dev))
     else:  # nothing is attended to
         out.zero_()
         if f32 is not None:
