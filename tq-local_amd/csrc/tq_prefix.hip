@@ -99,19 +99,30 @@ struct Slot {
     Item item;
     int first, n, step;
 };
-// Up to 64 items share the slots in proportion to their tiles, each with one at least; what is left over goes unused (count = 0).
-__device__ __forceinline__ Slot share_slots(const PrefixArgs& a, int slot, int lane) {
+// Up to 64 items of up to 64 prompts and SHARED_ROWS sequences share the slots in proportion to their tiles, each with one at least; what is
+// left over goes unused (count = 0).  All that it reads is asked for together: one wait for memory where a loop over an item's
+// sequences had one for each.
+constexpr int SHARED_ROWS = 256;
+struct Shared {
+    int own[SHARED_ROWS / 64];  // of sequence 64 i + lane
+    Range range;                // of prompt `lane`
+};
+__device__ __forceinline__ Slot share_slots(const PrefixArgs& a, int slot, int lane, Shared& s) {
+#pragma unroll
+    for (int i = 0; i < SHARED_ROWS / 64; ++i) s.own[i] = 64 * i + lane < a.batch ? own_of(a, 64 * i + lane) : 0;
+    s.range = lane < a.prompts ? range_of(a, lane) : Range{0, 0};
     const Item mine = find_item(a, lane, lane);
-    int tiles = 0;
-    if (mine.count) {
-        const Range range = range_of(a, mine.p);
-        tiles = tiles_of(range.end - range.lo);
-        if (a.own_lens) {
-            for (int m = 0; m < mine.count; ++m) tiles += tiles_of(own_of(a, mine.first + m));
-        } else {
-            tiles += mine.count * tiles_of((int)a.n_own);
-        }
+    // tiles of the sequences up to each
+    int before = 0, last = mine.first + mine.count - 1, tiles = 0;
+#pragma unroll
+    for (int i = 0; i < SHARED_ROWS / 64; ++i) {
+        const int up = scan_sum(tiles_of(s.own[i]), lane) + before;
+        const int to = __shfl(up, last & 63), from = __shfl(up, (mine.first - 1) & 63);
+        if (last >> 6 == i) tiles += to;
+        if (mine.first > 0 && (mine.first - 1) >> 6 == i) tiles -= from;
+        before = __builtin_amdgcn_readlane(up, 63);
     }
+    tiles = mine.count ? tiles + __shfl(tiles_of(s.range.end - s.range.lo), mine.p) : 0;
     const int total = __builtin_amdgcn_readlane(scan_sum(tiles, lane), 63);
     // (the sum of the shares does not pass what there is to share, whatever the roundings: these are far below 1)
     const int share = (int)((float)(a.n_slots - a.items) * ((float)tiles / (float)std::max(total, 1)));
@@ -173,17 +184,28 @@ __global__ __launch_bounds__(Tiles<RB>::T, 2) void prefix_kernel(PrefixArgs a, C
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = blockIdx.x, kvh = blockIdx.y;
     Slot at;
+    Range range;
+    int own_len = 0;  // of the item's sequence `lane`
     if (a.shared) {
-        at = share_slots(a, slot, lane);
+        Shared s;
+        at = share_slots(a, slot, lane, s);
+        if (at.item.count == 0) return;
+        range = {__builtin_amdgcn_readlane(s.range.lo, at.item.p), __builtin_amdgcn_readlane(s.range.end, at.item.p)};
+        const int row = at.item.first + lane;
+#pragma unroll
+        for (int i = 0; i < SHARED_ROWS / 64; ++i) {
+            const int x = __shfl(s.own[i], row & 63);
+            if (row >> 6 == i && lane < at.item.count) own_len = x;
+        }
     } else {
         const int it = slot % a.items;
         const Item item = find_item(a, it, lane);
         at = {{scalar(item.p), scalar(item.first), scalar(item.count)}, it, a.n_split, a.items};
+        if (at.item.count == 0) return;
+        if (lane < at.item.count) own_len = own_of(a, at.item.first + lane);
+        range = range_of(a, at.item.p);
     }
-    if (at.item.count == 0) return;
-    int own_len = 0;
-    if (lane < at.item.count) own_len = own_of(a, at.item.first + lane);
-    PrefixSource<RB> src(a, at, slot, kvh, range_of(a, at.item.p), own_len, lane);
+    PrefixSource<RB> src(a, at, slot, kvh, range, own_len, lane);
     if (src.split() == 0 && kvh == 0 && (int)threadIdx.x < at.item.count)
         a.row_slots[at.item.first + threadIdx.x] = make_int4(at.first, at.n, at.step, threadIdx.x);
     attend_tiles<KB, VB, QJL, RB, NQ>(codec, src, lane, wave);
@@ -202,7 +224,12 @@ struct PrefixRows {
     }
     __device__ __forceinline__ int64_t place(int64_t row) const { return row; }
 };
-__global__ __launch_bounds__(MERGE_T) void merge_kernel(Merge a, PrefixRows rows) { merge_rows(a, rows); }
+template <int ROWS>
+__global__ __launch_bounds__(MERGE_T) void merge_kernel(Merge a, PrefixRows rows) {
+    merge_rows<ROWS>(a, rows);
+}
+
+constexpr int FEW_ROWS = 2048;
 
 struct Plan {
     int row_blocks, per, items, n_split, n_slots;
@@ -293,7 +320,8 @@ extern "C" int tq_prefix_attention(const void* q, int q_type, int batch, int q_h
     if (!workspace || workspace_bytes < p.total() || !aligned16(workspace)) return TQ_ERR_WORKSPACE;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     int4* const row_slots = reinterpret_cast<int4*>(ws + p.o_bytes + p.ms_bytes);
-    const int shared = (cu_rows || prefix_starts || prefix_lens || own_lens) && p.items <= 64 && p.n_slots > p.items;
+    const int shared = (cu_rows || prefix_starts || prefix_lens || own_lens) && p.items <= 64 && prompts <= 64 && batch <= SHARED_ROWS &&
+                       p.n_slots > p.items;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const PrefixArgs a{prompts, batch, kv_heads, q_heads / kv_heads, p.per, p.items, cu_rows, batch / prompts,
                        prefix_starts, prefix_lens, own_lens, n_prefix, cap_prefix, n_own, cap_own,
@@ -314,7 +342,12 @@ extern "C" int tq_prefix_attention(const void* q, int q_type, int batch, int q_h
     TQ_CHECK_LAUNCH();
     const Merge m{(int64_t)batch * q_heads, c.part_o, c.part_ms, value_rotation, out_f32, out_16, q_type == 2, lse_out};
     const PrefixRows rows{q_heads, kv_heads, 32 * p.row_blocks, row_slots};
-    hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((m.all_rows + MERGE_ROWS - 1) / MERGE_ROWS)), dim3(MERGE_T), 0, s, m, rows);
+    // few rows are spread over more workgroups, which are done with theirs sooner
+    if (m.all_rows <= FEW_ROWS)
+        hipLaunchKernelGGL(merge_kernel<4>, dim3((unsigned)((m.all_rows + 3) / 4)), dim3(MERGE_T), 0, s, m, rows);
+    else
+        hipLaunchKernelGGL(merge_kernel<MERGE_ROWS>, dim3((unsigned)((m.all_rows + MERGE_ROWS - 1) / MERGE_ROWS)), dim3(MERGE_T), 0, s,
+                           m, rows);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
 }

@@ -208,8 +208,16 @@ struct Place {
     int left;
 };
 
-__device__ __forceinline__ float query_element(const Codec& a, int64_t i) {
-    return a.q_type == 1 ? static_cast<const float*>(a.q)[i] : tq::f16_to_f32(static_cast<const uint16_t*>(a.q)[i]);
+// Eight elements of an fp32 or fp16 query row, wherever it stands.
+__device__ __forceinline__ void query_elements(const Codec& a, int64_t at, float* y) {
+    if (a.q_type == 1) {
+        __builtin_memcpy(y, static_cast<const float*>(a.q) + at, 32);
+        return;
+    }
+    uint32_t w[4];
+    __builtin_memcpy(w, static_cast<const uint16_t*>(a.q) + at, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[2 * i] = tq::f16_to_f32(w[i] & 0xFFFFu), y[2 * i + 1] = tq::f16_to_f32(w[i] >> 16);
 }
 
 // Pairs of value codes looked up in LDS: entry e of the table is the pair (or the two pairs) that the byte e of the
@@ -317,8 +325,7 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
                 __builtin_memcpy(&x[s][0], static_cast<const uint16_t*>(a.q) + at + 16 * s, 16);  // rows past the last: some row
             } else {
                 float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = query_element(a, at + 16 * s + e);
+                query_elements(a, at + 16 * s, y);
                 split_terms<NQ>(y, x[s]);
             }
         }
@@ -711,33 +718,35 @@ struct Part {
     int n;
 };
 
-// MERGE_ROWS rows per workgroup: their splits weighed and added, then rotated back.  The matrix is read ahead of the partials,
+// ROWS rows per workgroup: their splits weighed and added, then rotated back.  The matrix is read ahead of the partials,
 // a quarter of its rows by a thread for its output dim.  `rows` says where a row's partials stand (find) and where its outputs
 // go (place).
 constexpr int MERGE_ROWS = 16, MERGE_T = 512, PARTS = MERGE_T / D, PART = D / PARTS;
-template <class Rows>
+template <int ROWS, class Rows>
 __device__ __forceinline__ void merge_rows(const Merge& a, const Rows& rows) {
-    __shared__ float s_w[MERGE_ROWS][MAX_SPLIT];
-    __shared__ float s_den[MERGE_ROWS];
-    __shared__ __align__(16) float s_o[MERGE_ROWS][D];
-    __shared__ float s_part[PARTS][MERGE_ROWS][D];
-    const int64_t row0 = (int64_t)blockIdx.x * MERGE_ROWS;
+    __shared__ float s_w[ROWS][MAX_SPLIT];
+    __shared__ float s_den[ROWS];
+    __shared__ __align__(16) float s_o[ROWS][D];
+    __shared__ float s_part[PARTS][ROWS][D];
+    const int64_t row0 = (int64_t)blockIdx.x * ROWS;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int j = threadIdx.x & 127, quarter = threadIdx.x >> 7;
     float m[PART];
 #pragma unroll
     for (int d = 0; d < PART; ++d) m[d] = a.rv[(PART * quarter + d) * D + j];
-    // 32 threads to a row, four dims each: the first splits' partials are on their way before the weights are known
-    constexpr int AHEAD = 8;
-    const int pk = threadIdx.x >> 5, pc = threadIdx.x & 31;
+    // 32 threads to a row and every SHARES-th of its splits, four dims each: the first splits' partials are on their way before the
+    // weights are known
+    constexpr int SHARES = MERGE_T / 32 / ROWS, AHEAD = 8 / SHARES;
+    static_assert(SHARES <= PARTS, "the shares' sums fit s_part");
+    const int pk = (threadIdx.x >> 5) / SHARES, share = (threadIdx.x >> 5) % SHARES, pc = threadIdx.x & 31;
     const Part mine = rows.find(std::min(row0 + pk, a.all_rows - 1));
     const float4* const part = reinterpret_cast<const float4*>(a.part_o + mine.at * D) + pc;
     const int64_t step4 = mine.step * (D / 4);
     float4 ahead[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) ahead[i] = i < mine.n ? part[i * step4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = share + SHARES * i < mine.n ? part[(share + SHARES * i) * step4] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-    for (int k = wave; k < MERGE_ROWS; k += MERGE_T / 64) {
+    for (int k = wave; k < ROWS; k += MERGE_T / 64) {
         const int64_t row = row0 + k;
         float2 ms = make_float2(-__builtin_inff(), 0.0f);
         if (row < a.all_rows) {
@@ -766,15 +775,22 @@ __device__ __forceinline__ void merge_rows(const Merge& a, const Rows& rows) {
             o.z = __builtin_fmaf(w, x.z, o.z), o.w = __builtin_fmaf(w, x.w, o.w);
         };
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) add(s_w[pk][i], ahead[i]);  // splits that there are not: 0 times 0
+        for (int i = 0; i < AHEAD; ++i) add(s_w[pk][share + SHARES * i], ahead[i]);  // splits that there are not: 0 times 0
 #pragma unroll 8
-        for (int i = AHEAD; i < mine.n; ++i) add(s_w[pk][i], part[i * step4]);
+        for (int i = share + SHARES * AHEAD; i < mine.n; i += SHARES) add(s_w[pk][i], part[i * step4]);
+        if constexpr (SHARES > 1) {
+            *reinterpret_cast<float4*>(&s_part[share][pk][4 * pc]) = o;
+            __syncthreads();
+            if (share == 0)
+#pragma unroll
+                for (int i = 1; i < SHARES; ++i) add(1.0f, *reinterpret_cast<const float4*>(&s_part[i][pk][4 * pc]));
+        }
         const float den = s_den[pk] == 0.0f ? 1.0f : s_den[pk];
-        *reinterpret_cast<float4*>(&s_o[pk][4 * pc]) = make_float4(o.x / den, o.y / den, o.z / den, o.w / den);
+        if (share == 0) *reinterpret_cast<float4*>(&s_o[pk][4 * pc]) = make_float4(o.x / den, o.y / den, o.z / den, o.w / den);
     }
     __syncthreads();
 #pragma unroll 1
-    for (int k = 0; k < MERGE_ROWS; ++k) {
+    for (int k = 0; k < ROWS; ++k) {
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int d = 0; d < PART; d += 4) {
@@ -786,7 +802,7 @@ __device__ __forceinline__ void merge_rows(const Merge& a, const Rows& rows) {
     }
     __syncthreads();
 #pragma unroll 1
-    for (int k = quarter; k < MERGE_ROWS; k += PARTS) {
+    for (int k = quarter; k < ROWS; k += PARTS) {
         const int64_t row = row0 + k;
         if (row >= a.all_rows) break;
         const float x = (s_part[0][k][j] + s_part[1][k][j]) + (s_part[2][k][j] + s_part[3][k][j]);

@@ -189,7 +189,7 @@ struct TreeRows {
         return ((int64_t)b * q_heads + hq) * T + (in - g * T);
     }
 };
-__global__ __launch_bounds__(MERGE_T) void merge_kernel(Merge a, TreeRows rows) { merge_rows(a, rows); }
+__global__ __launch_bounds__(MERGE_T) void merge_kernel(Merge a, TreeRows rows) { merge_rows<MERGE_ROWS>(a, rows); }
 
 struct Plan {
     int rows, row_blocks, n_split, n_slots;
