@@ -55,6 +55,7 @@ struct BoundsArgs {
     int8_t* lohi;
     float* step;
     int64_t cap, first, per_head, all;  // blocks to a head, and of all heads
+    int heads_next;                     // whether neighbouring waves have a block's heads, or a head's blocks
 };
 
 constexpr int BOUNDS_WAVES = 4;
@@ -62,7 +63,14 @@ __global__ __launch_bounds__(64 * BOUNDS_WAVES) void bounds_kernel(BoundsArgs a)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t at = (int64_t)blockIdx.x * BOUNDS_WAVES + wave;
     if (at >= a.all) return;
-    const int64_t group = at / a.per_head, block = at - group * a.per_head, b = group / a.heads, h = group - b * a.heads;
+    int64_t group, block;
+    if (a.heads_next) {
+        const int64_t place = at / a.heads, b = place / a.per_head;
+        block = place - b * a.per_head, group = b * a.heads + (at - place * a.heads);
+    } else {
+        group = at / a.per_head, block = at - group * a.per_head;
+    }
+    const int64_t b = group / a.heads, h = group - b * a.heads;
     const uint16_t* const k = a.k + b * a.k_sb + h * a.k_sh + block * BT * a.k_st;
     const int left = (int)std::min<int64_t>(a.tokens - block * BT, BT);
     // lane (c = lane % 16, t = lane / 16): channels [8 c, 8 c + 8) of the tokens t, t + 4, ...; past the last it again
@@ -384,7 +392,7 @@ extern "C" int tq_block_bounds(const uint16_t* k, int batch, int heads, int64_t 
     if (dim != D || !aligned16(k) || !aligned16(lohi) || ((k_sb | k_sh | k_st) & 7)) return TQ_ERR_UNSUPPORTED;
     const int64_t groups = (int64_t)batch * heads;
     if (per_head >= (int64_t)1 << 31 || groups * per_head >= (int64_t)1 << 31) return TQ_ERR_UNSUPPORTED;
-    const BoundsArgs a{k, heads, tokens, k_sb, k_sh, k_st, lohi, step, cap, first, per_head, groups * per_head};
+    const BoundsArgs a{k, heads, tokens, k_sb, k_sh, k_st, lohi, step, cap, first, per_head, groups * per_head, k_sh < k_st};
     hipLaunchKernelGGL(bounds_kernel, dim3((unsigned)((a.all + BOUNDS_WAVES - 1) / BOUNDS_WAVES)), dim3(64 * BOUNDS_WAVES), 0,
                        static_cast<hipStream_t>(stream), a);
     TQ_CHECK_LAUNCH();

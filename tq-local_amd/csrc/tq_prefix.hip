@@ -158,14 +158,15 @@ struct PrefixSource {
         return tile < shared_tiles ? -1 : __popcll(__ballot(own_tiles <= (int)tile - shared_tiles));
     }
     __device__ __forceinline__ Place place(int64_t tile) const {
-        const int s = owner(tile);
-        if (s < 0) {
-            const int t0 = lo + (int)tile * TK;
-            return {a.prefix, (int64_t)(at.item.p * a.kv_heads + kvh) * a.cap_prefix + t0, std::min(end - t0, TK)};
-        }
-        const int len = __builtin_amdgcn_readlane(own_lens, s), before = __builtin_amdgcn_readlane(own_tiles, s) - tiles_of(len);
-        const int t0 = ((int)tile - shared_tiles - before) * TK;
-        return {a.own, ((int64_t)(at.item.first + s) * a.kv_heads + kvh) * a.cap_own + t0, std::min(len - t0, TK)};
+        const int s = owner(tile), m = std::max(s, 0);
+        const bool mine = s >= 0;
+        const int len = __builtin_amdgcn_readlane(own_lens, m), before = __builtin_amdgcn_readlane(own_tiles, m) - tiles_of(len);
+        const int t0 = mine ? ((int)tile - shared_tiles - before) * TK : lo + (int)tile * TK;
+        const int64_t row = mine ? (int64_t)(at.item.first + m) : (int64_t)at.item.p;
+        const Cache &p = a.prefix, &o = a.own;
+        return {{mine ? o.k_codes : p.k_codes, mine ? o.k_signs : p.k_signs, mine ? o.v_codes : p.v_codes, mine ? o.k_norms : p.k_norms,
+                 mine ? o.k_rnorms : p.k_rnorms, mine ? o.v_norms : p.v_norms},
+                (row * a.kv_heads + kvh) * (mine ? a.cap_own : a.cap_prefix) + t0, std::min((mine ? len : end) - t0, TK)};
     }
     __device__ __forceinline__ uint32_t seen(int m, int64_t tile) const {
         const int s = owner(tile), left = place(tile).left;  // by the whole wave, ahead of what differs between lanes
