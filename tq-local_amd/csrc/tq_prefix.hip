@@ -32,22 +32,25 @@ __device__ __forceinline__ int clamp_to(int64_t x, int64_t n) { return (int)std:
 __device__ __forceinline__ int tiles_of(int tokens) { return (int)(((int64_t)tokens + TK - 1) / TK); }
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Prefix sums and maxima over the lanes of a wave.
-__device__ __forceinline__ int scan_sum(int x, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x += y;
-    }
-    return x;
+// Prefix sums and maxima (of numbers >= 0) over the lanes of a wave: within the rows of 16 lanes, then from row to row.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int x) {
+    return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ int scan_max(int x, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int y = __shfl_up(x, d);
-        if (lane >= d) x = std::max(x, y);
-    }
-    return x;
+template <class F>
+__device__ __forceinline__ int scan(int x, F join) {
+    x = join(x, moved<0x111, 0xF>(x));  // row_shr 1, 2, 4, 8
+    x = join(x, moved<0x112, 0xF>(x));
+    x = join(x, moved<0x114, 0xF>(x));
+    x = join(x, moved<0x118, 0xF>(x));
+    x = join(x, moved<0x142, 0xA>(x));  // row_bcast 15 to the second and fourth row, 31 to the upper two
+    return join(x, moved<0x143, 0xC>(x));
+}
+__device__ __forceinline__ int scan_sum(int x) {
+    return scan(x, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int scan_max(int x) {
+    return scan(x, [](int a, int b) { return std::max(a, b); });
 }
 
 // An item's prompt, its first sequence and how many it has (0: there is no such item).
@@ -68,9 +71,9 @@ __device__ __forceinline__ Item find_item(const PrefixArgs& a, int it, int lane)
         const int p = p0 + lane;
         int end = a.batch;
         if (p + 1 < a.prompts) end = clamp_to(a.cu_rows[p + 1], a.batch);
-        end = std::max(scan_max(end, lane), rows);
+        end = std::max(scan_max(end), rows);
         const int up = __shfl_up(end, 1), begin = lane == 0 ? rows : up;
-        const int last = scan_sum((end - begin + a.per - 1) / a.per, lane) + items;
+        const int last = scan_sum((end - begin + a.per - 1) / a.per) + items;
         const int n = std::min(64, a.prompts - p0);
         for (int i = 0; i < n; ++i) {
             const int e = __builtin_amdgcn_readlane(last, i), to = __builtin_amdgcn_readlane(end, i);
@@ -116,18 +119,19 @@ __device__ __forceinline__ Slot share_slots(const PrefixArgs& a, int slot, int l
     int before = 0, last = mine.first + mine.count - 1, tiles = 0;
 #pragma unroll
     for (int i = 0; i < SHARED_ROWS / 64; ++i) {
-        const int up = scan_sum(tiles_of(s.own[i]), lane) + before;
+        if (64 * i >= a.batch) break;
+        const int up = scan_sum(tiles_of(s.own[i])) + before;
         const int to = __shfl(up, last & 63), from = __shfl(up, (mine.first - 1) & 63);
         if (last >> 6 == i) tiles += to;
         if (mine.first > 0 && (mine.first - 1) >> 6 == i) tiles -= from;
         before = __builtin_amdgcn_readlane(up, 63);
     }
     tiles = mine.count ? tiles + __shfl(tiles_of(s.range.end - s.range.lo), mine.p) : 0;
-    const int total = __builtin_amdgcn_readlane(scan_sum(tiles, lane), 63);
+    const int total = __builtin_amdgcn_readlane(scan_sum(tiles), 63);
     // (the sum of the shares does not pass what there is to share, whatever the roundings: these are far below 1)
     const int share = (int)((float)(a.n_slots - a.items) * ((float)tiles / (float)std::max(total, 1)));
     const int n = mine.count ? std::min(std::min(1 + share, std::max(1, (tiles + MIN_TILES - 1) / MIN_TILES)), MAX_SPLIT) : 0;
-    const int end = scan_sum(n, lane), i = __popcll(__ballot(end <= slot));
+    const int end = scan_sum(n), i = __popcll(__ballot(end <= slot));
     if (i >= 64) return {{0, 0, 0}, 0, 0, 0};
     auto of_item = [&](int x) { return __builtin_amdgcn_readlane(x, i); };
     return {{of_item(mine.p), of_item(mine.first), of_item(mine.count)}, of_item(end - n), of_item(n), 1};
@@ -141,9 +145,9 @@ struct PrefixSource {
     const int slot, kvh, lo, end, shared_tiles, own_lens, own_tiles;  // the last two: of sequence `lane`, and with those before it
     int member[RB];
 
-    __device__ __forceinline__ PrefixSource(const PrefixArgs& a, const Slot& at, int slot, int kvh, Range range, int own_len, int lane)
+    __device__ __forceinline__ PrefixSource(const PrefixArgs& a, const Slot& at, int slot, int kvh, Range range, int own_len)
         : a(a), at(at), slot(slot), kvh(kvh), lo(scalar(range.lo)), end(scalar(range.end)), shared_tiles(tiles_of(end - lo)),
-          own_lens(own_len), own_tiles(scan_sum(tiles_of(own_len), lane)) {}
+          own_lens(own_len), own_tiles(scan_sum(tiles_of(own_len))) {}
     __device__ __forceinline__ int64_t query(int r) const {
         const uint32_t m = (uint32_t)r / (uint32_t)a.group, g = r - m * a.group;
         const bool live = (int)m < at.item.count;
@@ -206,7 +210,7 @@ __global__ __launch_bounds__(Tiles<RB>::T, 2) void prefix_kernel(PrefixArgs a, C
         if (lane < at.item.count) own_len = own_of(a, at.item.first + lane);
         range = range_of(a, at.item.p);
     }
-    PrefixSource<RB> src(a, at, slot, kvh, range, own_len, lane);
+    PrefixSource<RB> src(a, at, slot, kvh, range, own_len);
     if (src.split() == 0 && kvh == 0 && (int)threadIdx.x < at.item.count)
         a.row_slots[at.item.first + threadIdx.x] = make_int4(at.first, at.n, at.step, threadIdx.x);
     attend_tiles<KB, VB, QJL, RB, NQ>(codec, src, lane, wave);
