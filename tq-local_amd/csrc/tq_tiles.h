@@ -282,7 +282,8 @@ struct Tiles {
     };
     struct Sums {
         float4 o[W][32][32];  // chunks xor-swizzled by the row
-        float2 ms[W][32];
+        float2 ms[RB][W][32];
+        float4 by[RB][32][W / 4];  // what a row's sums of each wave are multiplied by
         float unit[W];
     };
     union Lds {
@@ -375,13 +376,16 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
     // a wave has 32 output dims of one of the matrices
     const int mat = wave >> 2, j0 = 32 * (wave & 3);
     const bool works = QJL || mat == 0;
-    float mrow[8][8];
+    Frag mt[8][2];
     if (works) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < 8; ++s) {
+            float y[8];
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-                __builtin_memcpy(&mrow[s][4 * e], &lds.m[(128 * mat + j0 + r) * 32 + ((4 * s + 2 * h + e) ^ r)], 16);
+                __builtin_memcpy(&y[4 * e], &lds.m[(128 * mat + j0 + r) * 32 + ((4 * s + 2 * h + e) ^ r)], 16);
+            split_terms<2>(y, mt[s]);
+        }
     }
 
     // ---- q R_k^T and q S^T as products of bf16 terms, a bf16 query one, any other two, the matrices two (what is left out,
@@ -393,15 +397,12 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
             f32x16 acc = zero16();
             if (works) {
 #pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    Frag mt[2];
-                    split_terms<2>(mrow[s], mt);
+                for (int s = 0; s < 8; ++s)
 #pragma unroll
                     for (int i = 1; i >= 0; --i)
 #pragma unroll
                         for (int j = NQ - 1; j >= 0; --j)
-                            if (i + j <= 1) acc = mfma_bf16(mt[i], x[s][j], acc);
-                }
+                            if (i + j <= 1) acc = mfma_bf16(mt[s][i], x[s][j], acc);
             }
             if (m + 1 < RB) load_queries(m + 1);
             // this lane: row r's dims j0 + 8 j + 4 h + (0..3)
@@ -660,42 +661,58 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
     for (; tile < whole; tile += step_tiles) step(tile, std::false_type{});
     for (; tile < tiles; tile += step_tiles) step(tile, std::true_type{});
 
-    // ---- the waves' sums, one block of rows at a time
+    // ---- the waves' sums, one block of rows at a time.  What a wave's sums weigh is found once for a row, beside the sums' way to LDS: every
+    // thread of a row for itself, it took half of the 6000 cycles of a block
     const float unit = __uint_as_float((uint32_t)(127 - shift) << 23);
+    __syncthreads();
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
-        __syncthreads();
         const float all = sum_of_halves(sum[m]);
-        if (h == 0) lds.s.ms[wave][r] = make_float2(top[m], all * unit);
+        if (h == 0) lds.s.ms[m][wave][r] = make_float2(top[m], all * unit);
+    }
+    if (lane == 0) lds.s.unit[wave] = unit;
+    __syncthreads();
+    if (wave == 0 && h < RB) {
+        float2 ms[W];
+        float best = -__builtin_inff();
+#pragma unroll
+        for (int k = 0; k < W; ++k) ms[k] = lds.s.ms[h][k][r], best = fmaxf(best, ms[k].x);
+        const float safe = best == -__builtin_inff() ? 0.0f : best;
+        float den = 0.0f, by[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            const float w = exp2_(ms[k].x - safe);
+            by[k] = w * lds.s.unit[k];
+            den = __builtin_fmaf(w, ms[k].y, den);
+        }
+#pragma unroll
+        for (int k = 0; k < W; k += 4) lds.s.by[h][r][k / 4] = make_float4(by[k], by[k + 1], by[k + 2], by[k + 3]);
+        if (32 * h + r < src.rows()) a.part_ms[src.partial() + 32 * h + r] = make_float2(best, den);
+    }
+#pragma unroll
+    for (int m = 0; m < RB; ++m) {
+        if (m) __syncthreads();
 #pragma unroll
         for (int d = 0; d < 4; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 lds.s.o[wave][r][(8 * d + 2 * j + h) ^ r] =
                     make_float4(o[m][d][4 * j], o[m][d][4 * j + 1], o[m][d][4 * j + 2], o[m][d][4 * j + 3]);
-        if (lane == 0) lds.s.unit[wave] = unit;
         __syncthreads();
         for (int i = threadIdx.x; i < 32 * 32; i += N::T) {
             const int row = i >> 5, ch = i & 31;
             if (32 * m + row >= src.rows()) continue;
-            float best = -__builtin_inff();
+            float by[W];
 #pragma unroll
-            for (int k = 0; k < W; ++k) best = fmaxf(best, lds.s.ms[k][row].x);
-            const float safe = best == -__builtin_inff() ? 0.0f : best;
+            for (int k = 0; k < W; k += 4) *reinterpret_cast<float4*>(&by[k]) = lds.s.by[m][row][k / 4];
             float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            float den = 0.0f;
 #pragma unroll
             for (int k = 0; k < W; ++k) {
-                const float2 ms = lds.s.ms[k][row];
-                const float w = exp2_(ms.x - safe), wu = w * lds.s.unit[k];
                 const float4 y = lds.s.o[k][row][ch ^ row];
-                den = __builtin_fmaf(w, ms.y, den);
-                x.x = __builtin_fmaf(wu, y.x, x.x), x.y = __builtin_fmaf(wu, y.y, x.y);
-                x.z = __builtin_fmaf(wu, y.z, x.z), x.w = __builtin_fmaf(wu, y.w, x.w);
+                x.x = __builtin_fmaf(by[k], y.x, x.x), x.y = __builtin_fmaf(by[k], y.y, x.y);
+                x.z = __builtin_fmaf(by[k], y.z, x.z), x.w = __builtin_fmaf(by[k], y.w, x.w);
             }
-            const int64_t at = src.partial() + 32 * m + row;
-            reinterpret_cast<float4*>(a.part_o + at * D)[ch] = x;
-            if (ch == 0) a.part_ms[at] = make_float2(best, den);
+            reinterpret_cast<float4*>(a.part_o + (src.partial() + 32 * m + row) * D)[ch] = x;
         }
     }
 }
