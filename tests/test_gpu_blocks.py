@@ -427,6 +427,31 @@ def test_left_padding(cuda):
         block_sparse_attention(q, layer, 4, attention_mask=mask)
 
 
+def test_captured_steps_with_a_mask(cuda):
+    """Every replay finds the mask's ranges anew, also where an eager step has had them."""
+    layer = make_layer(2, 2, 900, 4, True, seed=19)
+    layer.attend_blocks(4, sink=1, recent=1)
+    layer._tq_mask_contiguous = True
+    mask, q = torch.ones(2, 900, dtype=torch.bool, device="cuda"), randn((2, 8, 1, D), 5)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        q.add_(0.0)
+        with pytest.raises(ValueError, match="block_bounds"):
+            fused_attention(q, layer, 4, mask)
+    assert layer._bounds is None
+    lohi, step, known = (t[:, :, :900 // 64] if torch.is_tensor(t) else t for t in layer.block_bounds())
+    fused_attention(q, layer, 4, mask)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = fused_attention(q, layer, 4, mask)
+    for start in (0, 100, 333):
+        mask[1, :start] = False
+        graph.replay()
+        torch.cuda.synchronize()
+        blocks = select_ref(q[:, :, 0], lohi, step, 900, 4, 1, 1, [0, start], [900, 900])
+        check(out, blocks_ref(q[:, :, 0], layer, blocks, [0, start], [900, 900])[0][:, :, None])
+        check(fused_attention(q, layer, 4, mask), out.double(), 2 * TOL)
+
+
 def test_a_model_attending_to_blocks(cuda):
     """Every block kept: the logits of full attention; few kept: finite, and other ones."""
     from turboquant.adapters.transformers import disable_turboquant_attention, enable_turboquant_attention

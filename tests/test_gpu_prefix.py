@@ -350,3 +350,70 @@ def test_layers_that_cannot_be_shared_are_copied(cuda):
         share_prefix(Cache(layers=[make_layer(2, 2, 40, 4, True)]), [1, 2, 3])
     with pytest.raises(ValueError):
         share_prefix(Cache(layers=[make_layer(2, 2, 40, 4, True)]), 0)
+
+
+def test_masks_that_leave_a_row_nothing(cuda):
+    """A sequence whose row of the mask is empty, beside another of its prompt that is not: zero, and the others as they are."""
+    shared, copied = both((3, 2), 2, 100)
+    for layer in (shared, copied):
+        append(layer, 5, 2, 5, 50)
+    k, v = rows64(copied)
+    mask = torch.ones(5, 105, dtype=torch.bool, device="cuda")
+    mask[1] = False
+    added = torch.zeros(5, 1, 1, 105, device="cuda").masked_fill(~mask[:, None, None], -math.inf)
+    q = randn((5, 8, 1, D), 5)
+    ref, _ = attend64(q[:, :, 0], k, v, mask[:, None])
+    for m in (mask, mask.int(), mask[:, None, None], added):
+        got = shared_prefix_attention(q, shared, m)
+        check(got, ref[:, :, None], 2e-2)  # bf16 rows and weights: 2^-8 of the logits' terms and of the values
+        assert (got[1] == 0).all()
+    several = randn((5, 8, 3, D), 6)
+    for m in (mask, mask[:, None, None] & torch.ones(3, 105, dtype=torch.bool, device="cuda").tril(102)):
+        got = shared_prefix_attention(several, shared, m)  # a mask of tokens leaves the order of the new ones to hold
+        for i in range(3):
+            ref, _ = attend64(several[:, :, i], k[:, :, :103 + i], v[:, :, :103 + i], mask[:, None, :103 + i])
+            check(got[:, :, i], ref, 2e-2)
+
+
+def test_a_mask_known_to_be_ranges_is_not_looked_at(cuda):
+    """With the layer told so, a step with a mask can be captured."""
+    shared, copied = both((2, 3), 2, 100)
+    for layer in (shared, copied):
+        append(layer, 5, 2, 5, 50)
+    q, mask = randn((5, 8, 1, D), 5), torch.ones(5, 105, dtype=torch.bool, device="cuda")
+    mask[:2, :30] = False
+    want = shared_prefix_attention(q, shared, mask)
+    check(want, fused(q, copied, mask).double(), 2 * TOL)
+    shared._tq_mask_contiguous = True
+    shared_prefix_attention(q, shared, mask)  # the ranges of this mask are known, and yet looked for at every replay
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = shared_prefix_attention(q, shared, mask)
+    # (an eager call before the first replay has ranges of its own)
+    check(shared_prefix_attention(q, shared, mask), fused(q, copied, mask).double(), 2 * TOL)
+    for i in range(3):
+        mask[2:, :10 * i] = False
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, fused(q, copied, mask).double(), 2 * TOL)
+    shared._tq_mask_contiguous = False
+    check(shared_prefix_attention(q, shared, mask), fused(q, copied, mask).double(), 2e-2)
+
+
+def test_a_refused_call_changes_nothing(cuda):
+    shared, copied = both((2, 3), 2, 100)
+    for layer in (shared, copied):
+        append(layer, 5, 2, 5, 50)
+    q = randn((5, 8, 1, D), 5)
+    want = shared_prefix_attention(q, shared)
+    for rows in (torch.zeros(5, dtype=torch.bool), torch.tensor([], dtype=torch.int64), torch.tensor([4, 1])):
+        with pytest.raises(ValueError):
+            shared.batch_select_indices(rows)
+    assert torch.equal(shared_prefix_attention(q, shared), want)
+    first, other = make_layer(2, 2, 40, 4, True, dense=3), make_layer(2, 2, 40, 4, True)
+    other.attend_blocks(4)
+    with pytest.raises(ValueError):
+        share_prefix(Cache(layers=[first, other]), 3)
+    assert first._batch() == other._batch() == 2
+    other.attend_blocks(None)
+    assert share_prefix(Cache(layers=[first, other]), 3).layers[1].batch == 6

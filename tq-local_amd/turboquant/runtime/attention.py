@@ -70,10 +70,13 @@ def _valid_range(attention_mask: torch.Tensor | None, B: int, total: int, device
     hole (right padding followed by generated tokens) cannot take this path: with
     ``check_contiguous`` such masks raise ``_HoleyMask`` (one host sync to find out);
     callers that know the mask's shape pass False.  The result for one mask tensor is
-    computed once and reused by the following layers of the same forward.
+    computed once and reused by the following layers of the same forward; a call that is
+    being captured computes its own, which every replay then does from the mask as it is.
     """
     if attention_mask is None:
         return None, None
+    if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
+        return _compute_range(attention_mask, B, total, device, check_contiguous)
     c = getattr(_tls, "last_range", None)
     if (c is not None and c[0] is attention_mask and c[1] == attention_mask._version
             and c[2:6] == (B, total, check_contiguous, device)):
@@ -470,21 +473,31 @@ def block_sparse_attention(query_states: torch.Tensor, packed_layer: "PackedMSEL
 def _shared_ranges(layer: "SharedPrefixLayer", mask: torch.Tensor | None, device):
     """(prefix starts, prefix ends, own ends) of a step's mask, int32 or None.
 
-    The sequences of one prompt have to share its padding (one host sync to find out, for all layers of a forward);
-    ``_HoleyMask`` where they do not, or where a row's tokens are not one range."""
+    ``_HoleyMask`` where a row's tokens are not one range, or where the sequences of a prompt do not share its padding: a host
+    sync to find out, which a layer with ``_tq_mask_contiguous`` set spares (as for ``fused_attention``)."""
     if mask is None:
         return None, None, None
-    n, total = layer.prefix.packed_seq_length(), layer.get_seq_length()
-    key = (mask._version, n, total, tuple(layer.counts), device)
-    c = getattr(_tls, "last_shared", None)
-    if c is None or c[0] is not mask or c[1] != key:
-        starts, ends = _valid_range(mask, layer.batch, total, device)
-        first, last = starts[layer.first_of], ends.clamp(max=n)[layer.first_of]
-        apart = (starts != first[layer.prompt_of]) | (ends.clamp(max=n) != last[layer.prompt_of]) | (starts > n)
-        c = _tls.last_shared = (mask, key, None if bool(apart.any()) else (first, last, (ends - n).clamp(min=0)))
-    if c[2] is None:
+    if layer._tq_mask_contiguous is False:
         raise _HoleyMask
-    return c[2]
+    known = layer._tq_mask_contiguous is not None
+    n = layer.prefix.packed_seq_length()
+    starts, ends = _valid_range(mask, layer.batch, layer.get_seq_length(), device, check_contiguous=not known)
+    first, last = starts[layer.first_of], ends.clamp(max=n)[layer.first_of]
+    if not known and bool(((starts != first[layer.prompt_of]) | (ends.clamp(max=n) != last[layer.prompt_of]) | (starts > n)).any()):
+        raise _HoleyMask
+    return first, last, (ends - n).clamp(min=0)
+
+
+def _rows_mask(mask: torch.Tensor | None, B: int, Sq: int, total: int, device) -> torch.Tensor | None:
+    """The mask of a batch's last ``Sq`` of ``total`` tokens in four dimensions; without one, and of one [B, total], each sees those up to
+    its own."""
+    if mask is not None and mask.dim() == 4:
+        return mask[..., :total] if mask.dtype == torch.bool or mask.is_floating_point() else mask[..., :total] != 0
+    seen = None if mask is None else _attend_mask(mask, B, total)[:, None, None]
+    if Sq == 1:
+        return seen
+    up_to = torch.ones(Sq, total, dtype=torch.bool, device=device).tril(total - Sq)[None, None]
+    return up_to if seen is None else up_to & seen
 
 
 def shared_prefix_attention(query_states: torch.Tensor, layer: "SharedPrefixLayer",
@@ -493,7 +506,7 @@ def shared_prefix_attention(query_states: torch.Tensor, layer: "SharedPrefixLaye
 
     One query token per sequence, up to 64 query heads per KV head and a mask of one range per row (left padding of the
     prompts) run on the packed codes (``kernels.prefix_attention``), tokens kept dense merged by log-sum-exp; others
-    take the decoded rows and torch's attention, the Sq tokens being the sequences' last ones."""
+    take the decoded rows (``chunked_turboquant_attention``), the Sq tokens being the sequences' last ones."""
     B, Hq, Sq, D = query_states.shape
     prefix, own = layer.prefix, layer.own
     store, n_prefix, n_own, n_dense = prefix._store, prefix.packed_seq_length(), own.packed_seq_length(), own._dense_len
@@ -523,16 +536,8 @@ def shared_prefix_attention(query_states: torch.Tensor, layer: "SharedPrefixLaye
             return K.DenseAttention(q, store.H, n).add(*dense, n_dense, 0, n, 1.0 / math.sqrt(D), out=query_states.dtype,
                                                        prev=o_packed, prev_lse=lse, **more)
     keys, values = layer.dense_rows()
-    mask = attention_mask
-    if mask is None and Sq > 1:
-        mask = torch.ones(Sq, keys.shape[2], dtype=torch.bool, device=dev).tril(keys.shape[2] - Sq)
-    elif mask is not None:
-        if mask.dim() == 2:
-            mask = mask.bool()[:, None, None]
-        mask = mask[..., :keys.shape[2]]
-        mask = mask if mask.dtype == torch.bool else mask.to(query_states.dtype)
-    return F.scaled_dot_product_attention(query_states, keys.to(query_states.dtype), values.to(query_states.dtype), attn_mask=mask,
-                                          enable_gqa=group > 1)
+    mask = _rows_mask(attention_mask, B, Sq, keys.shape[2], dev)
+    return chunked_turboquant_attention(query_states, layer.without_tokens(), keys, values, group, mask)
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *,

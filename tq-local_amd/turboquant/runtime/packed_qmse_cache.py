@@ -662,11 +662,14 @@ class PackedMSELayer(CacheLayerMixin):
 
     def block_bounds(self) -> tuple[torch.Tensor, torch.Tensor, int]:
         """Bounds of the keys of the whole blocks of packed tokens, as decoded: (lohi, step, blocks), see
-        ``kernels.block_bounds``.  Blocks that have become whole since the last call are decoded for it."""
+        ``kernels.block_bounds``.  Blocks that have become whole since the last call are decoded for it, not while a graph is
+        captured, whose replays alone would write them: such a call is refused."""
         if self._store is None or self._split is not None:
             raise ValueError("block bounds need a one-group layer with packed tokens")
         B, H, D = self._shape
         n, b = self._store.length // K.BLOCK_TOKENS, self._bounds
+        if n > (0 if b is None else b.count) and torch.cuda.is_current_stream_capturing():
+            raise ValueError("blocks without bounds in a captured step: call block_bounds() before the capture")
         if b is None:
             b = self._bounds = _BlockBounds(B, H, n + max(1, self.reserve_tokens // K.BLOCK_TOKENS), D, self._store.device)
         elif n > b.lohi.shape[2]:

@@ -35,17 +35,16 @@ class SharedPrefixLayer(CacheLayerMixin):
         if len(counts) != store.B:
             raise ValueError(f"{len(counts)} numbers of sequences for {store.B} prompts")
         self.prefix = prefix
-        self.own = PackedMSELayer(prefix.bits, prefix.seed, prefix.grid_size, use_qjl_keys=prefix.use_qjl_keys,
-                                  quantize_decode=prefix.quantize_decode, reserve_tokens=prefix.reserve_tokens)
-        self.own.codecs, self.own.device, self.own.dtype = prefix.codecs, prefix.device, prefix.dtype
-        self.own.is_initialized = self.is_initialized = True
+        self.own = self.without_tokens()
+        self.is_initialized = True
         self.device, self.dtype = prefix.device, prefix.dtype
         self._force_dense = False
+        #: True: the caller knows every step's mask to be one range per row, with the padding of the prompt; False: not; None: looked at
+        self._tq_mask_contiguous: bool | None = getattr(prefix, "_tq_mask_contiguous", None)
         self._set_counts([int(n) for n in counts])
 
     def _set_counts(self, counts: list[int]) -> None:
-        if min(counts) < 0 or sum(counts) == 0:
-            raise ValueError(f"{counts} sequences")
+        self._check_counts(counts)
         self.counts = counts
         dev = self.prefix._store.device
         ends = torch.tensor(counts).cumsum(0)
@@ -54,6 +53,19 @@ class SharedPrefixLayer(CacheLayerMixin):
         self.first_of = (ends - torch.tensor(counts)).clamp(max=sum(counts) - 1).to(dev)
         even = len(set(counts)) == 1
         self.cu_rows = None if even else torch.cat((torch.zeros(1, dtype=torch.int64), ends)).int().to(dev)
+
+    def without_tokens(self) -> PackedMSELayer:
+        """A layer of the prompts' codec that holds nothing."""
+        p = self.prefix
+        layer = PackedMSELayer(p.bits, p.seed, p.grid_size, use_qjl_keys=p.use_qjl_keys, quantize_decode=p.quantize_decode,
+                               reserve_tokens=p.reserve_tokens)
+        layer.codecs, layer.device, layer.dtype, layer.is_initialized = p.codecs, p.device, p.dtype, True
+        return layer
+
+    @staticmethod
+    def _check_counts(counts: list[int]) -> None:
+        if min(counts) < 0 or sum(counts) == 0:
+            raise ValueError(f"{counts} sequences")
 
     @property
     def batch(self) -> int:
@@ -119,6 +131,7 @@ class SharedPrefixLayer(CacheLayerMixin):
         if (prompts.diff() < 0).any():
             raise ValueError(f"rows {rows.tolist()} do not keep the sequences in the order of their prompts")
         counts = torch.bincount(prompts, minlength=len(self.counts)).tolist()
+        self._check_counts(counts)
         if self.own._batch() is not None:
             self.own._take_rows(rows)
         self._set_counts(counts)
@@ -173,17 +186,23 @@ def share_prefix(cache: Cache, sequences: int | Sequence[int]) -> Cache:
     """A cache whose prompts are continued by several sequences each: ``sequences`` of them for every row, or a number for each.
 
     The packed layers of ``cache`` become the shared prompts of the result's layers; they are not copied, and the
-    given cache is to be used no further.  Layers that cannot be shared are copied for every sequence."""
-    layers = []
+    given cache is to be used no further.  Layers that cannot be shared are copied for every sequence.  Shared layers attend to
+    all of their tokens: a choice of blocks (``attend_blocks``) is refused."""
+    per_layer = []  # looked over before any layer is changed
     for layer in cache.layers:
         if not isinstance(layer, PackedMSELayer):
             raise ValueError(f"share_prefix takes packed layers, got {type(layer).__name__}")
         batch = layer._batch()
         if batch is None:
             raise ValueError("share_prefix: the prompts are not in the cache yet")
+        if layer._choice is not None:
+            raise ValueError("share_prefix: a layer attends to chosen blocks (attend_blocks(None) ends that)")
         counts = [int(sequences)] * batch if isinstance(sequences, int) else [int(n) for n in sequences]
         if len(counts) != batch or min(counts) < 0 or sum(counts) == 0:
             raise ValueError(f"share_prefix: {counts} sequences for {batch} prompts")
+        per_layer.append((batch, counts))
+    layers = []
+    for layer, (batch, counts) in zip(cache.layers, per_layer):
         if layer._store is not None and layer._split is None and not layer._dense_len and layer._store.length \
                 and layer._shape[2] == K.HEAD_DIM:
             layers.append(SharedPrefixLayer(layer, counts))
