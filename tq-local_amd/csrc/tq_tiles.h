@@ -100,10 +100,9 @@ struct Lut {
     }
 };
 
-// Four chunks of 8 elements from 32 codes (BITS words), in the order of position_of.
+// 32 codes (BITS words) one to a byte, in the order of position_of.
 template <int BITS>
-__device__ __forceinline__ void expand32(const uint32_t* w, const Lut<BITS>& lut, uint4* out) {
-    uint32_t q[8];
+__device__ __forceinline__ void unpack32(const uint32_t* w, uint32_t* q) {
     if constexpr (BITS == 4) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) q[2 * j] = w[j] & 0x0F0F0F0Fu, q[2 * j + 1] = (w[j] >> 4) & 0x0F0F0F0Fu;
@@ -126,26 +125,25 @@ __device__ __forceinline__ void expand32(const uint32_t* w, const Lut<BITS>& lut
 #pragma unroll
         for (int p = 0; p < 8; ++p) q[p] = (w[0] >> p) & 0x01010101u;
     }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        lut.four(q[2 * j], out[j].x, out[j].y);
-        lut.four(q[2 * j + 1], out[j].z, out[j].w);
-    }
+}
+// Chunk j of four from them.
+template <int BITS>
+__device__ __forceinline__ uint4 code_chunk(const uint32_t* q, int j, const Lut<BITS>& lut) {
+    uint4 x;
+    lut.four(q[2 * j], x.x, x.y);
+    lut.four(q[2 * j + 1], x.z, x.w);
+    return x;
 }
 
-// Four chunks from 32 sign bits, left where they are: bits i and i + 16 of the word (or of the word moved down by 8,
+// Chunk j of four from 32 sign bits, left where they are: bits i and i + 16 of the word (or of the word moved down by 8,
 // for i = 8..15) as the lowest mantissa bits of two fp16 numbers, 2^(p - 24) with p = i mod 8 for a set bit and 0 for a
 // clear one (the matrix cores keep subnormals).  The queries carry the 2^(7 - p), and sum_i s_i x_i = 2 sum_i bit_i x_i -
 // sum_i x_i.
-__device__ __forceinline__ void expand_signs(uint32_t w, uint4* out) {
-    const uint32_t v = w >> 8;
+__device__ __forceinline__ uint4 sign_chunk(uint32_t w, int j) {
+    uint32_t x[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        uint32_t x[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = (j < 2 ? w : v) & (0x00010001u << ((4 * j + k) & 7));
-        out[j] = make_uint4(x[0], x[1], x[2], x[3]);
-    }
+    for (int k = 0; k < 4; ++k) x[k] = (j < 2 ? w : w >> 8) & (0x00010001u << ((4 * j + k) & 7));
+    return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
 // ------------------------------------------------------------------ queries
@@ -272,13 +270,15 @@ template <int RB>
 struct Tiles {
     static constexpr int W = 8;
     static constexpr int T = 64 * W;
+    // What is read at a lane's place and many constants from there comes first: a read's own offset reaches 64 KB, and behind that every
+    // read had an address register to itself
     struct Parts {
-        uint32_t table[256 * 64];
-        uint4 v[W][16 * 16];
         // the rows' operands for the signs and for the codes (these go on to registers with one block of rows; two do not fit)
         uint4 qs[RB][8 * 64], qc[RB][8 * 64];
         uint16_t kn[W][32], vn[W][32];
         float ratio[W][32];
+        uint32_t table[256 * 64];
+        uint4 v[W][16 * 16];
     };
     struct Sums {
         float4 o[W][32][32];  // chunks xor-swizzled by the row
@@ -518,53 +518,55 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
             // |r| / |k|, in the units of the sign products
             if constexpr (QJL) lds.t.ratio[wave][r] = tq::f16_to_f32(rn) * 0x1p18f / tq::f16_to_f32(k);
         }
-        // ---- scores: |k| (<codes> + |r| / |k| <signs>), the sign products' sums going into the codes'
+        // ---- scores: |k| (<codes> + |r| / |k| <signs>), the sign products' sums going into the codes'.  A step's chunk of the keys is made
+        // beside the products of the one before, and what it takes of the queries is on its way from LDS since two steps
         f32x16 x[RB];
 #pragma unroll
         for (int m = 0; m < RB; ++m) x[m] = zero16();
-        if constexpr (QJL) {
+        constexpr int SIGNS = QJL ? 8 : 0, STEPS = SIGNS + 8;
+        Frag ring[2][RB];
+        auto ask = [&](int i) INLINE {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                uint4 f[4];
-                expand_signs(ws[u], f);
+            for (int m = 0; m < RB; ++m) {
+                if (i < SIGNS) ring[i % 2][m].q = lds.t.qs[m][i * 64 + lane];
+                else if (RB > 1) ring[i % 2][m].q = lds.t.qc[m][(i - SIGNS) * 64 + lane];
+            }
+        };
+        uint32_t code[8];
+        auto chunk = [&](int i) INLINE {
+            Frag f;
+            if (i < SIGNS) {
+                f.q = sign_chunk(ws[i >> 2], i & 3);
+            } else {
+                if (((i - SIGNS) & 3) == 0) unpack32<KB>(wk + KB * ((i - SIGNS) >> 2), code);
+                f.q = code_chunk<KB>(code, (i - SIGNS) & 3, klut);
+            }
+            return f;
+        };
+        ask(0);
+        Frag now = chunk(0);
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            if (i + 1 < STEPS) ask(i + 1);
+            if (QJL && i == SIGNS) {
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    Frag kf, qf;
-                    kf.q = f[j];
+                    const f32x4 r4 = *reinterpret_cast<const f32x4*>(&lds.t.ratio[wave][8 * j + 4 * h]);
 #pragma unroll
-                    for (int m = 0; m < RB; ++m) {
-                        qf.q = lds.t.qs[m][(4 * u + j) * 64 + lane];
-                        x[m] = mfma_f16(kf, qf, x[m]);
-                    }
-                }
-                if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);  // the registers hold a few operands at a time
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+                    for (int m = 0; m < RB; ++m)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 r4 = *reinterpret_cast<const f32x4*>(&lds.t.ratio[wave][8 * j + 4 * h]);
-#pragma unroll
-                for (int m = 0; m < RB; ++m)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[m][4 * j + e] = (x[m][4 * j + e] + sign0[m]) * r4[e];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            uint4 f[4];
-            expand32<KB>(wk + KB * u, klut, f);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                Frag kf, qf;
-                kf.q = f[j];
-#pragma unroll
-                for (int m = 0; m < RB; ++m) {
-                    if constexpr (RB > 1) qf.q = lds.t.qc[m][(4 * u + j) * 64 + lane];
-                    x[m] = mfma_f16(kf, RB > 1 ? qf : q[4 * u + j], x[m]);
+                        for (int e = 0; e < 4; ++e) x[m][4 * j + e] = (x[m][4 * j + e] + sign0[m]) * r4[e];
                 }
             }
-            if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);
+            Frag next;
+            if (i + 1 < STEPS) next = chunk(i + 1);
+#pragma unroll
+            for (int m = 0; m < RB; ++m)
+                x[m] = mfma_f16(now, RB > 1 || i < SIGNS ? ring[i % 2][m] : q[(i - SIGNS) & 7], x[m]);
+            now = next;
+            if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);  // the registers hold a few operands at a time
         }
         // the largest finite |v| of the tile: its exponent decides the unit (2^(e + 1) is above it)
         const int e5 = (norm >> 10) & 31, ve = e5 == 31 ? 0 : e5;
