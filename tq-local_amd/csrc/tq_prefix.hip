@@ -242,19 +242,34 @@ struct Plan {
     size_t total() const { return o_bytes + ms_bytes + slots_bytes; }
 };
 
-// 32 rows where the sequences of a prompt have no more, 64 else.  A workgroup fills a CU: as many splits as fill the CUs, as long as
-// none is left without a tile.
+// Blocks of 32 rows, or of 64, whose tiles are decoded once for twice the rows.  In graphs, us, 32 and 64 rows: two sequences behind 1037
+// tokens 15.6 and 19.1, 56 rows behind each of four times 8192 (3-bit Q_mse) 28.9 and 32.5, 128 behind 32768 63.9 and 59.8, 160 behind
+// three times 131072 345 and 321.  A tile of 64 rows takes 5/3 of one of 32, and a workgroup's start and end 46 and 38 tiles of 32
+// rows (46 is 8 more, 3 us).  A workgroup fills a CU: as many splits as fill the CUs, as long as none is left without a tile.
 bool make_plan(int batch, int q_heads, int kv_heads, int prompts, bool uneven, int max_rows, int64_t n_prefix, int64_t n_own, Plan& p) {
     const int group = q_heads / kv_heads, each = batch / prompts;
     const int most = uneven ? std::min(batch, std::max(max_rows, 1)) : each;
     if (group > 64 || kv_heads > 65535 || (int64_t)batch * q_heads >= (int64_t)1 << 26) return false;
     if (n_prefix + 64 * n_own >= (int64_t)1 << 29) return false;  // sums of 64 items' tiles fit 32 bits
-    p.row_blocks = (int64_t)most * group <= 32 ? 1 : 2;
-    p.per = 32 * p.row_blocks / group;
-    p.items = uneven ? (int)std::min<int64_t>(batch, (int64_t)batch / p.per + prompts) : prompts * ((each + p.per - 1) / p.per);
-    const int64_t tiles = (n_prefix + TK - 1) / TK + std::min(p.per, batch) * ((n_own + TK - 1) / TK);
-    const int64_t useful = std::min<int64_t>(std::max<int64_t>(1, (tiles + MIN_TILES - 1) / MIN_TILES), MAX_SPLIT);
-    p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)p.items * kv_heads), useful));
+    int64_t useful = 1;
+    // the plan for blocks of 32 row_blocks rows; returns what it takes, in thirds of a tile of 32 rows
+    auto take = [&](int row_blocks) {
+        p.row_blocks = row_blocks;
+        p.per = 32 * row_blocks / group;
+        p.items = uneven ? (int)std::min<int64_t>(batch, (int64_t)batch / p.per + prompts) : prompts * ((each + p.per - 1) / p.per);
+        const int64_t tiles = (n_prefix + TK - 1) / TK + std::min(p.per, batch) * ((n_own + TK - 1) / TK);
+        useful = std::min<int64_t>(std::max<int64_t>(1, (tiles + MIN_TILES - 1) / MIN_TILES), MAX_SPLIT);
+        p.n_split = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)p.items * kv_heads), useful));
+        // (uneven items are taken as full ones: how many there are the device knows)
+        const int64_t groups = (int64_t)(uneven ? (batch + p.per - 1) / p.per : p.items) * kv_heads;
+        const int64_t split = std::max<int64_t>(1, std::min<int64_t>(256 / groups, useful));
+        const int64_t rounds = (groups * split + 255) / 256, each_has = (tiles + split - 1) / split;
+        return rounds * (row_blocks == 1 ? 114 + 3 * each_has : 138 + 5 * each_has);
+    };
+    // (more than 32 query heads take 64 rows, a prompt's few rows 32)
+    const bool one = group <= 32, two = (int64_t)most * group > 32;
+    const int64_t of_two = two ? take(2) : 0, of_one = one ? take(1) : 0;
+    if (two && (!one || of_two < of_one)) take(2);
     p.n_slots = (int)std::max<int64_t>((int64_t)p.n_split * p.items, std::min<int64_t>(256 / kv_heads, useful * p.items));
     const size_t rows = (size_t)p.n_slots * kv_heads * 32 * p.row_blocks;
     p.o_bytes = rows * D * 4, p.ms_bytes = rows * 8, p.slots_bytes = (size_t)batch * 16;
