@@ -417,3 +417,26 @@ def test_a_refused_call_changes_nothing(cuda):
     assert first._batch() == other._batch() == 2
     other.attend_blocks(None)
     assert share_prefix(Cache(layers=[first, other]), 3).layers[1].batch == 6
+
+
+def test_both_attention_interfaces_take_shared_layers(cuda):
+    from turboquant.runtime.attention import turboquant_attention_forward, turboquant_prompt_forward
+
+    shared, copied = both((2, 1), 2, 90)
+    for layer in (shared, copied):
+        append(layer, 3, 2, 7, 50)
+    k, v = rows64(copied)
+    module = torch.nn.Module()
+    module._tq_cache_layer, module.num_key_value_groups = shared, 4
+    for S in (1, 3):
+        q = randn((3, 8, S, D), S)
+        want = shared_prefix_attention(q, shared).transpose(1, 2)
+        for forward in (turboquant_attention_forward, turboquant_prompt_forward):
+            got, _ = forward(module, q, None, None, None)
+            assert torch.equal(got, want)
+    got, _ = turboquant_prompt_forward(module, q, None, None, None, is_causal=False)
+    for i in range(3):
+        check(got[:, i], attend64(q[:, :, i], k, v)[0], 2e-2)  # bf16 rows and weights, as above
+    cu = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="packed sequences"):
+        turboquant_prompt_forward(module, q, None, None, None, cu_seq_lens_q=cu)

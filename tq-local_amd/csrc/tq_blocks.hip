@@ -6,9 +6,14 @@
 // a whole number below 2^22, the step a power of two, and so every score is exact in fp32, whatever the order of its sum.  The same
 // blocks are chosen everywhere, and a block's bounds are the same however its keys arrived.
 //
-//   bounds_kernel  a block per wave, 16 bytes of four keys a lane and load, all of a block's loads in flight together
+//   bounds_kernel  a block per wave, 16 bytes of four keys a lane and load, all of a block's loads in flight together.  Bound by memory:
+//                  8 sequences of 32768 tokens of 8 KV heads (537 MB) take 94 to 99 us, 5.4 to 5.7 TB/s; one of 131072 43 us, 6.3 TB/s
+//                  (part of it from the last-level cache); a block of each of 64 KV heads 4 us, first bytes and launch
 //   select_kernel  a KV head's whole choice per workgroup: scores by v_mfma_i32_16x16x64_i8, a column for a block, then the keep-th
-//                  largest by radix and the chosen numbers in order
+//                  largest by radix and the chosen numbers in order.  Bound by the steps that wait for one another: 32 of 129 blocks
+//                  for 8 KV heads take 6.3 us, 64 of 512 for 64 KV heads 10
+//   score_kernel   the scores of longer histories, spread over the CUs; the choice then reads 4 bytes of a block instead of 260.  128 of
+//                  2048 blocks for 32 KV heads take 14.5 us, the scores 6 of them (17 MB, 2.8 TB/s) and the choice 7
 
 #include <algorithm>
 
@@ -55,7 +60,9 @@ struct BoundsArgs {
     int8_t* lohi;
     float* step;
     int64_t cap, first, per_head, all;  // blocks to a head, and of all heads
-    int heads_next;                     // whether neighbouring waves have a block's heads, or a head's blocks
+    // whether neighbouring waves have a block's heads, or a head's blocks: what is next to one another in memory.  The 8 sequences above, us,
+    // a head's blocks and a block's heads: rows of a token together 99 and 94, rows of a head together 97 and 108
+    int heads_next;
 };
 
 constexpr int BOUNDS_WAVES = 4;
@@ -134,7 +141,7 @@ struct SelectArgs {
 
 constexpr int ST = 512, SW = ST / 64;  // threads and waves of a workgroup
 constexpr int TILE = 16;               // blocks of a matrix instruction
-constexpr int AHEAD = 4;               // tiles of a wave whose bounds are on their way together
+constexpr int AHEAD = 4;               // tiles of a wave whose bounds are on their way together: all that it has of 512 blocks
 constexpr uint32_t ALWAYS = 0xFFFFFFFFu;
 
 // The blocks of a row's range: [lo, lo + n).
@@ -378,8 +385,9 @@ __global__ __launch_bounds__(ST) void select_kernel(SelectArgs a, const uint32_t
     }
 }
 
-// One workgroup for a KV head's whole choice up to here, else its scores in a launch of their own, spread over the CUs: a workgroup takes its
-// bounds at about 36 GB/s.
+// One workgroup for a KV head's whole choice up to here, else its scores in a launch of their own, spread over the CUs: a workgroup alone takes
+// its bounds at about 36 GB/s, but a launch more is 4 us of the host.  In graphs, us, in one and in two launches: 128 blocks 6.5 and 8.0, 256
+// 7.4 and 8.1, 512 9.7 and 8.5 (from the host 13.4 and 17; for 256 KV heads 12.5 and 14.8), 1024 14.5 and 9.3, 2048 22.7 and 11.3.
 constexpr int FUSED_BLOCKS = 512;
 
 }  // namespace

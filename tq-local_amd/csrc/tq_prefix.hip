@@ -7,6 +7,16 @@
 //                  query heads.  Its tiles are the prompt's, which every row attends to, then the own tokens of its sequences, each of
 //                  which only that sequence's rows attend to.  The splits of an item share its tiles
 //   merge_kernel   the splits' partials of a row weighed and added, rotated back by R_v
+//
+// Cost (kernel and merge, in a graph).  Long prompts are bound by the tiles' decoding and softmax beside the matrix instructions, as the
+// trees are: three prompts of 131072 tokens with 21, 3 and 8 sequences (8 KV heads of 5 query heads, 4-bit Q_prod) take 319 us, the 458 MB of
+// codes at 1.4 TB/s, the products at 0.41 PFLOP/s (0.69 with the rows that fill the blocks up); vector instructions have 59% and matrix instructions 36% of a
+// SIMD's time, at the 1.9 GHz that this leaves.  32 sequences behind 32768 tokens (8 of 4 heads) take 60 us, 8 sequences behind each of
+// four padded prompts of 8192 tokens (4 of 7 heads, 3-bit Q_mse, fp16) 29.5.  Small calls are bound by what comes before the first tile
+// and after the last: two sequences behind 1037 tokens take 15.6, the kernel 12 (the first bytes from memory, the queries' rotation, the
+// table of values, the waves' meeting, 1 to 3 us each) and the merge 4.
+// A copy of the prompt for every sequence and tq_decode_attention (8 of 4 heads, 4-bit Q_prod): 16 sequences behind 32768 tokens 114 us,
+// here 43; 16 behind 8192 34 and 25; 4 behind 8192 16.4 and 20.5.
 
 #include "tq_tiles.h"
 
@@ -102,8 +112,9 @@ struct Slot {
     Item item;
     int first, n, step;
 };
-// Up to 64 items of up to 64 prompts and SHARED_ROWS sequences share the slots in proportion to their tiles, each with one at least; what is
-// left over goes unused (count = 0).  All that it reads is asked for together: one wait for memory where a loop over an item's
+// Where lengths may differ, up to 64 items of up to 64 prompts and SHARED_ROWS sequences share the slots in proportion to their tiles, each
+// with one at least; what is left over goes unused (count = 0).  Equal numbers of slots and shares, in graphs, us: two sequences behind each of a
+// prompt of 32768 tokens and seven of 2000 90 and 38, the three prompts above 339 and 315, eight equal prompts 103 and 105.  All that it reads is asked for together: one wait for memory where a loop over an item's
 // sequences had one for each.
 constexpr int SHARED_ROWS = 256;
 struct Shared {
@@ -234,6 +245,8 @@ __global__ __launch_bounds__(MERGE_T) void merge_kernel(Merge a, PrefixRows rows
     merge_rows<ROWS>(a, rows);
 }
 
+// Rows up to which the merge has 4 of them to a workgroup, which is done with them sooner; 16 beyond, which read the matrix R_v once for
+// more.  16 rows always and 4 always, in graphs, us: 64 rows 19.4 and 15.6, 1024 rows 63.3 and 59.8, 1280 rows 323.4 and 320.8.
 constexpr int FEW_ROWS = 2048;
 
 struct Plan {
@@ -362,7 +375,6 @@ extern "C" int tq_prefix_attention(const void* q, int q_type, int batch, int q_h
     TQ_CHECK_LAUNCH();
     const Merge m{(int64_t)batch * q_heads, c.part_o, c.part_ms, value_rotation, out_f32, out_16, q_type == 2, lse_out};
     const PrefixRows rows{q_heads, kv_heads, 32 * p.row_blocks, row_slots};
-    // few rows are spread over more workgroups, which are done with theirs sooner
     if (m.all_rows <= FEW_ROWS)
         hipLaunchKernelGGL(merge_kernel<4>, dim3((unsigned)((m.all_rows + 3) / 4)), dim3(MERGE_T), 0, s, m, rows);
     else

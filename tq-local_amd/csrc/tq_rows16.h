@@ -1,4 +1,4 @@
-// tq_rows16.h -- 16-bit matrix-core products over rows of 128 elements in LDS, shared by prompt and tree attention (gfx950).
+// tq_rows16.h -- 16-bit matrix-core products over rows of 128 elements in LDS, shared by the prompts' attention and that over packed tiles (gfx950).
 //
 // A row is 256 bytes, its 16-byte chunk c at slot c ^ swizzle(token): the low four bits of the token with the bits 0-1 on top, so
 // that the 16 rows of an operand's read, and the 4 x 2 rows that ds_read_b64_tr_b16 turns around, meet every bank once.

@@ -663,8 +663,8 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
     for (; tile < whole; tile += step_tiles) step(tile, std::false_type{});
     for (; tile < tiles; tile += step_tiles) step(tile, std::true_type{});
 
-    // ---- the waves' sums, one block of rows at a time.  What a wave's sums weigh is found once for a row, beside the sums' way to LDS: every
-    // thread of a row for itself, it took half of the 6000 cycles of a block
+    // ---- the waves' sums, one block of rows at a time.  What a wave's sums weigh is found once for a row, beside the sums' way to LDS (by every
+    // thread of a row for itself a call took 0.8 us more)
     const float unit = __uint_as_float((uint32_t)(127 - shift) << 23);
     __syncthreads();
 #pragma unroll
