@@ -480,3 +480,17 @@ def test_choices_that_are_none():
     for bad in ((2, 1, 2), (5, -1, 1), (5, 1, 0), (K.MAX_BLOCKS + 1, 1, 1)):
         with pytest.raises(ValueError):
             BlockChoice(*bad)
+
+
+@pytest.mark.parametrize("cap", [0, 130])
+def test_histories_without_tokens(cuda, cap):
+    layer = make_layer(2, 2, 130, 4, True)
+    cache = {name: t[:, :, :cap].contiguous() for name, t in arrays(layer).items()}
+    q, blocks = randn((2, 8, D), 5), torch.arange(3, dtype=torch.int32, device="cuda").expand(2, 2, 3)
+    got, lse = K.block_attention(q, blocks, **cache, **codec(layer), n_tokens=0, want_lse=True)
+    assert (got == 0).all() and (lse == -math.inf).all()
+    bounds = torch.zeros(2, 2, cap // 64, 2, D, dtype=torch.int8, device="cuda"), torch.zeros(2, 2, cap // 64, device="cuda")
+    assert (K.select_blocks(q, *bounds, n_tokens=0, keep=4) == -1).all()
+    before = [t.clone() for t in bounds]
+    K.block_bounds(torch.empty(2, 2, 0, D, dtype=torch.bfloat16, device="cuda"), *bounds)
+    assert all(torch.equal(a, b) for a, b in zip(bounds, before))

@@ -440,3 +440,30 @@ def test_both_attention_interfaces_take_shared_layers(cuda):
     cu = torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="packed sequences"):
         turboquant_prompt_forward(module, q, None, None, None, cu_seq_lens_q=cu)
+
+
+@pytest.mark.parametrize("cap", [0, 40])
+def test_caches_without_tokens(cuda, cap):
+    """No tokens at all, with room for some or without: zero and -inf."""
+    layer = make_layer(2, 2, 40, 4, True)
+    empty = {name: t[:, :, :cap].contiguous() for name, t in arrays(layer).items()}
+    own = {name: t[:1, :, :cap].expand(4, *t.shape[1:2], *t[:, :, :cap].shape[2:]).contiguous() for name, t in arrays(layer).items()}
+    q = randn((4, 8, D), 5)
+    for mine in (None, own):
+        got, lse = K.prefix_attention(q, empty, mine, n_prefix=0, **codec(layer), want_lse=True)
+        assert (got == 0).all() and (lse == -math.inf).all()
+    if cap:  # a sequence's own tokens alone
+        got = K.prefix_attention(q, empty, own, n_prefix=0, n_own=30, **codec(layer))
+        k, v = rows64(layer)
+        check(got, attend64(q, *(x[:1, :, :30].expand(4, -1, -1, -1) for x in (k, v)))[0])
+
+
+def test_as_many_query_heads_as_are_taken(cuda):
+    layer = make_layer(2, 1, 70, 4, True)
+    k, v = rows64(layer)
+    for group in (33, 47, 64):
+        q = randn((4, group, D), group)
+        got = K.prefix_attention(q, arrays(layer), None, n_prefix=70, **codec(layer))
+        check(got, attend64(q, k.repeat_interleave(2, 0), v.repeat_interleave(2, 0))[0])
+    with pytest.raises(Exception):
+        K.prefix_attention(randn((4, 65, D), 1), arrays(layer), None, n_prefix=70, **codec(layer))
