@@ -494,3 +494,15 @@ def test_histories_without_tokens(cuda, cap):
     before = [t.clone() for t in bounds]
     K.block_bounds(torch.empty(2, 2, 0, D, dtype=torch.bfloat16, device="cuda"), *bounds)
     assert all(torch.equal(a, b) for a, b in zip(bounds, before))
+
+
+def test_bounds_past_32_bits(cuda):
+    """Bounds of a KV head that begin past 2^32 bytes of their buffer: as of a small one."""
+    rows, q = randn((1, 5, 700, D), 3), randn((1, 10, D), 4)
+    cap = 1 << 22  # 256 bytes a block: 1 GB a head
+    both = [(torch.empty(1, 5, n, 2, D, dtype=torch.int8, device="cuda"), torch.empty(1, 5, n, device="cuda")) for n in (11, cap)]
+    for lohi, step in both:
+        K.block_bounds(rows, lohi, step)
+    assert torch.equal(both[0][0], both[1][0][:, :, :11]) and torch.equal(both[0][1], both[1][1][:, :, :11])
+    chosen = [K.select_blocks(q, *b, n_tokens=700, keep=4, n_blocks=11) for b in both]
+    assert torch.equal(*chosen) and torch.equal(chosen[0].cpu(), select_ref(q, *both[0], 700, 4, 1, 1))

@@ -467,3 +467,20 @@ def test_as_many_query_heads_as_are_taken(cuda):
         check(got, attend64(q, k.repeat_interleave(2, 0), v.repeat_interleave(2, 0))[0])
     with pytest.raises(Exception):
         K.prefix_attention(randn((4, 65, D), 1), arrays(layer), None, n_prefix=70, **codec(layer))
+
+
+def test_a_prompt_past_32_bits(cuda):
+    """Codes of a KV head that begin past 2^32 bytes of their buffer, and a prompt far into its row."""
+    layer = make_layer(1, 2, 200, 4, False, seed=11)
+    cap, H, first = (1 << 24) - 1, 5, 1 << 23  # 64 bytes a slot: 1 GB a head
+    big = {}
+    for name, t in arrays(layer).items():
+        if t is None:
+            big[name] = None
+            continue
+        big[name] = torch.empty(1, H, cap, *t.shape[3:], dtype=t.dtype, device="cuda")
+        big[name][:, :, first:first + 200] = t[:, :1, :200]
+    q = randn((3, H * 2, D), 5)
+    got = K.prefix_attention(q, big, None, n_prefix=first + 200, prefix_starts=i32([first]), **codec(layer))
+    k, v = (x[:, :1].expand(3, H, -1, -1) for x in rows64(layer))
+    check(got, attend64(q, k, v)[0])
