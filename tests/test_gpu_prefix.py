@@ -484,3 +484,21 @@ def test_a_prompt_past_32_bits(cuda):
     got = K.prefix_attention(q, big, None, n_prefix=first + 200, prefix_starts=i32([first]), **codec(layer))
     k, v = (x[:, :1].expand(3, H, -1, -1) for x in rows64(layer))
     check(got, attend64(q, k, v)[0])
+
+
+def test_attention_switched_off_and_on_again(cuda):
+    from turboquant.adapters.transformers import disable_turboquant_attention, enable_turboquant_attention
+
+    model = tiny_llama("cuda", torch.bfloat16, layers=2, heads=8, kv_heads=2)
+    ids = torch.randint(0, 94, (1, 40), generator=torch.Generator().manual_seed(3)).cuda()
+    with torch.no_grad():
+        cache = share_prefix(build_packed_mse_cache(model(input_ids=ids, use_cache=True).past_key_values, bits=4, use_qjl_keys=True,
+                                                    quantize_decode=True, norm_guard=False), 3)
+        mask = torch.ones(3, 40, dtype=torch.int64, device="cuda")
+        for i in range(4):
+            mask = torch.cat((mask, mask.new_ones(3, 1)), 1)
+            old = enable_turboquant_attention(model, cache) if i != 1 else None
+            out = model(input_ids=ids[:, i:i + 1].expand(3, 1), attention_mask=mask, past_key_values=cache, use_cache=True).logits
+            assert torch.isfinite(out).all() and cache.get_seq_length() == 41 + i
+            if i != 1:
+                disable_turboquant_attention(model, cache, old)

@@ -474,12 +474,13 @@ def _shared_ranges(layer: "SharedPrefixLayer", mask: torch.Tensor | None, device
     """(prefix starts, prefix ends, own ends) of a step's mask, int32 or None.
 
     ``_HoleyMask`` where a row's tokens are not one range, or where the sequences of a prompt do not share its padding: a host
-    sync to find out, which a layer with ``_tq_mask_contiguous`` set spares (as for ``fused_attention``)."""
+    sync to find out, which a caller spares who knows and says so in the layer's ``_tq_mask_contiguous``: True, every mask is
+    of such ranges, or False (as for ``fused_attention``)."""
     if mask is None:
         return None, None, None
-    if layer._tq_mask_contiguous is False:
+    known = getattr(layer, "_tq_mask_contiguous", None)
+    if known is False:
         raise _HoleyMask
-    known = layer._tq_mask_contiguous is not None
     n = layer.prefix.packed_seq_length()
     starts, ends = _valid_range(mask, layer.batch, layer.get_seq_length(), device, check_contiguous=not known)
     first, last = starts[layer.first_of], ends.clamp(max=n)[layer.first_of]

@@ -39,8 +39,6 @@ class SharedPrefixLayer(CacheLayerMixin):
         self.is_initialized = True
         self.device, self.dtype = prefix.device, prefix.dtype
         self._force_dense = False
-        #: True: the caller knows every step's mask to be one range per row, with the padding of the prompt; False: not; None: looked at
-        self._tq_mask_contiguous: bool | None = getattr(prefix, "_tq_mask_contiguous", None)
         self._set_counts([int(n) for n in counts])
 
     def _set_counts(self, counts: list[int]) -> None:
