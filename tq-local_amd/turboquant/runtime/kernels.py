@@ -1078,7 +1078,7 @@ def select_blocks(q: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, *, n_
         raise ValueError(f"select_blocks: keep {keep} (at most {MAX_BLOCKS}) with {sink} first and {recent} last blocks")
     seq_starts = _int32_on(seq_starts, dev, "seq_starts", (B,))
     seq_lens = _int32_on(seq_lens, dev, "seq_lens", (B,))
-    out = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    out = q.new_empty((B, Hkv, keep), dtype=torch.int32)
     if B and Hq:
         need = _lib.load().tq_select_blocks_workspace_bytes(B, Hkv, n_tokens)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None

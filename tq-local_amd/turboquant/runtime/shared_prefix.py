@@ -183,9 +183,9 @@ class SharedPrefixLayer(CacheLayerMixin):
 def share_prefix(cache: Cache, sequences: int | Sequence[int]) -> Cache:
     """A cache whose prompts are continued by several sequences each: ``sequences`` of them for every row, or a number for each.
 
-    The packed layers of ``cache`` become the shared prompts of the result's layers; they are not copied, and the
-    given cache is to be used no further; the attention backend is switched on for the new one.  Layers that cannot be shared are copied for every sequence.  Shared layers attend to
-    all of their tokens: a choice of blocks (``attend_blocks``) is refused."""
+    The packed layers of ``cache`` become the shared prompts of the result's layers; they are not copied, and the given cache is to
+    be used no further; the attention backend is switched on for the new one.  Layers that cannot be shared are copied for every
+    sequence.  Shared layers attend to all of their tokens: a choice of blocks (``attend_blocks``) is refused."""
     per_layer = []  # looked over before any layer is changed
     for layer in cache.layers:
         if not isinstance(layer, PackedMSELayer):
