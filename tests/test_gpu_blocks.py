@@ -2,6 +2,7 @@
 number (infinities, NaN, zeros, subnormal keys, equal scores), attention in 64 bits at block and tile edges, ranges and numbers that name
 nothing; the layer's choice kept in step with its tokens, and a run of all three."""
 
+import copy
 import math
 
 import numpy as np
@@ -506,3 +507,40 @@ def test_bounds_past_32_bits(cuda):
     assert torch.equal(both[0][0], both[1][0][:, :, :11]) and torch.equal(both[0][1], both[1][1][:, :, :11])
     chosen = [K.select_blocks(q, *b, n_tokens=700, keep=4, n_blocks=11) for b in both]
     assert torch.equal(*chosen) and torch.equal(chosen[0].cpu(), select_ref(q, *both[0], 700, 4, 1, 1))
+
+
+def test_bounds_that_another_stream_makes(cuda):
+    """A step on a stream that waits for the tokens alone attends to the same blocks as the step that makes the bounds, which is
+    still held up on its own stream."""
+    layer = make_layer(2, 2, 1500, 4, True, seed=21, reserve_tokens=64)
+    q, choice = randn((2, 8, 1, D), 5), BlockChoice(5, 1, 1)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def want():
+        n = layer.packed_seq_length()
+        lohi, step = (torch.from_numpy(t).cuda() for t in bounds_ref(layer._key_rows(0, n)))
+        return select_ref(q[:, :, 0], lohi, step, n, 5, 1, 1)
+
+    lohi, step, _ = layer.block_bounds()
+    lohi.zero_(), step.zero_()  # bounds by which the first blocks would be chosen
+    layer._forget_bounds(0)
+    for i in range(3):
+        torch.cuda.synchronize()
+        got = []
+        for s, held_up in ((streams[i % 2], 10_000_000), (streams[1 - i % 2], 0)):
+            with torch.cuda.stream(s):
+                if held_up:
+                    torch.cuda._sleep(held_up)
+                got.append(layer.choose_blocks(q, choice))
+        got.append(layer.choose_blocks(q, choice))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g.cpu(), want()) for g in got)
+        layer.update(*(kv_bf16((2, 2, 700, D), seed=90 + 2 * i + j) for j in range(2)))  # the buffers grow
+    with torch.cuda.stream(streams[0]):
+        torch.cuda._sleep(10_000_000)
+        layer.choose_blocks(q, choice)
+    with torch.cuda.stream(streams[1]):  # a copy is the stream's that makes it
+        other = copy.deepcopy(layer)
+        got = other.choose_blocks(q, choice)
+    torch.cuda.synchronize()
+    assert torch.equal(got.cpu(), want())

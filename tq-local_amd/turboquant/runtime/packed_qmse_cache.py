@@ -219,16 +219,50 @@ def _split_spec(sc: SplitCodecs) -> dict[str, tuple[tuple, torch.dtype] | None]:
 
 
 class _BlockBounds:
-    """Bounds of the keys of a layer's blocks of 64 tokens, the first ``count`` of them known."""
+    """Bounds of the keys of a layer's blocks of 64 tokens, the first ``count`` of them known.
+
+    A step makes what is missing on its own stream and the host counts it at once, so a step on another stream, which its caller
+    has wait for the tokens alone, waits here for whoever wrote bounds last (who had waited for those before)."""
 
     def __init__(self, B: int, H: int, cap: int, D: int, device: torch.device):
         self.lohi = torch.empty(B, H, cap, 2, D, dtype=torch.int8, device=device)
         self.step = torch.empty(B, H, cap, dtype=torch.float32, device=device)
         self.count = 0
+        self._home = K._stream_handle(self.step.device)  # the stream that the buffers are of
+        self._wrote: tuple[int, torch.cuda.Event] | None = None  # the stream that wrote last, and when
+
+    def ordered(self) -> None:
+        """The current stream waits for what others wrote, and the buffers are kept until it is done with them.  Not while it is
+        captured: a captured step takes bounds that were there before the capture."""
+        at = K._stream_handle(self.step.device)
+        other = self._wrote is not None and self._wrote[0] != at
+        if (at == self._home and not other) or torch.cuda.is_current_stream_capturing():
+            return
+        stream = torch.cuda.current_stream(self.step.device)
+        if other:
+            stream.wait_event(self._wrote[1])
+        if at != self._home:
+            for t in (self.lohi, self.step):
+                t.record_stream(stream)
+
+    def written(self) -> None:
+        """By the current stream."""
+        if torch.cuda.is_current_stream_capturing():
+            return
+        event = torch.cuda.Event() if self._wrote is None else self._wrote[1]
+        event.record(torch.cuda.current_stream(self.step.device))
+        self._wrote = K._stream_handle(self.step.device), event
 
     def take(self, rows: torch.Tensor | None, cap: int) -> None:
         """These batch rows of it, with room for ``cap`` blocks."""
+        self.ordered()
         self.lohi, self.step = K.gather_tokens([self.lohi, self.step], tokens=self.count, rows=rows, capacity=cap)
+        self._home = K._stream_handle(self.step.device)
+        self.written()
+
+    def __getstate__(self) -> dict:  # copies are the current stream's
+        self.ordered()
+        return {**self.__dict__, "_home": K._stream_handle(self.step.device), "_wrote": None}
 
 
 @dataclass(frozen=True)
@@ -674,11 +708,15 @@ class PackedMSELayer(CacheLayerMixin):
             b = self._bounds = _BlockBounds(B, H, n + max(1, self.reserve_tokens // K.BLOCK_TOKENS), D, self._store.device)
         elif n > b.lohi.shape[2]:
             b.take(None, max(n + self.reserve_tokens // K.BLOCK_TOKENS, 2 * b.lohi.shape[2]))
+        b.ordered()
+        if n <= b.count:
+            return b.lohi, b.step, b.count
         most = max(1, _BOUNDS_BYTES // (B * H * D * 2 * K.BLOCK_TOKENS))  # blocks decoded at once
         for first in range(b.count, n, most):
             to = min(first + most, n)
             K.block_bounds(self._key_rows(first * K.BLOCK_TOKENS, to * K.BLOCK_TOKENS), b.lohi, b.step, first=first)
             b.count = to
+        b.written()
         return b.lohi, b.step, b.count
 
     def choose_blocks(self, query: torch.Tensor, choice: BlockChoice, seq_starts: torch.Tensor | None = None,
