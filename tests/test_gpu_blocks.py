@@ -84,6 +84,23 @@ def test_bounds_of_special_keys(cuda):
     assert step[0, 0, 8] == 1.0 and step[0, 0, 9] == 2.0 and step[0, 0, 0] == 2.0 ** -100
 
 
+def test_bounds_of_numbers_far_below_the_step(cuda):
+    """Outward also where a number over the step has no fp32 of its own: behind an infinity, and of finite keys."""
+    k = torch.zeros(1, 1, 64 * 5, D, dtype=torch.bfloat16, device="cuda")
+    v = k.view(5, 64, D)
+    small = 2.0 ** torch.tensor([-40.0, -49, -50, -51, -60, -126, -133], device="cuda")
+    for block, largest in enumerate((math.inf, 2.0 ** 31, 2.0 ** 100, 2.0 ** 20, -math.inf)):
+        v[block] = 1.0
+        v[block, 0, 0] = largest
+        v[block, 3, 1:8], v[block, 4, 8:15] = small, -small
+        v[block, :, 16:23], v[block, :, 24:31] = small, -small  # nothing else in these channels
+        v[block, :, 32], v[block, :, 33] = 0.0, -0.0
+    lohi, step = bounds(k)
+    same_bounds(k, lohi, step)
+    assert (lohi[0, 0, :, 1, 16:23] == 1).all() and (lohi[0, 0, :, 0, 24:31] == -1).all()
+    assert (lohi[0, 0, :, :, 32:34] == 0).all()
+
+
 def test_bounds_hold_and_arrive_in_any_pieces(cuda):
     k = randn((2, 2, 300, D), 7)
     lohi, step = bounds(k, 5)

@@ -117,7 +117,9 @@ __global__ __launch_bounds__(64 * BOUNDS_WAVES) void bounds_kernel(BoundsArgs a)
         const uint32_t w = upper ? hi[j >> 1] : lo[j >> 1], bits = j & 1 ? w & 0xFFFF0000u : w << 16;
         // an infinity for NaN too
         const float v = __uint_as_float((bits & 0x80000000u) | std::min(bits & 0x7FFFFFFFu, 0x7F800000u)) * down;
-        const float r = fminf(fmaxf(upper ? __builtin_ceilf(v) : __builtin_floorf(v), -127.0f), 127.0f);
+        float r = fminf(fmaxf(upper ? __builtin_ceilf(v) : __builtin_floorf(v), -127.0f), 127.0f);
+        // a number less than 2^-149 of a step gives the product 0, and is rounded outward all the same
+        if (r == 0.0f && (bits << 1) != 0u && upper != (bool)(bits >> 31)) r = upper ? 1.0f : -1.0f;
         out[j >> 2] |= ((uint32_t)(int)r & 0xFFu) << (8 * (j & 3));
     }
     const int64_t to = group * a.cap + a.first + block;
