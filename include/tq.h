@@ -453,6 +453,9 @@ int tq_prefix_attention(const void* q, int q_type, int batch, int q_heads, int k
 #define TQ_MAX_BLOCKS 4096 /* blocks chosen for one KV head */
 int tq_block_bounds(const uint16_t* k, int batch, int heads, int64_t tokens, int dim, int64_t k_sb, int64_t k_sh, int64_t k_st,
                     int8_t* lohi, float* step, int64_t cap, int64_t first, void* stream);
+/* The same of keys of another type, k_type 0: bf16, 1: fp32, 2: fp16; the bounds are of the keys as they are given. */
+int tq_block_bounds_typed(const void* k, int k_type, int batch, int heads, int64_t tokens, int dim, int64_t k_sb, int64_t k_sh,
+                          int64_t k_st, int8_t* lohi, float* step, int64_t cap, int64_t first, void* stream);
 
 /*
  * tq_select_blocks: for each KV head of each row the `keep` blocks that its query heads may give the largest logits, by the bounds of

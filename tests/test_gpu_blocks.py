@@ -101,6 +101,49 @@ def test_bounds_of_numbers_far_below_the_step(cuda):
     assert (lohi[0, 0, :, :, 32:34] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("B,H,T,first", [(1, 1, 1, 0), (1, 2, 63, 0), (2, 3, 64, 2), (1, 2, 65, 1), (2, 4, 1000, 5)])
+def test_bounds_of_keys_of_other_types(cuda, dtype, B, H, T, first):
+    """Of the keys as given, not of what a rounding to bf16 leaves of them."""
+    k = (randn((B, T, H, D), 3, torch.float32) * 2.0 ** randn((B, T, H, 1), 4).float()).to(dtype).transpose(1, 2)
+    assert not torch.equal(k, k.bfloat16().to(dtype))
+    n = -(-T // 64)
+    lohi, step = bounds(k, first + n + 3, first)
+    same_bounds(k, lohi, step, first)
+    for t, v in ((lohi, 77), (step, -7.0)):  # the other blocks stay as they were
+        assert (t[:, :, :first] == v).all() and (t[:, :, first + n:] == v).all()
+    wide = torch.zeros(*k.shape[:3], D + 1, dtype=dtype, device="cuda")[..., 1:]  # rows at any element
+    wide.copy_(k)
+    assert all(torch.equal(a, b) for a, b in zip(bounds(k), bounds(wide)))
+
+
+def test_bounds_of_special_keys_of_other_types(cuda):
+    k = torch.zeros(1, 1, 64 * 10, D, dtype=torch.float16, device="cuda")
+    v = k.view(10, 64, D)
+    v[0, 3, 5] = 126.0625  # 126 in bf16
+    v[1, 5, 3], v[1, 6, 4] = math.inf, 2.0 ** -24
+    v[2, 0, 0] = -math.inf
+    v[3, 63, 127], v[3, 1, 2] = math.nan, -1.0
+    v[4, 9, 9] = -torch.tensor(math.nan)
+    v[5], v[6] = 65504.0, -65504.0
+    v[7, 1, 1] = -2.0 ** -24  # subnormal
+    v[8, 2, 2], v[8, 2, 3] = 127.0, -0.5
+    v[9] = -0.0
+    for t in (k, k.float()):
+        lohi, step = bounds(t)
+        same_bounds(t, lohi, step)
+        assert lohi[0, 0, 0, 1, 5] == 127 and step[0, 0, 0] == 1.0
+    k = torch.zeros(1, 1, 64 * 5, D, device="cuda")
+    v = k.view(5, 64, D)
+    v[0, 1, 1], v[0, 1, 2] = 2.0 ** -149, -2.0 ** -149
+    v[1], v[1, 5] = torch.finfo(torch.float32).max, -torch.finfo(torch.float32).max
+    v[2, 7, 7], v[2, 8, 8], v[2, 9, 9] = 2.0 ** 31, -2.0 ** -126, 2.0 ** -149
+    v[3, 7, 7], v[3, 8, 8] = 127.00001, -127.0
+    v[4, 0, 0], v[4, 0, 1] = -127.0 * 2.0 ** 100, 1.0 + 2.0 ** -23
+    lohi, step = bounds(k)
+    same_bounds(k, lohi, step)
+
+
 def test_bounds_hold_and_arrive_in_any_pieces(cuda):
     k = randn((2, 2, 300, D), 7)
     lohi, step = bounds(k, 5)

@@ -68,6 +68,20 @@ def test_block_bounds_rejects_on_host(status, change):
     assert _lib.load().tq_block_bounds(*dict(BOUNDS, **change).values()) == status
 
 
+@pytest.mark.parametrize("status,change", [
+    (INVALID, dict(k_type=3)), (INVALID, dict(k_type=-1)), (INVALID, dict(k=None)), (UNSUPPORTED, dict(st=132)),
+    (UNSUPPORTED, dict(k_type=2, st=132)), (UNSUPPORTED, dict(k_type=1, st=130)), (UNSUPPORTED, dict(k_type=1, k=ODD)),
+    (UNSUPPORTED, dict(k_type=1, lohi=ODD))])
+def test_block_bounds_of_other_types_rejects_on_host(status, change):
+    args = {"k": FAKE, "k_type": 0, **BOUNDS}
+    assert _lib.load().tq_block_bounds_typed(*dict(args, **change).values()) == status
+
+
+def test_block_bounds_takes_keys_of_three_types():
+    with pytest.raises(ValueError, match="fp16 or fp32"):
+        K.block_bounds(torch.zeros(1, 2, 64, 128, dtype=torch.float64), *lohi_step())
+
+
 SELECT = dict(q=FAKE, q_type=0, batch=1, q_heads=8, kv_heads=2, dim=128, q_sb=1024, q_sh=128, lohi=FAKE, step=FAKE, cap=40, blocks=40,
               n=2500, starts=None, lens=None, keep=8, sink=1, recent=2, out=FAKE, ws=None, wsb=0, stream=None)
 

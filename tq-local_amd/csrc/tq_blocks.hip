@@ -53,8 +53,15 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2, a), __builtin_bit_cast(s16x2, b)));
 }
 
+// fp32 bits as an integer whose order is theirs (NaN as above), and back.
+__device__ __forceinline__ int ordered(float x) {
+    const int b = __float_as_int(x);
+    return b ^ ((b >> 31) & 0x7FFFFFFF);
+}
+__device__ __forceinline__ uint32_t unordered(int x) { return (uint32_t)(x ^ ((x >> 31) & 0x7FFFFFFF)); }
+
 struct BoundsArgs {
-    const uint16_t* k;
+    const void* k;
     int heads;
     int64_t tokens, k_sb, k_sh, k_st;
     int8_t* lohi;
@@ -65,7 +72,26 @@ struct BoundsArgs {
     int heads_next;
 };
 
+// Whole numbers outward of eight channels' least or largest keys (fp32 bits) over a step (times `down`), four to a word.
+__device__ __forceinline__ uint2 outward8(const uint32_t* bits, bool upper, float down) {
+    uint32_t out[2] = {0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        // an infinity for NaN too
+        const float v = __uint_as_float((bits[j] & 0x80000000u) | std::min(bits[j] & 0x7FFFFFFFu, 0x7F800000u)) * down;
+        float r = fminf(fmaxf(upper ? __builtin_ceilf(v) : __builtin_floorf(v), -127.0f), 127.0f);
+        // a number less than 2^-149 of a step gives the product 0, and is rounded outward all the same
+        if (r == 0.0f && (bits[j] << 1) != 0u && upper != (bool)(bits[j] >> 31)) r = upper ? 1.0f : -1.0f;
+        out[j >> 2] |= ((uint32_t)(int)r & 0xFFu) << (8 * (j & 3));
+    }
+    return make_uint2(out[0], out[1]);
+}
+
+// TYPE: of the keys, 0: bf16, 1: fp32, 2: fp16.  16-bit keys are compared two at a time as they are; a bf16 or fp16 number is an fp32 one, so
+// the bounds are of the keys as given whatever their type.  fp32 keys are twice the bytes: the 8 sequences
+// above 190 to 194 us, 5.6 TB/s.
 constexpr int BOUNDS_WAVES = 4;
+template <int TYPE>
 __global__ __launch_bounds__(64 * BOUNDS_WAVES) void bounds_kernel(BoundsArgs a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t at = (int64_t)blockIdx.x * BOUNDS_WAVES + wave;
@@ -77,53 +103,79 @@ __global__ __launch_bounds__(64 * BOUNDS_WAVES) void bounds_kernel(BoundsArgs a)
     } else {
         group = at / a.per_head, block = at - group * a.per_head;
     }
-    const int64_t b = group / a.heads, h = group - b * a.heads;
-    const uint16_t* const k = a.k + b * a.k_sb + h * a.k_sh + block * BT * a.k_st;
+    const int64_t b = group / a.heads, h = group - b * a.heads, first = b * a.k_sb + h * a.k_sh + block * BT * a.k_st;
     const int left = (int)std::min<int64_t>(a.tokens - block * BT, BT);
     // lane (c = lane % 16, t = lane / 16): channels [8 c, 8 c + 8) of the tokens t, t + 4, ...; past the last it again
     const int c = lane & 15, t = lane >> 4;
-    uint4 x[BT / 4];
+    const bool upper = t == 1;  // lanes t = 0 write lo, t = 1 hi
+    uint32_t most = 0u;         // the largest absolute value, as fp32 bits
+    uint32_t mine[8];           // the lane's eight bounds
+    if constexpr (TYPE == 1) {
+        const float* const k = static_cast<const float*>(a.k) + first;
+        int lo[8], hi[8];
 #pragma unroll
-    for (int i = 0; i < BT / 4; ++i)
-        x[i] = *reinterpret_cast<const uint4*>(k + std::min(4 * i + t, left - 1) * a.k_st + 8 * c);
-    uint32_t lo[4], hi[4];
+        for (int j = 0; j < 8; ++j) lo[j] = 0x7FFFFFFF, hi[j] = (int)0x80000000u;
+        constexpr int SETS = 2;  // half of a block's loads in flight together, 64 registers
 #pragma unroll
-    for (int j = 0; j < 4; ++j) lo[j] = 0x7FFF7FFFu, hi[j] = 0x80008000u;
+        for (int s = 0; s < SETS; ++s) {
+            float4 x[BT / 4 / SETS][2];
 #pragma unroll
-    for (int i = 0; i < BT / 4; ++i) {
-        const uint32_t w[4] = {ordered(x[i].x), ordered(x[i].y), ordered(x[i].z), ordered(x[i].w)};
+            for (int i = 0; i < BT / 4 / SETS; ++i) {
+                const float* const row = k + std::min(4 * (BT / 4 / SETS * s + i) + t, left - 1) * a.k_st + 8 * c;
+                x[i][0] = *reinterpret_cast<const float4*>(row), x[i][1] = *reinterpret_cast<const float4*>(row + 4);
+            }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) lo[j] = min2(lo[j], w[j]), hi[j] = max2(hi[j], w[j]);
-    }
-    uint32_t most = 0u;  // the largest absolute value, as fp32 bits
+            for (int i = 0; i < BT / 4 / SETS; ++i) {
+                const float w[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w, x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 8; ++j) lo[j] = std::min(lo[j], ordered(w[j])), hi[j] = std::max(hi[j], ordered(w[j]));
+            }
+        }
 #pragma unroll
-        for (int d = 16; d < 64; d <<= 1)
-            lo[j] = min2(lo[j], (uint32_t)__shfl_xor((int)lo[j], d)), hi[j] = max2(hi[j], (uint32_t)__shfl_xor((int)hi[j], d));
-        lo[j] = ordered(lo[j]), hi[j] = ordered(hi[j]);  // its own inverse
-        const uint32_t l = lo[j] & 0x7FFF7FFFu, u = hi[j] & 0x7FFF7FFFu;
-        most = std::max(most, std::max(std::max(l << 16, l & 0x7FFF0000u), std::max(u << 16, u & 0x7FFF0000u)));
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+            for (int d = 16; d < 64; d <<= 1) lo[j] = std::min(lo[j], __shfl_xor(lo[j], d)), hi[j] = std::max(hi[j], __shfl_xor(hi[j], d));
+            const uint32_t l = unordered(lo[j]), u = unordered(hi[j]);
+            most = std::max(most, std::max(l & 0x7FFFFFFFu, u & 0x7FFFFFFFu));
+            mine[j] = upper ? u : l;
+        }
+    } else {
+        const uint16_t* const k = static_cast<const uint16_t*>(a.k) + first;
+        uint4 x[BT / 4];
+#pragma unroll
+        for (int i = 0; i < BT / 4; ++i)
+            x[i] = *reinterpret_cast<const uint4*>(k + std::min(4 * i + t, left - 1) * a.k_st + 8 * c);
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo[j] = 0x7FFF7FFFu, hi[j] = 0x80008000u;
+#pragma unroll
+        for (int i = 0; i < BT / 4; ++i) {
+            const uint32_t w[4] = {ordered(x[i].x), ordered(x[i].y), ordered(x[i].z), ordered(x[i].w)};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lo[j] = min2(lo[j], w[j]), hi[j] = max2(hi[j], w[j]);
+        }
+        auto fp32 = [](uint32_t half) {
+            if constexpr (TYPE == 2) return __float_as_uint(tq::f16_to_f32(half)); else return half << 16;
+        };
+        uint32_t largest = 0u;  // of two at a time
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int d = 16; d < 64; d <<= 1)
+                lo[j] = min2(lo[j], (uint32_t)__shfl_xor((int)lo[j], d)), hi[j] = max2(hi[j], (uint32_t)__shfl_xor((int)hi[j], d));
+            lo[j] = ordered(lo[j]), hi[j] = ordered(hi[j]);  // its own inverse
+            largest = max2(largest, max2(lo[j] & 0x7FFF7FFFu, hi[j] & 0x7FFF7FFFu));
+            const uint32_t w = upper ? hi[j] : lo[j];
+            mine[2 * j] = fp32(w & 0xFFFFu), mine[2 * j + 1] = fp32(w >> 16);
+        }
+        most = fp32(std::max(largest & 0xFFFFu, largest >> 16));
     }
 #pragma unroll
     for (int d = 1; d < 16; d <<= 1) most = std::max(most, (uint32_t)__shfl_xor((int)most, d));
     const int e = step_exponent(most);
-    const float down = power_of_two(-e);
-    // lanes t = 0 write lo, t = 1 hi
-    const bool upper = t == 1;
-    uint32_t out[2] = {0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t w = upper ? hi[j >> 1] : lo[j >> 1], bits = j & 1 ? w & 0xFFFF0000u : w << 16;
-        // an infinity for NaN too
-        const float v = __uint_as_float((bits & 0x80000000u) | std::min(bits & 0x7FFFFFFFu, 0x7F800000u)) * down;
-        float r = fminf(fmaxf(upper ? __builtin_ceilf(v) : __builtin_floorf(v), -127.0f), 127.0f);
-        // a number less than 2^-149 of a step gives the product 0, and is rounded outward all the same
-        if (r == 0.0f && (bits << 1) != 0u && upper != (bool)(bits >> 31)) r = upper ? 1.0f : -1.0f;
-        out[j >> 2] |= ((uint32_t)(int)r & 0xFFu) << (8 * (j & 3));
-    }
+    const uint2 out = outward8(mine, upper, power_of_two(-e));
     const int64_t to = group * a.cap + a.first + block;
-    if (t < 2) *reinterpret_cast<uint2*>(a.lohi + to * (2 * D) + t * D + 8 * c) = make_uint2(out[0], out[1]);
+    if (t < 2) *reinterpret_cast<uint2*>(a.lohi + to * (2 * D) + t * D + 8 * c) = out;
     if (lane == 0) a.step[to] = power_of_two(e);
 }
 
@@ -394,19 +446,27 @@ constexpr int FUSED_BLOCKS = 512;
 
 }  // namespace
 
-extern "C" int tq_block_bounds(const uint16_t* k, int batch, int heads, int64_t tokens, int dim, int64_t k_sb, int64_t k_sh,
-                               int64_t k_st, int8_t* lohi, float* step, int64_t cap, int64_t first, void* stream) {
-    if (!k || !lohi || !step || batch < 1 || heads < 1 || tokens < 1 || first < 0) return TQ_ERR_INVALID_ARGUMENT;
+extern "C" int tq_block_bounds_typed(const void* k, int k_type, int batch, int heads, int64_t tokens, int dim, int64_t k_sb, int64_t k_sh,
+                                     int64_t k_st, int8_t* lohi, float* step, int64_t cap, int64_t first, void* stream) {
+    if (!k || k_type < 0 || k_type > 2 || !lohi || !step || batch < 1 || heads < 1 || tokens < 1 || first < 0) return TQ_ERR_INVALID_ARGUMENT;
     const int64_t per_head = (tokens - 1) / BT + 1;
     if (first > cap - per_head) return TQ_ERR_INVALID_ARGUMENT;
-    if (dim != D || !aligned16(k) || !aligned16(lohi) || ((k_sb | k_sh | k_st) & 7)) return TQ_ERR_UNSUPPORTED;
+    if (dim != D || !aligned16(k) || !aligned16(lohi) || ((k_sb | k_sh | k_st) & (k_type == 1 ? 3 : 7))) return TQ_ERR_UNSUPPORTED;
     const int64_t groups = (int64_t)batch * heads;
     if (per_head >= (int64_t)1 << 31 || groups * per_head >= (int64_t)1 << 31) return TQ_ERR_UNSUPPORTED;
     const BoundsArgs a{k, heads, tokens, k_sb, k_sh, k_st, lohi, step, cap, first, per_head, groups * per_head, k_sh < k_st};
-    hipLaunchKernelGGL(bounds_kernel, dim3((unsigned)((a.all + BOUNDS_WAVES - 1) / BOUNDS_WAVES)), dim3(64 * BOUNDS_WAVES), 0,
-                       static_cast<hipStream_t>(stream), a);
+    const dim3 grid((unsigned)((a.all + BOUNDS_WAVES - 1) / BOUNDS_WAVES)), threads(64 * BOUNDS_WAVES);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (k_type == 0) hipLaunchKernelGGL(bounds_kernel<0>, grid, threads, 0, s, a);
+    else if (k_type == 1) hipLaunchKernelGGL(bounds_kernel<1>, grid, threads, 0, s, a);
+    else hipLaunchKernelGGL(bounds_kernel<2>, grid, threads, 0, s, a);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
+}
+
+extern "C" int tq_block_bounds(const uint16_t* k, int batch, int heads, int64_t tokens, int dim, int64_t k_sb, int64_t k_sh,
+                               int64_t k_st, int8_t* lohi, float* step, int64_t cap, int64_t first, void* stream) {
+    return tq_block_bounds_typed(k, 0, batch, heads, tokens, dim, k_sb, k_sh, k_st, lohi, step, cap, first, stream);
 }
 
 extern "C" size_t tq_select_blocks_workspace_bytes(int batch, int kv_heads, int64_t n_tokens) {

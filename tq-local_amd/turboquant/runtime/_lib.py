@@ -55,6 +55,7 @@ SIGNATURES: dict[str, tuple] = {
     "tq_prefix_attention": (_I, [_P, _I, _I, _I, _I, _I, _I64, _I64, _I, _P, _I, _P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I,
                                  _I, _I, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _SZ, _P]),
     "tq_block_bounds": (_I, [_P, _I, _I, _I64, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _P]),
+    "tq_block_bounds_typed": (_I, [_P, _I, _I, _I, _I64, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _P]),
     "tq_select_blocks": (_I, [_P, _I, _I, _I, _I, _I, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _P, _I, _I, _I, _P, _P, _SZ,
                               _P]),
     "tq_select_blocks_workspace_bytes": (_SZ, [_I, _I, _I64]),

@@ -1019,13 +1019,14 @@ MAX_SCORED = 32768  # blocks of a history that are chosen from (TQ_MAX_SCORED)
 
 
 def block_bounds(k: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, first: int = 0) -> None:
-    """Bounds of the keys of every 64 tokens of k [B, H, T, D] (bf16; other types are rounded to it), written for the blocks from
-    ``first`` on (tq_block_bounds).
+    """Bounds of the keys of every 64 tokens of k [B, H, T, D] (bf16, fp16 or fp32), written for the blocks from ``first`` on
+    (tq_block_bounds).
 
     ``lohi`` int8 [B, H, cap, 2, D] and ``step`` fp32 [B, H, cap]: no element of block j's keys is below lohi[j, 0] step[j] or above
     lohi[j, 1] step[j], channel by channel, up to 127 2^100.  The last block may have fewer than 64 tokens; the bounds are then of those.
     """
-    k = k if k.dim() == 4 and k.shape[2] == 0 else _as_encoder_input(k)
+    if k.dim() != 4 or k.shape[-1] != HEAD_DIM or k.dtype not in _QUERY_TYPES:
+        raise ValueError(f"block_bounds: expected k [B, H, T, {HEAD_DIM}] in bf16, fp16 or fp32, got {k.dtype} {tuple(k.shape)}")
     _no_gradient("block_bounds", k)
     _not_traced("block_bounds")
     _require_gpu(k)
@@ -1043,9 +1044,10 @@ def block_bounds(k: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, first:
         raise ValueError(f"block_bounds: blocks [{first}, {first + n}) of a capacity of {cap}")
     if k.numel() == 0:
         return
+    k = rows16(k)
     st = k.stride()
-    _on_device("tq_block_bounds", on, k.data_ptr(), B, H, T, D, st[0], st[1], st[2], lohi.data_ptr(), step.data_ptr(), cap, first,
-               _stream_handle(k.device))
+    _on_device("tq_block_bounds_typed", on, k.data_ptr(), _QUERY_TYPES[k.dtype], B, H, T, D, st[0], st[1], st[2], lohi.data_ptr(),
+               step.data_ptr(), cap, first, _stream_handle(k.device))
 
 
 def select_blocks(q: torch.Tensor, lohi: torch.Tensor, step: torch.Tensor, *, n_tokens: int, keep: int, sink: int = 1,
