@@ -502,3 +502,26 @@ def test_attention_switched_off_and_on_again(cuda):
             assert torch.isfinite(out).all() and cache.get_seq_length() == 41 + i
             if i != 1:
                 disable_turboquant_attention(model, cache, old)
+
+
+@pytest.mark.parametrize("large_first", [True, False])
+@pytest.mark.parametrize("n_prefix", [0, 40])
+@pytest.mark.parametrize("n,H,g,M", [(2, 64, 1, 1024), (9, 130, 4, 128)])
+def test_norms_of_neighbours_are_their_own(cuda, n, H, g, M, n_prefix, large_first):
+    """Sequences of one prompt whose values' norms are 2^29 apart, whichever come first in the waves' tiles: each as it is alone.  As many KV
+    heads as have a wave take tiles of both kinds, in blocks of 32 rows and of 64.  A weight times norm is rounded to fp16 in either call,
+    by half a step, 2^-11 of it (those below 2^-25 of the largest by 2^-36 of that): the outputs differ by 2^-10 of the weighted sum of the
+    values' sizes, and by the sums' roundings in fp32 and the exponents' (of numbers up to 64), below 2^-17 of it together."""
+    prompts, own, q, kw = setup((n,), H, g, 64, M, seed=27)
+    kw["n_prefix"] = n_prefix
+    large = torch.arange(n, device="cuda") < (n + 3) // 4
+    own._store.vn[:, :, :M] = torch.where(large if large_first else ~large, 2.0 ** 15, 2.0 ** -14).half()[:, None, None]
+    prompts._store.vn[:, :, :64] = 2.0 ** -14
+    _, f32 = call(prompts, own, q, dict(kw, want_f32=True))
+    (pk, pv), (ok, ov) = rows64(prompts), rows64(own)
+    for b in range(n):
+        mine = {name: t[b:b + 1].contiguous() for name, t in arrays(own).items()}
+        _, alone = K.prefix_attention(q[b:b + 1], arrays(prompts), mine, **kw, want_f32=True)
+        k, v = torch.cat((pk[:, :, :n_prefix], ok[b:b + 1]), 2), torch.cat((pv[:, :, :n_prefix], ov[b:b + 1]), 2)
+        sizes, _ = attend64(q[b:b + 1], k, v.abs())
+        assert ((f32[b] - alone[0]).double().abs() <= (2.0 ** -10 + 2.0 ** -17) * sizes[0]).all()

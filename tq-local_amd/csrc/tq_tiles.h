@@ -15,8 +15,9 @@
 //
 // Rounding.  Rotated queries and centroids are rounded once to fp16, by at most 2^-11 of each, 2^-11 / sqrt(3) root mean square (with
 // |q| = 11 and |k| = 20 a logit moves by 7e-4), value centroids too (their sum's errors are kept from adding up by the
-// codebook, see tq_value_codebook_f16), weights times norm p |v| once: to 11 bits down to 2^-25 of the largest norm's at the row's
-// reference, and by up to 2^-36 of it below.  Logits, maxima, weights, sums and outputs are fp32.
+// codebook, see tq_value_codebook_f16), weights times norm p |v| once: to 11 bits down to 2^-25 of the largest norm's, of the tiles that
+// the row attends to any of, at the row's reference, and by up to 2^-36 of it below.  Logits, maxima, weights, sums and outputs are
+// fp32.
 
 #pragma once
 
@@ -284,7 +285,7 @@ struct Tiles {
         float4 o[W][32][32];  // chunks xor-swizzled by the row
         float2 ms[RB][W][32];
         float4 by[RB][32][W / 4];  // what a row's sums of each wave are multiplied by
-        float unit[W];
+        float unit[RB][W][32];
     };
     union Lds {
         uint4 m[2 * 128 * 32];
@@ -499,9 +500,13 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
 #pragma unroll
         for (int d = 0; d < 4; ++d) o[m][d] = zero16();
     }
-    // weights and output sums are in units of 2^-shift, 2^-TOP_BIT of a power of two above the largest |v| so far: weights
-    // times norm then reach up to 2^(TOP_BIT + LAZY), and fp16 keeps its 11 bits down to 2^-14, 2^-25 of the reference's
-    int shift = TOP_BIT + 24;
+    // a row's weights and output sums are in units of 2^-shift, 2^-TOP_BIT of a power of two above the largest |v| of the tiles so far
+    // that it attends to any of: weights times norm then reach up to 2^(TOP_BIT + LAZY), and fp16 keeps its 11 bits down to 2^-14, 2^-25 of
+    // the reference's.  Tiles of others, as another sequence's own tokens, leave a row's unit alone; in whole tiles all rows' are one
+    int shift[RB];
+#pragma unroll
+    for (int m = 0; m < RB; ++m) shift[m] = TOP_BIT + 24;
+    int most_shift = TOP_BIT + 24;  // no row's is larger
     const uint32_t lane4 = (lane & 31) * 4;
     const uint8_t* const table = reinterpret_cast<const uint8_t*>(lds.t.table);
     uint8_t* const v8 = reinterpret_cast<uint8_t*>(lds.t.v[wave]);
@@ -570,8 +575,9 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
         }
         // the largest finite |v| of the tile: its exponent decides the unit (2^(e + 1) is above it)
         const int e5 = (norm >> 10) & 31, ve = e5 == 31 ? 0 : e5;
-        int need = 0;  // uniform: by how much the unit has to rise
-        if (__any(ve > 14 + TOP_BIT - shift)) {
+        bool rise = false;  // uniform: whether units may have to rise, to `limit`
+        int limit = 0;
+        if (__any(ve > 14 + TOP_BIT - most_shift)) {
             int e = 0;
             uint64_t largest = ~0ull;
 #pragma unroll
@@ -579,9 +585,9 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
                 const uint64_t set = __ballot(ve >> k & 1) & largest;
                 if (set) largest = set, e |= 1 << k;
             }
-            need = shift - (14 + TOP_BIT - std::max(e, 1));
+            rise = true, limit = 14 + TOP_BIT - std::max(e, 1);
+            if constexpr (!masked) most_shift = limit;
         }
-        shift -= need;
         if (tile + step_tiles < tiles) load_keys(tile + step_tiles);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -594,8 +600,11 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[m][4 * j + e] = __builtin_fmaf((float)k4[e], x[m][4 * j + e], 0.0f);
             }
+            int need = 0;  // by how much the row's unit rises
+            if (!masked && rise) need = shift[m] - limit;
             if constexpr (masked) {
-                const uint32_t word = src.seen(m, tile) >> (4 * h);
+                const uint32_t seen = src.seen(m, tile), word = seen >> (4 * h);
+                if (rise && seen) need = std::max(shift[m] - limit, 0);
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (!(word & (1u << (8 * (i >> 2) + (i & 3))))) x[m][i] = -__builtin_inff();
@@ -604,18 +613,19 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
 #pragma unroll
             for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[m][i]);
             // neither -inf nor NaN raises the reference
-            if (__any(__builtin_fmaf(mx, c[m], -top[m]) > LAZY) || need) {
+            if (__any(__builtin_fmaf(mx, c[m], -top[m]) > LAZY) || rise) {
                 mx = max_of_halves(mx) * c[m];
                 const float ref = mx > top[m] ? mx : top[m];
                 const float corr = exp2_(top[m] == ref ? -(float)need : top[m] - ref - (float)need);
                 top[m] = ref;
+                shift[m] -= need;
                 sum[m] *= corr;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[m][d][i] *= corr;
             }
-            const float base = (float)shift - (top[m] == -__builtin_inff() ? 0.0f : top[m]);
+            const float base = (float)shift[m] - (top[m] == -__builtin_inff() ? 0.0f : top[m]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const f16x4 v4 = *reinterpret_cast<const f16x4*>(&lds.t.vn[wave][8 * j + 4 * h]);
@@ -665,14 +675,13 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
 
     // ---- the waves' sums, one block of rows at a time.  What a wave's sums weigh is found once for a row, beside the sums' way to LDS (by every
     // thread of a row for itself a call took 0.8 us more)
-    const float unit = __uint_as_float((uint32_t)(127 - shift) << 23);
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < RB; ++m) {
         const float all = sum_of_halves(sum[m]);
-        if (h == 0) lds.s.ms[m][wave][r] = make_float2(top[m], all * unit);
+        const float unit = __uint_as_float((uint32_t)(127 - shift[m]) << 23);
+        if (h == 0) lds.s.ms[m][wave][r] = make_float2(top[m], all * unit), lds.s.unit[m][wave][r] = unit;
     }
-    if (lane == 0) lds.s.unit[wave] = unit;
     __syncthreads();
     if (wave == 0 && h < RB) {
         float2 ms[W];
@@ -684,7 +693,7 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
 #pragma unroll
         for (int k = 0; k < W; ++k) {
             const float w = exp2_(ms[k].x - safe);
-            by[k] = w * lds.s.unit[k];
+            by[k] = w * lds.s.unit[h][k][r];
             den = __builtin_fmaf(w, ms[k].y, den);
         }
 #pragma unroll
