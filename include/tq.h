@@ -493,6 +493,15 @@ int tq_block_attention(const uint16_t* q, int batch, int q_heads, int kv_heads, 
                        const float* key_centers, const float* qjl, const float* value_rotation, const float* value_centers,
                        float scale, float* out_f32, uint16_t* out_bf16, float* lse_out, void* workspace, size_t workspace_bytes,
                        void* stream);
+/* The same for queries of another type: q_type as for tq_prefix_attention, rows [batch][q_heads][dim] next to one another, 16-byte aligned, and
+ * used as they are given; out_16 the query's 16-bit type (bf16 for fp32 queries). */
+int tq_block_attention_typed(const void* q, int q_type, int batch, int q_heads, int kv_heads, int dim, const int32_t* blocks, int keep,
+                             const int32_t* seq_starts, const int32_t* seq_lens, int64_t n_tokens, int64_t cap,
+                             const uint8_t* k_codes, const uint16_t* k_norms, const uint8_t* k_signs, const uint16_t* k_rnorms,
+                             const uint8_t* v_codes, const uint16_t* v_norms, int key_bits, int value_bits, int has_qjl,
+                             const float* key_rotation, const float* key_centers, const float* qjl, const float* value_rotation,
+                             const float* value_centers, float scale, float* out_f32, uint16_t* out_16, float* lse_out,
+                             void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

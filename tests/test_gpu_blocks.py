@@ -312,6 +312,44 @@ def test_shapes(cuda, B, H, g, N, keep):
     check(got, blocks_ref(q, layer, blocks)[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("bits,qjl", BITS)
+@pytest.mark.parametrize("H,g", [(2, 4), (1, 1), (1, 7), (1, 8)])
+def test_queries_of_other_types(cuda, dtype, bits, qjl, H, g):
+    """Queries that are no bf16 numbers are not rounded to them, and outputs are in their type."""
+    layer = make_layer(2, H, 1000, bits, qjl, seed=25)
+    q = randn((2, H * g, D), 5, torch.float32).to(dtype)
+    assert not torch.equal(q, q.bfloat16().to(dtype))
+    blocks = some_blocks(2, H, 16, 5, 1)
+    kw = dict(**arrays(layer), **codec(layer), n_tokens=1000)
+    got, f32, lse = K.block_attention(q, blocks, **kw, want_f32=True, want_lse=True)
+    assert got.dtype == dtype and f32.dtype == torch.float32
+    ref, ref_lse = blocks_ref(q, layer, blocks)
+    check(got, ref)
+    check(f32, ref)
+    assert (lse.double() - ref_lse).abs().max() <= 4e-3
+    rows = torch.zeros(2, 3, H * g, D + 1, dtype=dtype, device="cuda")[:, 1, :, 1:]  # rows at any element
+    rows.copy_(q)
+    assert torch.equal(K.block_attention(rows, blocks, **kw), got)
+    assert torch.equal(K.block_attention(q[:, :, None], blocks, **kw), got)
+    exact = q.bfloat16()  # numbers that every type has
+    want = K.block_attention(exact, blocks, **kw, want_f32=True)[1]
+    assert torch.equal(K.block_attention(exact.to(dtype), blocks, **kw, want_f32=True)[1], want)  # the other terms add zeros
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("dense", [0, 30])
+@pytest.mark.parametrize("g", [4, 7])
+def test_layers_take_queries_of_other_types(cuda, dtype, dense, g):
+    layer = make_layer(2, 2, 1500, 4, True, seed=15, dense=dense)
+    q = randn((2, 2 * g, 1, D), 5, torch.float32).to(dtype)
+    got = block_sparse_attention(q, layer, keep=6)
+    assert got.shape == q.shape and got.dtype == dtype
+    check(got, sparse_ref(q, layer, 6, 1, 2))
+    empty = K.block_attention(q, torch.empty(2, 2, 0, dtype=torch.int32, device="cuda"), **arrays(layer), **codec(layer), n_tokens=1500)
+    assert empty.dtype == dtype and (empty == 0).all()
+
+
 def test_the_most_blocks(cuda):
     """As many as are taken, each of them of a short history and many times: like once."""
     layer = make_layer(1, 1, 130, 4, True, seed=5)

@@ -115,6 +115,14 @@ def test_block_attention_rejects_on_host(status, change):
     assert _lib.load().tq_block_attention(*dict(BLOCKS, **change).values()) == status
 
 
+@pytest.mark.parametrize("status,change", [(INVALID, dict(q_type=3)), (INVALID, dict(q_type=-1)), (INVALID, dict(q=None)),
+                                           (INVALID, dict(q_type=2, ob=None)), (UNSUPPORTED, dict(q_type=1, q=ODD)),
+                                           (UNSUPPORTED, dict(q_type=2, q_heads=18)), (WORKSPACE, dict(q_type=1, wsb=100))])
+def test_block_attention_of_other_types_rejects_on_host(status, change):
+    args = {"q": FAKE, "q_type": 0, **BLOCKS}
+    assert _lib.load().tq_block_attention_typed(*dict(args, **change).values()) == status
+
+
 def test_select_workspace_is_host_arithmetic():
     size = _lib.load().tq_select_blocks_workspace_bytes
     assert size(1, 2, 0) == size(1, 2, 1000) == 0 < size(1, 2, 100000) < size(2, 2, 100000)

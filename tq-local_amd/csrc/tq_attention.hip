@@ -340,10 +340,11 @@ __device__ __forceinline__ uint32_t win_off(const uint32_t* w, const uint32_t* s
 // One query head bh, MT threads (t = 0..MT-1): merge the split partials (maxima in the log2
 // domain), normalise, un-rotate by R_v.  Thread t reads R_v rows k in [16 (t / 32), 16 (t / 32)
 // + 16), columns 4 (t % 32) .. + 3, as float4.  Every thread of the workgroup calls it (barriers
-// inside).
+// inside).  F16: out_16 holds fp16, else bf16.
+template <bool F16 = false>
 __device__ __forceinline__ void merge_head(int bh, int t, int n_split, const float* __restrict__ part_o,
                                            const float* __restrict__ part_ml, const float* __restrict__ Rv,
-                                           float* __restrict__ out_f32, uint16_t* __restrict__ out_bf16,
+                                           float* __restrict__ out_f32, uint16_t* __restrict__ out_16,
                                            float* __restrict__ lse_out, float* so, float4 (*part)[D / 4],
                                            float (*red)[2]) {
     const int lane = t & 63, wv = t >> 6;
@@ -422,19 +423,20 @@ __device__ __forceinline__ void merge_head(int bh, int t, int n_split, const flo
 #pragma unroll
         for (int r = 0; r < MT / 32; ++r) a += pf[r * D + t];
         if (out_f32) out_f32[(size_t)bh * D + t] = a;
-        if (out_bf16) out_bf16[(size_t)bh * D + t] = (uint16_t)tq::f32_to_bf16(a);
+        if (out_16) out_16[(size_t)bh * D + t] = (uint16_t)(F16 ? tq::f32_to_f16(a) : tq::f32_to_bf16(a));
     }
 }
 
 // One workgroup per (batch row, query head).
+template <bool F16 = false>
 __global__ __launch_bounds__(MT) void merge_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml,
                                                    int n_split, const float* __restrict__ Rv,
-                                                   float* __restrict__ out_f32, uint16_t* __restrict__ out_bf16,
+                                                   float* __restrict__ out_f32, uint16_t* __restrict__ out_16,
                                                    float* __restrict__ lse_out) {
     __shared__ float so[D];
     __shared__ float4 part[MT / 32][D / 4];
     __shared__ float red[MT / 64][2];
-    merge_head(blockIdx.x, threadIdx.x, n_split, part_o, part_ml, Rv, out_f32, out_bf16, lse_out, so, part, red);
+    merge_head<F16>(blockIdx.x, threadIdx.x, n_split, part_o, part_ml, Rv, out_f32, out_16, lse_out, so, part, red);
 }
 
 // ------------------------------------------------------------------ q-side image
@@ -481,8 +483,10 @@ __device__ __forceinline__ void split3_bf16(const f32x4& a, const f32x4& b, u32x
 // operand loads are issued and before they are waited for: global loads complete in issue
 // order, so loads that mid() issues stay in flight through the products (and the barriers,
 // which wait for LDS only).
-template <bool QJL, int GC, int NW, bool KI8, bool QR, typename Mid>
-__device__ __forceinline__ void image_products(const uint16_t* __restrict__ q, int G, int bh0,
+// NQ = 3: q is fp32 (q_type 1) or fp16 (2), three bf16 terms exactly, as the matrix is.  Of their nine products the three smallest are left
+// out, 2^-23 of a product together, as an fp32 rounding.
+template <bool QJL, int GC, int NW, bool KI8, bool QR, int NQ = 1, typename Mid>
+__device__ __forceinline__ void image_products(const uint16_t* __restrict__ q, [[maybe_unused]] int q_type, int G, int bh0,
                                                const float* __restrict__ Rk, const float* __restrict__ S,
                                                float c_mse, PrepLds<GC, QR>& L, uint32_t* img, uint4* qst,
                                                int wave, int lane, int d0, Mid&& mid) {
@@ -493,17 +497,28 @@ __device__ __forceinline__ void image_products(const uint16_t* __restrict__ q, i
     const bool active = wave < NTILE;           // wave-uniform
     const int c = lane & 15, kq = lane >> 4;
     // A: lane (row c = query head, kq) holds q[c][32 s + 8 kq + e] for k-step s
-    u32x4 qa[4];
+    u32x4 qa[NQ][4];
     // B as loaded: rr[u][2 s + hf], lane l: row 16 t' + 8 hf + l / 8, floats 32 s + 4 (l mod 8) .. + 3
     f32x4 rr[TPW][8];
     // the group's query rows, 16 bytes per lane (rows >= G read as zero through the descriptor),
     // restaged in the wave's LDS slot below: one load per NH / 4 rows instead of four per lane,
     // most of them repeats of the same rows
-    u32x4 qv[NH / 4];
+    u32x4 qv[NQ == 1 ? 1 : 2][NH / 4];  // fp32 rows: twice the bytes
     if (active) {
-        const __amdgpu_buffer_rsrc_t rq = rsrc(q + (size_t)bh0 * D, (int64_t)G * D * 2);
+        if constexpr (NQ == 1) {
+            const __amdgpu_buffer_rsrc_t rq = rsrc(q + (size_t)bh0 * D, (int64_t)G * D * 2);
 #pragma unroll
-        for (int i = 0; i < NH / 4; ++i) qv[i] = __builtin_amdgcn_raw_buffer_load_b128(rq, (i * 64 + lane) * 16, 0, 0);
+            for (int i = 0; i < NH / 4; ++i) qv[0][i] = __builtin_amdgcn_raw_buffer_load_b128(rq, (i * 64 + lane) * 16, 0, 0);
+        } else {
+            const int step = q_type == 1 ? 32 : 16;  // bytes of a lane's eight elements
+            const __amdgpu_buffer_rsrc_t rq =
+                rsrc(reinterpret_cast<const uint8_t*>(q) + (size_t)bh0 * D * (step / 8), (int64_t)G * D * (step / 8));
+#pragma unroll
+            for (int i = 0; i < NH / 4; ++i) {
+                qv[0][i] = __builtin_amdgcn_raw_buffer_load_b128(rq, (i * 64 + lane) * step, 0, 0);
+                qv[1][i] = __builtin_amdgcn_raw_buffer_load_b128(rq, (i * 64 + lane) * step + 16, 0, 0);
+            }
+        }
 #pragma unroll
         for (int u = 0; u < TPW; ++u) {
             const int t = wave + u * NW;
@@ -522,16 +537,39 @@ __device__ __forceinline__ void image_products(const uint16_t* __restrict__ q, i
     __builtin_amdgcn_sched_barrier(0);
     if (!active) return;
     // the wave's own LDS slot: its accesses execute in order, no barrier needed
+    const int cr = c < NH ? c : 0;
+    if constexpr (NQ == 1) {
 #pragma unroll
-    for (int i = 0; i < NH / 4; ++i) qst[i * 64 + lane] = __builtin_bit_cast(uint4, qv[i]);
-    {
-        const int cr = c < NH ? c : 0;
+        for (int i = 0; i < NH / 4; ++i) qst[i * 64 + lane] = __builtin_bit_cast(uint4, qv[0][i]);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) qa[s] = __builtin_bit_cast(u32x4, qst[cr * 16 + 4 * s + kq]);
+        for (int s = 0; s < 4; ++s) qa[0][s] = __builtin_bit_cast(u32x4, qst[cr * 16 + 4 * s + kq]);
+    } else {
+        u32x4 terms[3][NH / 4];
+#pragma unroll
+        for (int i = 0; i < NH / 4; ++i) {
+            f32x4 a = __builtin_bit_cast(f32x4, qv[0][i]), b = __builtin_bit_cast(f32x4, qv[1][i]);
+            if (q_type == 2) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w0 = qv[0][i][e >> 1], w1 = qv[0][i][2 + (e >> 1)];
+                    a[e] = tq::f16_to_f32(e & 1 ? w0 >> 16 : w0 & 0xFFFFu), b[e] = tq::f16_to_f32(e & 1 ? w1 >> 16 : w1 & 0xFFFFu);
+                }
+            }
+            split3_bf16(a, b, terms[0][i], terms[1][i], terms[2][i]);
+        }
+#pragma unroll
+        for (int x = 0; x < 3; ++x) {
+#pragma unroll
+            for (int i = 0; i < NH / 4; ++i) qst[i * 64 + lane] = __builtin_bit_cast(uint4, terms[x][i]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) qa[x][s] = __builtin_bit_cast(u32x4, qst[cr * 16 + 4 * s + kq]);
+        }
     }
     if (c >= G) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) qa[s] = u32x4{0u, 0u, 0u, 0u};
+        for (int x = 0; x < NQ; ++x)
+#pragma unroll
+            for (int s = 0; s < 4; ++s) qa[x][s] = u32x4{0u, 0u, 0u, 0u};
     }
     // the same slot restages the matrix rows (2 KB per k-step; the qa reads above come first in
     // the wave's LDS order): lane (c, kq) takes row c's floats 32 s + 8 kq .. + 7, which lanes
@@ -550,9 +588,14 @@ __device__ __forceinline__ void image_products(const uint16_t* __restrict__ q, i
             const f32x4 b0 = rst[src], b1 = rst[src + 1];
             u32x4 hi, mid, lo;
             split3_bf16(b0, b1, hi, mid, lo);
-            acc = mfma_bf16(qa[s], lo, acc);
-            acc = mfma_bf16(qa[s], mid, acc);
-            acc = mfma_bf16(qa[s], hi, acc);
+            if constexpr (NQ == 3) {
+                acc = mfma_bf16(qa[2][s], hi, acc);
+                acc = mfma_bf16(qa[1][s], mid, acc);
+            }
+            acc = mfma_bf16(qa[0][s], lo, acc);
+            if constexpr (NQ == 3) acc = mfma_bf16(qa[1][s], hi, acc);
+            acc = mfma_bf16(qa[0][s], mid, acc);
+            acc = mfma_bf16(qa[0][s], hi, acc);
         }
         // lane (c, kq) holds rows 4 kq + i (query heads) of column j
         const int j = 16 * (t & 7) + c;
@@ -709,13 +752,14 @@ struct Og {
 // Blocks of TQ_BLOCK_TOKENS slots to attend to, instead of every slot of the range (LIST): `keep` numbers for each KV head of each batch row.
 struct BlockList {
     const int32_t* blocks;
-    int keep;
+    int keep, q_type;
 };
 struct NoList {};
 
 // X1 > 0: group 1's widths are group 0's plus X1 (the reference's default outlier_extra_bits
 // is 1), compile-time constants; X1 = 0: the widths come from og at run time.
-template <int KB, int VB, bool QJL, int GC, int OD = 0, int X1 = 0, bool LIST = false>
+// NQ: bf16 terms of a query, 1 for bf16 ones, 3 for fp32 and fp16 ones (LIST).
+template <int KB, int VB, bool QJL, int GC, int OD = 0, int X1 = 0, bool LIST = false, int NQ = 1>
 __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel(
     const uint16_t* __restrict__ q, int q_heads, int kv_heads, int G, const int32_t* __restrict__ seq_starts,
     const int32_t* __restrict__ seq_lens, int64_t n_tokens, int64_t cap, const uint8_t* __restrict__ kc,
@@ -727,6 +771,7 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
     std::conditional_t<LIST, BlockList, NoList> list) {
     constexpr bool SPL = OD > 0;
     static_assert(!(SPL && LIST), "chosen blocks: one-group layers only");
+    static_assert(LIST || NQ == 1, "queries of other types: chosen blocks only");
     static_assert(!SPL || OD <= OD1, "two-group layers: at most OD1 outlier dims per lane");
     using Sm = Smem<KB, VB, QJL, GC, OD>;
     using R = Rows<GC>;
@@ -1013,8 +1058,10 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
         E = 15 - e;
     }
     constexpr int PRO_SETS = Cfg<VB, GC, QJL, SPL>::PRO_SETS;
-    image_products<QJL, GC, NW, KI8, (GC == 1 || SPL)>(q, G, bh0, Rk, S, c_mse, sm.u.pro.ps, img, sm.u.pro.qst[wave], wave,
-                                                       lane, SPL ? og.d0 : D, [&] {
+    int q_type = 0;
+    if constexpr (LIST) q_type = list.q_type;
+    image_products<QJL, GC, NW, KI8, (GC == 1 || SPL), NQ>(q, q_type, G, bh0, Rk, S, c_mse, sm.u.pro.ps, img, sm.u.pro.qst[wave], wave,
+                                                           lane, SPL ? og.d0 : D, [&] {
         ck_e = Ck[tid & ((1 << KB) - 1)];
         cv_e = Cv[tid & ((1 << VB) - 1)];
         if constexpr (SPL) {
@@ -1723,7 +1770,9 @@ int launch_split(const SplitArgs& a, int groups, hipStream_t s, int* n_split_out
 // 4 query heads each; 35 MB) take 18 us, as many tokens in a row 17.6 and all 32768 of them 63; 32 of a chat's 129 blocks 13.8, 13.5 and 14.7; 128
 // of 2048 blocks for 64 KV heads of 7 query heads (3-bit Q_mse, 53 MB) 25.  The kernel's start (rotated queries and tables, 8 us) and the
 // merge (4) are the larger part of each.
-template <int KB, int VB, bool QJL, int GC>
+// fp16 and fp32 queries (NQ = 3) take 15.1, 18.9 and 24.2 (fp16 of 7 query heads for 64 KV heads, 128 blocks of 65536 tokens) where
+// bf16 ones take 13.7, 18.1 and 24.0.
+template <int KB, int VB, bool QJL, int GC, int NQ>
 int launch_blocks(const SplitArgs& a, const BlockList& list, int groups, hipStream_t s, int* n_split) {
     using C = Cfg<VB, GC, QJL>;
     const int64_t all = (int64_t)list.keep * TQ_BLOCK_TOKENS;
@@ -1733,7 +1782,7 @@ int launch_blocks(const SplitArgs& a, const BlockList& list, int groups, hipStre
     const int ns = (int)((all + tps - 1) / tps);
     *n_split = ns;
     if (a.po == nullptr) return TQ_OK;  // sizing query only
-    hipLaunchKernelGGL((split_kernel<KB, VB, QJL, GC, 0, 0, true>), dim3(ns, groups), dim3(C::NT), 0, s, a.q, a.q_heads, a.kv_heads,
+    hipLaunchKernelGGL((split_kernel<KB, VB, QJL, GC, 0, 0, true, NQ>), dim3(ns, groups), dim3(C::NT), 0, s, a.q, a.q_heads, a.kv_heads,
                        a.G, a.seq_starts, a.seq_lens, a.n_tokens, a.cap, a.kc, a.kn, a.ks, a.kr, a.vc, a.vn, a.Rk, a.S, a.c_mse,
                        a.c_qjl, a.Ck, a.Cv, a.scale, tps, ns, a.po, a.pml, a.og, list);
     return TQ_OK;
@@ -1741,7 +1790,9 @@ int launch_blocks(const SplitArgs& a, const BlockList& list, int groups, hipStre
 
 int dispatch_blocks(int value_bits, int has_qjl, const SplitArgs& a, const BlockList& list, int groups, hipStream_t s, int* ns) {
     auto launch = [&](auto kb, auto vb, auto qjl) {
-        return a.G <= 4 ? launch_blocks<kb, vb, qjl, 1>(a, list, groups, s, ns) : launch_blocks<kb, vb, qjl, 2>(a, list, groups, s, ns);
+        if (list.q_type == 0)
+            return a.G <= 4 ? launch_blocks<kb, vb, qjl, 1, 1>(a, list, groups, s, ns) : launch_blocks<kb, vb, qjl, 2, 1>(a, list, groups, s, ns);
+        return a.G <= 4 ? launch_blocks<kb, vb, qjl, 1, 3>(a, list, groups, s, ns) : launch_blocks<kb, vb, qjl, 2, 3>(a, list, groups, s, ns);
     };
     using std::integral_constant;
     const auto one = integral_constant<int, 1>{};
@@ -2207,7 +2258,7 @@ int decode_attention_impl(const uint16_t* q, int batch, int q_heads, int kv_head
     st = dispatch(value_bits, has_qjl, G, a, groups, s, &n_split, &tps);
     if (st != TQ_OK) return st;
     TQ_CHECK_LAUNCH();
-    hipLaunchKernelGGL(merge_kernel, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml, n_split, value_rotation,
+    hipLaunchKernelGGL(merge_kernel<false>, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml, n_split, value_rotation,
                        out_f32, out_bf16, lse_out);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
@@ -2393,7 +2444,7 @@ extern "C" int tq_decode_attention_groups(const uint16_t* q, int batch, int q_he
         st = dispatch_og(value_bits[0], has_qjl, G, sa, groups, s, &n_split, &tps);
         if (st != TQ_OK) return st;
         TQ_CHECK_LAUNCH();
-        hipLaunchKernelGGL(merge_kernel, dim3(batch * q_heads), dim3(MT), 0, s, sa.po, sa.pml, n_split, value_matrix,
+        hipLaunchKernelGGL(merge_kernel<false>, dim3(batch * q_heads), dim3(MT), 0, s, sa.po, sa.pml, n_split, value_matrix,
                            out_f32, out_bf16, lse_out);
         TQ_CHECK_LAUNCH();
         return TQ_OK;
@@ -2417,7 +2468,7 @@ extern "C" int tq_decode_attention_groups(const uint16_t* q, int batch, int q_he
         else hipLaunchKernelGGL((group_attn_kernel<8, false>), grid, dim3(GT), lds, s, a);
     }
     TQ_CHECK_LAUNCH();
-    hipLaunchKernelGGL(merge_kernel, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml, n_split, value_matrix,
+    hipLaunchKernelGGL(merge_kernel<false>, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml, n_split, value_matrix,
                        out_f32, out_bf16, lse_out);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
@@ -2439,17 +2490,17 @@ extern "C" size_t tq_block_attention_workspace_bytes(int batch, int q_heads, int
     return blocks_workspace(batch, q_heads, kv_heads, keep);
 }
 
-extern "C" int tq_block_attention(const uint16_t* q, int batch, int q_heads, int kv_heads, int dim, const int32_t* blocks, int keep,
+extern "C" int tq_block_attention_typed(const void* q, int q_type, int batch, int q_heads, int kv_heads, int dim, const int32_t* blocks, int keep,
                                   const int32_t* seq_starts, const int32_t* seq_lens, int64_t n_tokens, int64_t cap,
                                   const uint8_t* k_codes, const uint16_t* k_norms, const uint8_t* k_signs,
                                   const uint16_t* k_rnorms, const uint8_t* v_codes, const uint16_t* v_norms, int key_bits,
                                   int value_bits, int has_qjl, const float* key_rotation, const float* key_centers,
                                   const float* qjl, const float* value_rotation, const float* value_centers, float scale,
-                                  float* out_f32, uint16_t* out_bf16, float* lse_out, void* workspace, size_t workspace_bytes,
+                                  float* out_f32, uint16_t* out_16, float* lse_out, void* workspace, size_t workspace_bytes,
                                   void* stream) {
-    if (!q || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || !blocks || keep < 1 || n_tokens < 0 ||
+    if (!q || q_type < 0 || q_type > 2 || batch <= 0 || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || !blocks || keep < 1 || n_tokens < 0 ||
         cap < n_tokens || !key_rotation || !key_centers || !value_rotation || !value_centers || (has_qjl && !qjl) ||
-        (!out_f32 && !out_bf16 && !lse_out) || (n_tokens > 0 && (!k_codes || !k_norms || !v_codes || !v_norms)) ||
+        (!out_f32 && !out_16 && !lse_out) || (n_tokens > 0 && (!k_codes || !k_norms || !v_codes || !v_norms)) ||
         (has_qjl && n_tokens > 0 && (!k_signs || !k_rnorms)) || !(scale > 0.0f) || scale == __builtin_inff())
         return TQ_ERR_INVALID_ARGUMENT;
     const int G = q_heads / kv_heads;
@@ -2465,12 +2516,12 @@ extern "C" int tq_block_attention(const uint16_t* q, int batch, int q_heads, int
     if (!workspace || !aligned16(workspace)) return TQ_ERR_WORKSPACE;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int groups = batch * kv_heads;
-    SplitArgs a{q,        q_heads,  kv_heads, G,           seq_starts,    seq_lens,
+    SplitArgs a{static_cast<const uint16_t*>(q), q_heads,  kv_heads, G,           seq_starts,    seq_lens,
                 n_tokens, cap,      k_codes,  k_norms,     k_signs,       k_rnorms,
                 v_codes,  v_norms,  key_rotation, qjl,     scale * LOG2E, scale * LOG2E * QJL_SCALE,
                 key_centers, value_centers, scale, 0,      0,             nullptr,
                 nullptr};
-    const BlockList list{blocks, keep};
+    const BlockList list{blocks, keep, q_type};
     int n_split = 0;
     (void)dispatch_blocks(value_bits, has_qjl, a, list, groups, s, &n_split);  // sizing
     const Ws w = ws_layout(batch, q_heads, n_split);
@@ -2479,8 +2530,22 @@ extern "C" int tq_block_attention(const uint16_t* q, int batch, int q_heads, int
     a.pml = reinterpret_cast<float*>(static_cast<char*>(workspace) + w.pml);
     (void)dispatch_blocks(value_bits, has_qjl, a, list, groups, s, &n_split);
     TQ_CHECK_LAUNCH();
-    hipLaunchKernelGGL(merge_kernel, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml, n_split, value_rotation,
-                       out_f32, out_bf16, lse_out);
+    hipLaunchKernelGGL(q_type == 2 ? merge_kernel<true> : merge_kernel<false>, dim3(batch * q_heads), dim3(MT), 0, s, a.po, a.pml,
+                       n_split, value_rotation, out_f32, out_16, lse_out);
     TQ_CHECK_LAUNCH();
     return TQ_OK;
+}
+
+extern "C" int tq_block_attention(const uint16_t* q, int batch, int q_heads, int kv_heads, int dim, const int32_t* blocks, int keep,
+                                  const int32_t* seq_starts, const int32_t* seq_lens, int64_t n_tokens, int64_t cap,
+                                  const uint8_t* k_codes, const uint16_t* k_norms, const uint8_t* k_signs,
+                                  const uint16_t* k_rnorms, const uint8_t* v_codes, const uint16_t* v_norms, int key_bits,
+                                  int value_bits, int has_qjl, const float* key_rotation, const float* key_centers,
+                                  const float* qjl, const float* value_rotation, const float* value_centers, float scale,
+                                  float* out_f32, uint16_t* out_bf16, float* lse_out, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    return tq_block_attention_typed(q, 0, batch, q_heads, kv_heads, dim, blocks, keep, seq_starts, seq_lens, n_tokens, cap, k_codes,
+                                    k_norms, k_signs, k_rnorms, v_codes, v_norms, key_bits, value_bits, has_qjl, key_rotation,
+                                    key_centers, qjl, value_rotation, value_centers, scale, out_f32, out_bf16, lse_out, workspace,
+                                    workspace_bytes, stream);
 }

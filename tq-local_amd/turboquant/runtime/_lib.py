@@ -62,6 +62,8 @@ SIGNATURES: dict[str, tuple] = {
     "tq_block_attention_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
     "tq_block_attention": (_I, [_P, _I, _I, _I, _I, _P, _I, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P,
                                 _P, _F, _P, _P, _P, _P, _SZ, _P]),
+    "tq_block_attention_typed": (_I, [_P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P,
+                                      _P, _P, _F, _P, _P, _P, _P, _SZ, _P]),
     "tq_gather_tokens": (_I, [_I, _P, _P, _P, _I, _I, _I64, _I64, _I, _I64, _P, _P, _I64, _I64, _I64, _P]),
     "tq_keep_tokens": (_I, [_I, _P, _P, _I, _I, _I64, _I64, _I64, _P, _I64, _I64, _I, _P]),
     "tq_dequantize_group": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _I, _I, _P, _P, _P, _I, _P, _P]),

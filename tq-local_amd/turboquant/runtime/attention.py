@@ -173,7 +173,7 @@ def fused_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", 
         choice = packed_layer._choice if choice is None else choice
         blocks = None
         if choice is not None:
-            q = q if q.dtype in K._QUERY_TYPES else q.to(torch.bfloat16)
+            q = q if q.dtype in K._QUERY_TYPES else q.float()
             blocks = packed_layer.choose_blocks(q, choice, starts, p_ends)
         attend = K.decode_attention if blocks is None else functools.partial(K.block_attention, blocks=blocks)
         outs = attend(q, k_codes=store.kc, k_norms=store.kn, v_codes=store.vc, v_norms=store.vn, key=c.key, value=c.value,

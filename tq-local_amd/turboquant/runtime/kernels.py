@@ -1099,16 +1099,17 @@ def block_attention(q: torch.Tensor, blocks: torch.Tensor, *, k_codes: torch.Ten
 
     ``blocks`` int [B, Hkv, n], for each KV head the numbers of its blocks, in any order, n <= 4096.  Slots of a block outside
     [``seq_starts``, ``seq_lens``) and [0, ``n_tokens``) are left out, so is a number that names no slot (-1 as ``select_blocks`` leaves
-    it); a block named twice counts twice.  At most 8 query heads per KV head.  The rest, and what it returns, as for
-    ``decode_attention``.
+    it); a block named twice counts twice.  At most 8 query heads per KV head.  q [B, Hq, D] or [B, Hq, 1, D] in bf16, fp16 or fp32, of
+    which no bit is left out.  Returns [B, Hq, D] in q's dtype, then fp32 with ``want_f32``, then the fp32 log-sum-exp [B, Hq] with
+    ``want_lse``.  The rest as for ``decode_attention``.
     """
     q, B, Hq, q_sb, q_sh = _one_token("block_attention", q)
     _no_gradient("block_attention", q)
     _not_traced("block_attention")
     _require_gpu(q)
     dev, on, D = q.device, q.get_device(), HEAD_DIM
-    if q.dtype is not torch.bfloat16 or (q_sh != D and Hq != 1) or (q_sb != Hq * D and B != 1) or q.data_ptr() % 16:
-        q = q.to(torch.bfloat16, copy=True, memory_format=torch.contiguous_format)
+    if (q_sh != D and Hq != 1) or (q_sb != Hq * D and B != 1) or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
     has_qjl = qjl is not None
     cache = {"k_codes": k_codes, "k_norms": k_norms, "k_signs": k_signs, "k_rnorms": k_rnorms, "v_codes": v_codes, "v_norms": v_norms}
     (kc, kn, ks, kr, vc, vn), (_, Hkv, cap) = _packed_arrays("block_attention", cache, B, key, value, has_qjl, on)
@@ -1124,24 +1125,23 @@ def block_attention(q: torch.Tensor, blocks: torch.Tensor, *, k_codes: torch.Ten
     seq_starts = _int32_on(seq_starts, dev, "seq_starts", (B,))
     seq_lens = _int32_on(seq_lens, dev, "seq_lens", (B,))
     s = _logit_scale("block_attention", scale)
-    out = q.new_empty((B, Hq, D))
-    f32 = torch.empty((B, Hq, D), dtype=torch.float32, device=dev) if want_f32 else None
+    f32 = torch.empty((B, Hq, D), dtype=torch.float32, device=dev) if want_f32 or q.dtype is torch.float32 else None
+    out = q.new_empty((B, Hq, D)) if q.dtype is not torch.float32 else None
     lse = torch.empty((B, Hq), dtype=torch.float32, device=dev) if want_lse else None
     if B and Hq and keep:
         need = _lib.load().tq_block_attention_workspace_bytes(B, Hq, Hkv, D, keep)
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-        _on_device("tq_block_attention", on, q.data_ptr(), B, Hq, Hkv, D, blocks.data_ptr(), keep, _ptr(seq_starts), _ptr(seq_lens),
-                   n_tokens, cap, kc, kn, ks, kr, vc, vn, key.bits, value.bits, int(has_qjl), key.rotation.data_ptr(),
-                   key.centers.data_ptr(), _ptr(qjl), value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s,
-                   _ptr(f32), out.data_ptr(), _ptr(lse), ws.data_ptr(), max(need, 16), _stream_handle(dev))
+        _on_device("tq_block_attention_typed", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, D, blocks.data_ptr(), keep,
+                   _ptr(seq_starts), _ptr(seq_lens), n_tokens, cap, kc, kn, ks, kr, vc, vn, key.bits, value.bits, int(has_qjl),
+                   key.rotation.data_ptr(), key.centers.data_ptr(), _ptr(qjl), value.rotation.data_ptr(),
+                   attention_value_centers(value).data_ptr(), s, _ptr(f32), _ptr(out), _ptr(lse), ws.data_ptr(), max(need, 16),
+                   _stream_handle(dev))
     else:  # nothing is attended to
-        out.zero_()
-        if f32 is not None:
-            f32.zero_()
-        if lse is not None:
-            lse.fill_(float("-inf"))
-    outs = (out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
-    return outs if len(outs) > 1 else out
+        for t, x in ((out, 0.0), (f32, 0.0), (lse, float("-inf"))):
+            if t is not None:
+                t.fill_(x)
+    outs = (f32 if out is None else out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
+    return outs if len(outs) > 1 else outs[0]
 
 
 def rows16(t: torch.Tensor) -> torch.Tensor:
