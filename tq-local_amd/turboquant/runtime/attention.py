@@ -123,10 +123,10 @@ def _group_buffers(layer: "PackedMSELayer") -> list[dict]:
 
 def fused_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", n_kv_groups: int,
                     attention_mask: torch.Tensor | None = None,
-                    choice: "BlockChoice | None" = None) -> torch.Tensor | None:
+                    choice: "BlockChoice | None" = None, scale: float | None = None) -> torch.Tensor | None:
     """Decode attention of [B, Hq, 1, D] queries over a packed layer -> [B, Hq, 1, D].
 
-    The logit scale is 1/sqrt(D) (reference ``triton_kernels.py:285``).  Tokens
+    The logit scale is 1/sqrt(D) (reference ``triton_kernels.py:285``) unless ``scale`` is given.  Tokens
     kept dense (``quantize_decode=False``) are merged by log-sum-exp.  Outlier-split
     layers go through the channel-group kernel (where the reference returns None and
     its caller takes the chunked path).  The result has the query's dtype; an fp32
@@ -149,7 +149,7 @@ def fused_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", 
         return None
     n_packed = packed_layer.packed_seq_length()
     n_dense = packed_layer._dense_len
-    scale = 1.0 / math.sqrt(D)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     known = getattr(packed_layer, "_tq_mask_contiguous", None)
     if attention_mask is not None and known is False:
         return None
@@ -264,11 +264,10 @@ _ROW_BYTES = 64 << 20
 
 
 def _native_chunked(query: torch.Tensor, layer: "PackedMSELayer", new_key, new_value, mask, chunk_size: int,
-                    kv_heads: int) -> torch.Tensor:
+                    kv_heads: int, scale: float) -> torch.Tensor:
     """``chunked_turboquant_attention`` in libtq kernels: per segment of the packed history two
     decoder launches and one attention launch, one launch per dense part, one merge of the
     splits."""
-    scale = 1.0 / math.sqrt(query.shape[-1])
     q = query if query.dtype == torch.bfloat16 else query.float()
     if mask is not None and mask.dtype != torch.bool:
         mask = mask.float()
@@ -307,18 +306,19 @@ def _additive_mask(mask: torch.Tensor | None) -> torch.Tensor | None:
 def chunked_turboquant_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer",
                                  new_key: torch.Tensor | None = None, new_value: torch.Tensor | None = None,
                                  n_kv_groups: int = 1, attention_mask: torch.Tensor | None = None,
-                                 chunk_size: int = _DEFAULT_CHUNK_SIZE) -> torch.Tensor:
+                                 chunk_size: int = _DEFAULT_CHUNK_SIZE, scale: float | None = None) -> torch.Tensor:
     """Any-shape attention over a packed layer -> [B, Q, Sq, D] (reference runtime/attention.py:215-304).
 
     The packed history is decoded by libtq ``chunk_size`` tokens at a time into bf16 K / V
     rows (reference ``_decode_keys_range`` / ``_decode_values_range``), then the dense decode
-    buffer and ``new_key`` / ``new_value`` follow; logits are fp32 ``q . K / sqrt(D)`` plus
+    buffer and ``new_key`` / ``new_value`` follow; logits are fp32 ``q . K / sqrt(D)`` (or times ``scale``) plus
     the mask slice of each part, merged by an online softmax and normalised with the 1e-8
     clamp.  A boolean mask (True = attend) is applied as 0 / -inf; the reference adds
     ``mask.float()``, which is only right for additive masks.  Rows with nothing to attend
     to return zeros (the reference's running maximum turns them into NaN).
     """
     B, Q, Sq, D = query_states.shape
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     dense = (packed_layer._dense_keys, packed_layer._dense_values)
     parts = [t for t in (*dense, new_key, new_value) if t is not None]
     n_packed = packed_layer.packed_seq_length()
@@ -331,8 +331,7 @@ def chunked_turboquant_attention(query_states: torch.Tensor, packed_layer: "Pack
             and all(a is None or a.shape == b.shape for a, b in ((dense[0], dense[1]), (new_key, new_value)))
             and (n_packed == 0 or packed_layer._shape == (B, Q // n_kv_groups, D))):
         return _native_chunked(query_states, packed_layer, new_key, new_value, attention_mask, chunk_size,
-                               Q // n_kv_groups)
-    scale = 1.0 / math.sqrt(D)
+                               Q // n_kv_groups, scale)
     qf = query_states.float()
     mask = _additive_mask(attention_mask)
     m = torch.full((B, Q, Sq, 1), float("-inf"), device=qf.device)
@@ -502,13 +501,15 @@ def _rows_mask(mask: torch.Tensor | None, B: int, Sq: int, total: int, device) -
 
 
 def shared_prefix_attention(query_states: torch.Tensor, layer: "SharedPrefixLayer",
-                            attention_mask: torch.Tensor | None = None) -> torch.Tensor:
+                            attention_mask: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """Attention of sequences that continue shared packed prompts, [B, Hq, Sq, D] over a ``SharedPrefixLayer`` -> [B, Hq, Sq, D].
 
     One query token per sequence, up to 64 query heads per KV head and a mask of one range per row (left padding of the
     prompts) run on the packed codes (``kernels.prefix_attention``), tokens kept dense merged by log-sum-exp; others
-    take the decoded rows (``chunked_turboquant_attention``), the Sq tokens being the sequences' last ones."""
+    take the decoded rows (``chunked_turboquant_attention``), the Sq tokens being the sequences' last ones.  The logit scale is
+    1/sqrt(D) unless ``scale`` is given."""
     B, Hq, Sq, D = query_states.shape
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     prefix, own = layer.prefix, layer.own
     store, n_prefix, n_own, n_dense = prefix._store, prefix.packed_seq_length(), own.packed_seq_length(), own._dense_len
     if B != layer.batch or Hq % store.H:
@@ -526,7 +527,7 @@ def shared_prefix_attention(query_states: torch.Tensor, layer: "SharedPrefixLaye
                                 "v_codes": s.vc, "v_norms": s.vn}
             c = prefix.codecs
             kw = dict(n_prefix=n_prefix, n_own=n_own, key=c.key, value=c.value, qjl=c.qjl, cu_rows=layer.cu_rows,
-                      max_rows=max(layer.counts), prefix_starts=starts, prefix_lens=ends, own_lens=own_ends)
+                      max_rows=max(layer.counts), prefix_starts=starts, prefix_lens=ends, own_lens=own_ends, scale=scale)
             mine = arrays(own._store) if n_own else None
             if not n_dense:
                 return K.prefix_attention(query_states, arrays(store), mine, **kw).view(B, Hq, 1, D)
@@ -534,11 +535,11 @@ def shared_prefix_attention(query_states: torch.Tensor, layer: "SharedPrefixLaye
             q = query_states if query_states.dtype == torch.bfloat16 else query_states.float()
             n = K.DenseAttention.split_count(q, store.H, n_dense, K.DENSE_SPLITS)
             more = {} if own_ends is None else dict(starts=torch.zeros_like(own_ends), ends=own_ends, pos0=n_own)
-            return K.DenseAttention(q, store.H, n).add(*dense, n_dense, 0, n, 1.0 / math.sqrt(D), out=query_states.dtype,
+            return K.DenseAttention(q, store.H, n).add(*dense, n_dense, 0, n, scale, out=query_states.dtype,
                                                        prev=o_packed, prev_lse=lse, **more)
     keys, values = layer.dense_rows()
     mask = _rows_mask(attention_mask, B, Sq, keys.shape[2], dev)
-    return chunked_turboquant_attention(query_states, layer.without_tokens(), keys, values, group, mask)
+    return chunked_turboquant_attention(query_states, layer.without_tokens(), keys, values, group, mask, scale=scale)
 
 
 def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *,
@@ -582,10 +583,13 @@ def _hands_over_all(layer: "PackedMSELayer", query: torch.Tensor, key: torch.Ten
 def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, key: torch.Tensor,
                                  value: torch.Tensor, attention_mask: torch.Tensor | None, dropout: float = 0.0,
                                  scaling: float | None = None, is_causal: bool | None = None, **kwargs):
-    """HF attention-interface function: returns ([B, Sq, Hq, D], None)."""
+    """HF attention-interface function: returns ([B, Sq, Hq, D], None).  Logits are scaled by ``scaling`` (1/sqrt(D) without) on every
+    path, the prompt's before a layer is packed and the steps over it alike; the reference's steps leave it out
+    (``triton_kernels.py:285``)."""
     layer = getattr(module, "_tq_cache_layer", None)
     if getattr(layer, "shares_prompts", False):
-        return shared_prefix_attention(query, layer, attention_mask).transpose(1, 2).contiguous(), None
+        scale = None if scaling is None else K._logit_scale("shared_prefix_attention", scaling)
+        return shared_prefix_attention(query, layer, attention_mask, scale).transpose(1, 2).contiguous(), None
     if layer is None or _hands_over_all(layer, query, key, attention_mask):
         return _sdpa_fallback(module, query, key, value, attention_mask, scaling)
     if layer.packed_seq_length() == 0:  # the tokens before are dense: attended to as a norm-guarded layer's are
@@ -594,9 +598,10 @@ def turboquant_attention_forward(module: torch.nn.Module, query: torch.Tensor, k
             attention_mask = torch.ones(Sq, held, dtype=torch.bool, device=query.device).tril(held - Sq)
         return _sdpa_fallback(module, query, layer._dense_keys, layer._dense_values, attention_mask, scaling)
     n_kv_groups = getattr(module, "num_key_value_groups", 1)
-    out = fused_attention(query, layer, n_kv_groups, attention_mask) if query.shape[-2] == 1 else None
+    scale = None if scaling is None else K._logit_scale("fused_attention", scaling)
+    out = fused_attention(query, layer, n_kv_groups, attention_mask, scale=scale) if query.shape[-2] == 1 else None
     if out is None:  # several query tokens, or a shape / mask the fused kernel does not take
-        out = chunked_turboquant_attention(query, layer, n_kv_groups=n_kv_groups, attention_mask=attention_mask)
+        out = chunked_turboquant_attention(query, layer, n_kv_groups=n_kv_groups, attention_mask=attention_mask, scale=scale)
     return out.transpose(1, 2).contiguous(), None
 
 
