@@ -57,9 +57,14 @@ def _attend_mask(attention_mask: torch.Tensor, B: int, total: int) -> torch.Tens
 
 
 #: the ranges of the last mask seen, per host thread (an HF forward hands every layer the same
-#: mask tensor): (mask, its version counter, B, total, check) -> (starts, ends); holding the mask
+#: mask tensor): (mask, its version counter, B, total, check, device) -> (starts, ends); holding the mask
 #: keeps its memory from being reused by another tensor while the entry is live
 _tls = threading.local()
+
+
+def _version(t: torch.Tensor) -> int | None:
+    """A tensor's version counter; tensors made in inference mode have none, and nothing is kept for them."""
+    return None if t.is_inference() else t._version
 
 
 def _valid_range(attention_mask: torch.Tensor | None, B: int, total: int, device, check_contiguous: bool = True):
@@ -77,18 +82,18 @@ def _valid_range(attention_mask: torch.Tensor | None, B: int, total: int, device
         return None, None
     if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
         return _compute_range(attention_mask, B, total, device, check_contiguous)
+    key = _version(attention_mask), B, total, check_contiguous, device
     c = getattr(_tls, "last_range", None)
-    if (c is not None and c[0] is attention_mask and c[1] == attention_mask._version
-            and c[2:6] == (B, total, check_contiguous, device)):
-        if c[6] is None:
+    if c is not None and c[0] is attention_mask and c[1] == key and key[0] is not None:
+        if c[2] is None:
             raise _HoleyMask
-        return c[6]
+        return c[2]
     try:
         result = _compute_range(attention_mask, B, total, device, check_contiguous)
     except _HoleyMask:
-        _tls.last_range = (attention_mask, attention_mask._version, B, total, check_contiguous, device, None)
+        _tls.last_range = (attention_mask, key, None)
         raise
-    _tls.last_range = (attention_mask, attention_mask._version, B, total, check_contiguous, device, result)
+    _tls.last_range = (attention_mask, key, result)
     return result
 
 
