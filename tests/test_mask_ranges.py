@@ -49,3 +49,20 @@ def test_masks_made_in_inference_mode(computed):
         mask[1, 6] = True
         assert ranges(mask) == [[0, 4], [9, 9]]
     assert len(computed) == 4
+
+
+@pytest.mark.gpu
+def test_a_step_on_another_stream_finds_its_own_ranges(cuda, computed):
+    mask = torch.ones(2, 9, dtype=torch.bool, device="cuda")
+    mask[1, :4] = False
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(10_000_000)
+        first = A._valid_range(mask, 2, 9, mask.device, check_contiguous=False)
+    second = A._valid_range(mask, 2, 9, mask.device, check_contiguous=False)
+    assert len(computed) == 2 and second is not first
+    assert [t.tolist() for t in second] == [[0, 4], [9, 9]]
+    assert A._valid_range(mask, 2, 9, mask.device, check_contiguous=False) is second
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, second))

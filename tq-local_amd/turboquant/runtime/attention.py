@@ -57,8 +57,9 @@ def _attend_mask(attention_mask: torch.Tensor, B: int, total: int) -> torch.Tens
 
 
 #: the ranges of the last mask seen, per host thread (an HF forward hands every layer the same
-#: mask tensor): (mask, its version counter, B, total, check, device) -> (starts, ends); holding the mask
-#: keeps its memory from being reused by another tensor while the entry is live
+#: mask tensor): (mask, its version counter, B, total, check, device, stream) -> (starts, ends); holding the mask
+#: keeps its memory from being reused by another tensor while the entry is live.  A step on another stream finds its own:
+#: it does not wait for this one
 _tls = threading.local()
 
 
@@ -82,7 +83,8 @@ def _valid_range(attention_mask: torch.Tensor | None, B: int, total: int, device
         return None, None
     if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
         return _compute_range(attention_mask, B, total, device, check_contiguous)
-    key = _version(attention_mask), B, total, check_contiguous, device
+    key = (_version(attention_mask), B, total, check_contiguous, device,
+           K._stream_handle(attention_mask.device) if attention_mask.is_cuda else 0)
     c = getattr(_tls, "last_range", None)
     if c is not None and c[0] is attention_mask and c[1] == key and key[0] is not None:
         if c[2] is None:
