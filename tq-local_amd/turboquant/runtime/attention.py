@@ -63,6 +63,10 @@ def _attend_mask(attention_mask: torch.Tensor, B: int, total: int) -> torch.Tens
 _tls = threading.local()
 
 
+_UNKNOWN_MASK = ("a captured step cannot look whether its mask's rows are ranges of tokens: take the step with the same mask before the "
+                 "capture, or set _tq_mask_contiguous of the cache's layers")
+
+
 def _version(t: torch.Tensor) -> int | None:
     """A tensor's version counter; tensors made in inference mode have none, and nothing is kept for them."""
     return None if t.is_inference() else t._version
@@ -78,11 +82,19 @@ def _valid_range(attention_mask: torch.Tensor | None, B: int, total: int, device
     callers that know the mask's shape pass False.  The result for one mask tensor is
     computed once and reused by the following layers of the same forward; a call that is
     being captured computes its own, which every replay then does from the mask as it is.
+    A capture cannot look at the mask: what the step before it found of the same mask is taken
+    (replays are to have masks of the same kind), and without such a step the call is refused.
     """
     if attention_mask is None:
         return None, None
     if attention_mask.is_cuda and torch.cuda.is_current_stream_capturing():
-        return _compute_range(attention_mask, B, total, device, check_contiguous)
+        if check_contiguous:
+            c = getattr(_tls, "last_range", None)
+            if c is None or c[0] is not attention_mask or c[1][0] is None or c[1][:5] != (_version(attention_mask), B, total, True, device):
+                raise ValueError(_UNKNOWN_MASK)
+            if c[2] is None:
+                raise _HoleyMask
+        return _compute_range(attention_mask, B, total, device, False)
     key = (_version(attention_mask), B, total, check_contiguous, device,
            K._stream_handle(attention_mask.device) if attention_mask.is_cuda else 0)
     c = getattr(_tls, "last_range", None)
@@ -481,7 +493,7 @@ def _shared_ranges(layer: "SharedPrefixLayer", mask: torch.Tensor | None, device
 
     ``_HoleyMask`` where a row's tokens are not one range, or where the sequences of a prompt do not share its padding: a host
     sync to find out, which a caller spares who knows and says so in the layer's ``_tq_mask_contiguous``: True, every mask is
-    of such ranges, or False (as for ``fused_attention``)."""
+    of such ranges, or False (as for ``fused_attention``).  In a captured step what the step before found of the mask counts."""
     if mask is None:
         return None, None, None
     known = getattr(layer, "_tq_mask_contiguous", None)
@@ -490,8 +502,19 @@ def _shared_ranges(layer: "SharedPrefixLayer", mask: torch.Tensor | None, device
     n = layer.prefix.packed_seq_length()
     starts, ends = _valid_range(mask, layer.batch, layer.get_seq_length(), device, check_contiguous=not known)
     first, last = starts[layer.first_of], ends.clamp(max=n)[layer.first_of]
-    if not known and bool(((starts != first[layer.prompt_of]) | (ends.clamp(max=n) != last[layer.prompt_of]) | (starts > n)).any()):
-        raise _HoleyMask
+    if not known:
+        key = _version(mask), layer.counts, n, layer.get_seq_length()
+        c = getattr(_tls, "last_shared", None)
+        seen = c is not None and c[0] is mask and c[1] == key and key[0] is not None
+        if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+            if not seen:
+                raise ValueError(_UNKNOWN_MASK)
+            apart = c[2]
+        else:
+            apart = bool(((starts != first[layer.prompt_of]) | (ends.clamp(max=n) != last[layer.prompt_of]) | (starts > n)).any())
+            _tls.last_shared = mask, key, apart
+        if apart:
+            raise _HoleyMask
     return first, last, (ends - n).clamp(min=0)
 
 
