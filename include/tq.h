@@ -44,6 +44,9 @@ int tq_abi_version(void);
 /* Static, NUL-terminated description of a status code. */
 const char* tq_status_string(int status);
 
+/* *id (host) = the id of the graph capture that a stream is in, another for every capture; 0 outside one. */
+int tq_capture_id(void* stream, uint64_t* id);
+
 /*
  * Q_mse encoder (prefill and decode-append).
  * Replaces reference PackedMSELayer._encode_group (runtime/packed_qmse_cache.py:376-402)

@@ -4,7 +4,9 @@ import pytest
 import torch
 from transformers.cache_utils import Cache
 
+from turboquant.runtime import _lib
 from turboquant.runtime import attention as A
+from turboquant.runtime import kernels as K
 from turboquant.runtime import share_prefix
 
 from ._packed import D, make_layer, randn
@@ -130,3 +132,59 @@ def test_captured_steps_of_shared_layers_over_decoded_rows(cuda, hole):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, A.shared_prefix_attention(q, layer, mask)) and not torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_a_capture_finds_the_ranges_once_for_its_layers(cuda, computed):
+    """And anew in another capture, for another mask and behind a change of the mask within the capture."""
+    layers = [make_layer(2, 2, 300, 4, True, seed=i) for i in range(3)]
+    masks = [torch.ones(2, 300, dtype=torch.bool, device="cuda") for _ in range(2)]
+    masks[1][1, :7] = False
+    q = randn((2, 8, 1, D), 5)
+    for layer in layers:
+        layer._tq_mask_contiguous = True
+
+    def steps():
+        first = [A.fused_attention(q, layer, 4, masks[0]) for layer in layers]
+        other = [A.fused_attention(q, layer, 4, masks[1]) for layer in layers]
+        masks[1][0, :100] = False
+        changed = [A.fused_attention(q, layer, 4, masks[1]) for layer in layers]
+        masks[1][0, :100] = True
+        return first + other + changed
+
+    want = [t.clone() for t in steps()]
+    assert len(computed) == 3
+    graphs = []
+    for i in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = steps()
+        graphs.append((graph, out))
+        assert len(computed) == 6 + 3 * i
+    for _ in range(2):
+        for graph, out in reversed(graphs):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    masks[0][1, :60] = False
+    want = [t.clone() for t in steps()]
+    for graph, out in graphs:
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_captures_have_ids_of_their_own(cuda):
+    ids, x = [], torch.zeros(3, device="cuda")
+    assert K.capture_id(x.device) == 0
+    for _ in range(2):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ids.append(K.capture_id(x.device))
+            x.add_(1.0)
+            assert K.capture_id(x.device) == ids[-1]
+    assert 0 not in ids and ids[0] != ids[1] and K.capture_id(x.device) == 0
+
+
+def test_a_capture_id_needs_a_place_to_go():
+    assert _lib.load().tq_capture_id(None, None) == 1  # TQ_ERR_INVALID_ARGUMENT

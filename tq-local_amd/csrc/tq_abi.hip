@@ -15,6 +15,15 @@ extern "C" const char* tq_status_string(int status) {
     }
 }
 
+extern "C" int tq_capture_id(void* stream, uint64_t* id) {
+    if (!id) return TQ_ERR_INVALID_ARGUMENT;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long of = 0;
+    if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &of) != hipSuccess) return TQ_ERR_HIP;
+    *id = status == hipStreamCaptureStatusActive ? of : 0;
+    return TQ_OK;
+}
+
 // ------------------------------------------------------------------ value codebook in fp16
 // tq_decode_attention sums the values on fp16 matrix cores, so every value centroid enters as
 // one fp16 number.  Its rounding error is the same for every token that carries the code: over

@@ -64,6 +64,7 @@ SIGNATURES: dict[str, tuple] = {
                                 _P, _F, _P, _P, _P, _P, _SZ, _P]),
     "tq_block_attention_typed": (_I, [_P, _I, _I, _I, _I, _I, _P, _I, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P, _P, _P,
                                       _P, _P, _F, _P, _P, _P, _P, _SZ, _P]),
+    "tq_capture_id": (_I, [_P, _P]),
     "tq_gather_tokens": (_I, [_I, _P, _P, _P, _I, _I, _I64, _I64, _I, _I64, _P, _P, _I64, _I64, _I64, _P]),
     "tq_keep_tokens": (_I, [_I, _P, _P, _I, _I, _I64, _I64, _I64, _P, _I64, _I64, _I, _P]),
     "tq_dequantize_group": (_I, [_P, _P, _P, _P, _I64, _I64, _I64, _I, _P, _I, _I, _P, _P, _P, _I, _P, _P]),

@@ -80,8 +80,8 @@ def _valid_range(attention_mask: torch.Tensor | None, B: int, total: int, device
     hole (right padding followed by generated tokens) cannot take this path: with
     ``check_contiguous`` such masks raise ``_HoleyMask`` (one host sync to find out);
     callers that know the mask's shape pass False.  The result for one mask tensor is
-    computed once and reused by the following layers of the same forward; a call that is
-    being captured computes its own, which every replay then does from the mask as it is.
+    computed once and reused by the following layers of the same forward; a capture
+    computes its own, once on a stream too, which every replay then does from the mask as it is.
     A capture cannot look at the mask: what the step before it found of the same mask is taken
     (replays are to have masks of the same kind), and without such a step the call is refused.
     """
@@ -94,7 +94,14 @@ def _valid_range(attention_mask: torch.Tensor | None, B: int, total: int, device
                 raise ValueError(_UNKNOWN_MASK)
             if c[2] is None:
                 raise _HoleyMask
-        return _compute_range(attention_mask, B, total, device, False)
+        at = attention_mask.device
+        key = _version(attention_mask), B, total, device, K._stream_handle(at), K.capture_id(at)
+        c = getattr(_tls, "captured_range", None)
+        if c is None or c[0] is not attention_mask or c[1] != key or key[0] is None:
+            # (held until the next mask: the capture's later allocations leave the result alone)
+            c = _tls.captured_range = (attention_mask, key, _compute_range(attention_mask, B, total, device, False))
+        return c[2]
+    _tls.captured_range = None
     key = (_version(attention_mask), B, total, check_contiguous, device,
            K._stream_handle(attention_mask.device) if attention_mask.is_cuda else 0)
     c = getattr(_tls, "last_range", None)

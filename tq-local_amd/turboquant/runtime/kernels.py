@@ -63,6 +63,13 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(_stream_handle(device))
 
 
+def capture_id(device: torch.device) -> int:
+    """The id of the graph capture that the device's current stream is in; 0 outside one (tq_capture_id)."""
+    out = ctypes.c_uint64()
+    _lib.call("tq_capture_id", _stream_handle(device), ctypes.byref(out))
+    return out.value
+
+
 def _require_gpu(*tensors: torch.Tensor | None) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
