@@ -642,3 +642,26 @@ def test_bounds_that_another_stream_makes(cuda):
         got = other.choose_blocks(q, choice)
     torch.cuda.synchronize()
     assert torch.equal(got.cpu(), want())
+
+
+@pytest.mark.parametrize("known", [None, False])
+def test_masks_with_a_hole_are_attended_to_in_full(cuda, known):
+    """By a model's step; the call for one step over blocks refuses them."""
+    from turboquant.runtime.attention import turboquant_attention_forward, turboquant_prompt_forward
+
+    layer = make_layer(2, 2, 900, 4, True, seed=23)
+    layer.attend_blocks(4, sink=1, recent=1)
+    if known is not None:
+        layer._tq_mask_contiguous = known
+    module = torch.nn.Module()
+    module._tq_cache_layer, module.num_key_value_groups = layer, 4
+    mask = torch.ones(2, 900, dtype=torch.bool, device="cuda")
+    mask[1, 700:880] = False
+    q = randn((2, 8, 1, D), 5)
+    want, _ = attend64(q[:, :, 0], *rows64(layer), mask[:, None])
+    assert fused_attention(q, layer, 4, mask) is None
+    for forward in (turboquant_attention_forward, turboquant_prompt_forward):
+        got, _ = forward(module, q, None, None, mask[:, None, None])
+        check(got[:, 0], want, 2e-2)  # bf16 rows and weights: 2^-8 of the logits' terms and of the values
+    with pytest.raises(ValueError, match="one range"):
+        block_sparse_attention(q, layer, 4, attention_mask=mask)

@@ -164,7 +164,8 @@ def fused_attention(query_states: torch.Tensor, packed_layer: "PackedMSELayer", 
     not one contiguous range per row.  The cache layer's ``_tq_mask_contiguous`` (set by
     the generation loop from the prompt mask) spares the host sync of that last check.
 
-    A layer told to (``attend_blocks``), or a ``choice`` given here, attends to chosen blocks of the packed tokens.
+    A layer told to (``attend_blocks``), or a ``choice`` given here, attends to chosen blocks of the packed tokens.  Where None is
+    returned the caller's other path attends to all of them.
     """
     B, Hq, Sq, D = query_states.shape
     if Sq != 1:
@@ -480,7 +481,7 @@ def block_sparse_attention(query_states: torch.Tensor, packed_layer: "PackedMSEL
     The first ``sink`` blocks, the last ``recent`` and those that the query heads may give the largest logits, by bounds of the
     keys that the layer keeps (``PackedMSELayer.attend_blocks`` has every step of a model do it); tokens kept dense are all attended
     to.  A history of no more blocks is attended to in full.  One-group layers, up to 8 query heads per KV head, masks of one
-    range per row; others are refused."""
+    range per row; others, which a model's step would attend to in full, are refused."""
     from turboquant.runtime.packed_qmse_cache import BlockChoice
 
     B, Hq, Sq, D = query_states.shape

@@ -691,7 +691,9 @@ class PackedMSELayer(CacheLayerMixin):
         """From now on a decode step of the attention backend attends to ``keep`` blocks of 64 packed tokens for each KV head
         instead of to all of them: the first ``sink``, the last ``recent`` and those that its query may give the
         largest logits (``kernels.select_blocks``); dense tokens are attended to beside them.  ``None``: to all tokens again.
-        Steps of several tokens, layers split in channel groups and groups of more than 8 query heads attend to everything."""
+        Attended to in full are histories of no more blocks than ``keep`` and of more than 32768, and that by steps of several tokens,
+        layers split in channel groups, groups of more than 8 query heads and masks that leave out tokens inside a row's range (right padding with
+        tokens behind it), for which the interface takes the decoded rows."""
         self._choice = None if keep is None else BlockChoice(int(keep), int(sink), int(recent))
 
     def block_bounds(self) -> tuple[torch.Tensor, torch.Tensor, int]:
