@@ -8,8 +8,9 @@ import math
 import numpy as np
 import pytest
 import torch
+from transformers.cache_utils import Cache
 
-from turboquant.runtime import block_sparse_attention, fused_attention
+from turboquant.runtime import block_sparse_attention, fused_attention, share_prefix
 from turboquant.runtime import kernels as K
 from turboquant.runtime.packed_qmse_cache import BlockChoice
 from turboquant.runtime.synthetic import kv_bf16
@@ -665,3 +666,17 @@ def test_masks_with_a_hole_are_attended_to_in_full(cuda, known):
         check(got[:, 0], want, 2e-2)  # bf16 rows and weights: 2^-8 of the logits' terms and of the values
     with pytest.raises(ValueError, match="one range"):
         block_sparse_attention(q, layer, 4, attention_mask=mask)
+
+
+def test_bounds_are_counted_among_a_layers_bytes(cuda):
+    from turboquant.runtime.packed_qmse_cache import packed_cache_storage_bytes
+
+    layer = make_layer(2, 3, 1000, 4, True)
+    before = layer.storage_bytes()
+    layer.block_bounds()
+    assert layer.storage_bytes() - before == 2 * 3 * 15 * (2 * D + 4)
+    layer.crop(-200)
+    one = layer.storage_bytes()
+    assert one == before * 800 // 1000 + 2 * 3 * 12 * (2 * D + 4)
+    shared = share_prefix(Cache(layers=[layer]), 2)
+    assert packed_cache_storage_bytes(shared) == one

@@ -260,6 +260,10 @@ class _BlockBounds:
         self._home = K._stream_handle(self.step.device)
         self.written()
 
+    def storage_bytes(self) -> int:
+        B, H, _, *row = self.lohi.shape
+        return B * H * self.count * (prod(row) + self.step.element_size())
+
     def __getstate__(self) -> dict:  # copies are the current stream's
         self.ordered()
         return {**self.__dict__, "_home": K._stream_handle(self.step.device), "_wrote": None}
@@ -843,7 +847,7 @@ class PackedMSELayer(CacheLayerMixin):
         return -1
 
     def storage_bytes(self) -> int:
-        """Logical storage (N valid tokens, as the reference counts it; :874-885)."""
+        """Logical storage (N valid tokens, as the reference counts it; :874-885), and the bounds of the blocks that have them."""
         total = 0
         for p in (self.keys_packed, self.values_packed, self._keys_qjl, self._keys_outlier, self._values_outlier,
                   self._keys_outlier_qjl):
@@ -852,6 +856,8 @@ class PackedMSELayer(CacheLayerMixin):
         for d in (self._dense_keys, self._dense_values):
             if d is not None:
                 total += d.numel() * d.element_size()
+        if self._bounds is not None:
+            total += self._bounds.storage_bytes()
         return int(total)
 
 
