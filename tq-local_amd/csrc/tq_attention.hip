@@ -1034,6 +1034,7 @@ __global__ __launch_bounds__((Cfg<VB, GC, QJL, (OD > 0)>::NT)) void split_kernel
     Kd kset[NSET];
     Vd vset[NSET];
     static_assert(!SPL || (NSET == 2 && NB == 1), "two-group layers: group 1's loads serve the two blocks of a round");
+    static_assert(!LIST || NB == 1, "chosen blocks: a step is skipped by what its one block holds");
     OdT oset[2];  // two-group layers: rounds of even / odd parity
 
     // ------------------------------------------------------------ prologue

@@ -36,8 +36,9 @@ constexpr int MIN_TILES = 8;   // tiles of a split
 constexpr int MAX_SPLIT = 64;  // partials a merge wave weighs with one lane each
 constexpr float LOG2E = 1.44269504f;
 // Log2 that a score may exceed its row's reference by, and of the largest weight times norm at the reference: 15 together, what fp16
-// holds.  The less a score may exceed it the smaller the weights that keep their bits, and the more often references rise: with 4 the
-// calls of the header, with their merges, take 159 and 71 us, with 8 156 and 69, with 2 160 and 72
+// holds.  The less a score may exceed it the smaller the weights that keep their bits, and the more often references rise: trees of 16
+// nodes of 4 heads over 8 sequences of 32768 tokens (8 KV heads, 4-bit Q_prod), and of 64 nodes of 7 heads over 4 of 8192 (4 KV heads, 3-bit
+// Q_mse), take with their merges 159 and 71 us with 4, 156 and 69 with 8, 160 and 72 with 2
 constexpr float LAZY = 4.0f;
 constexpr int TOP_BIT = 11;
 constexpr float QJL_SCALE = 1.2533141373155003f / D;  // sqrt(pi/2) / D
@@ -59,13 +60,12 @@ __device__ __forceinline__ float sum_of_halves(float x) {
     const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(y[0]) + __uint_as_float(y[1]);
 }
-__device__ __forceinline__ f32x16 fill16(float x) {
+__device__ __forceinline__ f32x16 zero16() {
     f32x16 z;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) z[i] = x;
+    for (int i = 0; i < 16; ++i) z[i] = 0.0f;
     return z;
 }
-__device__ __forceinline__ f32x16 zero16() { return fill16(0.0f); }
 
 // ------------------------------------------------------------------ codes to fp16 rows
 
