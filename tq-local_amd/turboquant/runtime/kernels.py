@@ -975,7 +975,8 @@ def prefix_attention(q: torch.Tensor, prefix: dict, own: dict | None = None, *, 
     slots.  Prompt p is continued by B / P sequences, those of prompt 0 first, or with ``cu_rows`` int [P + 1], ascending from 0 to B,
     by the sequences [cu_rows[p], cu_rows[p + 1]); ``max_rows``, the most sequences of one prompt where the caller knows it, is what the
     kernel's blocks are then sized for.  ``prefix_starts`` / ``prefix_lens`` int [P]: prompt p is the slots [start, len) of its row;
-    ``own_lens`` int [B]: a sequence's own tokens are the slots [0, len) of its row.  Returns [B, Hq, D] in q's dtype, then fp32 with
+    ``own_lens`` int [B]: a sequence's own tokens are the slots [0, len) of its row.  Whatever q's type, the products' operands are fp16
+    and their sums fp32.  Returns [B, Hq, D] in q's dtype, then fp32 with
     ``want_f32``, then the fp32 log-sum-exp [B, Hq] of the scaled logits with ``want_lse``.
     """
     q, B, Hq, q_sb, q_sh = _one_token("prefix_attention", q)
