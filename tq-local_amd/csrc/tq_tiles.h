@@ -613,7 +613,7 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
 #pragma unroll
             for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[m][i]);
             // neither -inf nor NaN raises the reference
-            if (__any(__builtin_fmaf(mx, c[m], -top[m]) > LAZY) || rise) {
+            if (__any(__builtin_fmaf(mx, c[m], -top[m]) > LAZY || need > 0)) {
                 mx = max_of_halves(mx) * c[m];
                 const float ref = mx > top[m] ? mx : top[m];
                 const float corr = exp2_(top[m] == ref ? -(float)need : top[m] - ref - (float)need);
