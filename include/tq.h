@@ -426,8 +426,9 @@ int tq_keep_tokens(int n_buffers, void* const* buffers, const int* row_bytes, in
  *   out_f32, out_16  [batch][q_heads][dim], fp32 and the query's 16-bit type (bf16 for fp32 queries); at least one.  lse_out
  *            [batch][q_heads] (nullable; -inf for a sequence without tokens, whose output is 0)
  *   workspace  device scratch of tq_prefix_attention_workspace_bytes(); `uneven`: whether cu_rows is given
- * The products' operands are fp16 whatever the query's type (rotated queries, centroids, weights times norms in a unit of the row's own); sums
- * and softmax statistics are fp32.
+ * The products' operands are fp16: rotated queries (two terms of fp16 and fp32 ones for the codes' products), centroids, weights times norms
+ * in a unit of the row's own; sums and softmax statistics are fp32.  Centroids that fp16 holds badly may be given times a factor, and their
+ * rotation divided by it.
  * Offsets that descend or leave [0, batch] are taken as empty prompts and as the ends of the batch.  TQ_ERR_UNSUPPORTED beyond
  * 2^29 tokens (64 n_own counted), 2^26 query rows or 64 query heads per KV head.
  */

@@ -525,3 +525,21 @@ def test_norms_of_neighbours_are_their_own(cuda, n, H, g, M, n_prefix, large_fir
         k, v = torch.cat((pk[:, :, :n_prefix], ok[b:b + 1]), 2), torch.cat((pv[:, :, :n_prefix], ov[b:b + 1]), 2)
         sizes, _ = attend64(q[b:b + 1], k, v.abs())
         assert ((f32[b] - alone[0]).double().abs() <= (2.0 ** -10 + 2.0 ** -17) * sizes[0]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("bits", [1, 2, 3, 4])
+@pytest.mark.parametrize("each", [2, 12])
+def test_rotated_queries_keep_their_bits(cuda, dtype, bits, each):
+    """Of one token's logits, where the centroids are fp16 numbers, what is left is the rotation's products (two bf16 terms each: up to 2^-16 of
+    one, 2^-16 / sqrt 3 root mean square, is left out) and sums in fp32: of a logit scale |k| <q R^T, C> with |q| = sqrt 128, |k| about 20
+    and |C| about 1 1.6e-5 root mean square.  One fp16 term of a rotated query (2^-11 / sqrt 12 and more) leaves 2e-4."""
+    layer = make_layer(8, 2, 1, bits, False, seed=29)
+    c = layer.codecs.value
+    exact = K.CodecParams(c.bits, c.rotation, c.centers.half().float(), c.boundaries)
+    layer.codecs = copy.copy(layer.codecs)
+    layer.codecs.key = layer.codecs.value = exact
+    q = randn((8 * each, 8, D), 5, torch.float32).to(dtype)
+    _, lse = K.prefix_attention(q, arrays(layer), None, n_prefix=1, **codec(layer), want_lse=True)
+    _, ref = reference(q, layer, None, [each] * 8)
+    assert ((lse.double() - ref) ** 2).mean().sqrt() <= 5e-5

@@ -12,7 +12,7 @@
 // trees are: three prompts of 131072 tokens with 21, 3 and 8 sequences (8 KV heads of 5 query heads, 4-bit Q_prod) take 319 us, the 458 MB of
 // codes at 1.4 TB/s, the products at 0.41 PFLOP/s (0.69 with the rows that fill the blocks up); vector instructions have 59% and matrix instructions 36% of a
 // SIMD's time, at the 1.9 GHz that this leaves.  32 sequences behind 32768 tokens (8 of 4 heads) take 60 us, 8 sequences behind each of
-// four padded prompts of 8192 tokens (4 of 7 heads, 3-bit Q_mse, fp16) 29.5.  Small calls are bound by what comes before the first tile
+// four padded prompts of 8192 tokens (4 of 7 heads, 3-bit Q_mse, fp16) 30.  Small calls are bound by what comes before the first tile
 // and after the last: two sequences behind 1037 tokens take 15.6, the kernel 12 (the first bytes from memory, the queries' rotation, the
 // table of values, the waves' meeting, 1 to 3 us each) and the merge 4.
 // A copy of the prompt for every sequence and tq_decode_attention (8 of 4 heads, 4-bit Q_prod): 16 sequences behind 32768 tokens 114 us,
@@ -194,6 +194,9 @@ struct PrefixSource {
     __device__ __forceinline__ void take_row(int m, int r) { member[m] = r / a.group; }
 };
 
+// fp16 and fp32 queries (NQ = 2) keep their bits behind the rotation too, in two fp16 terms (LO): 32 sequences behind 32768 tokens (8 of 4 heads,
+// 4-bit Q_prod, fp16) take 68.6 us and 60.2 with one term, the padded prompts above 29.9 and 28.9, and lose 5.4e-4 and 7.1e-4 of an output's
+// norm, 2.5e-4 with scaled codebooks as well.
 template <int KB, int VB, bool QJL, int RB, int NQ>
 __global__ __launch_bounds__(Tiles<RB>::T, 2) void prefix_kernel(PrefixArgs a, Codec codec) {
     const int lane = threadIdx.x & 63;
@@ -224,7 +227,7 @@ __global__ __launch_bounds__(Tiles<RB>::T, 2) void prefix_kernel(PrefixArgs a, C
     PrefixSource<RB> src(a, at, slot, kvh, range, own_len);
     if (src.split() == 0 && kvh == 0 && (int)threadIdx.x < at.item.count)
         a.row_slots[at.item.first + threadIdx.x] = make_int4(at.first, at.n, at.step, threadIdx.x);
-    attend_tiles<KB, VB, QJL, RB, NQ>(codec, src, lane, wave);
+    attend_tiles<KB, VB, QJL, RB, NQ, (NQ > 1)>(codec, src, lane, wave);
 }
 
 // Rows of [batch][q head].

@@ -14,8 +14,9 @@
 // codes at a time (PairTable), and turned around by ds_read_b64_tr_b16.
 //
 // Rounding.  Rotated queries and centroids are rounded once to fp16, by at most 2^-11 of each, 2^-11 / sqrt(3) root mean square (with
-// |q| = 11 and |k| = 20 a logit moves by 7e-4), value centroids too (their sum's errors are kept from adding up by the
-// codebook, see tq_value_codebook_f16), weights times norm p |v| once: to 11 bits down to 2^-25 of the largest norm's, of the tiles that
+// |q| = 11 and |k| = 20 a logit moves by 7e-4; the queries' part of it goes with LO, most of the centroids' where the caller gives them times a
+// factor that fp16 holds them well with, and the rotation divided by it), value centroids too (their sum's errors are kept from adding up
+// by the codebook, see tq_value_codebook_f16, or that factor), weights times norm p |v| once: to 11 bits down to 2^-25 of the largest norm's, of the tiles that
 // the row attends to any of, at the row's reference, and by up to 2^-36 of it below.  Logits, maxima, weights, sums and outputs are
 // fp32.
 
@@ -267,7 +268,7 @@ struct PairTable {
 // 32 RB rows of a KV head to a workgroup, all of them in every wave; the waves take the tiles of 32 tokens in turn.  A lane
 // is a token and half of its dims: the keys' codes and signs become its A operands in registers; the values' codes go,
 // 16 tokens at a time, through 4 KB of LDS of the wave's own.  No barrier until the waves' sums meet at the end.
-template <int RB>
+template <int RB, bool LO = false>
 struct Tiles {
     static constexpr int W = 8;
     static constexpr int T = 64 * W;
@@ -276,6 +277,7 @@ struct Tiles {
     struct Parts {
         // the rows' operands for the signs and for the codes (these go on to registers with one block of rows; two do not fit)
         uint4 qs[RB][8 * 64], qc[RB][8 * 64];
+        uint4 ql[LO ? RB : 1][LO ? 8 * 64 : 1];  // what fp16 leaves of the codes'
         uint16_t kn[W][32], vn[W][32];
         float ratio[W][32];
         uint32_t table[256 * 64];
@@ -302,9 +304,12 @@ struct Tiles {
 //   seen(m, tile)      bit t: whether row 32 m + lane % 32 attends to the tile's token t
 //   rows(), partial()  rows whose sums are wanted, and where they go
 //   prefetch(), publish(), take_row()  its own loads: asked for, shared in LDS, and taken by a lane for row 32 m + lane % 32
-template <int KB, int VB, bool QJL, int RB, int NQ, class Source>
+//
+// LO: the rotated queries are two fp16 terms for the codes' products (the signs' weigh a tenth of them), which leave out 2^-22 of a
+// number, for queries of more bits than bf16 ones.
+template <int KB, int VB, bool QJL, int RB, int NQ, bool LO = false, class Source>
 __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int lane, int wave) {
-    using N = Tiles<RB>;
+    using N = Tiles<RB, LO>;
     constexpr int W = N::W;
     __shared__ typename N::Lds lds;
     __shared__ float s_centers[1 << VB];
@@ -425,24 +430,32 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
             const float up = __uint_as_float((uint32_t)(127 + e) << 23);
             // what is next to one another goes out together
             if (mat == 0) {
-                uint8_t* const to = reinterpret_cast<uint8_t*>(lds.t.qc[m]) + operand_offset(position_of<KB>(j0 + 4 * h)) + 16 * r;
+                auto write = [&](uint4* operands) INLINE {
+                    uint8_t* const to = reinterpret_cast<uint8_t*>(operands) + operand_offset(position_of<KB>(j0 + 4 * h)) + 16 * r;
+                    if constexpr (KB == 3 || KB == 1) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<uint2*>(to + operand_offset(position_of<KB>(e))) =
+                                make_uint2(pack_f16(acc[e], acc[4 + e]), pack_f16(acc[8 + e], acc[12 + e]));
+                    } else if constexpr (KB == 4) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            *reinterpret_cast<uint32_t*>(to + operand_offset(position_of<KB>(8 * (i >> 1) + (i & 1)))) =
+                                pack_f16(acc[4 * (i >> 1) + (i & 1)], acc[4 * (i >> 1) + (i & 1) + 2]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            *reinterpret_cast<uint16_t*>(to + operand_offset(position_of<KB>(8 * (i >> 2) + (i & 3)))) =
+                                (uint16_t)tq::f32_to_f16(acc[i]);
+                    }
+                };
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[i] *= up;
-                if constexpr (KB == 3 || KB == 1) {
+                write(lds.t.qc[m]);
+                if constexpr (LO) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        *reinterpret_cast<uint2*>(to + operand_offset(position_of<KB>(e))) =
-                            make_uint2(pack_f16(acc[e], acc[4 + e]), pack_f16(acc[8 + e], acc[12 + e]));
-                } else if constexpr (KB == 4) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint32_t*>(to + operand_offset(position_of<KB>(8 * (i >> 1) + (i & 1)))) =
-                            pack_f16(acc[4 * (i >> 1) + (i & 1)], acc[4 * (i >> 1) + (i & 1) + 2]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        *reinterpret_cast<uint16_t*>(to + operand_offset(position_of<KB>(8 * (i >> 2) + (i & 3)))) =
-                            (uint16_t)tq::f32_to_f16(acc[i]);
+                    for (int i = 0; i < 16; ++i) acc[i] -= tq::f16_to_f32(tq::f32_to_f16(acc[i]));
+                    write(lds.t.ql[m]);
                 }
             } else if (QJL) {
                 uint8_t* const to = reinterpret_cast<uint8_t*>(lds.t.qs[m]) + operand_offset(sign_position_of(j0 + 4 * h)) + 16 * r;
@@ -528,13 +541,18 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
         f32x16 x[RB];
 #pragma unroll
         for (int m = 0; m < RB; ++m) x[m] = zero16();
-        constexpr int SIGNS = QJL ? 8 : 0, STEPS = SIGNS + 8;
+        // A code's chunk meets the queries' lower terms, then their higher ones
+        constexpr int SIGNS = QJL ? 8 : 0, TERMS = LO ? 2 : 1, STEPS = SIGNS + 8 * TERMS;
+        auto chunk_of = [](int i) INLINE { return i < SIGNS ? i : SIGNS + (i - SIGNS) / TERMS; };
+        auto lower = [](int i) INLINE { return LO && i >= SIGNS && (i - SIGNS) % TERMS == 0; };
         Frag ring[2][RB];
         auto ask = [&](int i) INLINE {
 #pragma unroll
             for (int m = 0; m < RB; ++m) {
+                const int c = chunk_of(i) - SIGNS;
                 if (i < SIGNS) ring[i % 2][m].q = lds.t.qs[m][i * 64 + lane];
-                else if (RB > 1) ring[i % 2][m].q = lds.t.qc[m][(i - SIGNS) * 64 + lane];
+                else if (lower(i)) ring[i % 2][m].q = lds.t.ql[m][c * 64 + lane];
+                else if (RB > 1) ring[i % 2][m].q = lds.t.qc[m][c * 64 + lane];
             }
         };
         uint32_t code[8];
@@ -566,11 +584,12 @@ __device__ __forceinline__ void attend_tiles(const Codec& a, Source& src, int la
                 }
             }
             Frag next;
-            if (i + 1 < STEPS) next = chunk(i + 1);
+            const bool turn = i + 1 < STEPS && chunk_of(i + 1) != chunk_of(i);
+            if (turn) next = chunk(chunk_of(i + 1));
 #pragma unroll
             for (int m = 0; m < RB; ++m)
-                x[m] = mfma_f16(now, RB > 1 || i < SIGNS ? ring[i % 2][m] : q[(i - SIGNS) & 7], x[m]);
-            now = next;
+                x[m] = mfma_f16(now, RB > 1 || i < SIGNS || lower(i) ? ring[i % 2][m] : q[(chunk_of(i) - SIGNS) & 7], x[m]);
+            if (turn) now = next;
             if constexpr (RB > 1) __builtin_amdgcn_sched_barrier(0);  // the registers hold a few operands at a time
         }
         // the largest finite |v| of the tile: its exponent decides the unit (2^(e + 1) is above it)
