@@ -1,5 +1,7 @@
 """The fp16 codebook of a layer's values is there before its first attention, which may be a captured one."""
 
+import dataclasses
+
 import pytest
 import torch
 
@@ -35,3 +37,39 @@ def test_a_layers_first_attention_captured(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("values", [False, True])
+@pytest.mark.parametrize("bits", [1, 2, 3, 4])
+def test_scaled_codebooks(bits, values):
+    """The same products of rotated queries and centroids, from centroids that fp16 holds better."""
+    c = layer_codecs(128, bits, 0, False, "cpu").value
+    rotation, centers = K.scaled_codec(c, values)
+    assert K.scaled_codec(c, values)[0] is rotation and rotation.dtype == centers.dtype == torch.float32
+    assert torch.equal(centers, centers.half().float())
+    at = torch.argmax(c.rotation.abs())
+    s = (c.rotation.flatten()[at].double() / rotation.flatten()[at]).item()
+    assert 1.0 <= s < 2.0 + 1e-6 and (rotation * s - c.rotation).abs().max() <= 2.0 ** -23
+    x = c.centers.double()
+    middle = (x[1:] + x[:-1]) / 2
+    n = 1 << 16
+    grid = (torch.arange(n).double() + 0.5) / n * 2 - 1
+    weight = (1 - grid ** 2) ** 62.5
+    share = torch.zeros(1 << bits).double().index_add_(0, torch.bucketize(grid, middle), weight) / weight.sum()
+    size = lambda e: (share * e ** 2).sum().sqrt() / (share * x ** 2).sum().sqrt()  # noqa: E731
+    err = centers.double() / s - x
+    assert size(err) <= 0.8 * size(x.half().double() - x)
+    if values:
+        assert abs((share * err).sum()) <= 1e-6 * (share * x ** 2).sum().sqrt()
+
+
+def test_scaled_codebooks_go_with_their_codec():
+    """A codec with another codebook does not keep the first one's; codebooks past fp16's range, and of one number, have one."""
+    c = layer_codecs(128, 2, 0, False, "cpu").value
+    K.scaled_codec(c, True)
+    other = dataclasses.replace(c, centers=c.centers * 0.7)
+    assert other.attn_values is None and not torch.equal(K.scaled_codec(other, True)[1], K.scaled_codec(c, True)[1])
+    exact = dataclasses.replace(c, centers=torch.tensor([-0.5, -0.25, 0.25, 0.5]))
+    assert torch.equal(K.scaled_codec(exact, False)[1], exact.centers) and torch.equal(K.scaled_codec(exact, False)[0], c.rotation)
+    large = dataclasses.replace(c, centers=torch.tensor([-6e4, -1.0, 1.0, 6e4]))
+    assert torch.isfinite(K.scaled_codec(large, True)[1]).all()

@@ -543,3 +543,17 @@ def test_rotated_queries_keep_their_bits(cuda, dtype, bits, each):
     _, lse = K.prefix_attention(q, arrays(layer), None, n_prefix=1, **codec(layer), want_lse=True)
     _, ref = reference(q, layer, None, [each] * 8)
     assert ((lse.double() - ref) ** 2).mean().sqrt() <= 5e-5
+
+
+@pytest.mark.parametrize("bits,qjl", BITS)
+@pytest.mark.parametrize("size", [1.0, 1e-3])
+@pytest.mark.parametrize("each", [2, 12])
+def test_fp32_queries_lose_little_to_fp16_codebooks(cuda, bits, qjl, size, each):
+    """Of the output's norm: keys' centroids 1.2e-4 of a key, which moves a logit of |q| = sqrt 128 and |k| = 20 by 2.4e-4; values' 1.5e-4;
+    weights times norms 1.7e-4; signs' queries 0.8e-4: 3.4e-4 together.  With queries of a thousandth all tokens weigh the same, the values
+    nearly cancel, and the errors' mean would be what is left."""
+    counts = (each,)
+    prompts, own, q, kw = setup(counts, 2, 4, 8192, 64, bits, qjl, torch.float32, seed=31)
+    q = q * size
+    ref, _ = reference(q, prompts, own, counts)
+    assert (call(prompts, own, q, kw).double() - ref).norm() <= 4e-4 * ref.norm()

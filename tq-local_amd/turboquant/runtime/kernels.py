@@ -25,9 +25,10 @@ part).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from array import array
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
@@ -94,7 +95,7 @@ class CodecParams:
     """Device-resident parameters of one Q_mse codec (rotation, codebook).
 
     ``attn_centers`` caches the codebook's fp16 form for the decode attention's value sums
-    (``attention_value_centers``).
+    (``attention_value_centers``), ``attn_keys`` and ``attn_values`` what ``scaled_codec`` makes.
     """
 
     bits: int
@@ -102,6 +103,8 @@ class CodecParams:
     centers: torch.Tensor  # fp32 [2^bits]
     boundaries: torch.Tensor  # fp32 [2^bits - 1]
     attn_centers: torch.Tensor | None = None  # fp32 [2^bits], fp16-exact values
+    attn_keys: tuple[torch.Tensor, torch.Tensor] | None = field(default=None, init=False, repr=False, compare=False)
+    attn_values: tuple[torch.Tensor, torch.Tensor] | None = field(default=None, init=False, repr=False, compare=False)
 
 
 @dataclass
@@ -345,6 +348,44 @@ def attention_value_centers(codec: CodecParams | GroupCodec) -> torch.Tensor:
         host = value_codebook_f16(codec.centers.detach().cpu().numpy(), codec.bits, dim)
         codec.attn_centers = torch.from_numpy(host).to(codec.centers.device)
     return codec.attn_centers
+
+
+@functools.lru_cache(maxsize=64)
+def _codebook_scale(centers: bytes, mean: float) -> float:
+    """The s of 2^14 in [1, 2) for which s C is nearest to fp16 numbers: the least sum of the squared errors and ``mean`` times their
+    mean's square, weighed by the codes' shares among a rotated vector's coordinates, whose density is (1 - x^2)^((D - 3) / 2)."""
+    c = np.frombuffer(centers, dtype=np.float32).astype(np.float64)
+    grid = np.linspace(-1.0, 1.0, (1 << 14) + 1)
+    below = np.cumsum((1.0 - grid ** 2) ** ((HEAD_DIM - 3) / 2))
+    order = np.sort(c)
+    ends = np.interp(0.5 * (order[1:] + order[:-1]), grid, below / below[-1])
+    share = np.diff(ends, prepend=0.0, append=1.0)[np.argsort(np.argsort(c))][:, None]
+    s = 1.0 + np.arange(1 << 14) / (1 << 14)
+    x = c[:, None] * s
+    with np.errstate(over="ignore", invalid="ignore"):  # past fp16's range
+        err = (x.astype(np.float16) - x) / s
+        loss = (share * err ** 2).sum(0) + mean * (share * err).sum(0) ** 2
+    return float(s[np.argmin(np.nan_to_num(loss, nan=np.inf))])
+
+
+def scaled_codec(codec: CodecParams, values: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """(R / s, s C rounded to fp16), both fp32, in which <q R^T, C> = <q (R / s)^T, s C> and (sum w C) R = (sum w s C) (R / s) lose less to
+    fp16 centroids: of a key's norm 1.2e-4 where those of C itself lose 2.2e-4 with 4 bits, 0.9e-4 and 1.7e-4 with 3, 0.05e-4 and 0.7e-4 with
+    2.  ``values``: the errors' mean is kept small before their size (2^15 times its square counts), as it adds up over the tokens of an
+    even softmax where the values cancel; 1.5e-4, 1.1e-4 and 0.1e-4 then.  Computed once per codec, on the host; a captured call that none
+    came before has the codebooks as they are."""
+    made = codec.attn_values if values else codec.attn_keys
+    if made is None:
+        if codec.centers.is_cuda and torch.cuda.is_current_stream_capturing():
+            return codec.rotation, attention_value_centers(codec) if values else codec.centers
+        centers = codec.centers.detach()
+        s = _codebook_scale(np.ascontiguousarray(centers.cpu().numpy(), dtype=np.float32).tobytes(), 2.0 ** 15 if values else 0.0)
+        made = codec.rotation.detach() / s, (centers.double() * s).half().float()
+        if values:
+            codec.attn_values = made
+        else:
+            codec.attn_keys = made
+    return made
 
 
 def decode_attention(q: torch.Tensor, *, k_codes: torch.Tensor, k_norms: torch.Tensor, v_codes: torch.Tensor,
@@ -975,8 +1016,8 @@ def prefix_attention(q: torch.Tensor, prefix: dict, own: dict | None = None, *, 
     slots.  Prompt p is continued by B / P sequences, those of prompt 0 first, or with ``cu_rows`` int [P + 1], ascending from 0 to B,
     by the sequences [cu_rows[p], cu_rows[p + 1]); ``max_rows``, the most sequences of one prompt where the caller knows it, is what the
     kernel's blocks are then sized for.  ``prefix_starts`` / ``prefix_lens`` int [P]: prompt p is the slots [start, len) of its row;
-    ``own_lens`` int [B]: a sequence's own tokens are the slots [0, len) of its row.  Whatever q's type, the products' operands are fp16
-    and their sums fp32.  Returns [B, Hq, D] in q's dtype, then fp32 with
+    ``own_lens`` int [B]: a sequence's own tokens are the slots [0, len) of its row.  The products' operands are fp16, rotated
+    queries of fp16 and fp32 two such terms, and their sums fp32.  Returns [B, Hq, D] in q's dtype, then fp32 with
     ``want_f32``, then the fp32 log-sum-exp [B, Hq] of the scaled logits with ``want_lse``.
     """
     q, B, Hq, q_sb, q_sh = _one_token("prefix_attention", q)
@@ -993,6 +1034,7 @@ def prefix_attention(q: torch.Tensor, prefix: dict, own: dict | None = None, *, 
         if sh[1] != Hkv:
             raise ValueError(f"own: {sh[1]} KV heads, the prompts have {Hkv}")
     _check_codec(key, value, qjl, on)
+    (key_rotation, key_centers), (value_rotation, value_centers) = scaled_codec(key, False), scaled_codec(value, True)
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads for {Hkv} KV heads")
     if not 0 <= n_prefix <= cap or not 0 <= n_own <= own_cap:
@@ -1014,8 +1056,8 @@ def prefix_attention(q: torch.Tensor, prefix: dict, own: dict | None = None, *, 
         at, at_own = array("Q", shared), array("Q", mine)
         _on_device("tq_prefix_attention", on, q.data_ptr(), _QUERY_TYPES[dtype], B, Hq, Hkv, D, q_sb, q_sh, P, _ptr(cu_rows), rows,
                    _ptr(prefix_starts), _ptr(prefix_lens), n_prefix, cap, at.buffer_info()[0], _ptr(own_lens), n_own,
-                   own_cap, at_own.buffer_info()[0], key.bits, value.bits, int(has_qjl), key.rotation.data_ptr(),
-                   key.centers.data_ptr(), _ptr(qjl), value.rotation.data_ptr(), attention_value_centers(value).data_ptr(), s,
+                   own_cap, at_own.buffer_info()[0], key.bits, value.bits, int(has_qjl), key_rotation.data_ptr(),
+                   key_centers.data_ptr(), _ptr(qjl), value_rotation.data_ptr(), value_centers.data_ptr(), s,
                    _ptr(f32), _ptr(out), _ptr(lse), ws.data_ptr(), max(need, 16), _stream_handle(dev))
     outs = (f32 if out is None else out,) + ((f32,) if want_f32 else ()) + ((lse,) if want_lse else ())
     return outs if len(outs) > 1 else outs[0]

@@ -32,7 +32,7 @@ from turboquant.quantization.turboquant_mse import (
     generate_qjl_matrix,
     random_rotation_matrix,
 )
-from turboquant.runtime.kernels import HEAD_DIM, CodecParams, GroupCodec, group_matrix, value_codebook_f16
+from turboquant.runtime.kernels import HEAD_DIM, CodecParams, GroupCodec, group_matrix, scaled_codec, value_codebook_f16
 
 #: widest code libtq's channel-group kernels pack
 MAX_GROUP_BITS = 8
@@ -101,6 +101,8 @@ def layer_codecs(dim: int, bits: int, seed: int, use_qjl_keys: bool, device: tor
         qjl = generate_qjl_matrix(dim, seed + QJL_SEED_OFFSET).to(device)
     else:
         kc, qjl = value, None
+    if dim == HEAD_DIM:  # for the attention behind shared prompts, on the host too (2 to 10 ms)
+        scaled_codec(kc, False), scaled_codec(value, True)
     out = LayerCodecs(bits=bits, use_qjl_keys=use_qjl_keys, key=kc, value=value, qjl=qjl)
     _device_cache[key] = out
     return out
