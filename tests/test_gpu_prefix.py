@@ -557,3 +557,30 @@ def test_fp32_queries_lose_little_to_fp16_codebooks(cuda, bits, qjl, size, each)
     q = q * size
     ref, _ = reference(q, prompts, own, counts)
     assert (call(prompts, own, q, kw).double() - ref).norm() <= 4e-4 * ref.norm()
+
+
+def test_a_codec_made_by_hand_on_several_streams(cuda):
+    """Its codebooks are made at the first call, on that call's stream, and taken by calls on others."""
+    prompts, own, q, kw = setup((3, 4), 2, 4, 300, 20, seed=33)
+    want = call(prompts, own, q, kw)
+    torch.cuda.synchronize()
+    kw.update({name: K.CodecParams(c.bits, c.rotation, c.centers, c.boundaries) for name, c in (("key", kw["key"]), ("value", kw["value"]))})
+    outs = []
+    for held_up in (10_000_000, 0):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            if held_up:
+                torch.cuda._sleep(held_up)
+            outs.append(call(prompts, own, q, kw))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs.append(call(prompts, own, q, kw))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    alone = {name: K.CodecParams(c.bits, c.rotation, c.centers, c.boundaries) for name, c in (("key", kw["key"]), ("value", kw["value"]))}
+    K.attention_value_centers(alone["value"])
+    with torch.cuda.graph(graph := torch.cuda.CUDAGraph()):  # a capture that nothing came before
+        out = call(prompts, own, q, dict(kw, **alone))
+    graph.replay()
+    torch.cuda.synchronize()
+    check(out, reference(q, prompts, own, (3, 4))[0])

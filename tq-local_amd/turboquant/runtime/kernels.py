@@ -381,6 +381,8 @@ def scaled_codec(codec: CodecParams, values: bool) -> tuple[torch.Tensor, torch.
         centers = codec.centers.detach()
         s = _codebook_scale(np.ascontiguousarray(centers.cpu().numpy(), dtype=np.float32).tobytes(), 2.0 ** 15 if values else 0.0)
         made = codec.rotation.detach() / s, (centers.double() * s).half().float()
+        if centers.is_cuda:  # kept for calls on every stream
+            torch.cuda.current_stream(centers.device).synchronize()
         if values:
             codec.attn_values = made
         else:
