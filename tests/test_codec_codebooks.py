@@ -73,3 +73,18 @@ def test_scaled_codebooks_go_with_their_codec():
     assert torch.equal(K.scaled_codec(exact, False)[1], exact.centers) and torch.equal(K.scaled_codec(exact, False)[0], c.rotation)
     large = dataclasses.replace(c, centers=torch.tensor([-6e4, -1.0, 1.0, 6e4]))
     assert torch.isfinite(K.scaled_codec(large, True)[1]).all()
+
+
+def test_codebooks_are_searched_for_once(monkeypatch):
+    """Codecs made by hand of the same centroids; each keeps a tensor of its own."""
+    c = layer_codecs(128, 4, 0, False, "cpu").value
+    K._value_codebook.cache_clear()
+    searched, search = [], K.value_codebook_f16
+    monkeypatch.setattr(K, "value_codebook_f16", lambda *a: searched.append(a) or search(*a))
+    codecs = [K.CodecParams(4, c.rotation, c.centers.clone(), c.boundaries) for _ in range(3)]
+    made = [K.attention_value_centers(x) for x in codecs]
+    assert len(searched) == 1 and all(torch.equal(m, c.attn_centers) for m in made)
+    made[0].zero_()
+    assert torch.equal(K.attention_value_centers(K.CodecParams(4, c.rotation, c.centers, c.boundaries)), made[1])
+    K.attention_value_centers(dataclasses.replace(codecs[0], centers=c.centers * 0.9, attn_centers=None))
+    assert len(searched) == 2

@@ -336,17 +336,23 @@ def value_codebook_f16(centers: np.ndarray, bits: int, dim: int = HEAD_DIM) -> n
     return out
 
 
+@functools.lru_cache(maxsize=64)
+def _value_codebook(centers: bytes, bits: int, dim: int) -> np.ndarray:
+    return value_codebook_f16(np.frombuffer(centers, dtype=np.float32), bits, dim)
+
+
 def attention_value_centers(codec: CodecParams | GroupCodec) -> torch.Tensor:
     """The value codebook tq_decode_attention is given: ``value_codebook_f16`` of the
     codec's centers (at the group's dimension for a channel group), on the codec's
-    device, computed once per codec."""
+    device, computed once per codec and searched for once per codebook (1 ms with 4 bits, more
+    than a short call)."""
     if codec.attn_centers is None:
         if codec.centers.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a value codec's attention codebook is made on the host: call attention_value_centers(codec) "
                                "before the graph is captured")
         dim = codec.dim if isinstance(codec, GroupCodec) else HEAD_DIM
-        host = value_codebook_f16(codec.centers.detach().cpu().numpy(), codec.bits, dim)
-        codec.attn_centers = torch.from_numpy(host).to(codec.centers.device)
+        centers = np.ascontiguousarray(codec.centers.detach().cpu().numpy(), dtype=np.float32).tobytes()
+        codec.attn_centers = torch.tensor(_value_codebook(centers, codec.bits, dim), device=codec.centers.device)
     return codec.attn_centers
 
 
