@@ -338,6 +338,20 @@ def test_queries_of_other_types(cuda, dtype, bits, qjl, H, g):
     assert torch.equal(K.block_attention(exact.to(dtype), blocks, **kw, want_f32=True)[1], want)  # the other terms add zeros
 
 
+@pytest.mark.parametrize("bits,qjl", BITS)
+@pytest.mark.parametrize("size", [1.0, 1e-3])
+@pytest.mark.parametrize("g", [4, 7])
+def test_fp32_queries_lose_little_to_fp16_values(cuda, bits, qjl, size, g):
+    """Of the output's norm: values' centroids up to 1.5e-4, weights times norms up to 2^-11 / sqrt 3 = 2.8e-4: 3.2e-4 together.  With queries of a
+    thousandth all tokens weigh the same, the values nearly cancel, and the centroids' mean error would be what is left."""
+    layer = make_layer(1, 2, 16384, bits, qjl, seed=27)
+    q = randn((1, 2 * g, D), 5, torch.float32) * size
+    every = torch.arange(256, dtype=torch.int32, device="cuda").expand(1, 2, 256)
+    got = K.block_attention(q, every, **arrays(layer), **codec(layer), n_tokens=16384)
+    ref, _ = attend64(q, *rows64(layer))
+    assert (got.double() - ref).norm() <= 3.3e-4 * ref.norm()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("dense", [0, 30])
 @pytest.mark.parametrize("g", [4, 7])

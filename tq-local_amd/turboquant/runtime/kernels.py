@@ -1172,6 +1172,7 @@ def block_attention(q: torch.Tensor, blocks: torch.Tensor, *, k_codes: torch.Ten
     cache = {"k_codes": k_codes, "k_norms": k_norms, "k_signs": k_signs, "k_rnorms": k_rnorms, "v_codes": v_codes, "v_norms": v_norms}
     (kc, kn, ks, kr, vc, vn), (_, Hkv, cap) = _packed_arrays("block_attention", cache, B, key, value, has_qjl, on)
     _check_codec(key, value, qjl, on)
+    value_rotation, value_centers = scaled_codec(value, True)
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"{Hq} query heads for {Hkv} KV heads")
     if not 0 <= n_tokens <= cap:
@@ -1191,9 +1192,8 @@ def block_attention(q: torch.Tensor, blocks: torch.Tensor, *, k_codes: torch.Ten
         ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         _on_device("tq_block_attention_typed", on, q.data_ptr(), _QUERY_TYPES[q.dtype], B, Hq, Hkv, D, blocks.data_ptr(), keep,
                    _ptr(seq_starts), _ptr(seq_lens), n_tokens, cap, kc, kn, ks, kr, vc, vn, key.bits, value.bits, int(has_qjl),
-                   key.rotation.data_ptr(), key.centers.data_ptr(), _ptr(qjl), value.rotation.data_ptr(),
-                   attention_value_centers(value).data_ptr(), s, _ptr(f32), _ptr(out), _ptr(lse), ws.data_ptr(), max(need, 16),
-                   _stream_handle(dev))
+                   key.rotation.data_ptr(), key.centers.data_ptr(), _ptr(qjl), value_rotation.data_ptr(), value_centers.data_ptr(), s,
+                   _ptr(f32), _ptr(out), _ptr(lse), ws.data_ptr(), max(need, 16), _stream_handle(dev))
     else:  # nothing is attended to
         for t, x in ((out, 0.0), (f32, 0.0), (lse, float("-inf"))):
             if t is not None:

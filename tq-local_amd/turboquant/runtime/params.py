@@ -101,7 +101,7 @@ def layer_codecs(dim: int, bits: int, seed: int, use_qjl_keys: bool, device: tor
         qjl = generate_qjl_matrix(dim, seed + QJL_SEED_OFFSET).to(device)
     else:
         kc, qjl = value, None
-    if dim == HEAD_DIM:  # for the attention behind shared prompts, on the host too (2 to 10 ms)
+    if dim == HEAD_DIM:  # for the attention behind shared prompts and over blocks, on the host too (2 to 10 ms)
         scaled_codec(kc, False), scaled_codec(value, True)
     out = LayerCodecs(bits=bits, use_qjl_keys=use_qjl_keys, key=kc, value=value, qjl=qjl)
     _device_cache[key] = out
